@@ -129,7 +129,7 @@ __device__ __forceinline__ float block_magnitude(float v) {
 }
 // The IEEE divide for rare fallbacks, as a call: inlined, the compiler may evaluate it on every
 // path before the branch that needs it.
-__device__ __noinline__ float fdiv_slow(float a, float b) { return __fdiv_rn(a, b); }
+static __device__ __noinline__ float fdiv_slow(float a, float b) { return __fdiv_rn(a, b); }
 
 // mag / 127 correctly rounded, without the IEEE divide's branchy slow path: q0 = mag * y with
 // y = RN(1/127), then one remainder correction r = mag - q0 * 127 (exact, by FMA), q = q0 + r * y
@@ -221,7 +221,7 @@ __device__ __forceinline__ void quantize_blocks_warp(const float *v, int8_t *q, 
 }
 
 // Out of line: the persistent decode kernel calls it from two places every layer.
-__device__ __noinline__ float quantize_block_warp(float v, int8_t *q, int *bsum) {
+static __device__ __noinline__ float quantize_block_warp(float v, int8_t *q, int *bsum) {
     float scale;
     quantize_blocks_warp<1>(&v, q, &scale, bsum);
     return scale;

@@ -6,7 +6,7 @@
 // (runtime.py:281-299); here one device arena is laid out at creation, every step is the
 // same fixed sequence of fused kernels reading its sizes from device memory, and decode
 // steps replay one captured CUDA graph.
-#include "../../include/nc_cuda.h"
+#include "nc_api.cuh"
 #include "nc_attention.cuh"
 #include "nc_gemm_f32.cuh"
 #include "nc_lm_head_tc.cuh"
@@ -34,7 +34,7 @@ using namespace nc;
 // ---- errors ---------------------------------------------------------------------------------
 static thread_local std::string g_error;
 
-static int32_t fail(int32_t code, const char *fmt, ...) {
+int32_t nc::fail(int32_t code, const char *fmt, ...) {
     char buf[1024];
     va_list ap;
     va_start(ap, fmt);
@@ -43,20 +43,6 @@ static int32_t fail(int32_t code, const char *fmt, ...) {
     g_error = buf;
     return code;
 }
-
-#define CUDA_TRY(expr)                                                                       \
-    do {                                                                                     \
-        cudaError_t e_ = (expr);                                                             \
-        if (e_ != cudaSuccess)                                                               \
-            return fail(NC_ERR_CUDA, "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_), \
-                        __FILE__, __LINE__);                                                 \
-    } while (0)
-
-#define NC_TRY(expr)                  \
-    do {                              \
-        int32_t s_ = (expr);          \
-        if (s_ != NC_OK) return s_;   \
-    } while (0)
 
 extern "C" int32_t nc_last_error(char *buf, int64_t size) {
     if (buf && size > 0) {
@@ -98,17 +84,6 @@ extern "C" int32_t nc_device_synchronize(void) {
 
 // ---- kernel launchers (shared by the fused-group ABI and the model) -------------------------
 namespace {
-
-// Every kernel of the step is launched with programmatic stream serialization (PDL): it may
-// begin while its predecessor runs, prefetch immutable data (weights), and wait in-kernel for
-// the predecessor's results.  NC_PDL=0 in the environment turns it off (for A/B timing).
-bool pdl_enabled() {
-    static const bool on = [] {
-        const char *v = std::getenv("NC_PDL");
-        return !(v && v[0] == '0');
-    }();
-    return on;
-}
 
 // NC_SPLIT_ATTENTION=0 keeps few-row attention at one CTA per query head.
 bool split_attention_enabled() {
@@ -154,40 +129,6 @@ bool tc_head_enabled() {
 bool tc_i8_enabled() {
     const char *v = std::getenv("NC_TC_I8");
     return v && v[0] == '1';
-}
-
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 148;
-    return sms > 0 ? sms : 148;
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
-template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return cudaSuccess;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
-int32_t check_launch(const char *what) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(NC_ERR_CUDA, "launching %s: %s", what, cudaGetErrorString(e));
-    return NC_OK;
 }
 
 int32_t launch_norm(cudaStream_t st, float *normed, const float *x, const float *w, int8_t *xq, float *xs,
