@@ -205,6 +205,79 @@ int32_t nc_quantize_int8_rows(void **p, const int64_t *s, void *stream);
  * it against the IEEE divide on every non-negative float and reports the differences (0). */
 int32_t nc_selfcheck_div127(int64_t *mismatches);
 
+/* ---- 1b. serving operators ------------------------------------------------------------------
+ * A paged key/value cache held in 4 bits, and the log probabilities of a step's tokens.  They keep the
+ * p[] / s[] convention; they have no counterpart in the reference.  Element types: 0 float32, 1 float16,
+ * 2 bfloat16.  Nothing is allocated, nothing synchronizes, and calls on one stream follow one another; calls
+ * that may overlap need scratch of their own.  Scratch is given zeroed once; each call leaves what the next
+ * one needs.
+ *
+ * The cache.  A pool of `pages` pages of `page bytes` each.  A layer's part of a page begins at `layer offset`
+ * and takes kv_heads * page * d * 5 / 4 bytes: `page` positions (a multiple of 16) of every head, keys and
+ * values, in blocks of 32 along the head dimension (d: 32, 64, 96 or 128), each block with an f16 scale and
+ * zero and sixteen levels (layout and rounding: nanocompile_b200/csrc/nc_kv4.cuh).  Sequence i's position t
+ * is in page table[i][t / page].  Rows of a call: row_start[i] .. row_start[i + 1] - 1 are sequence i's last
+ * positions before lengths[i] (row_start null: one row of each sequence); row_start[0] = 0, ascending.
+ * A position whose page is not in 0..pages-1 (or that has no rotation angle) is left out, and the smallest
+ * such sequence is put into the error word (device u64, set to all ones before; nullable). */
+
+/* Quantises rows of keys and values into the cache; keys are rotated first (RoPE, as nc_attention does)
+ * where there is a table.  Rows before position 0 are left out.
+ * p: [0] pool  [1] keys [rows, kv, d]  [2] values [rows, kv, d]  [3] table i32[seqs, width]
+ *    [4] lengths i32[seqs], after the append  [5] row_start i32[seqs + 1] (nullable)
+ *    [6] cos f32[positions, d/2]  [7] sin (both nullable)  [8] error word (nullable)
+ * s: rows, seqs, kv_heads, d, page, pages, page bytes, layer offset, width, key row stride (elements),
+ *    value row stride, element type, positions */
+int32_t nc_kv4_append(void **p, const int64_t *s, void *stream);
+
+/* The values that rows' keys and values stand for (zeros where there is no position).
+ * p: [0] keys f32[rows, kv, d]  [1] values f32[rows, kv, d]  [2] pool  [3] table  [4] lengths
+ *    [5] row_start (nullable)  [6] error word (nullable)
+ * s: rows, seqs, kv_heads, d, page, pages, page bytes, layer offset, width */
+int32_t nc_kv4_read(void **p, const int64_t *s, void *stream);
+
+/* Attention of rows over the cache: row r at position t sees positions 0..t of its sequence; a row that sees
+ * nothing gets zeros and a log-sum of -inf.  Queries are rotated where there is a table.  float32 calls
+ * keep float32 accuracy (queries and probabilities as two f16 parts); 16-bit calls round each to one.
+ * p: [0] out [rows, heads, d]  [1] q [rows, heads, d]  [2] pool  [3] table  [4] lengths
+ *    [5] row_start (nullable)  [6] cos  [7] sin (nullable)  [8] log-sums f32[rows, heads] (nullable)
+ *    [9] scratch (device, >= nc_kv4_attention_scratch_bytes)  [10] error word (nullable)
+ * s: rows, seqs, kv_heads, d, page, pages, page bytes, layer offset, width, heads, q row stride, out row
+ *    stride, element type of q and out, positions, scale as float32 bits, the most rows of a sequence,
+ *    the most positions of a sequence, scratch bytes */
+int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream);
+int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_rows,
+                                       int64_t max_length);
+
+/* Forks, reorders, grows, cuts and frees sequences: new sequence i continues old sequence parent[i] (outside
+ * 0..seqs-1: none, length 0) with length clamp(length + grow[i], 0, width * page).  Pages are shared; the last
+ * page of a sequence, where not full, is its own (copied where it was shared).  Fresh pages are the lowest
+ * free ids, in the order of the new table.  The old table is left as it is.  If pages are missing or the
+ * table names pages outside the pool, the new table is the old one and nothing is copied.
+ * p: [0] new table i32[seqs, width]  [1] new lengths i32[seqs]  [2] table  [3] lengths
+ *    [4] status i64[4]: pages missing (-1: bad table), pages in use, pages copied, highest id in use + 1
+ *    [5] pool  [6] scratch (device, >= nc_kv_pages_scratch_bytes)  [7] parent i32[seqs] (null: each its own)
+ *    [8] grow i32[seqs] (null: 0)
+ * s: seqs, width, pages, page, page bytes (all layers), scratch bytes */
+int32_t nc_kv_pages_update(void **p, const int64_t *s, void *stream);
+
+/* Moves the n pages in use to the ids 0..n-1: those from n on go to the free ids below n, in order.
+ * p: as nc_kv_pages_update, without [1] (null), [7] and [8]; status as there (copied: pages moved).  s: as there. */
+int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream);
+int64_t nc_kv_pages_scratch_bytes(int64_t seqs, int64_t width, int64_t pages);
+
+/* Log probabilities of given tokens, entropy and the best alternatives of rows of logits.  Alternatives are
+ * ordered by value, the lowest index first among equals, a NaN before all else (np.argmax's order).  Logits of
+ * -inf have no share; a row of nothing else gets log probabilities and a log-sum of -inf and entropy 0.
+ * A target outside the vocabulary gets a NaN, and the smallest such row is put into the error word.
+ * p: [0] log probabilities f32[rows, targets]  [1] entropy f32[rows] (nullable)  [2] log-sums f32[rows] (nullable)
+ *    [3] top ids i64[rows, k]  [4] top log probabilities f32[rows, k]  [5] logits [rows, vocab]
+ *    [6] targets i64[rows, targets]  [7] scratch (device, >= nc_token_logprobs_scratch_bytes)
+ *    [8] error word (device u64, nullable)
+ * s: rows, vocab, logit row stride (elements), element type, targets, k (0..32), scratch bytes */
+int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream);
+int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
+
 /* ---- 2. the model runtime ---------------------------------------------------------------- */
 
 typedef struct nc_model nc_model;

@@ -22,11 +22,11 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = [HERE / "csrc" / "nc_cuda.cu"]
+SOURCES = [HERE / "csrc" / "nc_cuda.cu", HERE / "csrc" / "nc_serving.cu"]
 TARGET = HERE / "libnc_cuda.so"
 STAMP = TARGET.with_name(TARGET.name + ".stamp")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fmad=false",
-              "-Xcompiler", "-fPIC", "-shared"]
+              "-Xcompiler", "-fPIC", "-shared", "--threads", "2"]
 
 
 def depends() -> list[Path]:

@@ -1,0 +1,569 @@
+// nc_kv4_attention.cuh -- attention of query rows over a paged 4-bit cache (nc_kv4.cuh).
+//
+//   out[r, h] = sum_t softmax_t(scale * q[r, h] . k[t, h / G]) v[t, h / G],  t = 0 .. position of row r,
+// with q rotated (RoPE) where there is a table; zeros, and a log-sum of -inf, for a row that sees nothing.
+//
+// The products are matrix instructions on the codes themselves.  A code c in the low bits of an f16 is the
+// subnormal c 2^-24, in bits 4-7 it is 16 c 2^-24, so one AND makes a pair of operands from packed codes,
+// exactly; the 2^-24 and the 16 go into the queries.  The blocks' parameters stay outside the products:
+//   q . k[t]   = sum_b scale_k[t, b] (q . code)_b + zero_k[t, b] (sum of q over b)
+//   sum p v    = sum_b (p[t] scale_v[t, b]) (code - 7.5)  + (sum_t p[t] (zero_v + 7.5 scale_v)[t, b])
+// the first of each line by mma m16n8k16 (S^T = K Q^T with positions as rows; O^T = V^T P^T), the rest in
+// 32 bits.  Values average to little where their codes average to 7.5 scales: without the 7.5 the two sums
+// of the second line would cancel.
+//
+// Accuracy.  The matrix unit truncates its sums, at a place set by its operands' exponent fields: a sum of
+// products with subnormals loses up to ten bits.  So the values' codes are brought to normal numbers by the
+// subtraction of the 7.5 (one FMA for two), and the scores of float32 and float16 callers (HL) are made exact:
+// q is brought below 2^11 by a power of two and split into two whole numbers q = hi + lo 2^-11 of at most 11
+// bits, whose 32 products with a code fit the unit's bits, in an accumulator for each part.  p scale_v is split
+// into two f16 parts (22 bits), summed over one step and added to the running sum in float32.
+// bfloat16 callers take one f16 part of q and of p scale_v.
+//
+// Probabilities are held relative to ref = (running maximum) - k, where k lifts p scale_v to just below
+// 2^15 for the largest scale_v seen (k <= 15): any power of two cancels in sum p v / sum p, so the f16 range
+// costs nothing and no size of input leaves it.
+//
+// A CTA has the columns (row, head of the group) of one kv head, 8 NT of them; its warps take steps of 64
+// or 32 positions in turn, each with its own reference and sums, and meet in shared memory at the end.  A warp
+// copies its steps into its own ring of stages (cp.async, from before the queries are ready) and waits for
+// nobody else.  Few columns and a long cache are split over CTAs as well (chunks of whole steps); the last
+// CTA to finish joins the parts in their order, so results do not depend on the schedule.
+#pragma once
+
+#include "nc_kv4.cuh"
+
+namespace nc {
+
+// Tiles that a warp takes at a time: about 5 KB, and few enough values in registers for 16 warps on an SM.
+__host__ __device__ constexpr int kv4_step_tiles(int d) { return d <= 64 ? 4 : 2; }
+
+struct Kv4AttnArgs {
+    Kv4Rows at;
+    Kv4Pool pool;
+    void *out;                         // [rows][heads][d]
+    const void *q;                     // [rows][heads][d]
+    const float *cos_tab, *sin_tab;    // [positions][d / 2] or null
+    float *lse;                        // [rows][heads] or null
+    unsigned int *counter;             // [groups], zero before the call and after it
+    float *part;                       // [groups][splits][8 NT][d + 2]
+    int64_t q_stride, out_stride, positions;
+    uint64_t page_magic;               // ceil(2^37 / tiles of a page): the tile's page by a multiplication
+    float scale_log2e;
+    int type, heads, group, col_blocks, splits, chunk;   // chunk: steps of a split
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint2 &b) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// Pairs of codes less 7.5, times 2^-9 (exact), from c 2^-24 (multiplier 2^15) or 16 c 2^-24 (2^11).
+__device__ __forceinline__ uint32_t centred(uint32_t v, uint32_t multiplier) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(multiplier), "r"(0xa380a380u));
+    return r;
+}
+constexpr uint32_t CODE_LOW = 0x78007800u, CODE_HIGH = 0x68006800u;
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ void copy16_async(void *smem, const void *global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int D, int NT, bool HL, int W, int ST>
+struct Kv4AttnShape {
+    static constexpr int NB = D / 32, VB = kv4_vb(NB), COLS = 8 * NT, PARTS = HL ? 2 : 1;
+    static constexpr int TILES = kv4_step_tiles(D), STEP = TILES * KV4_TILE;   // positions of a step
+    static constexpr int MT = TILES < 4 / NT ? TILES : 4 / NT;         // tiles whose scores are held at a time
+    static constexpr int STAGE = TILES * 20 * D;                       // bytes
+    static constexpr int RING = W * ST * STAGE;
+    static constexpr int MERGE = W * COLS * (D + 2) * 4;               // shares the ring's bytes
+    static constexpr int BODY = RING > MERGE ? RING : MERGE;
+    static constexpr int QF = NB * 2 * NT * PARTS * 32 * 8;
+    static constexpr int SMEM = BODY + QF + COLS * (NB + 4) * 4;
+    static constexpr int CTAS = NT == 1 ? 16 / W : 8 / W;              // wanted on an SM
+};
+
+template <int D, int NT, bool HL, int W, int ST>
+__global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)) kv4_attention_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using S = Kv4AttnShape<D, NT, HL, W, ST>;
+    constexpr int NB = S::NB, VB = S::VB, COLS = S::COLS, MT = S::MT, TILES = S::TILES, STEP = S::STEP;
+    extern __shared__ __align__(128) char smem[];
+    uint2 *const qf = (uint2 *)(smem + S::BODY);                       // [block][half][nt][part][lane]
+    float *const qsum = (float *)(smem + S::BODY + S::QF);             // [block][col]
+    float *const qscale = qsum + NB * COLS;                            // [col]
+    int2 *const qrow = (int2 *)(qscale + COLS);                        // [col] row and head
+    int *const qpos = (int *)(qrow + COLS);                            // [col]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+
+    release_dependents();
+    wait_for_producer();
+    const int split = (int)(blockIdx.x % a.splits);
+    const unsigned group = blockIdx.x / a.splits;
+    const int cb = a.col_blocks - 1 - (int)(group % a.col_blocks);     // the longest histories first
+    const int head = (int)(group / a.col_blocks % a.pool.kv);
+    const int seq = (int)(group / a.col_blocks / a.pool.kv);
+    const int length = a.at.lengths[seq];
+    const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
+    const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;
+    if (row0 < 0 || nr <= 0 || (int64_t)row0 + nr > a.at.rows) return;
+    const int cols = nr * a.group, col0 = cb * COLS;                   // the entry point bounds rows * group
+    if (col0 >= cols) return;
+    const int ncol = min(cols - col0, COLS);
+    // Positions 0 .. end - 1 are seen by the block's last row, all of 0 .. first by every row of it.
+    const int first = length - nr + col0 / a.group, last = length - nr + (col0 + ncol - 1) / a.group;
+    const int end = last < 0 ? 0 : last + 1;
+    const int steps = min((end + STEP - 1) / STEP, a.splits * a.chunk);   // no more than the call provides for
+    const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;
+    if (split >= active) return;
+
+    char *const ring = smem + warp * ST * S::STAGE;
+    const int step0 = split * a.chunk + warp, step_end = min(steps, split * a.chunk + a.chunk);
+    const int tiles_per_page = a.at.page / KV4_TILE;
+    const int32_t *const table = a.at.table + (int64_t)seq * a.at.width;
+    // Where the lane's tile (lane % TILES) of a step lies; null past the end or where the table names no page.
+    auto tile_at = [&](int step) -> const char * {
+        const int tile = step * TILES + lane % TILES;
+        if (step >= step_end || tile * KV4_TILE >= end) return nullptr;
+        const int j = (int)((uint64_t)tile * a.page_magic >> 37);
+        const int page = j < a.at.width ? table[j] : -1;
+        if (page < 0 || page >= a.at.pages) {
+            if (a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+            return nullptr;
+        }
+        return a.pool.base + page * a.pool.page_bytes + ((int64_t)head * tiles_per_page + (tile - j * tiles_per_page)) * (20 * D);
+    };
+    auto issue = [&](int stage, const char *from) {
+        constexpr int PIECES = 20 * D / 16;                            // 16-byte pieces of a tile
+        char *const to = ring + stage * S::STAGE;
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) {
+            const char *const src = (const char *)__shfl_sync(0xffffffffu, (unsigned long long)from, k);
+            if (src)
+#pragma unroll
+                for (int i = 0; i < (PIECES + 31) / 32; ++i)
+                    if (i * 32 + 32 <= PIECES || i * 32 + lane < PIECES)
+                        copy16_async(to + k * 20 * D + (i * 32 + lane) * 16, src + (i * 32 + lane) * 16);
+        }
+    };
+    uint32_t held[ST];                                                 // which tiles of the steps in flight are there
+    int next = step0;
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) {
+        const char *const from = tile_at(next);
+        held[s] = __ballot_sync(0xffffffffu, from != nullptr);
+        issue(s, from);
+        copies_commit();
+        next += W;
+    }
+    const char *from_next = tile_at(next);
+
+    // The queries: rotated, brought to the f16 range, in the B operand's order.
+    for (int col = warp; col < COLS; col += W) {
+        const bool have = col < ncol;
+        const int r = have ? (col0 + col) / a.group : 0;
+        const int64_t row = row0 + r;
+        const int h = head * a.group + (have ? col0 + col - r * a.group : 0);
+        const int pos = have ? length - nr + r : -1;
+        const bool known = have && pos >= 0 && (!a.cos_tab || pos < a.positions);
+        if (have && pos >= 0 && !known && a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)seq);
+        float v[NB];
+        uint32_t mag = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            v[b] = known ? kv4_rotated(a.q, row * a.q_stride + (int64_t)h * D, 32 * b + lane, D, a.type, a.cos_tab,
+                                       a.sin_tab, pos)
+                         : 0.0f;
+            mag = max(mag, __float_as_uint(v[b]) & 0x7fffffffu);
+        }
+        mag = __reduce_max_sync(0xffffffffu, mag);
+        int e = 0;                                                     // |q| 2^e < 2^11
+        if (mag != 0 && mag < 0x7f800000u) e = 10 - ((int)(mag >> 23) - 127);
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        if (lane == 0) {
+            qscale[col] = fmul(a.scale_log2e, pow2i(24 - e));
+            qrow[col] = make_int2(row0 + r, h);
+            qpos[col] = known ? pos : -1;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float x = fmul(v[b], pow2i(e));
+            float hi = HL ? rintf(x) : __half2float(__float2half_rn(x));
+            const float lo = HL ? rintf(fmul(x - hi, 2048.0f)) : 0.0f;
+            float sum = HL ? __fmaf_rn(lo, 0x1p-11f, hi) : x;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) qsum[b * COLS + col] = fmul(sum, 0x1p-24f);
+            // dimension 8 c' + i of the block: nibble i -> k half (i >> 1) & 1, register i & 1, f16 half i >> 2
+            const int i = lane & 7, cc = lane >> 3;
+            const float unit = (i & 1) ? 0.0625f : 1.0f;
+            const int64_t at = (((b * 2 + ((i >> 1) & 1)) * NT + (col >> 3)) * S::PARTS) * 32 + 4 * (col & 7) + cc;
+            __half *const to = (__half *)(qf + at) + (i & 1) * 2 + (i >> 2);
+            *to = __float2half_rn(fmul(hi, unit));
+            if (HL) to[32 * 4] = __float2half_rn(fmul(lo, unit));
+        }
+    }
+    __syncthreads();
+
+    float ref[NT][2], l[NT][2], o[NB][2][NT][4], oz[NB][NT][2];
+    float f[NT][2];
+    int pos[NT][2];
+    int lift = 15;                                                     // k: the same for all columns
+    float top[NT][2];                                                  // the running maximum
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int col = 8 * nt + 2 * c + e;
+            top[nt][e] = ref[nt][e] = -INFINITY;
+            l[nt][e] = 0.0f;
+            f[nt][e] = qscale[col];
+            pos[nt][e] = qpos[col];
+        }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            oz[b][nt][0] = oz[b][nt][1] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[b][k][nt][e] = 0.0f;
+        }
+
+    int stage = 0;
+#pragma unroll 1
+    for (int step = step0; step < step_end; step += W) {
+        // Start the copies ST - 1 steps ahead, into the stage that the last step read.
+        issue(stage == 0 ? ST - 1 : stage - 1, from_next);
+        copies_commit();
+        held[ST - 1] = __ballot_sync(0xffffffffu, from_next != nullptr);
+        next += W;
+        from_next = tile_at(next);
+        copies_wait<ST - 1>();
+        __syncwarp();
+        const uint32_t whole = held[0];
+#pragma unroll
+        for (int s = 0; s + 1 < ST; ++s) held[s] = held[s + 1];
+        const char *const buf = ring + stage * S::STAGE;
+        const bool edge = (step + 1) * STEP > first + 1 || whole != 0xffffffffu;
+
+#pragma unroll 1
+        for (int sub = 0; sub < TILES; sub += MT) {
+            const char *const tiles = buf + sub * 20 * D;
+            float sc[MT][NT][4];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t ka[MT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint2 w = *(const uint2 *)(tiles + mt * 20 * D + kv4_code_word(VB, b, lane, 0) * 4);
+                    ka[mt][0][0] = w.x & 0x000f000fu;
+                    ka[mt][0][1] = w.y & 0x000f000fu;
+                    ka[mt][0][2] = w.x & 0x00f000f0u;
+                    ka[mt][0][3] = w.y & 0x00f000f0u;
+                    ka[mt][1][0] = w.x >> 8 & 0x000f000fu;
+                    ka[mt][1][1] = w.y >> 8 & 0x000f000fu;
+                    ka[mt][1][2] = w.x >> 8 & 0x00f000f0u;
+                    ka[mt][1][3] = w.y >> 8 & 0x00f000f0u;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint2 *const qb = qf + (b * 2 * NT + nt) * S::PARTS * 32 + lane;
+                    const uint2 q0 = qb[0], q1 = qb[NT * S::PARTS * 32];
+                    const uint2 r0 = HL ? qb[32] : q0, r1 = HL ? qb[NT * S::PARTS * 32 + 32] : q1;
+                    const float2 zs = *(const float2 *)(qsum + b * COLS + 8 * nt + 2 * c);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_f16(acc, ka[mt][0], q0);
+                        mma_f16(acc, ka[mt][1], q1);
+                        if (HL) {
+                            float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(low, ka[mt][0], r0);
+                            mma_f16(low, ka[mt][1], r1);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[e] = __fmaf_rn(low[e], 0x1p-11f, acc[e]);
+                        }
+                        const uint2 par = *(const uint2 *)(tiles + mt * 20 * D + 8 * D + kv4_param_word(NB, b, g) * 4);
+                        const float2 p0 = unpack_f16(par.x), p1 = unpack_f16(par.y);     // (scale, zero)
+                        float *const s = sc[mt][nt];
+                        s[0] = __fmaf_rn(p0.x, acc[0], b ? __fmaf_rn(p0.y, zs.x, s[0]) : fmul(p0.y, zs.x));
+                        s[1] = __fmaf_rn(p0.x, acc[1], b ? __fmaf_rn(p0.y, zs.y, s[1]) : fmul(p0.y, zs.y));
+                        s[2] = __fmaf_rn(p1.x, acc[2], b ? __fmaf_rn(p1.y, zs.x, s[2]) : fmul(p1.y, zs.x));
+                        s[3] = __fmaf_rn(p1.x, acc[3], b ? __fmaf_rn(p1.y, zs.y, s[3]) : fmul(p1.y, zs.y));
+                    }
+                }
+            }
+            const int t0 = step * STEP + sub * KV4_TILE + g;       // the lane's positions: t0 + 16 mt + 8 k
+            // The values' parameters, and the lift that their largest scale allows.
+            auto value_params = [&](int mt, int b) {
+                uint2 w = *(const uint2 *)(tiles + mt * 20 * D + 18 * D + kv4_param_word(NB, b, g) * 4);
+                if (edge) {                                            // past the end: whatever was there before
+                    const bool there = (whole >> (sub + mt) & 1) != 0;
+                    if (!there || t0 + 16 * mt >= end) w.x = 0;
+                    if (!there || t0 + 16 * mt + 8 >= end) w.y = 0;
+                }
+                return w;
+            };
+            uint32_t big = 0;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint2 w = value_params(mt, b);
+                    big = __vmaxu2(big, __vmaxu2(w.x, w.y));
+                }
+            big = __reduce_max_sync(0xffffffffu, big & 0x7fffu);       // scales are not negative; below 2^(exponent + 1)
+            lift = min(lift, max(29 - (int)(big >> 10), -1));
+
+            uint32_t seen[MT][NT];                                     // bits: score e of the tile counts
+            float alpha[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    seen[mt][nt] = 15u;
+                    if (edge) {                                        // masked scores are -inf
+                        const bool there = (whole >> (sub + mt) & 1) != 0;
+                        uint32_t ok = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool in = there && t0 + 16 * mt + 8 * (e >> 1) <= pos[nt][e & 1];
+                            if (in) ok |= 1u << e;
+                            else sc[mt][nt][e] = -INFINITY;
+                        }
+                        seen[mt][nt] = ok;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most[e & 1] = fmaxf(most[e & 1], sc[mt][nt][e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], x));
+                    top[nt][e] = fmaxf(top[nt][e], fmul(most[e], f[nt][e]));
+                    const bool none = top[nt][e] == -INFINITY;         // nothing seen so far: no reference yet
+                    const float base = none ? 0.0f : top[nt][e] - (float)lift;
+                    alpha[nt][e] = fast_exp2(ref[nt][e] - base);       // 0 at the first position seen
+                    ref[nt][e] = none ? -INFINITY : base;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float &s = sc[mt][nt][2 * k + e];
+                            s = fast_exp2(__fmaf_rn(s, f[nt][e], -base));
+                            sum += s;
+                        }
+                    l[nt][e] = __fmaf_rn(l[nt][e], alpha[nt][e], sum);
+                }
+            }
+            // P V, block by block.
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float acc[2][NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    oz[b][nt][0] = fmul(oz[b][nt][0], alpha[nt][0]);
+                    oz[b][nt][1] = fmul(oz[b][nt][1], alpha[nt][1]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[k][nt][e] = 0.0f;
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint2 w = *(const uint2 *)(tiles + mt * 20 * D + 10 * D + kv4_code_word(VB, b, lane, 0) * 4);
+                    uint32_t va[2][4];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t x = k ? w.x >> 8 : w.x, y = k ? w.y >> 8 : w.y;
+                        va[k][0] = centred(x & 0x000f000fu, CODE_LOW);
+                        va[k][1] = centred(x & 0x00f000f0u, CODE_HIGH);
+                        va[k][2] = centred(y & 0x000f000fu, CODE_LOW);
+                        va[k][3] = centred(y & 0x00f000f0u, CODE_HIGH);
+                    }
+                    const uint2 vp = value_params(mt, b);
+                    float2 par[2] = {unpack_f16(vp.x), unpack_f16(vp.y)};   // (scale, zero)
+                    par[0].y = __fmaf_rn(7.5f, par[0].x, par[0].y);
+                    par[1].y = __fmaf_rn(7.5f, par[1].x, par[1].y);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint2 hi, lo;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float p0 = sc[mt][nt][2 * k], p1 = sc[mt][nt][2 * k + 1];
+                            float x0 = fmul(p0, par[k].x), x1 = fmul(p1, par[k].x);
+                            float y0 = __fmaf_rn(p0, par[k].y, oz[b][nt][0]), y1 = __fmaf_rn(p1, par[k].y, oz[b][nt][1]);
+                            if (edge) {                                // a masked position counts for nothing, NaN or not
+                                if (!(seen[mt][nt] >> (2 * k) & 1)) x0 = 0.0f, y0 = oz[b][nt][0];
+                                if (!(seen[mt][nt] >> (2 * k + 1) & 1)) x1 = 0.0f, y1 = oz[b][nt][1];
+                            }
+                            oz[b][nt][0] = y0;
+                            oz[b][nt][1] = y1;
+                            const uint32_t h = pack_f16(x0, x1);
+                            (k ? hi.y : hi.x) = transpose_8x8(h);
+                            if (HL) {
+                                const float2 back = unpack_f16(h);
+                                (k ? lo.y : lo.x) = transpose_8x8(pack_f16(x0 - back.x, x1 - back.y));
+                            }
+                        }
+                        mma_f16(acc[0][nt], va[0], hi);
+                        mma_f16(acc[1][nt], va[1], hi);
+                        if (HL) {
+                            mma_f16(acc[0][nt], va[0], lo);
+                            mma_f16(acc[1][nt], va[1], lo);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[b][k][nt][e] = __fmaf_rn(o[b][k][nt][e], alpha[nt][e & 1], acc[k][nt][e]);
+            }
+        }
+        __syncwarp();
+        stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    copies_wait<0>();
+    __syncthreads();
+
+    // The warps' parts meet: [warp][col][D] values, then [warp][col] (reference, sum).
+    float *const mo = (float *)smem;
+    float2 *const ml = (float2 *)(mo + W * COLS * D);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[nt][e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            const int col = 8 * nt + 2 * c + e;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float z = oz[b][nt][e];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+                float4 v;                                              // 2^9: the codes' unit
+                v.x = __fmaf_rn(o[b][0][nt][e], 512.0f, z);
+                v.y = __fmaf_rn(o[b][0][nt][2 + e], 512.0f, z);
+                v.z = __fmaf_rn(o[b][1][nt][e], 512.0f, z);
+                v.w = __fmaf_rn(o[b][1][nt][2 + e], 512.0f, z);
+                *(float4 *)(mo + ((warp * COLS + col) * D + 32 * b + 4 * g)) = v;
+            }
+            if (g == 0) ml[warp * COLS + col] = make_float2(ref[nt][e], sum);
+        }
+    __syncthreads();
+
+    // Four dimensions of a column to a thread; weights of the parts relative to their largest reference.
+    const bool alone = active == 1;
+    float *const part = alone ? nullptr : a.part + ((int64_t)group * a.splits + split) * (COLS * (D + 2));
+    auto finish = [&](int col, int i, const float4 &v, float sum, float base) {
+        const int64_t row = qrow[col].x;
+        const int h = qrow[col].y;
+        const float inv = sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
+        const int64_t at = row * a.out_stride + (int64_t)h * D + i;
+        if (sum == 0.0f) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) kv_store(a.out, at + k, a.type, 0.0f);
+        } else {
+            kv_store(a.out, at, a.type, fmul(v.x, inv));
+            kv_store(a.out, at + 1, a.type, fmul(v.y, inv));
+            kv_store(a.out, at + 2, a.type, fmul(v.z, inv));
+            kv_store(a.out, at + 3, a.type, fmul(v.w, inv));
+        }
+        if (i == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.0f ? -INFINITY : fmul(base + log2f(sum), 0.6931471805599453f);
+    };
+    for (int at = threadIdx.x; at < ncol * (D / 4); at += 32 * W) {
+        const int col = at / (D / 4), i = at % (D / 4) * 4;
+        float2 rl[W];
+        float base = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            rl[w] = ml[w * COLS + col];
+            base = fmaxf(base, rl[w].x);
+        }
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float x = rl[w].x == -INFINITY ? 0.0f : fast_exp2(rl[w].x - base);
+            const float4 y = *(const float4 *)(mo + (w * COLS + col) * D + i);
+            v.x = __fmaf_rn(y.x, x, v.x);
+            v.y = __fmaf_rn(y.y, x, v.y);
+            v.z = __fmaf_rn(y.z, x, v.z);
+            v.w = __fmaf_rn(y.w, x, v.w);
+            sum = __fmaf_rn(rl[w].y, x, sum);
+        }
+        if (alone) {
+            finish(col, i, v, sum, base);
+        } else {
+            *(float4 *)(part + col * D + i) = v;
+            if (i == 0) *(float2 *)(part + COLS * D + 2 * col) = make_float2(base, sum);
+        }
+    }
+    if (alone) return;
+
+    // The last CTA of the group joins the splits' parts, in their order.
+    __shared__ unsigned int arrived;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) arrived = atomicAdd(a.counter + group, 1u);
+    __syncthreads();
+    if (arrived != (unsigned)active - 1) return;
+    __threadfence();
+    if (threadIdx.x == 0) a.counter[group] = 0;
+    const float *const parts = a.part + (int64_t)group * a.splits * (COLS * (D + 2));
+    for (int at = threadIdx.x; at < ncol * (D / 4); at += 32 * W) {
+        const int col = at / (D / 4), i = at % (D / 4) * 4;
+        float base = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int s = 0; s < active; ++s) {
+            const float *const p = parts + (int64_t)s * (COLS * (D + 2));
+            const float2 rl = __ldcg((const float2 *)(p + COLS * D + 2 * col));
+            const float4 y = __ldcg((const float4 *)(p + col * D + i));
+            const float to = fmaxf(base, rl.x);
+            const float x = rl.x == -INFINITY ? 0.0f : fast_exp2(rl.x - to), old = base == -INFINITY ? 0.0f : fast_exp2(base - to);
+            v.x = __fmaf_rn(v.x, old, fmul(y.x, x));
+            v.y = __fmaf_rn(v.y, old, fmul(y.y, x));
+            v.z = __fmaf_rn(v.z, old, fmul(y.z, x));
+            v.w = __fmaf_rn(v.w, old, fmul(y.w, x));
+            sum = __fmaf_rn(sum, old, fmul(rl.y, x));
+            base = to;
+        }
+        finish(col, i, v, sum, base);
+    }
+}
+
+}  // namespace nc

@@ -1,0 +1,380 @@
+// nc_serving.cu -- the serving entry points of include/nc_cuda.h: the paged 4-bit key/value cache
+// (append, read, attention, page updates) and token log probabilities.
+//
+// nanocompile keeps its history as float32 arrays that a step returns and takes back
+// (nanocompile/models/qwen2.py:232-271) and chooses tokens by argmax on the host
+// (nanocompile/models/qwen2.py:348-368); these operators have no counterpart there.
+#include "nc_api.cuh"
+#include "nc_kv4_attention.cuh"
+#include "nc_kv_pages.cuh"
+#include "nc_logprobs.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+using namespace nc;
+
+namespace {
+
+constexpr int64_t I32 = (int64_t(1) << 31) - 1;
+
+bool misaligned(const void *p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) != 0; }
+
+int32_t check_type(int64_t type) {
+    if (type < KV_F32 || type > KV_BF16) return fail(NC_ERR_ARGUMENT, "element type %lld: 0 float32, 1 float16, 2 bfloat16", (long long)type);
+    return NC_OK;
+}
+
+// The sizes that append, read and attention share.
+int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, const void *lengths, const void *row_start,
+                   void *error, int64_t rows, int64_t seqs, int64_t kv, int64_t d, int64_t page, int64_t pages,
+                   int64_t page_bytes, int64_t offset, int64_t width) {
+    if (rows < 0 || seqs < 0 || rows > I32 || seqs > I32 || kv <= 0 || kv > 65535)
+        return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows, %lld sequences, %lld kv heads", (long long)rows, (long long)seqs, (long long)kv);
+    if (d != 32 && d != 64 && d != 96 && d != 128)
+        return fail(NC_ERR_ARGUMENT, "head dimension %lld: the 4-bit cache serves 32, 64, 96 and 128", (long long)d);
+    if (page <= 0 || page % KV4_TILE || page > 1024) return fail(NC_ERR_ARGUMENT, "page size %lld: a multiple of 16 positions, 1024 at most", (long long)page);
+    if (pages < 0 || pages > I32 || width < 0 || width * page > I32)
+        return fail(NC_ERR_ARGUMENT, "bad cache extent: %lld pages, %lld of a sequence", (long long)pages, (long long)width);
+    const int64_t layer = kv * page * d * 5 / 4;
+    if (offset < 0 || offset % 16 || page_bytes % 16 || offset + layer > page_bytes || misaligned(base, 16))
+        return fail(NC_ERR_ARGUMENT, "a layer takes %lld bytes of a page at a 16-byte boundary; offset %lld in pages of %lld bytes",
+                    (long long)layer, (long long)offset, (long long)page_bytes);
+    if (!row_start && rows != seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of %lld sequences need row_start", (long long)rows, (long long)seqs);
+    if (rows && (!base || !table || !lengths)) return fail(NC_ERR_ARGUMENT, "null pool, table or lengths");
+    at->table = (const int32_t *)table;
+    at->lengths = (const int32_t *)lengths;
+    at->row_start = (const int32_t *)row_start;
+    at->error = (unsigned long long *)error;
+    at->rows = rows;
+    at->seqs = (int)seqs;
+    at->width = (int)width;
+    at->page = (int)page;
+    at->pages = (int)pages;
+    pool->base = (char *)base + offset;
+    pool->page_bytes = page_bytes;
+    pool->kv = (int)kv;
+    pool->d = (int)d;
+    return NC_OK;
+}
+
+float bits_to_f32(int64_t bits) {
+    const uint32_t u = (uint32_t)bits;
+    float f;
+    std::memcpy(&f, &u, 4);
+    return f;
+}
+
+// How a call's work is cut: 8 nt columns and `chunk` steps of positions to a CTA.
+struct AttnPlan {
+    int nt, col_blocks, splits, chunk;
+    int64_t groups;
+};
+constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: their finish counters lead the scratch
+constexpr int KV4_WARPS = 4, KV4_STAGES = 2;
+
+AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length) {
+    AttnPlan p;
+    const int64_t cols = heads / kv * max_rows;
+    p.nt = cols <= 8 ? 1 : cols <= 16 || d > 64 ? 2 : 4;
+    p.col_blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
+    p.groups = seqs * kv * p.col_blocks;
+    const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, steps = std::max<int64_t>(1, (max_length + step - 1) / step);
+    const int64_t target = 148 * 6;
+    int64_t splits = p.groups >= target || p.groups > KV4_COUNTERS || p.groups == 0 ? 1 : target / p.groups;
+    splits = std::max<int64_t>(1, std::min(splits, (steps + KV4_WARPS - 1) / KV4_WARPS));
+    int64_t chunk = (steps + splits - 1) / splits;
+    chunk = (chunk + KV4_WARPS - 1) / KV4_WARPS * KV4_WARPS;
+    p.chunk = (int)chunk;
+    p.splits = (int)((steps + chunk - 1) / chunk);
+    return p;
+}
+
+int64_t kv4_scratch(const AttnPlan &p, int64_t d) {
+    return p.splits == 1 ? 256 : 4 * KV4_COUNTERS + p.groups * p.splits * 8 * p.nt * (d + 2) * 4;
+}
+
+template <int D, int NT, bool HL>
+int32_t launch_kv4_attention_t(cudaStream_t st, const Kv4AttnArgs &a, int64_t ctas) {
+    using S = Kv4AttnShape<D, NT, HL, KV4_WARPS, KV4_STAGES>;
+    auto kernel = kv4_attention_kernel<D, NT, HL, KV4_WARPS, KV4_STAGES>;
+    static std::atomic<uint64_t> allowed{0};       // devices whose limit is raised
+    int device = 0;
+    CUDA_TRY(cudaGetDevice(&device));
+    if (!(allowed.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        CUDA_TRY(allow_smem(kernel, S::SMEM));
+        if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    }
+    CUDA_TRY(launch_k(kernel, (unsigned)ctas, 32 * KV4_WARPS, S::SMEM, st, a));
+    return check_launch("kv4_attention_kernel");
+}
+
+template <int D, bool HL>
+int32_t launch_kv4_attention_n(cudaStream_t st, const Kv4AttnArgs &a, int nt, int64_t ctas) {
+    switch (nt) {
+        case 1: return launch_kv4_attention_t<D, 1, HL>(st, a, ctas);
+        case 2: return launch_kv4_attention_t<D, 2, HL>(st, a, ctas);
+        default:
+            if constexpr (D <= 64) return launch_kv4_attention_t<D, 4, HL>(st, a, ctas);
+            return fail(NC_ERR_ARGUMENT, "no kernel of %d columns for head dimension %d", 8 * nt, D);
+    }
+}
+
+template <int D>
+int32_t launch_kv4_attention_d(cudaStream_t st, const Kv4AttnArgs &a, int nt, int64_t ctas) {
+    return a.type != KV_BF16 ? launch_kv4_attention_n<D, true>(st, a, nt, ctas) : launch_kv4_attention_n<D, false>(st, a, nt, ctas);
+}
+
+}  // namespace
+
+extern "C" int32_t nc_kv4_append(void **p, const int64_t *s, void *stream) {
+    Kv4AppendArgs a{};
+    NC_TRY(kv4_common(&a.at, &a.pool, p[0], p[3], p[4], p[5], p[8], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8]));
+    NC_TRY(check_type(s[11]));
+    if (a.at.rows == 0) return NC_OK;
+    a.keys = p[1];
+    a.values = p[2];
+    a.cos_tab = (const float *)p[6];
+    a.sin_tab = (const float *)p[7];
+    a.key_stride = s[9];
+    a.value_stride = s[10];
+    a.type = (int)s[11];
+    a.positions = s[12];
+    const int64_t line = (int64_t)a.pool.kv * a.pool.d;
+    if (!a.keys || !a.values || !a.cos_tab != !a.sin_tab) return fail(NC_ERR_ARGUMENT, "null keys or values, or half a rotation table");
+    if (a.key_stride < line || a.value_stride < line) return fail(NC_ERR_ARGUMENT, "rows of %lld values overlap", (long long)line);
+    const int64_t warps = a.at.rows * a.pool.kv * (a.pool.d / 32) * 2, ctas = (warps + 7) / 8;
+    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
+    CUDA_TRY(launch_k(kv4_append_kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, a));
+    return check_launch("kv4_append_kernel");
+}
+
+extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {
+    Kv4ReadArgs a{};
+    NC_TRY(kv4_common(&a.at, &a.pool, p[2], p[3], p[4], p[5], p[6], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8]));
+    if (a.at.rows == 0) return NC_OK;
+    a.keys = (float *)p[0];
+    a.values = (float *)p[1];
+    if (!a.keys || !a.values) return fail(NC_ERR_ARGUMENT, "null keys or values");
+    const int64_t warps = a.at.rows * a.pool.kv * 2, ctas = (warps + 7) / 8;
+    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
+    CUDA_TRY(launch_k(kv4_read_kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, a));
+    return check_launch("kv4_read_kernel");
+}
+
+extern "C" int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_rows,
+                                                  int64_t max_length) {
+    if (seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || d <= 0 || max_rows <= 0 || max_length < 0) return 256;
+    return kv4_scratch(kv4_plan(seqs, heads, kv_heads, d, max_rows, max_length), d);
+}
+
+extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
+    Kv4AttnArgs a{};
+    NC_TRY(kv4_common(&a.at, &a.pool, p[2], p[3], p[4], p[5], p[10], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8]));
+    NC_TRY(check_type(s[12]));
+    const int64_t heads = s[9], max_rows = s[15], max_length = s[16], scratch = s[17];
+    if (heads <= 0 || heads % a.pool.kv) return fail(NC_ERR_ARGUMENT, "%lld query heads do not share %d KV heads evenly", (long long)heads, a.pool.kv);
+    if (a.at.rows == 0 || a.at.seqs == 0) return NC_OK;
+    a.out = p[0];
+    a.q = p[1];
+    a.cos_tab = (const float *)p[6];
+    a.sin_tab = (const float *)p[7];
+    a.lse = (float *)p[8];
+    a.q_stride = s[10];
+    a.out_stride = s[11];
+    a.type = (int)s[12];
+    a.positions = s[13];
+    const float scale = bits_to_f32(s[14]);
+    if (!(scale > 0.0f) || scale > 1e30f) return fail(NC_ERR_ARGUMENT, "a score scale of %g: positive", scale);
+    a.scale_log2e = scale * 1.4426950408889634f;
+    const uint64_t tiles = (uint64_t)a.at.page / KV4_TILE;
+    a.page_magic = ((uint64_t(1) << 37) + tiles - 1) / tiles;
+    a.heads = (int)heads;
+    a.group = (int)(heads / a.pool.kv);
+    if (!a.out || !a.q || !a.cos_tab != !a.sin_tab) return fail(NC_ERR_ARGUMENT, "null output or queries, or half a rotation table");
+    if (a.q_stride < heads * a.pool.d || a.out_stride < heads * a.pool.d) return fail(NC_ERR_ARGUMENT, "rows of %lld values overlap", (long long)(heads * a.pool.d));
+    if (max_rows <= 0 || max_rows > a.at.rows || max_length < 0 || max_length > I32 || (!a.at.row_start && max_rows != 1))
+        return fail(NC_ERR_ARGUMENT, "at most %lld rows and %lld positions of a sequence", (long long)max_rows, (long long)max_length);
+    const AttnPlan plan = kv4_plan(a.at.seqs, heads, a.pool.kv, a.pool.d, max_rows, max_length);
+    a.col_blocks = plan.col_blocks;
+    a.splits = plan.splits;
+    a.chunk = plan.chunk;
+    if (plan.splits > 1) {
+        if (!p[9] || misaligned(p[9], 16) || scratch < kv4_scratch(plan, a.pool.d))
+            return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch, (long long)kv4_scratch(plan, a.pool.d));
+        a.counter = (unsigned int *)p[9];
+        a.part = (float *)((char *)p[9] + 4 * KV4_COUNTERS);
+    }
+    const int64_t ctas = plan.groups * plan.splits;
+    if (ctas > I32 || a.at.rows * a.group > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (a.pool.d) {
+        case 32: return launch_kv4_attention_d<32>(st, a, plan.nt, ctas);
+        case 64: return launch_kv4_attention_d<64>(st, a, plan.nt, ctas);
+        case 96: return launch_kv4_attention_d<96>(st, a, plan.nt, ctas);
+        default: return launch_kv4_attention_d<128>(st, a, plan.nt, ctas);
+    }
+}
+
+// ---- pages --------------------------------------------------------------------------------------
+
+namespace {
+
+// refs, tails, owner and fresh by page; first, need, offset by sequence; the copy list; its length.
+int64_t kvp_list(int64_t seqs, int64_t pages) { return 2 * std::max(seqs, pages); }
+
+int32_t kvp_args(KvPagesArgs *a, void **p, const int64_t *s, int table, int status, int scratch) {
+    const int64_t seqs = s[0], width = s[1], pages = s[2], page = s[3], page_bytes = s[4];
+    if (seqs < 0 || width < 0 || pages < 0 || page <= 0 || seqs > I32 || pages > I32 / 2 || width * page > I32 || seqs * width > I32)
+        return fail(NC_ERR_ARGUMENT, "bad cache extent: %lld sequences of %lld pages of %lld positions, %lld pages", (long long)seqs,
+                    (long long)width, (long long)page, (long long)pages);
+    if (page_bytes <= 0 || page_bytes % 16 || misaligned(p[5], 16)) return fail(NC_ERR_ARGUMENT, "pages of %lld bytes: a multiple of 16 at a 16-byte boundary", (long long)page_bytes);
+    if (seqs && (!p[0] || !p[table] || !p[table + 1] || !p[5] || !p[status] || !p[scratch] || misaligned(p[scratch], 16)))
+        return fail(NC_ERR_ARGUMENT, "null table, lengths, pool, status or scratch");
+    if (p[0] == p[table] && seqs) return fail(NC_ERR_ARGUMENT, "the new table is the old one");
+    if (s[5] < nc_kv_pages_scratch_bytes(seqs, width, pages))
+        return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)s[5], (long long)nc_kv_pages_scratch_bytes(seqs, width, pages));
+    a->new_table = (int32_t *)p[0];
+    a->table = (const int32_t *)p[table];
+    a->lengths = (const int32_t *)p[table + 1];
+    a->status = (int64_t *)p[status];
+    int32_t *w = (int32_t *)p[scratch];
+    a->copies = w;
+    w += 4;
+    for (int32_t **x : {&a->refs, &a->tails, &a->owner, &a->fresh}) *x = w, w += pages;
+    for (int32_t **x : {&a->first, &a->need, &a->offset}) *x = w, w += seqs;
+    a->list = w;
+    a->seqs = (int)seqs;
+    a->width = (int)width;
+    a->pages = (int)pages;
+    a->page = (int)page;
+    return NC_OK;
+}
+
+int32_t kvp_copy(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page_bytes) {
+    CUDA_TRY(launch_k(kv_pages_copy_kernel, KVP_COPY_CTAS, KVP_COPY_THREADS, 0, st, (char *)pool, page_bytes, a.list, a.copies));
+    return check_launch("kv_pages_copy_kernel");
+}
+
+}  // namespace
+
+extern "C" int64_t nc_kv_pages_scratch_bytes(int64_t seqs, int64_t width, int64_t pages) {
+    (void)width;
+    if (seqs < 0 || pages < 0) return 16;
+    return 16 + 4 * (4 * pages + 3 * seqs + kvp_list(seqs, pages));
+}
+
+// p: [0] new table [1] new lengths [2] table [3] lengths [4] status [5] pool [6] scratch [7] parent [8] grow
+extern "C" int32_t nc_kv_pages_update(void **p, const int64_t *s, void *stream) {
+    KvPagesArgs a{};
+    NC_TRY(kvp_args(&a, p, s, 2, 4, 6));
+    if (a.seqs == 0) return NC_OK;
+    if (!p[1] || p[1] == p[3]) return fail(NC_ERR_ARGUMENT, "the new lengths are null or the old ones");
+    a.new_lengths = (int32_t *)p[1];
+    a.parent = (const int32_t *)p[7];
+    a.grow = (const int32_t *)p[8];
+    CUDA_TRY(launch_k(kv_pages_update_kernel, 1, KVP_THREADS, 0, (cudaStream_t)stream, a));
+    NC_TRY(check_launch("kv_pages_update_kernel"));
+    return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
+}
+
+extern "C" int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream) {
+    KvPagesArgs a{};
+    NC_TRY(kvp_args(&a, p, s, 2, 4, 6));
+    if (a.seqs == 0) return NC_OK;
+    CUDA_TRY(launch_k(kv_pages_compact_kernel, 1, KVP_THREADS, 0, (cudaStream_t)stream, a));
+    NC_TRY(check_launch("kv_pages_compact_kernel"));
+    return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
+}
+
+// ---- token log probabilities ----------------------------------------------------------------------
+
+namespace {
+
+struct LogprobPlan {
+    int ept, segs;
+};
+
+// The longest segments that still give every SM two CTAs; longer ones have fewer parts to join.
+LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int64_t type) {
+    const int epts[2][3] = {{64, 16, 4}, {64, 16, 8}};
+    const int skew = type == KV_F32 ? 3 : 7;
+    LogprobPlan p{};
+    for (int ept : epts[type == KV_F32 ? 0 : 1]) {
+        const int64_t segs = (vocab + skew + LP_THREADS * ept - 1) / (LP_THREADS * ept);
+        if (segs > LP_SEGS) break;
+        p = {ept, (int)segs};
+        if (rows * segs >= 2 * 148) break;
+    }
+    return p;
+}
+
+template <int TYPE, int EPT>
+int32_t launch_logprobs(cudaStream_t st, const LogprobArgs &a, int64_t rows) {
+    CUDA_TRY(launch_k(logprobs_kernel<TYPE, EPT>, (unsigned)(rows * a.segs), LP_THREADS, 0, st, a));
+    return check_launch("logprobs_kernel");
+}
+
+}  // namespace
+
+extern "C" int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k) {
+    if (rows <= 0 || vocab <= 0 || k < 0) return 4 * LP_ROWS;
+    int64_t most = 0;
+    for (int type : {KV_F32, KV_F16}) most = std::max<int64_t>(most, logprob_plan(std::min<int64_t>(rows, LP_ROWS), vocab, type).segs);
+    return 4 * LP_ROWS + std::min<int64_t>(rows, LP_ROWS) * most * (16 + 8 * k);
+}
+
+extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {
+    const int64_t rows = s[0], vocab = s[1], type = s[3], ntargets = s[4], k = s[5], scratch = s[6];
+    LogprobArgs a{};
+    NC_TRY(check_type(type));
+    if (rows < 0 || vocab <= 0 || vocab >= (int64_t(1) << 32) - 1 || ntargets < 0 || ntargets > I32)
+        return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows of %lld logits, %lld targets", (long long)rows, (long long)vocab, (long long)ntargets);
+    if (k < 0 || k > LP_MAX_TOP || k > vocab)
+        return fail(NC_ERR_ARGUMENT, "%lld alternatives: at most %d, and no more than the vocabulary's %lld", (long long)k, LP_MAX_TOP, (long long)vocab);
+    if (s[2] < vocab) return fail(NC_ERR_ARGUMENT, "rows of %lld logits overlap at a stride of %lld", (long long)vocab, (long long)s[2]);
+    if (rows == 0) return NC_OK;
+    const LogprobPlan plan = logprob_plan(std::min<int64_t>(rows, LP_ROWS), vocab, type);
+    if (plan.segs == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is beyond %d segments", (long long)vocab, LP_SEGS);
+    if (!p[5] || (ntargets && (!p[0] || !p[6])) || (k && (!p[3] || !p[4])) || misaligned(p[5], type == KV_F32 ? 4 : 2))
+        return fail(NC_ERR_ARGUMENT, "null or misaligned logits, targets or outputs");
+    if (plan.segs > 1 && (!p[7] || misaligned(p[7], 16) || scratch < nc_token_logprobs_scratch_bytes(rows, vocab, k)))
+        return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch,
+                    (long long)nc_token_logprobs_scratch_bytes(rows, vocab, k));
+    a.out = (float *)p[0];
+    a.entropy = (float *)p[1];
+    a.lse = (float *)p[2];
+    a.top = (int64_t *)p[3];
+    a.top_logprobs = (float *)p[4];
+    a.logits = (const char *)p[5];
+    a.targets = (const int64_t *)p[6];
+    a.error = (unsigned long long *)p[8];
+    a.stride = s[2];
+    a.vocab = vocab;
+    a.ntargets = (int)ntargets;
+    a.k = (int)k;
+    a.segs = plan.segs;
+    if (plan.segs > 1) {
+        a.counter = (unsigned int *)p[7];
+        a.part = (float4 *)((char *)p[7] + 4 * LP_ROWS);
+        a.part_top = (unsigned long long *)(a.part + std::min<int64_t>(rows, LP_ROWS) * plan.segs);
+    }
+    const cudaStream_t st = (cudaStream_t)stream;
+    for (int64_t first = 0; first < rows; first += LP_ROWS) {
+        const int64_t n = std::min<int64_t>(rows - first, LP_ROWS);
+        a.row_first = first;
+        int32_t status;
+        if (type == KV_F32)
+            status = plan.ept == 64 ? launch_logprobs<KV_F32, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_F32, 16>(st, a, n)
+                                                                                            : launch_logprobs<KV_F32, 4>(st, a, n);
+        else if (type == KV_F16)
+            status = plan.ept == 64 ? launch_logprobs<KV_F16, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_F16, 16>(st, a, n)
+                                                                                            : launch_logprobs<KV_F16, 8>(st, a, n);
+        else
+            status = plan.ept == 64 ? launch_logprobs<KV_BF16, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_BF16, 16>(st, a, n)
+                                                                                             : launch_logprobs<KV_BF16, 8>(st, a, n);
+        NC_TRY(status);
+    }
+    return NC_OK;
+}

@@ -67,7 +67,9 @@ _P64, _P32, _PF = ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int32)
 GROUP_ENTRY_POINTS = ("nc_gather_rows", "nc_rms_norm_quantize", "nc_quantize_blocks", "nc_matmul_i8_vnni",
                       "nc_matmul_i8_tc", "nc_matmul_i8_f32", "nc_matmul_f32", "nc_lm_head_argmax",
                       "nc_lm_head_argmax_noalloc", "nc_attention", "nc_attention_cache", "nc_expf_exact",
-                      "nc_lm_head_q8_prepare", "nc_lm_head_q8_argmax", "nc_quantize_int8_rows")
+                      "nc_lm_head_q8_prepare", "nc_lm_head_q8_argmax", "nc_quantize_int8_rows",
+                      "nc_kv4_append", "nc_kv4_read", "nc_kv4_attention", "nc_kv_pages_update", "nc_kv_pages_compact",
+                      "nc_token_logprobs")
 
 
 def library() -> ctypes.CDLL:
@@ -91,6 +93,9 @@ def library() -> ctypes.CDLL:
             "nc_selfcheck_div127": ([_P64], _i32),
             "nc_lm_head_scratch_bytes": ([_i64, _i64], _i64),
             "nc_lm_head_q8_scratch_bytes": ([_i64, _i64], _i64),
+            "nc_kv4_attention_scratch_bytes": ([_i64] * 6, _i64),
+            "nc_kv_pages_scratch_bytes": ([_i64] * 3, _i64),
+            "nc_token_logprobs_scratch_bytes": ([_i64] * 3, _i64),
             "nc_device_count": ([_P32], _i32),
             "nc_set_device": ([_i32], _i32),
             "nc_device_alloc": ([_i64, ctypes.POINTER(_vp)], _i32),
