@@ -6,10 +6,13 @@
 // LM head's argmax).  A logit of -inf adds nothing; a row of nothing else has log probabilities of
 // -inf and entropy 0.
 //
-// One pass over the logits, which bound it: a CTA takes a segment of a row into registers with one
-// burst of 16-byte loads, so its maximum is known before the first exponential and nothing is read
-// twice.  The segment's best k: the k-th largest of 32 maxima (each of eight threads' values) is a
-// lower bound that at least k values reach; the few that do are ranked by comparing each with all.
+// One pass over the logits, which bound it.  A CTA streams a segment of a row in batches of four 16-byte vectors to
+// a thread, the next batch's loads in flight while one is worked on.  Each thread keeps its own maximum and sums,
+// rescaled only by a batch with a larger value, and leaves the maximum of each batch (a block of 16 or 32
+// logits) in shared memory: no barrier and nothing of the top is in the loop.  The top k lie in the blocks whose maxima
+// reach the k-th largest one, T.  T comes from ranking the blocks that reach the k-th largest of 32 threads' groups'
+// maxima (about as many as k); those k blocks are read again and their values from T up ranked.  Where more
+// blocks end in T than can be read again, equals are as good as their index: the first k in the row's order are taken.
 // The last CTA of a row joins the segments, in their order.
 #pragma once
 
@@ -18,8 +21,11 @@
 namespace nc {
 
 constexpr int LP_THREADS = 256;
+constexpr int LP_CTAS = 4;             // resident on an SM
+constexpr int LP_VECS = 4;             // vectors of a batch, for each thread
+constexpr int LP_BATCHES = 32;         // of a segment at most: their maxima are kept
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_CAND = LP_MAX_TOP * LP_MAX_TOP;   // candidates ranked at once; more (masses of equal values) take rounds
+constexpr int LP_CAND = 1024;          // room for candidates: the values of LP_CAND / 8 N blocks
 constexpr int LP_ROWS = 4096;          // rows of a launch at most: their finish counters
 constexpr int LP_SEGS = LP_THREADS;    // segments of a row at most
 
@@ -34,13 +40,17 @@ struct LogprobArgs {
     unsigned long long *part_top;      // [rows][segs][k]
     unsigned long long *error;         // null, or the smallest row with a target outside the vocabulary
     int64_t stride, vocab, row_first;
+    int64_t seg_vecs;                  // vectors of a segment
     int ntargets, k, segs;
 };
 
 // Orders (value, index): larger values first, then lower indices.  -0 counts as +0, every NaN as the largest.
+__device__ __forceinline__ uint32_t lp_order(float x) { return x != x ? 0xffffffffu : ordered_bits(x == 0.0f ? 0.0f : x); }
+__device__ __forceinline__ float lp_value(uint32_t order) {
+    return order == 0xffffffffu ? __uint_as_float(0x7fc00000u) : from_ordered_bits(order);
+}
 __device__ __forceinline__ unsigned long long lp_key(float x, uint32_t index) {
-    uint32_t u = x != x ? 0xffffffffu : ordered_bits(x == 0.0f ? 0.0f : x);
-    return (unsigned long long)u << 32 | (0xffffffffu - index);
+    return (unsigned long long)lp_order(x) << 32 | (0xffffffffu - index);
 }
 
 template <int TYPE>
@@ -71,14 +81,59 @@ __device__ __forceinline__ void lp_unpack(const uint4 &w, float *x) {
     }
 }
 
-__device__ __forceinline__ float lp_block_max(float v, float *buf) {
+// The larger of two, a NaN if either is one.
+__device__ __forceinline__ float lp_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The vector whose first element is element e of a row of n, -inf outside the row; for the row's ends only.
+template <int TYPE>
+__device__ __noinline__ uint4 lp_partial(const char *row, int64_t e, int64_t n) {
+    constexpr int N = LpVec<TYPE>::N;
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int j = 0; j < N; ++j) {
+        const bool in = e + j >= 0 && e + j < n;
+        if constexpr (TYPE == KV_F32) {
+            w[j] = in ? ((const uint32_t *)row)[e + j] : 0xff800000u;
+        } else {
+            const uint32_t v = in ? ((const uint16_t *)row)[e + j] : TYPE == KV_F16 ? 0xfc00u : 0xff80u;
+            w[j >> 1] |= v << (16 * (j & 1));
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A maximum with the sums relative to it.
+struct LpSums {
+    float m, s, e;
+};
+__device__ __forceinline__ float lp_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr float LP_LEAST = -1000.0f;   // exp is 0 below: keeps 0 * -inf out of the entropy
+__device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
+    const float m = lp_max(a.m, b.m), to = m == -INFINITY ? 0.0f : m;
+    const float da = lp_max(a.m - to, LP_LEAST), db = lp_max(b.m - to, LP_LEAST);
+    const float wa = lp_exp2(da * LP_LOG2E), wb = lp_exp2(db * LP_LOG2E);
+    LpSums r;
+    r.m = m;
+    r.s = __fmaf_rn(a.s, wa, b.s * wb);
+    r.e = __fmaf_rn(wa, __fmaf_rn(a.s, da, a.e), wb * __fmaf_rn(b.s, db, b.e));
+    return r;
+}
+__device__ __forceinline__ LpSums lp_warp_join(LpSums v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = nan_max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = buf[0];
-#pragma unroll
-    for (int w = 1; w < LP_THREADS / 32; ++w) v = nan_max(v, buf[w]);
+    for (int o = 16; o > 0; o >>= 1) {
+        LpSums w;
+        w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+        w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+        w.e = __shfl_xor_sync(0xffffffffu, v.e, o);
+        v = lp_join(v, w);
+    }
     return v;
 }
 
@@ -93,142 +148,212 @@ __device__ __forceinline__ void lp_rank(const unsigned long long *keys, int n, i
 }
 
 struct LpShared {
-    float warp_max[LP_THREADS / 32], group_max[32];
-    float2 sums[LP_THREADS / 32];
+    uint32_t block[LP_BATCHES][LP_THREADS];                        // maxima, in order
+    uint32_t group_max[32];
+    LpSums sums[LP_THREADS / 32];
     unsigned long long cand[LP_CAND], best[LP_MAX_TOP], round[LP_THREADS / 32], heads[LP_SEGS];
-    float4 parts[LP_SEGS];
-    int count;
-    float bound;
+    int count, greater, equal;
+    uint32_t kth;
     unsigned int arrived;
 };
 
-// EPT elements per thread: a segment is EPT * 256 elements.
-template <int TYPE, int EPT>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int N = LpVec<TYPE>::N, VECS = EPT / N, SIZE = TYPE == KV_F32 ? 4 : 2;
+__device__ __forceinline__ unsigned long long lp_warp_max(unsigned long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, o);
+        v = other > v ? other : v;
+    }
+    return v;
+}
+// The largest of the block's keys, in every thread.  The caller's next write to `round` comes after a barrier.
+__device__ __forceinline__ unsigned long long lp_block_max(unsigned long long v, unsigned long long *round) {
+    v = lp_warp_max(v);
+    if ((threadIdx.x & 31) == 0) round[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = round[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 32; ++w) v = round[w] > v ? round[w] : v;
+    return v;
+}
+
+// The k best keys of a segment, in order, to sh.best (0 past its end); `mine`: the largest of the thread's blocks.
+template <int TYPE>
+__device__ __forceinline__ void lp_segment_top(const LogprobArgs &a, LpShared &sh, const char *base, int skew, int64_t seg0,
+                                               int64_t v_end, int batches, uint32_t mine) {
+    constexpr int N = LpVec<TYPE>::N, SIZE = LP_VECS * N, MOST = LP_CAND / SIZE;      // values of a block; blocks to read again
+    constexpr int64_t BATCH = LP_THREADS * LP_VECS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t quarter = mine;                                       // of eight threads
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) quarter = max(quarter, __shfl_xor_sync(0xffffffffu, quarter, o));
+    if ((lane & 7) == 0) sh.group_max[tid >> 3] = quarter;
+    if (tid == 0) sh.count = sh.greater = sh.equal = 0;
+    if (tid < a.k) sh.best[tid] = 0;
+    __syncthreads();
+    const uint32_t group = sh.group_max[lane];
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        const uint32_t other = sh.group_max[j];
+        rank += other > group || (other == group && j < lane);
+    }
+    const uint32_t bound = __shfl_sync(0xffffffffu, group, __ffs(__ballot_sync(0xffffffffu, rank == a.k - 1)) - 1);
+    if (mine >= bound)
+        for (int i = 0; i < batches; ++i)
+            if (sh.block[i][tid] >= bound) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < LP_CAND) sh.cand[at] = (unsigned long long)sh.block[i][tid] << 32 | (uint32_t)(i * LP_THREADS + tid);
+            }
+    __syncthreads();
+    uint32_t kth = 0;                                              // T, in order
+    if (sh.count <= LP_CAND) {
+        for (int i = tid; i < sh.count; i += LP_THREADS) {
+            const unsigned long long key = sh.cand[i];
+            int above = 0;
+            for (int j = 0; j < sh.count; ++j) above += sh.cand[j] > key;
+            if (above == a.k - 1) sh.kth = (uint32_t)(key >> 32);
+        }
+        __syncthreads();
+        kth = sh.kth;
+    } else {                                                       // bit by bit: the largest T that k blocks reach
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t trial = kth | 1u << bit;
+            int n = 0;
+            for (int i = 0; i < batches; ++i) n += sh.block[i][tid] >= trial;
+            n = warp_sum_int(n);
+            if (lane == 0) sh.round[warp] = n;
+            __syncthreads();
+            n = 0;
+            for (int w = 0; w < LP_THREADS / 32; ++w) n += (int)sh.round[w];
+            if (n >= a.k) kth = trial;
+            __syncthreads();
+        }
+    }
+    // The blocks above T, then those that end in it.
+    int *const list = (int *)sh.heads;                             // MOST block numbers at most, before the heads are used
+    if (mine >= kth)
+        for (int i = 0; i < batches; ++i)
+            if (sh.block[i][tid] >= kth) {
+                if (sh.block[i][tid] > kth) list[atomicAdd(&sh.greater, 1)] = i * LP_THREADS + tid;     // fewer than k
+                else atomicAdd(&sh.equal, 1);
+            }
+    __syncthreads();
+    const int greater = sh.greater;
+    const bool all = greater + sh.equal <= MOST;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (all && mine >= kth)
+        for (int i = 0; i < batches; ++i)
+            if (sh.block[i][tid] == kth) list[atomicAdd(&sh.greater, 1)] = i * LP_THREADS + tid;
+    __syncthreads();
+    const int blocks = sh.greater;
+    for (int at = warp; at < blocks; at += LP_THREADS / 32)
+#pragma unroll
+        for (int u = lane; u < SIZE; u += 32) {
+            const int64_t v = seg0 + list[at] / LP_THREADS * BATCH + list[at] % LP_THREADS + u / N * LP_THREADS;
+            const int64_t e = v * N - skew + u % N;
+            if (v >= v_end || e < 0 || e >= a.vocab) continue;
+            const unsigned long long key = lp_key(kv_load(base, e, TYPE), (uint32_t)e);
+            const uint32_t order = (uint32_t)(key >> 32);
+            if (all ? order >= kth : order > kth) sh.cand[atomicAdd(&sh.count, 1)] = key;
+        }
+    __syncthreads();
+    if (!all) {                                                    // the first k equals, in the row's order
+        int found = 0;
+        for (int64_t e0 = max((int64_t)0, seg0 * N - skew); found < a.k && e0 < min(a.vocab, v_end * N - skew); e0 += LP_THREADS) {
+            const int64_t e = e0 + tid;
+            const unsigned long long key = e < min(a.vocab, v_end * N - skew) ? lp_key(kv_load(base, e, TYPE), (uint32_t)e) : 0;
+            const bool is = key != 0 && (uint32_t)(key >> 32) == kth;
+            if (is) sh.cand[atomicAdd(&sh.count, 1)] = key;
+            found += __syncthreads_count(is);
+        }
+        __syncthreads();
+    }
+    lp_rank(sh.cand, sh.count, a.k, sh.best);
+    __syncthreads();
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int N = LpVec<TYPE>::N, SIZE = TYPE == KV_F32 ? 4 : 2;
+    constexpr int64_t BATCH = LP_THREADS * LP_VECS;                // vectors
     __shared__ LpShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    release_dependents();
+    wait_for_producer();
     const int seg = (int)(blockIdx.x % a.segs);
     const int64_t local = blockIdx.x / a.segs, row = a.row_first + local;
-    wait_for_producer();
     const char *const base = a.logits + row * a.stride * SIZE;
     // Vectors lie on 16-byte boundaries: element e of the row is element e + skew of the vectors.
     const int skew = (int)(((uintptr_t)base & 15) / SIZE);
     const char *const aligned = base - skew * SIZE;
-    const int64_t v0 = (int64_t)seg * (LP_THREADS * VECS) + tid;
-    float x[EPT];
-    uint4 raw[VECS];
+    const int64_t v_end = min((int64_t)(seg + 1) * a.seg_vecs, (a.vocab + skew + N - 1) / N);
+
+    const int64_t v_low = skew ? 1 : 0, v_high = min(v_end, (a.vocab + skew) / N);       // whole vectors
+    auto fetch = [&](int64_t first, uint4 (&raw)[LP_VECS]) {
+        const char *const from = aligned + (first + tid) * 16;
+        if (first >= v_low && first + BATCH <= v_high) {
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-        const int64_t e = (v0 + i * LP_THREADS) * N - skew;        // the vector's first element
-        if (e >= 0 && e + N <= a.vocab) raw[i] = __ldcs((const uint4 *)(aligned + (v0 + i * LP_THREADS) * 16));
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-        const int64_t e = (v0 + i * LP_THREADS) * N - skew;
-        if (e >= 0 && e + N <= a.vocab) {
-            lp_unpack<TYPE>(raw[i], x + i * N);
+            for (int i = 0; i < LP_VECS; ++i) raw[i] = __ldcs((const uint4 *)(from + i * LP_THREADS * 16));
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                x[i * N + j] = e + j >= 0 && e + j < a.vocab ? kv_load(base, e + j, TYPE) : -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) top = nan_max(top, x[i * N + j]);
-    }
-    // 32 maxima, each of the eight threads of one quarter warp, for the top's bound.
-    float quarter = top;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) quarter = nan_max(quarter, __shfl_xor_sync(0xffffffffu, quarter, o));
-    if ((lane & 7) == 0) sh.group_max[tid >> 3] = quarter;
-    if (tid == 0) sh.count = 0;
-    const float M = lp_block_max(quarter, sh.warp_max);
-
-    const float L2E = 1.4426950408889634f;
-    const float base_m = M == -INFINITY ? 0.0f : M;
-    float s = 0.0f, es = 0.0f;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const float d = x[i] - base_m;
-        float p;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(d * L2E));
-        s += p;
-        es = __fmaf_rn(p, fmaxf(d, -1000.0f), es);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        es += __shfl_xor_sync(0xffffffffu, es, o);
-    }
-    if (lane == 0) sh.sums[warp] = make_float2(s, es);
-
-    if (a.k) {
-        if (warp == 0) {
-            const unsigned long long mine = lp_key(sh.group_max[lane], lane);
-            int rank = 0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) rank += lp_key(sh.group_max[j], j) > mine;
-            if (rank == a.k - 1) sh.bound = sh.group_max[lane];
-        }
-        __syncthreads();
-        const float bound = sh.bound;
-        // Values at or above the bound (a NaN always is); padding is told from a logit of -inf by its index.
-        if (!(top < bound)) {
-#pragma unroll
-            for (int i = 0; i < EPT; ++i) {
-                if (!(x[i] < bound) || bound != bound) {
-                    const int64_t e = (v0 + i / N * LP_THREADS) * N - skew + i % N;
-                    if (e >= 0 && e < a.vocab && (bound == bound || x[i] != x[i])) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < LP_CAND) sh.cand[at] = lp_key(x[i], (uint32_t)e);
-                    }
-                }
+            for (int i = 0; i < LP_VECS; ++i) {
+                constexpr uint32_t none = TYPE == KV_F32 ? 0xff800000u : TYPE == KV_F16 ? 0xfc00fc00u : 0xff80ff80u;
+                const int64_t v = first + tid + i * LP_THREADS;
+                raw[i] = make_uint4(none, none, none, none);
+                if (v >= v_low && v < v_high) raw[i] = __ldcs((const uint4 *)(from + i * LP_THREADS * 16));
+                else if (v < v_end) raw[i] = lp_partial<TYPE>(base, v * N - skew, a.vocab);
             }
         }
-        if (tid < a.k) sh.best[tid] = 0;
-        __syncthreads();
-        if (sh.count <= LP_CAND) {
-            lp_rank(sh.cand, sh.count, a.k, sh.best);
-        } else {                                                   // more equals than that: the best, k times over
-            unsigned long long last = ~0ull;
-            for (int r = 0; r < a.k; ++r) {
-                unsigned long long mine = 0;
+    };
+
+    LpSums sum{-INFINITY, 0.0f, 0.0f};
+    const int64_t seg0 = (int64_t)seg * a.seg_vecs;
+    uint4 raw[LP_VECS], ahead[LP_VECS];
+    fetch(seg0, raw);
+    int batches = 0;
+    for (int64_t first = seg0; first < v_end; first += BATCH, ++batches) {
+        fetch(first + BATCH, ahead);
+        float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) {
-                    const int64_t e = (v0 + i / N * LP_THREADS) * N - skew + i % N;
-                    if (e >= 0 && e < a.vocab) {
-                        const unsigned long long key = lp_key(x[i], (uint32_t)e);
-                        if (key < last && key > mine) mine = key;
-                    }
-                }
+        for (int i = 0; i < LP_VECS; ++i) {
+            float x[N];
+            lp_unpack<TYPE>(raw[i], x);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
-                    mine = other > mine ? other : mine;
-                }
-                if (lane == 0) sh.round[warp] = mine;
-                __syncthreads();
-                mine = sh.round[0];
+            for (int j = 0; j < N; ++j) top = lp_max(top, x[j]);
+        }
+        if (a.k) sh.block[batches][tid] = lp_order(top);
+        if (!(top <= sum.m)) {                                     // a larger value, or a NaN
+            const float d = lp_max(sum.m - top, LP_LEAST), w = lp_exp2(d * LP_LOG2E);
+            sum.e = w * __fmaf_rn(sum.s, d, sum.e);
+            sum.s *= w;
+            sum.m = top;
+        }
+        const float to = sum.m == -INFINITY ? 0.0f : sum.m;
 #pragma unroll
-                for (int w = 1; w < LP_THREADS / 32; ++w) mine = sh.round[w] > mine ? sh.round[w] : mine;
-                if (tid == 0) sh.best[r] = mine;
-                last = mine;
-                __syncthreads();
+        for (int i = 0; i < LP_VECS; ++i) {
+            float x[N];
+            lp_unpack<TYPE>(raw[i], x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float d = lp_max(x[j] - to, LP_LEAST), p = lp_exp2(d * LP_LOG2E);
+                sum.s += p;
+                sum.e = __fmaf_rn(p, d, sum.e);
             }
         }
+#pragma unroll
+        for (int i = 0; i < LP_VECS; ++i) raw[i] = ahead[i];
     }
+    if (a.k) lp_segment_top<TYPE>(a, sh, base, skew, seg0, v_end, batches, lp_order(sum.m));
+    sum = lp_warp_join(sum);
+    if (lane == 0) sh.sums[warp] = sum;
     __syncthreads();
-    s = es = 0.0f;
+    sum = sh.sums[0];
 #pragma unroll
-    for (int w = 0; w < LP_THREADS / 32; ++w) {
-        s += sh.sums[w].x;
-        es += sh.sums[w].y;
-    }
+    for (int w = 1; w < LP_THREADS / 32; ++w) sum = lp_join(sum, sh.sums[w]);
 
-    float row_m = M, row_s = s, row_e = es;
     if (a.segs > 1) {
-        if (tid == 0) a.part[local * a.segs + seg] = make_float4(M, s, es, 0.0f);
+        if (tid == 0) a.part[local * a.segs + seg] = make_float4(sum.m, sum.s, sum.e, 0.0f);
         if (tid < a.k) a.part_top[(local * a.segs + seg) * a.k + tid] = sh.best[tid];
         __threadfence();
         __syncthreads();
@@ -236,47 +361,37 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
         __syncthreads();
         if (sh.arrived != (unsigned)a.segs - 1) return;
         __threadfence();
-        if (tid == 0) a.counter[local] = 0;
-        for (int i = tid; i < a.segs; i += LP_THREADS) sh.parts[i] = __ldcg(a.part + local * a.segs + i);
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        row_m = -INFINITY;
-        for (int i = 0; i < a.segs; ++i) row_m = nan_max(row_m, sh.parts[i].x);
-        const float to = row_m == -INFINITY ? 0.0f : row_m;
-        row_s = row_e = 0.0f;
-        for (int i = 0; i < a.segs; ++i) {
-            const float4 p = sh.parts[i];
-            if (p.x == -INFINITY) continue;
-            float w;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((p.x - to) * L2E));
-            row_s = __fmaf_rn(p.y, w, row_s);
-            row_e = __fmaf_rn(w, __fmaf_rn(p.y, fmaxf(p.x - to, -1000.0f), p.z), row_e);
+        if (tid == 0) {
+            a.counter[local] = 0;
+            sh.count = 0;
         }
+        sum = LpSums{-INFINITY, 0.0f, 0.0f};
+        if (tid < a.segs) {
+            const float4 p = __ldcg(a.part + local * a.segs + tid);
+            sum = LpSums{p.x, p.y, p.z};
+        }
+        const unsigned long long *const tops = a.part_top + local * a.segs * a.k;
+        unsigned long long head = 0, floor_key = 0;
+        if (a.k && tid < a.segs) {
+            head = __ldcg(tops + tid * a.k);
+            floor_key = __ldcg(tops + tid * a.k + a.k - 1);
+            sh.heads[tid] = head;
+        }
+        sum = lp_warp_join(sum);
+        if (lane == 0) sh.sums[warp] = sum;
+        __syncthreads();
+        sum = sh.sums[0];
+#pragma unroll
+        for (int w = 1; w < LP_THREADS / 32; ++w) sum = lp_join(sum, sh.sums[w]);
         if (a.k) {
             // A key below the k-th largest of the segments' best, or below a segment's own k-th best, has
             // k better ones: at most k * k keys are left to rank.
-            const unsigned long long *const tops = a.part_top + local * a.segs * a.k;
-            unsigned long long floor_key = 0, best = 0;
-            if (tid < a.segs) {
-                best = __ldcg(tops + tid * a.k);
-                floor_key = __ldcg(tops + tid * a.k + a.k - 1);
-                sh.heads[tid] = best;
-            }
-            __syncthreads();
             if (tid < a.segs) {
                 int rank = 0;
-                for (int i = 0; i < a.segs; ++i) rank += sh.heads[i] > best;
-                if (rank == a.k - 1 && best > floor_key) floor_key = best;
+                for (int i = 0; i < a.segs; ++i) rank += sh.heads[i] > head;
+                if (rank == a.k - 1 && head > floor_key) floor_key = head;
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, floor_key, o);
-                floor_key = other > floor_key ? other : floor_key;
-            }
-            if (lane == 0) sh.round[warp] = floor_key;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < LP_THREADS / 32; ++w) floor_key = sh.round[w] > floor_key ? sh.round[w] : floor_key;
+            floor_key = lp_block_max(floor_key, sh.round);
             for (int i = tid; i < a.segs * a.k; i += LP_THREADS) {
                 const unsigned long long key = __ldcg(tops + i);
                 if (key != 0 && key >= floor_key) sh.cand[atomicAdd(&sh.count, 1)] = key;
@@ -288,12 +403,12 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     }
 
     // The row's results.
-    const float log_s = logf(row_s);
-    const bool none = row_m == -INFINITY;
-    const float shift = none ? 0.0f : row_m;
+    const float log_s = logf(sum.s);
+    const bool none = sum.m == -INFINITY;
+    const float shift = none ? 0.0f : sum.m;
     if (tid == 0) {
-        if (a.entropy) a.entropy[row] = none ? 0.0f : log_s - row_e / row_s;
-        if (a.lse) a.lse[row] = none ? -INFINITY : row_m + log_s;
+        if (a.entropy) a.entropy[row] = none ? 0.0f : log_s - fdiv(sum.e, sum.s);
+        if (a.lse) a.lse[row] = none ? -INFINITY : sum.m + log_s;
     }
     for (int j = tid; j < a.ntargets; j += LP_THREADS) {
         const int64_t t = a.targets[row * a.ntargets + j];

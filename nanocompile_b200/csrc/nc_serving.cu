@@ -293,26 +293,31 @@ extern "C" int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream)
 namespace {
 
 struct LogprobPlan {
-    int ept, segs;
+    int segs;
+    int64_t seg_vecs;
 };
 
-// The longest segments that still give every SM two CTAs; longer ones have fewer parts to join.
+// Segments to a row: the fewest elements' time over the waves of CTAs that the card holds at once, a segment's
+// start and end counted as 4096 elements and its share of the join as 16.
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int64_t type) {
-    const int epts[2][3] = {{64, 16, 4}, {64, 16, 8}};
-    const int skew = type == KV_F32 ? 3 : 7;
-    LogprobPlan p{};
-    for (int ept : epts[type == KV_F32 ? 0 : 1]) {
-        const int64_t segs = (vocab + skew + LP_THREADS * ept - 1) / (LP_THREADS * ept);
-        if (segs > LP_SEGS) break;
-        p = {ept, (int)segs};
-        if (rows * segs >= 2 * 148) break;
+    const int n = type == KV_F32 ? 4 : 8;
+    const int64_t vecs = (vocab + 2 * (n - 1)) / n, slots = 148 * LP_CTAS;      // at any alignment
+    const int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS, fewest = (vecs + longest - 1) / longest;
+    int64_t best = -1;
+    LogprobPlan p{0, 0};
+    for (int64_t segs = fewest; segs <= LP_SEGS && (segs == fewest || vecs / segs >= LP_THREADS); ++segs) {
+        const int64_t waves = (rows * segs + slots - 1) / slots, cost = waves * (vecs * n / segs + 4096) + 16 * segs;
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        p.seg_vecs = (vecs + segs - 1) / segs;
+        p.segs = (int)((vecs + p.seg_vecs - 1) / p.seg_vecs);
     }
     return p;
 }
 
-template <int TYPE, int EPT>
+template <int TYPE>
 int32_t launch_logprobs(cudaStream_t st, const LogprobArgs &a, int64_t rows) {
-    CUDA_TRY(launch_k(logprobs_kernel<TYPE, EPT>, (unsigned)(rows * a.segs), LP_THREADS, 0, st, a));
+    CUDA_TRY(launch_k(logprobs_kernel<TYPE>, (unsigned)(rows * a.segs), LP_THREADS, 0, st, a));
     return check_launch("logprobs_kernel");
 }
 
@@ -355,6 +360,7 @@ extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {
     a.ntargets = (int)ntargets;
     a.k = (int)k;
     a.segs = plan.segs;
+    a.seg_vecs = plan.seg_vecs;
     if (plan.segs > 1) {
         a.counter = (unsigned int *)p[7];
         a.part = (float4 *)((char *)p[7] + 4 * LP_ROWS);
@@ -364,17 +370,8 @@ extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {
     for (int64_t first = 0; first < rows; first += LP_ROWS) {
         const int64_t n = std::min<int64_t>(rows - first, LP_ROWS);
         a.row_first = first;
-        int32_t status;
-        if (type == KV_F32)
-            status = plan.ept == 64 ? launch_logprobs<KV_F32, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_F32, 16>(st, a, n)
-                                                                                            : launch_logprobs<KV_F32, 4>(st, a, n);
-        else if (type == KV_F16)
-            status = plan.ept == 64 ? launch_logprobs<KV_F16, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_F16, 16>(st, a, n)
-                                                                                            : launch_logprobs<KV_F16, 8>(st, a, n);
-        else
-            status = plan.ept == 64 ? launch_logprobs<KV_BF16, 64>(st, a, n) : plan.ept == 16 ? launch_logprobs<KV_BF16, 16>(st, a, n)
-                                                                                             : launch_logprobs<KV_BF16, 8>(st, a, n);
-        NC_TRY(status);
+        NC_TRY(type == KV_F32 ? launch_logprobs<KV_F32>(st, a, n) : type == KV_F16 ? launch_logprobs<KV_F16>(st, a, n)
+                                                                                  : launch_logprobs<KV_BF16>(st, a, n));
     }
     return NC_OK;
 }
