@@ -10,10 +10,10 @@
 // a thread, the next batch's loads in flight while one is worked on.  Each thread keeps its own maximum and sums,
 // rescaled only by a batch with a larger value, and leaves the maximum of each batch (a block of 16 or 32
 // logits) in shared memory: no barrier and nothing of the top is in the loop.  The top k lie in the blocks whose maxima
-// reach the k-th largest one, T.  T comes from ranking the blocks that reach the k-th largest of 32 threads' groups'
-// maxima (about as many as k); those k blocks are read again and their values from T up ranked.  Where more
-// blocks end in T than can be read again, equals are as good as their index: the first k in the row's order are taken.
-// The last CTA of a row joins the segments, in their order.
+// reach the k-th largest one, T.  The k-th largest of the maxima of 32 groups of threads is a bound that about as
+// many blocks as k reach: they are read again and their values from there up ranked.  Where that is more blocks than are
+// read at once, T is found among them, or bit by bit; where more end in T than are read at once, the first k of its equals
+// in the row's order are taken.  The last CTA of a row joins the segments, in their order.
 #pragma once
 
 #include "nc_kv4.cuh"
@@ -104,7 +104,7 @@ __device__ __noinline__ uint4 lp_partial(const char *row, int64_t e, int64_t n) 
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A maximum with the sums relative to it.
+// Sums relative to a maximum: s = sum exp(x - m), e = sum exp(x - m) (x - m); m is -inf with no sums.
 struct LpSums {
     float m, s, e;
 };
@@ -125,6 +125,48 @@ __device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
     r.e = __fmaf_rn(wa, __fmaf_rn(a.s, da, a.e), wb * __fmaf_rn(b.s, db, b.e));
     return r;
 }
+// Two floats to an instruction.
+__device__ __forceinline__ uint64_t lp_pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 lp_unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t lp_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The largest value of a vector, a NaN if there is one.
+template <int TYPE>
+__device__ __forceinline__ float lp_vector_max(const uint4 &w) {
+    if constexpr (TYPE == KV_F32) {
+        return lp_max(lp_max(__uint_as_float(w.x), __uint_as_float(w.y)), lp_max(__uint_as_float(w.z), __uint_as_float(w.w)));
+    } else if constexpr (TYPE == KV_F16) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+        const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+        return lp_max(m.x, m.y);
+    } else {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&w);
+        const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+        return lp_max(m.x, m.y);
+    }
+}
+
 __device__ __forceinline__ LpSums lp_warp_join(LpSums v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -137,14 +179,27 @@ __device__ __forceinline__ LpSums lp_warp_join(LpSums v) {
     return v;
 }
 
+// How many of the n keys are above keys[i], for i < n: four neighbouring threads share an i.  Calls use(i, key, above) in
+// one thread for each i.
+template <typename F>
+__device__ __forceinline__ void lp_ranks(const unsigned long long *keys, int n, F use) {
+    const int part = threadIdx.x & 3;
+    for (int base = 0; base < n; base += LP_THREADS / 4) {
+        const int i = base + (threadIdx.x >> 2);
+        const unsigned long long mine = i < n ? keys[i] : ~0ull;
+        int above = 0;
+#pragma unroll 4
+        for (int j = part; j < n; j += 4) above += keys[j] > mine;
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 2);
+        if (part == 0 && i < n) use(i, mine, above);
+    }
+}
 // The k best of the n keys in `keys` (distinct), in order, to out.
 __device__ __forceinline__ void lp_rank(const unsigned long long *keys, int n, int k, unsigned long long *out) {
-    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
-        const unsigned long long mine = keys[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += keys[j] > mine;
-        if (rank < k) out[rank] = mine;
-    }
+    lp_ranks(keys, n, [&](int, unsigned long long key, int above) {
+        if (above < k) out[above] = key;
+    });
 }
 
 struct LpShared {
@@ -199,24 +254,43 @@ __device__ __forceinline__ void lp_segment_top(const LogprobArgs &a, LpShared &s
     }
     const uint32_t bound = __shfl_sync(0xffffffffu, group, __ffs(__ballot_sync(0xffffffffu, rank == a.k - 1)) - 1);
     if (mine >= bound)
-        for (int i = 0; i < batches; ++i)
-            if (sh.block[i][tid] >= bound) {
+#pragma unroll 4
+        for (int i = 0; i < batches; ++i) {
+            const uint32_t most = sh.block[i][tid];
+            if (most >= bound) {
                 const int at = atomicAdd(&sh.count, 1);
-                if (at < LP_CAND) sh.cand[at] = (unsigned long long)sh.block[i][tid] << 32 | (uint32_t)(i * LP_THREADS + tid);
+                if (at < LP_CAND) sh.cand[at] = (unsigned long long)most << 32 | (uint32_t)(i * LP_THREADS + tid);
             }
-    __syncthreads();
-    uint32_t kth = 0;                                              // T, in order
-    if (sh.count <= LP_CAND) {
-        for (int i = tid; i < sh.count; i += LP_THREADS) {
-            const unsigned long long key = sh.cand[i];
-            int above = 0;
-            for (int j = 0; j < sh.count; ++j) above += sh.cand[j] > key;
-            if (above == a.k - 1) sh.kth = (uint32_t)(key >> 32);
         }
+    __syncthreads();
+    int *const list = (int *)sh.heads;                             // MOST block numbers; the heads come later
+    uint32_t kth = 0;
+    bool all = false;
+    const int reached = sh.count;
+    if (reached <= MOST) {                                         // few enough to be read again as they are
+        kth = bound;
+        all = true;
+        if (tid < reached) list[tid] = (int)(uint32_t)sh.cand[tid];
+        if (tid == 0) sh.greater = reached;
+    } else if (reached <= LP_CAND) {                               // T, and the blocks above it (fewer than k), then those that end in it
+        lp_ranks(sh.cand, reached, [&](int, unsigned long long key, int above) {
+            if (above == a.k - 1) sh.kth = (uint32_t)(key >> 32);
+        });
         __syncthreads();
         kth = sh.kth;
-    } else {                                                       // bit by bit: the largest T that k blocks reach
-        for (int bit = 31; bit >= 0; --bit) {
+        for (int i = tid; i < reached; i += LP_THREADS) {
+            const uint32_t most = (uint32_t)(sh.cand[i] >> 32);
+            if (most > kth) list[atomicAdd(&sh.greater, 1)] = (int)(uint32_t)sh.cand[i];
+            else if (most == kth) atomicAdd(&sh.equal, 1);
+        }
+        __syncthreads();
+        all = sh.greater + sh.equal <= MOST;
+        __syncthreads();
+        if (all)
+            for (int i = tid; i < reached; i += LP_THREADS)
+                if ((uint32_t)(sh.cand[i] >> 32) == kth) list[atomicAdd(&sh.greater, 1)] = (int)(uint32_t)sh.cand[i];
+    } else {                                                       // masses of equals, or of good blocks in few threads:
+        for (int bit = 31; bit >= 0; --bit) {                      // bit by bit, the largest T that k blocks reach
             const uint32_t trial = kth | 1u << bit;
             int n = 0;
             for (int i = 0; i < batches; ++i) n += sh.block[i][tid] >= trial;
@@ -228,35 +302,28 @@ __device__ __forceinline__ void lp_segment_top(const LogprobArgs &a, LpShared &s
             if (n >= a.k) kth = trial;
             __syncthreads();
         }
+        for (int i = 0; i < batches; ++i)
+            if (sh.block[i][tid] > kth) list[atomicAdd(&sh.greater, 1)] = i * LP_THREADS + tid;
     }
-    // The blocks above T, then those that end in it.
-    int *const list = (int *)sh.heads;                             // MOST block numbers at most, before the heads are used
-    if (mine >= kth)
-        for (int i = 0; i < batches; ++i)
-            if (sh.block[i][tid] >= kth) {
-                if (sh.block[i][tid] > kth) list[atomicAdd(&sh.greater, 1)] = i * LP_THREADS + tid;     // fewer than k
-                else atomicAdd(&sh.equal, 1);
-            }
     __syncthreads();
-    const int greater = sh.greater;
-    const bool all = greater + sh.equal <= MOST;
     if (tid == 0) sh.count = 0;
+    const int values = sh.greater * SIZE;
     __syncthreads();
-    if (all && mine >= kth)
-        for (int i = 0; i < batches; ++i)
-            if (sh.block[i][tid] == kth) list[atomicAdd(&sh.greater, 1)] = i * LP_THREADS + tid;
-    __syncthreads();
-    const int blocks = sh.greater;
-    for (int at = warp; at < blocks; at += LP_THREADS / 32)
+    for (int base_at = tid; base_at < values; base_at += 4 * LP_THREADS) {
+        unsigned long long key[4];
 #pragma unroll
-        for (int u = lane; u < SIZE; u += 32) {
-            const int64_t v = seg0 + list[at] / LP_THREADS * BATCH + list[at] % LP_THREADS + u / N * LP_THREADS;
+        for (int m = 0; m < 4; ++m) {
+            const int at = base_at + m * LP_THREADS, block = list[min(at, values - 1) / SIZE], u = at % SIZE;
+            const int64_t v = seg0 + block / LP_THREADS * BATCH + block % LP_THREADS + u / N * LP_THREADS;
             const int64_t e = v * N - skew + u % N;
-            if (v >= v_end || e < 0 || e >= a.vocab) continue;
-            const unsigned long long key = lp_key(kv_load(base, e, TYPE), (uint32_t)e);
-            const uint32_t order = (uint32_t)(key >> 32);
-            if (all ? order >= kth : order > kth) sh.cand[atomicAdd(&sh.count, 1)] = key;
+            key[m] = at < values && v < v_end && e >= 0 && e < a.vocab ? lp_key(kv_load(base, e, TYPE), (uint32_t)e) : 0;
         }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const uint32_t order = (uint32_t)(key[m] >> 32);
+            if (key[m] != 0 && (all ? order >= kth : order > kth)) sh.cand[atomicAdd(&sh.count, 1)] = key[m];
+        }
+    }
     __syncthreads();
     if (!all) {                                                    // the first k equals, in the row's order
         int found = 0;
@@ -308,42 +375,48 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __g
     };
 
     LpSums sum{-INFINITY, 0.0f, 0.0f};
+    float2 pair = make_float2(0.0f, 0.0f), epair = pair;           // the two halves of the thread's sums
     const int64_t seg0 = (int64_t)seg * a.seg_vecs;
     uint4 raw[LP_VECS], ahead[LP_VECS];
     fetch(seg0, raw);
     int batches = 0;
     for (int64_t first = seg0; first < v_end; first += BATCH, ++batches) {
         fetch(first + BATCH, ahead);
-        float top = -INFINITY;
+        float top = lp_vector_max<TYPE>(raw[0]);
 #pragma unroll
-        for (int i = 0; i < LP_VECS; ++i) {
-            float x[N];
-            lp_unpack<TYPE>(raw[i], x);
-#pragma unroll
-            for (int j = 0; j < N; ++j) top = lp_max(top, x[j]);
-        }
+        for (int i = 1; i < LP_VECS; ++i) top = lp_max(top, lp_vector_max<TYPE>(raw[i]));
         if (a.k) sh.block[batches][tid] = lp_order(top);
-        if (!(top <= sum.m)) {                                     // a larger value, or a NaN
+        if (!(top <= sum.m)) {                                   // a larger value, or a NaN
+            const float s = pair.x + pair.y, e = epair.x + epair.y;
             const float d = lp_max(sum.m - top, LP_LEAST), w = lp_exp2(d * LP_LOG2E);
-            sum.e = w * __fmaf_rn(sum.s, d, sum.e);
-            sum.s *= w;
+            pair = make_float2(s * w, 0.0f);
+            epair = make_float2(w * __fmaf_rn(s, d, e), 0.0f);
             sum.m = top;
         }
         const float to = sum.m == -INFINITY ? 0.0f : sum.m;
+        const uint64_t unit = lp_pair(LP_LOG2E, LP_LOG2E), from = lp_pair(-to, -to);
+        uint64_t s2 = lp_pair(pair.x, pair.y), e2 = lp_pair(epair.x, epair.y);
 #pragma unroll
         for (int i = 0; i < LP_VECS; ++i) {
             float x[N];
             lp_unpack<TYPE>(raw[i], x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float d = lp_max(x[j] - to, LP_LEAST), p = lp_exp2(d * LP_LOG2E);
-                sum.s += p;
-                sum.e = __fmaf_rn(p, d, sum.e);
+            for (int j = 0; j < N; j += 2) {
+                const float2 d = lp_unpair(lp_add2(lp_pair(x[j], x[j + 1]), from));
+                const uint64_t d2 = lp_pair(lp_max(d.x, LP_LEAST), lp_max(d.y, LP_LEAST));
+                const float2 u = lp_unpair(lp_mul2(d2, unit));
+                const uint64_t p = lp_pair(lp_exp2(u.x), lp_exp2(u.y));
+                s2 = lp_add2(s2, p);
+                e2 = lp_fma2(p, d2, e2);
             }
         }
+        pair = lp_unpair(s2);
+        epair = lp_unpair(e2);
 #pragma unroll
         for (int i = 0; i < LP_VECS; ++i) raw[i] = ahead[i];
     }
+    sum.s = pair.x + pair.y;
+    sum.e = epair.x + epair.y;
     if (a.k) lp_segment_top<TYPE>(a, sh, base, skew, seg0, v_end, batches, lp_order(sum.m));
     sum = lp_warp_join(sum);
     if (lane == 0) sh.sums[warp] = sum;
@@ -405,23 +478,22 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __g
     // The row's results.
     const float log_s = logf(sum.s);
     const bool none = sum.m == -INFINITY;
-    const float shift = none ? 0.0f : sum.m;
     if (tid == 0) {
         if (a.entropy) a.entropy[row] = none ? 0.0f : log_s - fdiv(sum.e, sum.s);
         if (a.lse) a.lse[row] = none ? -INFINITY : sum.m + log_s;
     }
+    auto logprob = [&](float x) { return none ? -INFINITY : (x - sum.m) - log_s; };
     for (int j = tid; j < a.ntargets; j += LP_THREADS) {
         const int64_t t = a.targets[row * a.ntargets + j];
         float v = __uint_as_float(0x7fc00000u);
-        if (t >= 0 && t < a.vocab) v = none ? -INFINITY : (kv_load(base, t, TYPE) - shift) - log_s;
+        if (t >= 0 && t < a.vocab) v = logprob(kv_load(base, t, TYPE));
         else if (a.error) atomicMin(a.error, (unsigned long long)row);
         a.out[row * a.ntargets + j] = v;
     }
     if (tid < a.k) {
         const unsigned long long key = sh.best[tid];
-        const int64_t t = 0xffffffffu - (uint32_t)key;
-        a.top[row * a.k + tid] = t;
-        a.top_logprobs[row * a.k + tid] = none ? -INFINITY : (kv_load(base, t, TYPE) - shift) - log_s;
+        a.top[row * a.k + tid] = 0xffffffffu - (uint32_t)key;
+        a.top_logprobs[row * a.k + tid] = logprob(lp_value((uint32_t)(key >> 32)));
     }
 }
 

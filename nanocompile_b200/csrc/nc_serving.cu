@@ -26,6 +26,17 @@ int32_t check_type(int64_t type) {
     return NC_OK;
 }
 
+// Raises a kernel's limit of shared memory, once on each device (`allowed`: a bit for each).
+template <typename K>
+int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) {
+    int device = 0;
+    CUDA_TRY(cudaGetDevice(&device));
+    if (device < 64 && (allowed->load(std::memory_order_relaxed) >> device & 1)) return NC_OK;
+    CUDA_TRY(allow_smem(kernel, bytes));
+    if (device < 64) allowed->fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    return NC_OK;
+}
+
 // The sizes that append, read and attention share.
 int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, const void *lengths, const void *row_start,
                    void *error, int64_t rows, int64_t seqs, int64_t kv, int64_t d, int64_t page, int64_t pages,
@@ -99,13 +110,8 @@ template <int D, int NT, bool HL>
 int32_t launch_kv4_attention_t(cudaStream_t st, const Kv4AttnArgs &a, int64_t ctas) {
     using S = Kv4AttnShape<D, NT, HL, KV4_WARPS, KV4_STAGES>;
     auto kernel = kv4_attention_kernel<D, NT, HL, KV4_WARPS, KV4_STAGES>;
-    static std::atomic<uint64_t> allowed{0};       // devices whose limit is raised
-    int device = 0;
-    CUDA_TRY(cudaGetDevice(&device));
-    if (!(allowed.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-        CUDA_TRY(allow_smem(kernel, S::SMEM));
-        if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
-    }
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(kernel, S::SMEM, &allowed));
     CUDA_TRY(launch_k(kernel, (unsigned)ctas, 32 * KV4_WARPS, S::SMEM, st, a));
     return check_launch("kv4_attention_kernel");
 }
