@@ -104,22 +104,39 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t u) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-// One block by one warp, lane = dimension in the block: the lane's code; the parameters' word in all lanes.
-__device__ __forceinline__ uint32_t kv4_quantise(float x, uint32_t *params) {
-    const uint32_t key = ordered_bits(x);
-    const float low = from_ordered_bits(__reduce_min_sync(0xffffffffu, key));
-    const float high = from_ordered_bits(__reduce_max_sync(0xffffffffu, key));
-    const bool nan = __any_sync(0xffffffffu, x != x);   // the extremes are found as float maxima, which pass a NaN over
+// A block of 32 values in four neighbouring lanes, eight each: the lane's eight codes in a word, the block's parameters.
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t *params) {
+    float low = x[0], high = x[0];
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        low = fminf(low, x[i]);
+        high = fmaxf(high, x[i]);
+        nan = nan || x[i] != x[i];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    const uint32_t votes = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 28);
+    nan = (votes & 15u) != 0;
     const float limit = 65504.0f;
     const float z = fminf(fmaxf(low, -limit), limit);
     const float w = fminf(fmul(fsub(high, low), 1.0f / 15.0f), limit);
     const float bad = __uint_as_float(0x7fc00000u);
     const __half zero = __float2half_rn(nan ? bad : z), scale = __float2half_rn(nan ? bad : w);
     *params = (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(zero) << 16;
-    const float s = __half2float(scale);
+    const float s = __half2float(scale), from = __half2float(zero);
     if (!(s > 0.0f)) return 0;
-    const float q = floorf(fadd(fmul(fsub(x, __half2float(zero)), fdiv(1.0f, s)), 0.5f));
-    return (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
+    const float inv = fdiv(1.0f, s);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = fadd(fmul(fsub(x[i], from), inv), 0.5f);
+        word |= (uint32_t)(int)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);     // rounds towards zero: floor, as q >= 0
+    }
+    return word;
 }
 
 struct Kv4AppendArgs {
@@ -143,45 +160,177 @@ __device__ __forceinline__ float kv4_rotated(const void *p, int64_t base, int i,
     return i < half ? fsub(fmul(x, c), fmul(y, s)) : fadd(fmul(x, c), fmul(y, s));
 }
 
-// A warp per (row, kv head, block, key or value).
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendArgs a) {
+// Eight values from element `at` (of 16-byte aligned memory where `vectors`).
+__device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bool vectors, float (&x)[8]) {
+    if (!vectors) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = kv_load(p, at + i, type);
+    } else if (type == KV_F32) {
+        const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 w = *(const uint4 *)((const uint16_t *)p + at);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (type == KV_F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(u[i] << 16);
+                x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+// The append and the read go by tiles: the rows of a call that fall into one tile are one piece of work for a warp
+// and head, keys or values, with lane 4 g + c at dimensions 32 b + 8 c .. of positions g and 8 + g: for keys the
+// lane's words are the ones it writes, for values two shuffles turn them.  A CTA looks through `window` rows for
+// the first rows of tiles.  One row of each sequence (a decode step) is the same with tiles of one row.
+struct Kv4TileRows {
+    char *tile;                    // of the first head, or null: no page
+    int64_t row, position;         // of the first row
+    int count, t0;                 // rows of the tile, its first position in the tile
+    int seq;
+};
+
+// Calls work(rows) for each tile whose first row is among the CTA's window, all threads of the CTA alike.
+template <typename F>
+__device__ __forceinline__ void kv4_tiles(const Kv4Rows &at, const Kv4Pool &pool, int window, F work) {
+    const int lane = threadIdx.x & 31;
+    const int64_t first = (int64_t)blockIdx.x * window, r = first + lane;
+    int seq = 0, position = -1, count = 0;
+    bool starts = false;
+    if (lane < window && r < at.rows) {
+        seq = kv4_sequence(at, r);
+        const int64_t after = at.row_start ? at.row_start[seq + 1] - r : 1;      // rows to the sequence's end
+        const int64_t begin = at.row_start ? at.row_start[seq] : r;
+        position = (int)(at.lengths[seq] - after);
+        if (after > 0 && position < 0) {                             // before position 0: a piece of one row
+            starts = true;
+            count = 1;
+        } else if (after > 0) {
+            starts = r == begin || position % KV4_TILE == 0;
+            count = (int)min(after, (int64_t)(KV4_TILE - position % KV4_TILE));
+        } else {                                                     // belongs to no sequence
+            starts = true;
+            count = 1;
+            position = -1;
+        }
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, starts); left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        Kv4TileRows t;
+        t.seq = __shfl_sync(0xffffffffu, seq, k);
+        t.row = first + k;
+        t.position = __shfl_sync(0xffffffffu, position, k);
+        t.count = __shfl_sync(0xffffffffu, count, k);
+        t.t0 = (int)(t.position & (KV4_TILE - 1));
+        t.tile = nullptr;
+        if (t.position >= 0) {
+            const int page = kv4_page(at, t.seq, (int)t.position);
+            if (page >= 0) t.tile = pool.base + page * pool.page_bytes + (int64_t)((int)t.position % at.page / KV4_TILE) * (20 * pool.d);
+        }
+        work(t);
+    }
+}
+constexpr int KV4_TILE_WARPS = 4;
+
+template <int NB>
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int window, bool vectors) {
+    constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2;
+    release_dependents();
     wait_for_producer();
-    const int lane = threadIdx.x & 31, nb = a.pool.d / 32, vb = kv4_vb(nb), d = a.pool.d;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (item >= a.at.rows * a.pool.kv * nb * 2) return;
-    const int which = (int)(item & 1);
-    const int b = (int)((item >> 1) % nb), head = (int)((item >> 1) / nb % a.pool.kv);
-    const int64_t row = (item >> 1) / nb / a.pool.kv;
-    const int seq = kv4_sequence(a.at, row);
-    const int64_t after = a.at.row_start ? a.at.row_start[seq + 1] - row : 1;
-    const int64_t position = a.at.lengths[seq] - after;
-    if (position < 0 || after <= 0) return;
-    if (a.cos_tab && position >= a.positions) {
-        if (a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)seq);
-        return;
-    }
-    const int page = kv4_page(a.at, seq, (int)position);
-    if (page < 0) return;
-    float x;
-    if (which == 0)
-        x = kv4_rotated(a.keys, row * a.key_stride + head * d, 32 * b + lane, d, a.type, a.cos_tab, a.sin_tab, position);
-    else
-        x = kv_load(a.values, row * a.value_stride + head * d + 32 * b + lane, a.type);
-    uint32_t params;
-    const uint32_t code = kv4_quantise(x, &params);
-    const int inside = (int)(position % a.at.page), t = inside & 15, g = t & 7, c = (t & 7) >> 1, j = t >> 3, h = t & 1;
-    char *tile = a.pool.base + page * a.pool.page_bytes +
-                 ((int64_t)head * (a.at.page / KV4_TILE) + inside / KV4_TILE) * (20 * d) + which * 10 * d;
-    uint32_t v = code << (4 * (lane & (which == 0 ? 7 : 3)));
-    v |= __shfl_xor_sync(0xffffffffu, v, 1);
-    v |= __shfl_xor_sync(0xffffffffu, v, 2);
-    if (which == 0) {
-        v |= __shfl_xor_sync(0xffffffffu, v, 4);
-        if ((lane & 7) == 0) ((uint32_t *)tile)[kv4_code_word(vb, b, 4 * g + (lane >> 3), j)] = v;
-    } else if ((lane & 3) == 0) {
-        ((uint16_t *)tile)[kv4_code_word(vb, b, 4 * (lane >> 2) + c, j) * 2 + h] = (uint16_t)v;
-    }
-    if (lane == 0) ((uint32_t *)(tile + 8 * d))[kv4_param_word(nb, b, t)] = params;
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int job = blockIdx.y * KV4_TILE_WARPS + (threadIdx.x >> 5);     // 2 head + (0 keys, 1 values)
+    const int head = job >> 1, which = job & 1;
+    kv4_tiles(a.at, a.pool, window, [&](const Kv4TileRows &rows) {
+        if (!rows.tile || head >= a.pool.kv) return;
+        int count = rows.count;
+        if (a.cos_tab && rows.position + count > a.positions) {
+            if (a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)rows.seq);
+            count = (int)(a.positions - rows.position);
+        }
+        char *const tile = rows.tile + (int64_t)head * (a.at.page / KV4_TILE) * (20 * D) + which * 10 * D;
+        const void *const p = which ? a.values : a.keys;
+        const int64_t stride = which ? a.value_stride : a.key_stride;
+        const bool full = count == KV4_TILE;
+        bool in[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) in[j] = 8 * j + g >= rows.t0 && 8 * j + g < rows.t0 + count;
+#pragma unroll
+        for (int b0 = 0; b0 < NB; b0 += VB) {
+            uint32_t words[VB][2], params[VB][2];
+#pragma unroll
+            for (int v = 0; v < VB; ++v)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int t = 8 * j + g, i0 = 32 * (b0 + v) + 8 * c;
+                    const int64_t at = (rows.row + t - rows.t0) * stride + (int64_t)head * D;
+                    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    if (in[j]) {
+                        kv_load8(p, at + i0, a.type, vectors, x);
+                        if (which == 0 && a.cos_tab) {                // as kv4_rotated, eight at a time
+                            const bool low = i0 < HALF;
+                            const int k = low ? i0 : i0 - HALF;
+                            const int64_t angle = (rows.position + t - rows.t0) * HALF + k;
+                            float y[8], cs[8], sn[8];
+                            kv_load8(p, at + (low ? i0 + HALF : k), a.type, vectors, y);
+                            kv_load8(a.cos_tab, angle, KV_F32, vectors, cs);
+                            kv_load8(a.sin_tab, angle, KV_F32, vectors, sn);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                x[i] = low ? fsub(fmul(x[i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[i], cs[i]), fmul(y[i], sn[i]));
+                        }
+                    }
+                    words[v][j] = kv4_quantise(x, &params[v][j]);
+                }
+            if (which) {
+                // Value words: lane 4 g' + c' takes dimension group g' of positions 2 c' and 2 c' + 1.
+#pragma unroll
+                for (int v = 0; v < VB; ++v)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t even = __shfl_sync(0xffffffffu, words[v][j], 8 * c + (g >> 1));
+                        const uint32_t odd = __shfl_sync(0xffffffffu, words[v][j], 8 * c + 4 + (g >> 1));
+                        words[v][j] = __byte_perm(even, odd, g & 1 ? 0x7632 : 0x5410);
+                    }
+            }
+            uint32_t *const codes = (uint32_t *)tile + kv4_code_word(VB, b0, lane, 0);
+            if (full) {
+                if constexpr (VB == 2) *(uint4 *)codes = make_uint4(words[0][0], words[0][1], words[1][0], words[1][1]);
+                else *(uint2 *)codes = make_uint2(words[0][0], words[0][1]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VB; ++v)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (which == 0) {
+                            if (in[j]) codes[2 * v + j] = words[v][j];
+                        } else {
+                            const int t = 8 * j + 2 * c;
+                            uint16_t *const shorts = (uint16_t *)(codes + 2 * v + j);
+                            if (t >= rows.t0 && t < rows.t0 + count) shorts[0] = (uint16_t)words[v][j];
+                            if (t + 1 >= rows.t0 && t + 1 < rows.t0 + count) shorts[1] = (uint16_t)(words[v][j] >> 16);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int v = 0; v < VB; ++v)
+                if (c == v) {
+                    uint32_t *const to = (uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b0 + v, g);
+                    if (full) {
+                        *(uint2 *)to = make_uint2(params[v][0], params[v][1]);
+                    } else {
+                        if (in[0]) to[0] = params[v][0];
+                        if (in[1]) to[1] = params[v][1];
+                    }
+                }
+        }
+    });
 }
 
 struct Kv4ReadArgs {
@@ -190,38 +339,52 @@ struct Kv4ReadArgs {
     float *keys, *values;          // [rows][kv][d]
 };
 
-// The values the rows' positions stand for; zeros for a row without a position.  A warp per
-// (row, kv head, key or value).
-__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4ReadArgs a) {
+// The values the rows' positions stand for; zeros for a row without a position.
+template <int NB>
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a, int window, bool vectors) {
+    constexpr int D = 32 * NB, VB = kv4_vb(NB);
+    release_dependents();
     wait_for_producer();
-    const int lane = threadIdx.x & 31, nb = a.pool.d / 32, vb = kv4_vb(nb), d = a.pool.d;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (item >= a.at.rows * a.pool.kv * 2) return;
-    const int which = (int)(item & 1), head = (int)((item >> 1) % a.pool.kv);
-    const int64_t row = (item >> 1) / a.pool.kv;
-    const int seq = kv4_sequence(a.at, row);
-    const int64_t after = a.at.row_start ? a.at.row_start[seq + 1] - row : 1;
-    const int64_t position = a.at.lengths[seq] - after;
-    const int page = position >= 0 && after > 0 ? kv4_page(a.at, seq, (int)position) : -1;
-    float *out = (which == 0 ? a.keys : a.values) + (row * a.pool.kv + head) * d;
-    if (page < 0) {
-        for (int b = 0; b < nb; ++b) out[32 * b + lane] = 0.0f;
-        return;
-    }
-    const int inside = (int)(position % a.at.page), t = inside & 15, g = t & 7, c = (t & 7) >> 1, j = t >> 3, h = t & 1;
-    const char *tile = a.pool.base + page * a.pool.page_bytes +
-                       ((int64_t)head * (a.at.page / KV4_TILE) + inside / KV4_TILE) * (20 * d) + which * 10 * d;
-    for (int b = 0; b < nb; ++b) {
-        uint32_t code;
-        if (which == 0)
-            code = ((const uint32_t *)tile)[kv4_code_word(vb, b, 4 * g + (lane >> 3), j)] >> (4 * (lane & 7)) & 15u;
-        else
-            code = ((const uint16_t *)tile)[kv4_code_word(vb, b, 4 * (lane >> 2) + c, j) * 2 + h] >> (4 * (lane & 3)) & 15u;
-        const uint32_t par = ((const uint32_t *)(tile + 8 * d))[kv4_param_word(nb, b, t)];
-        const float s = __half2float(__ushort_as_half((unsigned short)(par & 0xffff)));
-        const float z = __half2float(__ushort_as_half((unsigned short)(par >> 16)));
-        out[32 * b + lane] = fadd(z, fmul(s, (float)code));
-    }
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int job = blockIdx.y * KV4_TILE_WARPS + (threadIdx.x >> 5);
+    const int head = job >> 1, which = job & 1;
+    kv4_tiles(a.at, a.pool, window, [&](const Kv4TileRows &rows) {
+        if (head >= a.pool.kv) return;
+        const char *const tile = rows.tile ? rows.tile + (int64_t)head * (a.at.page / KV4_TILE) * (20 * D) + which * 10 * D : nullptr;
+        float *const out = which ? a.values : a.keys;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint2 w = make_uint2(0, 0), par = make_uint2(0, 0);
+            if (tile) {
+                w = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
+                par = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, g));
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t word = j ? w.y : w.x;
+                if (which) {
+                    // Back to lane 4 g + c: groups 2 c (low half) and 2 c + 1 of position g, half-word g & 1 of lane 4 g' + g / 2.
+                    const uint32_t low = __shfl_sync(0xffffffffu, word, 8 * c + (g >> 1));
+                    const uint32_t high = __shfl_sync(0xffffffffu, word, 8 * c + 4 + (g >> 1));
+                    word = __byte_perm(low, high, g & 1 ? 0x7632 : 0x5410);
+                }
+                const int t = 8 * j + g;
+                if (t < rows.t0 || t >= rows.t0 + rows.count) continue;
+                const float2 sz = __half22float2(*reinterpret_cast<const __half2 *>(j ? &par.y : &par.x));
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = tile ? fadd(sz.y, fmul(sz.x, (float)(word >> (4 * i) & 15u))) : 0.0f;
+                float *const to = out + ((rows.row + t - rows.t0) * a.pool.kv + head) * D + 32 * b + 8 * c;
+                if (vectors) {
+                    *(float4 *)to = make_float4(x[0], x[1], x[2], x[3]);
+                    *(float4 *)(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) to[i] = x[i];
+                }
+            }
+        }
+    });
 }
 
 }  // namespace nc

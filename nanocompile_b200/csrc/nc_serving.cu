@@ -41,7 +41,7 @@ int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) 
 int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, const void *lengths, const void *row_start,
                    void *error, int64_t rows, int64_t seqs, int64_t kv, int64_t d, int64_t page, int64_t pages,
                    int64_t page_bytes, int64_t offset, int64_t width) {
-    if (rows < 0 || seqs < 0 || rows > I32 || seqs > I32 || kv <= 0 || kv > 65535)
+    if (rows < 0 || seqs < 0 || rows > I32 || seqs > I32 || kv <= 0 || kv > 32768)
         return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows, %lld sequences, %lld kv heads", (long long)rows, (long long)seqs, (long long)kv);
     if (d != 32 && d != 64 && d != 96 && d != 128)
         return fail(NC_ERR_ARGUMENT, "head dimension %lld: the 4-bit cache serves 32, 64, 96 and 128", (long long)d);
@@ -68,6 +68,12 @@ int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, co
     pool->kv = (int)kv;
     pool->d = (int)d;
     return NC_OK;
+}
+
+// Rows that a CTA looks through for tiles: a tile's worth, or one where there are few rows or each is a sequence's only one.
+int kv4_window(const Kv4Rows &at) { return at.row_start && at.rows >= 16 * at.seqs && at.rows >= 1024 ? KV4_TILE : 1; }
+dim3 kv4_tile_grid(const Kv4Rows &at, const Kv4Pool &pool, int window) {
+    return dim3((unsigned)((at.rows + window - 1) / window), (unsigned)((2 * pool.kv + KV4_TILE_WARPS - 1) / KV4_TILE_WARPS));
 }
 
 float bits_to_f32(int64_t bits) {
@@ -150,9 +156,18 @@ extern "C" int32_t nc_kv4_append(void **p, const int64_t *s, void *stream) {
     const int64_t line = (int64_t)a.pool.kv * a.pool.d;
     if (!a.keys || !a.values || !a.cos_tab != !a.sin_tab) return fail(NC_ERR_ARGUMENT, "null keys or values, or half a rotation table");
     if (a.key_stride < line || a.value_stride < line) return fail(NC_ERR_ARGUMENT, "rows of %lld values overlap", (long long)line);
-    const int64_t warps = a.at.rows * a.pool.kv * (a.pool.d / 32) * 2, ctas = (warps + 7) / 8;
-    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
-    CUDA_TRY(launch_k(kv4_append_kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, a));
+    const int64_t bytes = a.type == KV_F32 ? 4 : 2;
+    const bool vectors = !misaligned(a.keys, 16) && !misaligned(a.values, 16) && a.key_stride * bytes % 16 == 0 &&
+                         a.value_stride * bytes % 16 == 0 && !misaligned(a.cos_tab, 16) && !misaligned(a.sin_tab, 16);
+    const int window = kv4_window(a.at);
+    const dim3 grid = kv4_tile_grid(a.at, a.pool, window);
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (a.pool.d) {
+        case 32: CUDA_TRY(launch_k(kv4_append_kernel<1>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        case 64: CUDA_TRY(launch_k(kv4_append_kernel<2>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        case 96: CUDA_TRY(launch_k(kv4_append_kernel<3>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        default: CUDA_TRY(launch_k(kv4_append_kernel<4>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+    }
     return check_launch("kv4_append_kernel");
 }
 
@@ -163,9 +178,16 @@ extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {
     a.keys = (float *)p[0];
     a.values = (float *)p[1];
     if (!a.keys || !a.values) return fail(NC_ERR_ARGUMENT, "null keys or values");
-    const int64_t warps = a.at.rows * a.pool.kv * 2, ctas = (warps + 7) / 8;
-    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
-    CUDA_TRY(launch_k(kv4_read_kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, a));
+    const bool vectors = !misaligned(a.keys, 16) && !misaligned(a.values, 16);
+    const int window = kv4_window(a.at);
+    const dim3 grid = kv4_tile_grid(a.at, a.pool, window);
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (a.pool.d) {
+        case 32: CUDA_TRY(launch_k(kv4_read_kernel<1>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        case 64: CUDA_TRY(launch_k(kv4_read_kernel<2>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        case 96: CUDA_TRY(launch_k(kv4_read_kernel<3>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        default: CUDA_TRY(launch_k(kv4_read_kernel<4>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+    }
     return check_launch("kv4_read_kernel");
 }
 
