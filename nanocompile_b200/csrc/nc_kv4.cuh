@@ -104,39 +104,80 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t u) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
+// The smaller and the larger of two, a NaN if either is one.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Two floats to an instruction.  A packed multiplication and a packed addition after it may become one FMA (seen, with
+// -fmad=false and .rn too): where both roundings count, one of the two is not packed.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // A block of 32 values in four neighbouring lanes, eight each: the lane's eight codes in a word, the block's parameters.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t *params) {
     float low = x[0], high = x[0];
-    bool nan = x[0] != x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
-        low = fminf(low, x[i]);
-        high = fmaxf(high, x[i]);
-        nan = nan || x[i] != x[i];
+        low = min_nan(low, x[i]);
+        high = max_nan(high, x[i]);
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
-    const uint32_t votes = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 28);
-    nan = (votes & 15u) != 0;
     const float limit = 65504.0f;
-    const float z = fminf(fmaxf(low, -limit), limit);
-    const float w = fminf(fmul(fsub(high, low), 1.0f / 15.0f), limit);
-    const float bad = __uint_as_float(0x7fc00000u);
-    const __half zero = __float2half_rn(nan ? bad : z), scale = __float2half_rn(nan ? bad : w);
+    const float z = min_nan(max_nan(low, -limit), limit);
+    // An infinite range, or none between infinities of one sign, counts as the largest; a NaN among the values stays one.
+    const float w = low != low ? low : fminf(fmul(fsub(high, low), 1.0f / 15.0f), limit);
+    const __half zero = __float2half_rn(z), scale = __float2half_rn(w);
     *params = (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(zero) << 16;
     const float s = __half2float(scale), from = __half2float(zero);
     if (!(s > 0.0f)) return 0;
     const float inv = fdiv(1.0f, s);
+    const uint64_t from2 = pack2(-from, -from), inv2 = pack2(inv, inv);
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float q = fadd(fmul(fsub(x[i], from), inv), 0.5f);
-        word |= (uint32_t)(int)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);     // rounds towards zero: floor, as q >= 0
+    for (int i = 6; i >= 0; i -= 2) {
+        float2 q = unpack2(mul2(add2(pack2(x[i], x[i + 1]), from2), inv2));
+        q.x = fadd(q.x, 0.5f);
+        q.y = fadd(q.y, 0.5f);
+        // 2^23 + the clamped code, rounded towards zero: floor, as it is not negative.  The code is in the low bits.
+        const uint32_t a = __float_as_uint(__fadd_rz(fminf(fmaxf(q.x, 0.0f), 15.0f), 8388608.0f));
+        const uint32_t b = __float_as_uint(__fadd_rz(fminf(fmaxf(q.y, 0.0f), 15.0f), 8388608.0f));
+        word = (word * 16 + b) * 16 + a;
     }
-    return word;
+    return word - 0x4b000000u * 0x11111111u;       // what the eight 2^23 have added, modulo 2^32
 }
 
 struct Kv4AppendArgs {
@@ -166,11 +207,11 @@ __device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bo
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = kv_load(p, at + i, type);
     } else if (type == KV_F32) {
-        const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
+        const float4 a = __ldg((const float4 *)((const float *)p + at)), b = __ldg((const float4 *)((const float *)p + at + 4));
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
         x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
-        const uint4 w = *(const uint4 *)((const uint16_t *)p + at);
+        const uint4 w = __ldg((const uint4 *)((const uint16_t *)p + at));
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -81,12 +81,6 @@ __device__ __forceinline__ void lp_unpack(const uint4 &w, float *x) {
     }
 }
 
-// The larger of two, a NaN if either is one.
-__device__ __forceinline__ float lp_max(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 // The vector whose first element is element e of a row of n, -inf outside the row; for the row's ends only.
 template <int TYPE>
 __device__ __noinline__ uint4 lp_partial(const char *row, int64_t e, int64_t n) {
@@ -116,8 +110,8 @@ __device__ __forceinline__ float lp_exp2(float x) {
 constexpr float LP_LOG2E = 1.4426950408889634f;
 constexpr float LP_LEAST = -1000.0f;   // exp is 0 below: keeps 0 * -inf out of the entropy
 __device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
-    const float m = lp_max(a.m, b.m), to = m == -INFINITY ? 0.0f : m;
-    const float da = lp_max(a.m - to, LP_LEAST), db = lp_max(b.m - to, LP_LEAST);
+    const float m = max_nan(a.m, b.m), to = m == -INFINITY ? 0.0f : m;
+    const float da = max_nan(a.m - to, LP_LEAST), db = max_nan(b.m - to, LP_LEAST);
     const float wa = lp_exp2(da * LP_LOG2E), wb = lp_exp2(db * LP_LOG2E);
     LpSums r;
     r.m = m;
@@ -125,45 +119,19 @@ __device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
     r.e = __fmaf_rn(wa, __fmaf_rn(a.s, da, a.e), wb * __fmaf_rn(b.s, db, b.e));
     return r;
 }
-// Two floats to an instruction.
-__device__ __forceinline__ uint64_t lp_pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 lp_unpair(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t lp_mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // The largest value of a vector, a NaN if there is one.
 template <int TYPE>
 __device__ __forceinline__ float lp_vector_max(const uint4 &w) {
     if constexpr (TYPE == KV_F32) {
-        return lp_max(lp_max(__uint_as_float(w.x), __uint_as_float(w.y)), lp_max(__uint_as_float(w.z), __uint_as_float(w.w)));
+        return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
     } else if constexpr (TYPE == KV_F16) {
         const __half2 *h = reinterpret_cast<const __half2 *>(&w);
         const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-        return lp_max(m.x, m.y);
+        return max_nan(m.x, m.y);
     } else {
         const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&w);
         const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-        return lp_max(m.x, m.y);
+        return max_nan(m.x, m.y);
     }
 }
 
@@ -384,34 +352,34 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __g
         fetch(first + BATCH, ahead);
         float top = lp_vector_max<TYPE>(raw[0]);
 #pragma unroll
-        for (int i = 1; i < LP_VECS; ++i) top = lp_max(top, lp_vector_max<TYPE>(raw[i]));
+        for (int i = 1; i < LP_VECS; ++i) top = max_nan(top, lp_vector_max<TYPE>(raw[i]));
         if (a.k) sh.block[batches][tid] = lp_order(top);
         if (!(top <= sum.m)) {                                   // a larger value, or a NaN
             const float s = pair.x + pair.y, e = epair.x + epair.y;
-            const float d = lp_max(sum.m - top, LP_LEAST), w = lp_exp2(d * LP_LOG2E);
+            const float d = max_nan(sum.m - top, LP_LEAST), w = lp_exp2(d * LP_LOG2E);
             pair = make_float2(s * w, 0.0f);
             epair = make_float2(w * __fmaf_rn(s, d, e), 0.0f);
             sum.m = top;
         }
         const float to = sum.m == -INFINITY ? 0.0f : sum.m;
-        const uint64_t unit = lp_pair(LP_LOG2E, LP_LOG2E), from = lp_pair(-to, -to);
-        uint64_t s2 = lp_pair(pair.x, pair.y), e2 = lp_pair(epair.x, epair.y);
+        const uint64_t unit = pack2(LP_LOG2E, LP_LOG2E), from = pack2(-to, -to);
+        uint64_t s2 = pack2(pair.x, pair.y), e2 = pack2(epair.x, epair.y);
 #pragma unroll
         for (int i = 0; i < LP_VECS; ++i) {
             float x[N];
             lp_unpack<TYPE>(raw[i], x);
 #pragma unroll
             for (int j = 0; j < N; j += 2) {
-                const float2 d = lp_unpair(lp_add2(lp_pair(x[j], x[j + 1]), from));
-                const uint64_t d2 = lp_pair(lp_max(d.x, LP_LEAST), lp_max(d.y, LP_LEAST));
-                const float2 u = lp_unpair(lp_mul2(d2, unit));
-                const uint64_t p = lp_pair(lp_exp2(u.x), lp_exp2(u.y));
-                s2 = lp_add2(s2, p);
-                e2 = lp_fma2(p, d2, e2);
+                const float2 d = unpack2(add2(pack2(x[j], x[j + 1]), from));
+                const uint64_t d2 = pack2(max_nan(d.x, LP_LEAST), max_nan(d.y, LP_LEAST));
+                const float2 u = unpack2(mul2(d2, unit));
+                const uint64_t p = pack2(lp_exp2(u.x), lp_exp2(u.y));
+                s2 = add2(s2, p);
+                e2 = fma2(p, d2, e2);
             }
         }
-        pair = lp_unpair(s2);
-        epair = lp_unpair(e2);
+        pair = unpack2(s2);
+        epair = unpack2(e2);
 #pragma unroll
         for (int i = 0; i < LP_VECS; ++i) raw[i] = ahead[i];
     }

@@ -269,7 +269,8 @@ int32_t kvp_args(KvPagesArgs *a, void **p, const int64_t *s, int table, int stat
     a->status = (int64_t *)p[status];
     int32_t *w = (int32_t *)p[scratch];
     a->copies = w;
-    w += 4;
+    a->words = w + 4;
+    w += 4 + KVP_WORDS;
     for (int32_t **x : {&a->refs, &a->tails, &a->owner, &a->fresh}) *x = w, w += pages;
     for (int32_t **x : {&a->first, &a->need, &a->offset}) *x = w, w += seqs;
     a->list = w;
@@ -278,6 +279,24 @@ int32_t kvp_args(KvPagesArgs *a, void **p, const int64_t *s, int table, int stat
     a->pages = (int)pages;
     a->page = (int)page;
     return NC_OK;
+}
+
+// One CTA for up to four pages or table entries to a thread (its barriers are cheaper), else a cluster.
+cudaError_t launch_pages(void (*kernel)(KvPagesArgs), cudaStream_t st, const KvPagesArgs &a) {
+    const bool many = (int64_t)a.seqs * a.width + a.pages > 4 * KVP_THREADS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = many ? KVP_CLUSTER : 1;
+    cfg.blockDim = KVP_THREADS;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = many ? KVP_CLUSTER : 1;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 int32_t kvp_copy(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page_bytes) {
@@ -289,8 +308,8 @@ int32_t kvp_copy(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page
 
 extern "C" int64_t nc_kv_pages_scratch_bytes(int64_t seqs, int64_t width, int64_t pages) {
     (void)width;
-    if (seqs < 0 || pages < 0) return 16;
-    return 16 + 4 * (4 * pages + 3 * seqs + kvp_list(seqs, pages));
+    if (seqs < 0 || pages < 0) return 0;
+    return 4 * (4 + KVP_WORDS + 4 * pages + 3 * seqs + kvp_list(seqs, pages));
 }
 
 // p: [0] new table [1] new lengths [2] table [3] lengths [4] status [5] pool [6] scratch [7] parent [8] grow
@@ -302,7 +321,7 @@ extern "C" int32_t nc_kv_pages_update(void **p, const int64_t *s, void *stream) 
     a.new_lengths = (int32_t *)p[1];
     a.parent = (const int32_t *)p[7];
     a.grow = (const int32_t *)p[8];
-    CUDA_TRY(launch_k(kv_pages_update_kernel, 1, KVP_THREADS, 0, (cudaStream_t)stream, a));
+    CUDA_TRY(launch_pages(kv_pages_update_kernel, (cudaStream_t)stream, a));
     NC_TRY(check_launch("kv_pages_update_kernel"));
     return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
 }
@@ -311,7 +330,7 @@ extern "C" int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream)
     KvPagesArgs a{};
     NC_TRY(kvp_args(&a, p, s, 2, 4, 6));
     if (a.seqs == 0) return NC_OK;
-    CUDA_TRY(launch_k(kv_pages_compact_kernel, 1, KVP_THREADS, 0, (cudaStream_t)stream, a));
+    CUDA_TRY(launch_pages(kv_pages_compact_kernel, (cudaStream_t)stream, a));
     NC_TRY(check_launch("kv_pages_compact_kernel"));
     return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
 }
