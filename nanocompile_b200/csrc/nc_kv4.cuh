@@ -207,11 +207,11 @@ __device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bo
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = kv_load(p, at + i, type);
     } else if (type == KV_F32) {
-        const float4 a = __ldg((const float4 *)((const float *)p + at)), b = __ldg((const float4 *)((const float *)p + at + 4));
+        const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
         x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
     } else {
-        const uint4 w = __ldg((const uint4 *)((const uint16_t *)p + at));
+        const uint4 w = *(const uint4 *)((const uint16_t *)p + at);
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -281,13 +281,22 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Rows &at, const Kv4Pool &pool
 constexpr int KV4_TILE_WARPS = 4;
 
 template <int NB>
-__global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int window, bool vectors) {
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS, 6) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int window, bool vectors) {
     constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2;
     release_dependents();
     wait_for_producer();
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int job = blockIdx.y * KV4_TILE_WARPS + (threadIdx.x >> 5);     // 2 head + (0 keys, 1 values)
     const int head = job >> 1, which = job & 1;
+    if (head < a.pool.kv) {                                          // the rows are on their way while their tiles are looked up
+        const int size = a.type == KV_F32 ? 4 : 2, lines = (D * size + 127) / 128;
+        for (int i = lane; i < window * lines; i += 32) {
+            const int64_t r = (int64_t)blockIdx.x * window + i / lines;
+            if (r < a.at.rows)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"((const char *)(which ? a.values : a.keys) +
+                             (r * (which ? a.value_stride : a.key_stride) + (int64_t)head * D) * size + min(i % lines * 128, D * size - 1)));
+        }
+    }
     kv4_tiles(a.at, a.pool, window, [&](const Kv4TileRows &rows) {
         if (!rows.tile || head >= a.pool.kv) return;
         int count = rows.count;
@@ -393,13 +402,15 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_read_kernel(const __g
         if (head >= a.pool.kv) return;
         const char *const tile = rows.tile ? rows.tile + (int64_t)head * (a.at.page / KV4_TILE) * (20 * D) + which * 10 * D : nullptr;
         float *const out = which ? a.values : a.keys;
+        uint2 codes[NB], params[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint2 w = make_uint2(0, 0), par = make_uint2(0, 0);
-            if (tile) {
-                w = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
-                par = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, g));
-            }
+            codes[b] = tile ? *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0)) : make_uint2(0, 0);
+            params[b] = tile ? *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, g)) : make_uint2(0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint2 w = codes[b];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint32_t word = j ? w.y : w.x;
@@ -411,7 +422,7 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_read_kernel(const __g
                 }
                 const int t = 8 * j + g;
                 if (t < rows.t0 || t >= rows.t0 + rows.count) continue;
-                const float2 sz = __half22float2(*reinterpret_cast<const __half2 *>(j ? &par.y : &par.x));
+                const float2 sz = __half22float2(*reinterpret_cast<const __half2 *>(j ? &params[b].y : &params[b].x));
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = tile ? fadd(sz.y, fmul(sz.x, (float)(word >> (4 * i) & 15u))) : 0.0f;

@@ -17,8 +17,8 @@
 //
 // The bookkeeping is one CTA, or a cluster of eight where there is much of it: warps read the live table entries
 // once and count in global memory (atomics on integers, whose order does not matter), prefix sums over the cluster find
-// the free pages.  It is bound by the latency of its few dependent steps.  The page copies are a second kernel over
-// the list that the first one leaves, bound by memory.
+// the free pages.  It is bound by the latency of its few dependent steps, so it leaves the rest to a second kernel of
+// many CTAs: the page copies, bound by memory, and the new table.
 #pragma once
 
 #include <climits>
@@ -28,7 +28,8 @@
 namespace nc {
 
 constexpr int KVP_THREADS = 1024;
-constexpr int KVP_COPY_CTAS = 148 * 4, KVP_COPY_THREADS = 256;
+constexpr int KVP_COPY_CTAS = 148 * 5, KVP_COPY_THREADS = 256;
+constexpr int KVP_TABLE_CTAS = 64;             // of them also write the new table, first
 constexpr int KVP_COPY_CHUNK = 16384;          // bytes of a page that a CTA copies at a time
 
 struct KvPagesArgs {
@@ -38,12 +39,13 @@ struct KvPagesArgs {
     int32_t *refs, *tails, *owner;             // [pages]
     int32_t *fresh;                            // [pages]: the free pages that are taken
     int32_t *first, *need, *offset;            // [seqs]: first fresh entry, how many, where they start in `fresh`
-    int32_t *list, *copies;                    // list [2 * max(seqs, pages)]: (from, to); copies [1]
+    int32_t *list;                             // [2 * max(seqs, pages)]: (from, to), `to` by its place in `fresh` for an update
     int32_t *words;                            // [KVP_WORDS]: what the cluster's CTAs tell one another
     int seqs, width, pages, page;
 };
 constexpr int KVP_CLUSTER = 8;
-enum KvpWord : int { KVP_BAD = 0, KVP_HIGHEST = 1, KVP_LOW = 2, KVP_SUMS = 4, KVP_WORDS = KVP_SUMS + 2 * KVP_CLUSTER };
+// KVP_STATE: 0 the new table as planned, 1 the old one again.
+enum KvpWord : int { KVP_BAD = 0, KVP_STATE = 1, KVP_COPIES = 2, KVP_USED = 3, KVP_LOW = 4, KVP_SUMS = 8, KVP_WORDS = KVP_SUMS + 4 * KVP_CLUSTER };
 constexpr int KVP_UNIT = 256;                  // table entries of a sequence that a warp takes
 
 // The kernel's threads: of one CTA or of a cluster.
@@ -61,59 +63,56 @@ struct KvpTeam {
         threads = size * KVP_THREADS;
         parity = 0;
     }
-    // A barrier that orders global memory; what another CTA wrote is read past L1.
+    // A barrier that orders global memory (release and acquire for the cluster); what another CTA wrote is read past L1.
     __device__ __forceinline__ void sync() const {
         if (size == 1) {
             __syncthreads();
         } else {
-            __threadfence();
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
     }
 };
 
-// Exclusive prefix sum over the block's threads; *total gets the sum.  `buf`: 33 ints.
-__device__ __forceinline__ int block_exclusive_sum(int v, int *buf, int *total) {
+// Exclusive prefix sums of two counts (packed into 64 bits: neither passes 32) over the team; *total gets their sums.
+struct KvpCounts {
+    int a, b;
+};
+__device__ __forceinline__ KvpCounts team_exclusive_sum(KvpTeam &team, int32_t *words, KvpCounts v, unsigned long long *buf, KvpCounts *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    const unsigned long long mine = (unsigned long long)(unsigned)v.b << 32 | (unsigned)v.a;
+    unsigned long long x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();                            // the last call's readers are done with buf
     if (lane == 31) buf[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int w = lane < KVP_THREADS / 32 ? buf[lane] : 0;
+    unsigned long long w = buf[lane];           // KVP_THREADS / 32 = 32 warps: every warp sums them for itself
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+    }
+    const unsigned long long before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    unsigned long long all = __shfl_sync(0xffffffffu, w, 31), at = x - mine + (warp ? before : 0);
+    if (team.size > 1) {
+        unsigned long long *const sums = (unsigned long long *)(words + KVP_SUMS) + team.parity * KVP_CLUSTER;
+        team.parity ^= 1;
+        if (threadIdx.x == 0) sums[team.rank] = all;
+        team.sync();
+        all = 0;
+#pragma unroll
+        for (int r = 0; r < KVP_CLUSTER; ++r) {
+            const unsigned long long y = __ldcg(sums + r);
+            if (r < team.rank) at += y;
+            all += y;
         }
-        buf[lane] = w;
     }
-    __syncthreads();
-    *total = buf[31];
-    return x - v + (warp ? buf[warp - 1] : 0);
-}
-// The same over the team.
-__device__ __forceinline__ int team_exclusive_sum(KvpTeam &team, int32_t *words, int v, int *buf, int *total) {
-    int mine = block_exclusive_sum(v, buf, total);
-    if (team.size == 1) return mine;
-    int32_t *const sums = words + KVP_SUMS + team.parity * KVP_CLUSTER;
-    team.parity ^= 1;
-    if (threadIdx.x == 0) sums[team.rank] = *total;
-    team.sync();
-    *total = 0;
-#pragma unroll
-    for (int r = 0; r < KVP_CLUSTER; ++r) {
-        const int x = __ldcg(sums + r);
-        if (r < team.rank) mine += x;
-        *total += x;
-    }
-    return mine;
+    *total = KvpCounts{(int)(unsigned)all, (int)(all >> 32)};
+    return KvpCounts{(int)(unsigned)at, (int)(at >> 32)};
 }
 
 __device__ __forceinline__ int pages_of(int length, int page) { return (int)(((int64_t)length + page - 1) / page); }
@@ -146,20 +145,19 @@ __device__ __forceinline__ void kvp_units(const KvpTeam &team, const KvPagesArgs
 
 // The new table is the old one, and nothing is copied.
 __device__ __forceinline__ void kvp_refuse(const KvpTeam &team, const KvPagesArgs &a, int short_of, int used) {
-    const int64_t n = (int64_t)a.seqs * a.width;
-    for (int64_t i = team.thread; i < n; i += team.threads) a.new_table[i] = a.table[i];
     for (int i = team.thread; i < a.seqs; i += team.threads)
         if (a.new_lengths) a.new_lengths[i] = a.lengths[i];
     if (team.thread == 0) {
         a.status[0] = short_of;
         a.status[1] = used;
         a.status[2] = a.status[3] = 0;
-        *a.copies = 0;
+        a.words[KVP_STATE] = 1;
+        a.words[KVP_COPIES] = 0;
     }
 }
 
 __global__ void __launch_bounds__(KVP_THREADS) kv_pages_update_kernel(const __grid_constant__ KvPagesArgs a) {
-    __shared__ int buf[33];
+    __shared__ unsigned long long buf[32];
     release_dependents();
     wait_for_producer();
     KvpTeam team;
@@ -168,7 +166,7 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_pages_update_kernel(const __gr
         a.refs[i] = a.tails[i] = 0;
         a.owner[i] = INT_MAX;
     }
-    if (team.thread < KVP_SUMS) a.words[team.thread] = 0;
+    if (team.thread < KVP_SUMS) a.words[team.thread] = 0;          // KVP_STATE among them
     team.sync();
     // Every reference that the new table keeps.
     kvp_units(team, a, [&](int i, int j0) {
@@ -215,33 +213,31 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_pages_update_kernel(const __gr
             a.need[i] = need;
             a.new_lengths[i] = s.after;
         }
-        int total, copies;
-        const int at = team_exclusive_sum(team, a.words, need, buf, &total);
-        const int place = team_exclusive_sum(team, a.words, copy, buf, &copies);
+        KvpCounts total;
+        const KvpCounts at = team_exclusive_sum(team, a.words, KvpCounts{need, copy}, buf, &total);
         if (i < a.seqs) {
-            a.offset[i] = wanted + at;
+            a.offset[i] = wanted + at.a;
             if (copy) {
-                a.list[2 * (copied + place)] = source;
-                a.list[2 * (copied + place) + 1] = wanted + at;        // becomes the page id below
+                a.list[2 * (copied + at.b)] = source;
+                a.list[2 * (copied + at.b) + 1] = wanted + at.a;
             }
         }
-        wanted += total;
-        copied += copies;
+        wanted += total.a;
+        copied += total.b;
     }
     // The free pages, lowest first, and the pages in use.
     int found = 0;
     for (int base = 0; base < a.pages; base += team.threads) {
         const int id = base + team.thread;
         const bool free = id < a.pages && __ldcg(a.refs + id) == 0;
-        int total;
-        const int at = found + team_exclusive_sum(team, a.words, free, buf, &total);
+        KvpCounts total;
+        const int at = found + team_exclusive_sum(team, a.words, KvpCounts{free, 0}, buf, &total).a;
         if (free && at < wanted) a.fresh[at] = id;
-        found += total;
+        found += total.a;
     }
-    const int kept = a.pages - found;
-    team.sync();
     if (found < wanted) {
         // The pages that the old table uses, for the caller to see.
+        team.sync();
         for (int i = team.thread; i < a.pages; i += team.threads) a.tails[i] = 0;
         team.sync();
         int used = 0;
@@ -252,47 +248,28 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_pages_update_kernel(const __gr
                 if (id >= 0 && id < a.pages) used += atomicExch(a.tails + id, 1) == 0;
             }
         });
-        int total;
-        team_exclusive_sum(team, a.words, used, buf, &total);
-        kvp_refuse(team, a, wanted - found, total);
+        KvpCounts total;
+        team_exclusive_sum(team, a.words, KvpCounts{used, 0}, buf, &total);
+        kvp_refuse(team, a, wanted - found, total.a);
         return;
     }
-    int top = 0;
-    kvp_units(team, a, [&](int i, int j0) {
-        const int first = __ldcg(a.first + i), need = __ldcg(a.need + i), offset = __ldcg(a.offset + i);
-        const int source = a.parent ? a.parent[i] : i;
-#pragma unroll
-        for (int k = 0; k < KVP_UNIT / 32; ++k) {
-            const int j = j0 + 32 * k + lane;
-            if (j >= a.width) break;
-            int id = -1;
-            if (j < first) id = a.table[(int64_t)source * a.width + j];
-            else if (j - first < need) id = __ldcg(a.fresh + offset + j - first);
-            a.new_table[(int64_t)i * a.width + j] = id;
-            top = max(top, id + 1);
-        }
-    });
-    for (int i = team.thread; i < copied; i += team.threads) a.list[2 * i + 1] = __ldcg(a.fresh + __ldcg(a.list + 2 * i + 1));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top) atomicMax(a.words + KVP_HIGHEST, top);
-    team.sync();
     if (team.thread == 0) {
         a.status[0] = 0;
-        a.status[1] = kept + wanted;
+        a.status[1] = a.pages - found + wanted;
         a.status[2] = copied;
-        a.status[3] = __ldcg(a.words + KVP_HIGHEST);
-        *a.copies = copied;
+        a.status[3] = 0;                                           // raised as the table is written
+        a.words[KVP_COPIES] = copied;
     }
 }
 
 __global__ void __launch_bounds__(KVP_THREADS) kv_pages_compact_kernel(const __grid_constant__ KvPagesArgs a) {
-    __shared__ int buf[33];
+    __shared__ unsigned long long buf[32];
     release_dependents();
     wait_for_producer();
     KvpTeam team;
     const int lane = threadIdx.x & 31;
     for (int i = team.thread; i < a.pages; i += team.threads) a.refs[i] = 0;
-    if (team.thread < KVP_SUMS) a.words[team.thread] = 0;
+    if (team.thread < KVP_SUMS) a.words[team.thread] = 0;          // KVP_STATE among them
     team.sync();
     kvp_units(team, a, [&](int i, int j0) {
         const int n = pages_of(max(0, a.lengths[i]), a.page);
@@ -315,58 +292,93 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_pages_compact_kernel(const __g
     int used = 0;
     for (int base = 0; base < a.pages; base += team.threads) {
         const int id = base + team.thread;
-        int total;
-        const int below = used + team_exclusive_sum(team, a.words, id < a.pages && __ldcg(a.refs + id), buf, &total);
+        KvpCounts total;
+        const int live = id < a.pages && __ldcg(a.refs + id);
+        const int below = used + team_exclusive_sum(team, a.words, KvpCounts{live, 0}, buf, &total).a;
         if (id < a.pages) a.owner[id] = below;
-        used += total;
+        used += total.a;
     }
     team.sync();
     // The k-th hole below `used` takes the k-th page in use from `used` on.
-    const int low = used < a.pages ? __ldcg(a.owner + used) : used, holes = used - low;
+    const int low = used < a.pages ? __ldcg(a.owner + used) : used;
     for (int id = team.thread; id < a.pages; id += team.threads) {
         const int below = __ldcg(a.owner + id);
         const bool live = __ldcg(a.refs + id) != 0;
         if (id < used && !live) a.list[2 * (id - below) + 1] = id;
         if (id >= used && live) a.list[2 * (below - low)] = id;
     }
-    team.sync();
-    kvp_units(team, a, [&](int i, int j0) {
-        const int n = min(a.width, pages_of(max(0, a.lengths[i]), a.page));
-#pragma unroll
-        for (int k = 0; k < KVP_UNIT / 32; ++k) {
-            const int j = j0 + 32 * k + lane;
-            if (j >= a.width) break;
-            int id = -1;
-            if (j < n) {
-                id = a.table[(int64_t)i * a.width + j];
-                if (id >= used) id = __ldcg(a.list + 2 * (__ldcg(a.owner + id) - low) + 1);
-            }
-            a.new_table[(int64_t)i * a.width + j] = id;
-        }
-    });
     if (team.thread == 0) {
         a.status[0] = 0;
-        a.status[1] = used;
-        a.status[2] = holes;
-        a.status[3] = used;
-        *a.copies = holes;
+        a.status[1] = a.status[3] = used;
+        a.status[2] = a.words[KVP_COPIES] = used - low;
+        a.words[KVP_USED] = used;
+        a.words[KVP_LOW] = low;
     }
 }
 
-// The listed pages, in chunks; no page is both read and written.
-__global__ void __launch_bounds__(KVP_COPY_THREADS) kv_pages_copy_kernel(char *pool, int64_t page_bytes, const int32_t *list,
-                                                                        const int32_t *copies) {
+// The new table, by the first CTAs, and the listed pages, in chunks; no page is both read and written.
+template <bool UPDATE>
+__global__ void __launch_bounds__(KVP_COPY_THREADS) kv_pages_write_kernel(const __grid_constant__ KvPagesArgs a, char *pool, int64_t page_bytes) {
     release_dependents();
     wait_for_producer();
+    const int lane = threadIdx.x & 31;
+    if (blockIdx.x < KVP_TABLE_CTAS) {
+        const bool refused = a.words[KVP_STATE] != 0;
+        const unsigned chunks = (a.width + KVP_UNIT - 1) / KVP_UNIT, units = chunks * a.seqs;
+        int top = 0;
+        for (unsigned u = (blockIdx.x * KVP_COPY_THREADS + threadIdx.x) >> 5; u < units; u += KVP_TABLE_CTAS * KVP_COPY_THREADS / 32) {
+            const int i = (int)(u / chunks), j0 = (int)(u % chunks) * KVP_UNIT;
+            int first, end, offset = 0, source = i, used = 0, low = 0;      // entries before `first` are old, before `end` fresh
+            if (refused) {
+                first = end = a.width;
+            } else if (UPDATE) {
+                first = a.first[i];
+                end = first + a.need[i];
+                offset = a.offset[i];
+                source = a.parent ? a.parent[i] : i;
+            } else {
+                first = end = min(a.width, pages_of(max(0, a.lengths[i]), a.page));
+                used = a.words[KVP_USED];
+                low = a.words[KVP_LOW];
+            }
+#pragma unroll
+            for (int k = 0; k < KVP_UNIT / 32; ++k) {
+                const int j = j0 + 32 * k + lane;
+                if (j >= a.width) break;
+                int id = -1;
+                if (j < first) {
+                    id = a.table[(int64_t)source * a.width + j];
+                    if (!UPDATE && !refused && id >= used) id = a.list[2 * (a.owner[id] - low) + 1];
+                } else if (j < end) {
+                    id = a.fresh[offset + j - first];
+                }
+                a.new_table[(int64_t)i * a.width + j] = id;
+                top = max(top, id + 1);
+            }
+        }
+        if (UPDATE && !refused) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0 && top) atomicMax((long long *)a.status + 3, (long long)top);
+        }
+    }
     const int64_t chunks = (page_bytes + KVP_COPY_CHUNK - 1) / KVP_COPY_CHUNK;
-    const int64_t items = *copies * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t items = a.words[KVP_COPIES] * chunks;
+    // From the last CTA on, as the first ones have the table.
+    for (int64_t item = gridDim.x - 1 - blockIdx.x; item < items; item += gridDim.x) {
         const int64_t k = item / chunks, at = item % chunks * KVP_COPY_CHUNK;
         const int64_t n = page_bytes - at < KVP_COPY_CHUNK ? page_bytes - at : KVP_COPY_CHUNK;
-        const uint4 *const from = (const uint4 *)(pool + list[2 * k] * page_bytes + at);
-        uint4 *const to = (uint4 *)(pool + list[2 * k + 1] * page_bytes + at);
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < n / 16; i += KVP_COPY_THREADS) to[i] = __ldcs(from + i);
+        const int32_t to_page = UPDATE ? a.fresh[a.list[2 * k + 1]] : a.list[2 * k + 1];
+        const uint4 *const from = (const uint4 *)(pool + a.list[2 * k] * page_bytes + at);
+        uint4 *const to = (uint4 *)(pool + to_page * page_bytes + at);
+        if (n == KVP_COPY_CHUNK) {
+            uint4 v[KVP_COPY_CHUNK / 16 / KVP_COPY_THREADS];
+#pragma unroll
+            for (int i = 0; i < KVP_COPY_CHUNK / 16 / KVP_COPY_THREADS; ++i) v[i] = __ldcs(from + i * KVP_COPY_THREADS + threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < KVP_COPY_CHUNK / 16 / KVP_COPY_THREADS; ++i) __stcs(to + i * KVP_COPY_THREADS + threadIdx.x, v[i]);
+        } else {
+            for (int64_t i = threadIdx.x; i < n / 16; i += KVP_COPY_THREADS) to[i] = __ldcs(from + i);
+        }
     }
 }
 

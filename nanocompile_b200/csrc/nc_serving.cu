@@ -268,9 +268,8 @@ int32_t kvp_args(KvPagesArgs *a, void **p, const int64_t *s, int table, int stat
     a->lengths = (const int32_t *)p[table + 1];
     a->status = (int64_t *)p[status];
     int32_t *w = (int32_t *)p[scratch];
-    a->copies = w;
-    a->words = w + 4;
-    w += 4 + KVP_WORDS;
+    a->words = w;                              // pairs of them are 64-bit sums
+    w += KVP_WORDS;
     for (int32_t **x : {&a->refs, &a->tails, &a->owner, &a->fresh}) *x = w, w += pages;
     for (int32_t **x : {&a->first, &a->need, &a->offset}) *x = w, w += seqs;
     a->list = w;
@@ -299,9 +298,10 @@ cudaError_t launch_pages(void (*kernel)(KvPagesArgs), cudaStream_t st, const KvP
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-int32_t kvp_copy(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page_bytes) {
-    CUDA_TRY(launch_k(kv_pages_copy_kernel, KVP_COPY_CTAS, KVP_COPY_THREADS, 0, st, (char *)pool, page_bytes, a.list, a.copies));
-    return check_launch("kv_pages_copy_kernel");
+template <bool UPDATE>
+int32_t launch_pages_write(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page_bytes) {
+    CUDA_TRY(launch_k(kv_pages_write_kernel<UPDATE>, KVP_COPY_CTAS, KVP_COPY_THREADS, 0, st, a, (char *)pool, page_bytes));
+    return check_launch("kv_pages_write_kernel");
 }
 
 }  // namespace
@@ -309,7 +309,7 @@ int32_t kvp_copy(cudaStream_t st, const KvPagesArgs &a, void *pool, int64_t page
 extern "C" int64_t nc_kv_pages_scratch_bytes(int64_t seqs, int64_t width, int64_t pages) {
     (void)width;
     if (seqs < 0 || pages < 0) return 0;
-    return 4 * (4 + KVP_WORDS + 4 * pages + 3 * seqs + kvp_list(seqs, pages));
+    return 4 * (KVP_WORDS + 4 * pages + 3 * seqs + kvp_list(seqs, pages));
 }
 
 // p: [0] new table [1] new lengths [2] table [3] lengths [4] status [5] pool [6] scratch [7] parent [8] grow
@@ -323,7 +323,7 @@ extern "C" int32_t nc_kv_pages_update(void **p, const int64_t *s, void *stream) 
     a.grow = (const int32_t *)p[8];
     CUDA_TRY(launch_pages(kv_pages_update_kernel, (cudaStream_t)stream, a));
     NC_TRY(check_launch("kv_pages_update_kernel"));
-    return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
+    return launch_pages_write<true>((cudaStream_t)stream, a, p[5], s[4]);
 }
 
 extern "C" int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream) {
@@ -332,7 +332,7 @@ extern "C" int32_t nc_kv_pages_compact(void **p, const int64_t *s, void *stream)
     if (a.seqs == 0) return NC_OK;
     CUDA_TRY(launch_pages(kv_pages_compact_kernel, (cudaStream_t)stream, a));
     NC_TRY(check_launch("kv_pages_compact_kernel"));
-    return kvp_copy((cudaStream_t)stream, a, p[5], s[4]);
+    return launch_pages_write<false>((cudaStream_t)stream, a, p[5], s[4]);
 }
 
 // ---- token log probabilities ----------------------------------------------------------------------
