@@ -18,7 +18,8 @@
 // q is brought below 2^11 by a power of two and split into two whole numbers q = hi + lo 2^-11 of at most 11
 // bits, whose 32 products with a code fit the unit's bits, in an accumulator for each part.  p scale_v is split
 // into two f16 parts (22 bits), summed over one step and added to the running sum in float32.
-// bfloat16 callers take one f16 part of q and of p scale_v.
+// bfloat16 callers take one f16 part of q, of p and of p scale_v, and have the parameters' sums made by the matrix unit
+// too: sum_b zero_k (sum of q over b) with the sums of q in two parts, sum_t p zero_v and sum_t p scale_v as eight more rows.
 //
 // Probabilities are held relative to ref = (running maximum) - k, where k lifts p scale_v to just below
 // 2^15 for the largest scale_v seen (k <= 15): any power of two cancels in sum p v / sum p, so the f16 range
@@ -30,6 +31,8 @@
 // nobody else.  Few columns and a long cache are split over CTAs as well (chunks of whole steps); the last
 // CTA to finish joins the parts in their order, so results do not depend on the schedule.
 #pragma once
+
+#include <type_traits>
 
 #include "nc_kv4.cuh"
 
@@ -58,6 +61,21 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], c
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
+__device__ __forceinline__ void mma_f16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -82,6 +100,8 @@ __device__ __forceinline__ uint32_t pack_f16(float low, float high) {
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
+// Whether a block's parameters are those of a NaN (no others are not finite).
+__device__ __forceinline__ bool nan_params(uint32_t w) { return (w & 0x7fffu) > 0x7c00u || (w >> 16 & 0x7fffu) > 0x7c00u; }
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -105,7 +125,7 @@ struct Kv4AttnShape {
     static constexpr int MERGE = W * COLS * (D + 2) * 4;               // shares the ring's bytes
     static constexpr int BODY = RING > MERGE ? RING : MERGE;
     static constexpr int QF = NB * 2 * NT * PARTS * 32 * 8;
-    static constexpr int SMEM = BODY + QF + COLS * (NB + 4) * 4;
+    static constexpr int SMEM = BODY + QF + COLS * (NB + 4) * 4 + NT * 32 * 4;
     static constexpr int CTAS = NT == 1 ? 16 / W : 8 / W;              // wanted on an SM
 };
 
@@ -113,12 +133,14 @@ template <int D, int NT, bool HL, int W, int ST>
 __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)) kv4_attention_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using S = Kv4AttnShape<D, NT, HL, W, ST>;
     constexpr int NB = S::NB, VB = S::VB, COLS = S::COLS, MT = S::MT, TILES = S::TILES, STEP = S::STEP;
+    constexpr int ZB = NB == 3 ? 4 : NB;                               // places of a k8 operand for the blocks' zeros
     extern __shared__ __align__(128) char smem[];
     uint2 *const qf = (uint2 *)(smem + S::BODY);                       // [block][half][nt][part][lane]
     float *const qsum = (float *)(smem + S::BODY + S::QF);             // [block][col]
     float *const qscale = qsum + NB * COLS;                            // [col]
     int2 *const qrow = (int2 *)(qscale + COLS);                        // [col] row and head
     int *const qpos = (int *)(qrow + COLS);                            // [col]
+    uint32_t *const qz = (uint32_t *)(qpos + COLS);                    // [nt][lane]: sums of q as B operands (not HL)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 
     release_dependents();
@@ -183,6 +205,9 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     }
     const char *from_next = tile_at(next);
 
+    if (!HL)
+        for (int i = threadIdx.x; i < NT * 32; i += 32 * W) qz[i] = 0;
+    if (!HL) __syncthreads();
     // The queries: rotated, brought to the f16 range, in the B operand's order.
     for (int col = warp; col < COLS; col += W) {
         const bool have = col < ncol;
@@ -202,8 +227,8 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
             mag = max(mag, __float_as_uint(v[b]) & 0x7fffffffu);
         }
         mag = __reduce_max_sync(0xffffffffu, mag);
-        int e = 0;                                                     // |q| 2^e < 2^11
-        if (mag != 0 && mag < 0x7f800000u) e = 10 - ((int)(mag >> 23) - 127);
+        int e = 0;                                                     // |q| 2^e < 2^11, or 2^15 for one part
+        if (mag != 0 && mag < 0x7f800000u) e = (HL ? 10 : 14) - ((int)(mag >> 23) - 127);
         e = e < -100 ? -100 : e > 100 ? 100 : e;
         if (lane == 0) {
             qscale[col] = fmul(a.scale_log2e, pow2i(24 - e));
@@ -219,6 +244,12 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane == 0) qsum[b * COLS + col] = fmul(sum, 0x1p-24f);
+            if (!HL && lane < 2) {                                     // k = b its f16 part, k = ZB + b the rest
+                const float z = fmul(sum, 0x1p-24f);
+                const __half part = __float2half_rn(z);
+                const int k = b + lane * ZB;
+                ((__half *)(qz + (col >> 3) * 32 + 4 * (col & 7) + (k >> 1)))[k & 1] = lane ? __float2half_rn(z - __half2float(part)) : part;
+            }
             // dimension 8 c' + i of the block: nibble i -> k half (i >> 1) & 1, register i & 1, f16 half i >> 2
             const int i = lane & 7, cc = lane >> 3;
             const float unit = (i & 1) ? 0.0625f : 1.0f;
@@ -230,7 +261,8 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     }
     __syncthreads();
 
-    float ref[NT][2], l[NT][2], o[NB][2][NT][4], oz[NB][NT][2];
+    constexpr int OZ = HL ? NB : 1;                                    // sums of zeros: by block, or rows g of one operand
+    float ref[NT][2], l[NT][2], o[NB][2][NT][4], oz[OZ][NT][2];
     float f[NT][2];
     int pos[NT][2];
     int lift = 15;                                                     // k: the same for all columns
@@ -249,7 +281,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            oz[b][nt][0] = oz[b][nt][1] = 0.0f;
+            oz[b % OZ][nt][0] = oz[b % OZ][nt][1] = 0.0f;
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -271,12 +303,40 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
 #pragma unroll
         for (int s = 0; s + 1 < ST; ++s) held[s] = held[s + 1];
         const char *const buf = ring + stage * S::STAGE;
-        const bool edge = (step + 1) * STEP > first + 1 || whole != 0xffffffffu;
+        const bool at_edge = (step + 1) * STEP > first + 1 || whole != 0xffffffffu;
 
-#pragma unroll 1
-        for (int sub = 0; sub < TILES; sub += MT) {
+        // EDGE: some position of the step is past the end, masked for some row, or has no page.
+        auto body = [&](auto edge_tag, int sub) {
+            constexpr bool EDGE = decltype(edge_tag)::value;
             const char *const tiles = buf + sub * 20 * D;
+            const int t0 = step * STEP + sub * KV4_TILE + g;           // the lane's positions: t0 + 16 mt + 8 k
+            // Whether there is anything at position t0 - g + i of tile mt.
+            auto there = [&](int mt, int i) { return (whole >> (sub + mt) & 1) != 0 && t0 - g + 16 * mt + i < end; };
             float sc[MT][NT][4];
+            if constexpr (!HL) {
+                // Scores begin with the zeros' part.
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t z0, z1;                                   // zeros of positions g and 8 + g, blocks 2 c and 2 c + 1
+                    const uint32_t *const par = (const uint32_t *)(tiles + mt * 20 * D + 8 * D) + g * NB * 2;
+                    if constexpr (NB == 1) {
+                        const uint2 w = *(const uint2 *)par;
+                        z0 = __byte_perm(w.x, w.x, 0x3232);
+                        z1 = __byte_perm(w.y, w.y, 0x3232);
+                    } else {
+                        const int b = NB == 2 ? 0 : 2 * (c & 1);
+                        const uint2 w = *(const uint2 *)(par + b * 2);
+                        const uint2 v = NB == 3 && b == 2 ? make_uint2(0, 0) : *(const uint2 *)(par + (NB == 3 && b == 2 ? 0 : b + 1) * 2);
+                        z0 = __byte_perm(w.x, v.x, 0x7632);
+                        z1 = __byte_perm(w.y, v.y, 0x7632);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.0f;
+                        mma_f16_k8(sc[mt][nt], z0, z1, qz[nt * 32 + lane]);
+                    }
+                }
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 uint32_t ka[MT][2][4];
@@ -297,37 +357,41 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
                     const uint2 *const qb = qf + (b * 2 * NT + nt) * S::PARTS * 32 + lane;
                     const uint2 q0 = qb[0], q1 = qb[NT * S::PARTS * 32];
                     const uint2 r0 = HL ? qb[32] : q0, r1 = HL ? qb[NT * S::PARTS * 32 + 32] : q1;
-                    const float2 zs = *(const float2 *)(qsum + b * COLS + 8 * nt + 2 * c);
+                    const float2 zs = HL ? *(const float2 *)(qsum + b * COLS + 8 * nt + 2 * c) : make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
                         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         mma_f16(acc, ka[mt][0], q0);
                         mma_f16(acc, ka[mt][1], q1);
-                        if (HL) {
+                        const uint2 par = *(const uint2 *)(tiles + mt * 20 * D + 8 * D + kv4_param_word(NB, b, g) * 4);
+                        float *const s = sc[mt][nt];
+                        if constexpr (HL) {
                             float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             mma_f16(low, ka[mt][0], r0);
                             mma_f16(low, ka[mt][1], r1);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) acc[e] = __fmaf_rn(low[e], 0x1p-11f, acc[e]);
+                            const float2 p0 = unpack_f16(par.x), p1 = unpack_f16(par.y);     // (scale, zero)
+                            s[0] = __fmaf_rn(p0.x, acc[0], b ? __fmaf_rn(p0.y, zs.x, s[0]) : fmul(p0.y, zs.x));
+                            s[1] = __fmaf_rn(p0.x, acc[1], b ? __fmaf_rn(p0.y, zs.y, s[1]) : fmul(p0.y, zs.y));
+                            s[2] = __fmaf_rn(p1.x, acc[2], b ? __fmaf_rn(p1.y, zs.x, s[2]) : fmul(p1.y, zs.x));
+                            s[3] = __fmaf_rn(p1.x, acc[3], b ? __fmaf_rn(p1.y, zs.y, s[3]) : fmul(p1.y, zs.y));
+                        } else {
+                            const float p0 = unpack_f16(par.x).x, p1 = unpack_f16(par.y).x;
+                            s[0] = __fmaf_rn(p0, acc[0], s[0]);
+                            s[1] = __fmaf_rn(p0, acc[1], s[1]);
+                            s[2] = __fmaf_rn(p1, acc[2], s[2]);
+                            s[3] = __fmaf_rn(p1, acc[3], s[3]);
                         }
-                        const uint2 par = *(const uint2 *)(tiles + mt * 20 * D + 8 * D + kv4_param_word(NB, b, g) * 4);
-                        const float2 p0 = unpack_f16(par.x), p1 = unpack_f16(par.y);     // (scale, zero)
-                        float *const s = sc[mt][nt];
-                        s[0] = __fmaf_rn(p0.x, acc[0], b ? __fmaf_rn(p0.y, zs.x, s[0]) : fmul(p0.y, zs.x));
-                        s[1] = __fmaf_rn(p0.x, acc[1], b ? __fmaf_rn(p0.y, zs.y, s[1]) : fmul(p0.y, zs.y));
-                        s[2] = __fmaf_rn(p1.x, acc[2], b ? __fmaf_rn(p1.y, zs.x, s[2]) : fmul(p1.y, zs.x));
-                        s[3] = __fmaf_rn(p1.x, acc[3], b ? __fmaf_rn(p1.y, zs.y, s[3]) : fmul(p1.y, zs.y));
                     }
                 }
             }
-            const int t0 = step * STEP + sub * KV4_TILE + g;       // the lane's positions: t0 + 16 mt + 8 k
-            // The values' parameters, and the lift that their largest scale allows.
+            // The values' parameters of positions g and 8 + g, and the lift that their largest scale allows.
             auto value_params = [&](int mt, int b) {
                 uint2 w = *(const uint2 *)(tiles + mt * 20 * D + 18 * D + kv4_param_word(NB, b, g) * 4);
-                if (edge) {                                            // past the end: whatever was there before
-                    const bool there = (whole >> (sub + mt) & 1) != 0;
-                    if (!there || t0 + 16 * mt >= end) w.x = 0;
-                    if (!there || t0 + 16 * mt + 8 >= end) w.y = 0;
+                if (EDGE) {                                            // past the end: whatever was there before
+                    if (!there(mt, g)) w.x = 0;
+                    if (!there(mt, 8 + g)) w.y = 0;
                 }
                 return w;
             };
@@ -337,7 +401,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const uint2 w = value_params(mt, b);
-                    big = __vmaxu2(big, __vmaxu2(w.x, w.y));
+                    big = max_f16x2(big, max_f16x2(w.x, w.y));         // a NaN is passed over
                 }
             big = __reduce_max_sync(0xffffffffu, big & 0x7fffu);       // scales are not negative; below 2^(exponent + 1)
             lift = min(lift, max(29 - (int)(big >> 10), -1));
@@ -350,12 +414,11 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     seen[mt][nt] = 15u;
-                    if (edge) {                                        // masked scores are -inf
-                        const bool there = (whole >> (sub + mt) & 1) != 0;
+                    if (EDGE) {                                        // masked scores are -inf
                         uint32_t ok = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const bool in = there && t0 + 16 * mt + 8 * (e >> 1) <= pos[nt][e & 1];
+                            const bool in = (whole >> (sub + mt) & 1) != 0 && t0 + 16 * mt + 8 * (e >> 1) <= pos[nt][e & 1];
                             if (in) ok |= 1u << e;
                             else sc[mt][nt][e] = -INFINITY;
                         }
@@ -386,13 +449,47 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
                 }
             }
             // P V, block by block.
+            uint2 ph[MT][NT];                                          // not HL: p as B operands, positions 2 c, 2 c + 1, ..
+            if constexpr (!HL) {
+                float zacc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) zacc[nt][0] = zacc[nt][1] = zacc[nt][2] = zacc[nt][3] = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    // Rows b: the zeros of block b, rows 4 + b: its scales, at positions 2 c, 2 c + 1, 8 + 2 c, 8 + 2 c + 1.
+                    const uint32_t *const par = (const uint32_t *)(tiles + mt * 20 * D + 18 * D) + (2 * c * NB + (g & 3)) * 2;
+                    const bool row = NB == 4 || (g & 3) < NB;
+                    uint2 w = row ? *(const uint2 *)par : make_uint2(0, 0), v = row ? *(const uint2 *)(par + 2 * NB) : make_uint2(0, 0);
+                    if (EDGE) {                                        // nothing there, or a NaN: that is dealt with below
+                        if (!there(mt, 2 * c) || nan_params(w.x)) w.x = 0;
+                        if (!there(mt, 8 + 2 * c) || nan_params(w.y)) w.y = 0;
+                        if (!there(mt, 2 * c + 1) || nan_params(v.x)) v.x = 0;
+                        if (!there(mt, 9 + 2 * c) || nan_params(v.y)) v.y = 0;
+                    }
+                    const uint32_t pick = g < 4 ? 0x7632 : 0x5410;
+                    const uint32_t za[4] = {__byte_perm(w.x, v.x, pick), 0, __byte_perm(w.y, v.y, pick), 0};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        ph[mt][nt] = make_uint2(transpose_8x8(pack_f16(sc[mt][nt][0], sc[mt][nt][1])),
+                                                transpose_8x8(pack_f16(sc[mt][nt][2], sc[mt][nt][3])));
+                        mma_f16(zacc[nt], za, ph[mt][nt]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    oz[0][nt][0] = __fmaf_rn(oz[0][nt][0], alpha[nt][0], zacc[nt][0]);
+                    oz[0][nt][1] = __fmaf_rn(oz[0][nt][1], alpha[nt][1], zacc[nt][1]);
+                }
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 float acc[2][NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    oz[b][nt][0] = fmul(oz[b][nt][0], alpha[nt][0]);
-                    oz[b][nt][1] = fmul(oz[b][nt][1], alpha[nt][1]);
+                    if (HL) {
+                        oz[b % OZ][nt][0] = fmul(oz[b % OZ][nt][0], alpha[nt][0]);
+                        oz[b % OZ][nt][1] = fmul(oz[b % OZ][nt][1], alpha[nt][1]);
+                    }
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -410,36 +507,65 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
                         va[k][2] = centred(y & 0x000f000fu, CODE_LOW);
                         va[k][3] = centred(y & 0x00f000f0u, CODE_HIGH);
                     }
-                    const uint2 vp = value_params(mt, b);
-                    float2 par[2] = {unpack_f16(vp.x), unpack_f16(vp.y)};   // (scale, zero)
-                    par[0].y = __fmaf_rn(7.5f, par[0].x, par[0].y);
-                    par[1].y = __fmaf_rn(7.5f, par[1].x, par[1].y);
+                    if constexpr (HL) {
+                        const uint2 vp = value_params(mt, b);
+                        float2 par[2] = {unpack_f16(vp.x), unpack_f16(vp.y)};   // (scale, zero)
+                        par[0].y = __fmaf_rn(7.5f, par[0].x, par[0].y);
+                        par[1].y = __fmaf_rn(7.5f, par[1].x, par[1].y);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        uint2 hi, lo;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float *const z = oz[b % OZ][nt];
+                            uint2 hi, lo;
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float p0 = sc[mt][nt][2 * k], p1 = sc[mt][nt][2 * k + 1];
-                            float x0 = fmul(p0, par[k].x), x1 = fmul(p1, par[k].x);
-                            float y0 = __fmaf_rn(p0, par[k].y, oz[b][nt][0]), y1 = __fmaf_rn(p1, par[k].y, oz[b][nt][1]);
-                            if (edge) {                                // a masked position counts for nothing, NaN or not
-                                if (!(seen[mt][nt] >> (2 * k) & 1)) x0 = 0.0f, y0 = oz[b][nt][0];
-                                if (!(seen[mt][nt] >> (2 * k + 1) & 1)) x1 = 0.0f, y1 = oz[b][nt][1];
-                            }
-                            oz[b][nt][0] = y0;
-                            oz[b][nt][1] = y1;
-                            const uint32_t h = pack_f16(x0, x1);
-                            (k ? hi.y : hi.x) = transpose_8x8(h);
-                            if (HL) {
+                            for (int k = 0; k < 2; ++k) {
+                                const float p0 = sc[mt][nt][2 * k], p1 = sc[mt][nt][2 * k + 1];
+                                float x0 = fmul(p0, par[k].x), x1 = fmul(p1, par[k].x);
+                                float y0 = __fmaf_rn(p0, par[k].y, z[0]), y1 = __fmaf_rn(p1, par[k].y, z[1]);
+                                if (EDGE) {                            // a masked position counts for nothing, NaN or not
+                                    if (!(seen[mt][nt] >> (2 * k) & 1)) x0 = 0.0f, y0 = z[0];
+                                    if (!(seen[mt][nt] >> (2 * k + 1) & 1)) x1 = 0.0f, y1 = z[1];
+                                }
+                                z[0] = y0;
+                                z[1] = y1;
+                                const uint32_t h = pack_f16(x0, x1);
+                                (k ? hi.y : hi.x) = transpose_8x8(h);
                                 const float2 back = unpack_f16(h);
                                 (k ? lo.y : lo.x) = transpose_8x8(pack_f16(x0 - back.x, x1 - back.y));
                             }
-                        }
-                        mma_f16(acc[0][nt], va[0], hi);
-                        mma_f16(acc[1][nt], va[1], hi);
-                        if (HL) {
+                            mma_f16(acc[0][nt], va[0], hi);
+                            mma_f16(acc[1][nt], va[1], hi);
                             mma_f16(acc[0][nt], va[0], lo);
                             mma_f16(acc[1][nt], va[1], lo);
+                        }
+                    } else {
+                        const uint32_t *const par = (const uint32_t *)(tiles + mt * 20 * D + 18 * D) + (2 * c * NB + b) * 2;
+                        uint2 even = *(const uint2 *)par, odd = *(const uint2 *)(par + 2 * NB);
+                        if (EDGE) {
+                            if (!there(mt, 2 * c) || nan_params(even.x)) even.x = 0;
+                            if (!there(mt, 8 + 2 * c) || nan_params(even.y)) even.y = 0;
+                            if (!there(mt, 2 * c + 1) || nan_params(odd.x)) odd.x = 0;
+                            if (!there(mt, 9 + 2 * c) || nan_params(odd.y)) odd.y = 0;
+                        }
+                        const uint32_t s0 = __byte_perm(even.x, odd.x, 0x5410), s1 = __byte_perm(even.y, odd.y, 0x5410);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint2 x = make_uint2(mul_f16x2(ph[mt][nt].x, s0), mul_f16x2(ph[mt][nt].y, s1));
+                            mma_f16(acc[0][nt], va[0], x);
+                            mma_f16(acc[1][nt], va[1], x);
+                        }
+                    }
+                    if (EDGE && !HL) {                                 // a NaN's columns that see its position
+                        const uint2 vp = value_params(mt, b);
+                        const bool nan0 = nan_params(vp.x), nan1 = nan_params(vp.y);
+                        if (__any_sync(0xffffffffu, nan0 || nan1)) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const bool hit = (nan0 && (seen[mt][nt] >> e & 1)) || (nan1 && (seen[mt][nt] >> (2 + e) & 1));
+                                    if (__ballot_sync(0xffffffffu, hit) & (0x11111111u << c))
+                                        acc[0][nt][e] = acc[0][nt][2 + e] = acc[1][nt][e] = acc[1][nt][2 + e] = __uint_as_float(0x7fc00000u);
+                                }
                         }
                     }
                 }
@@ -451,6 +577,11 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
                         for (int e = 0; e < 4; ++e)
                             o[b][k][nt][e] = __fmaf_rn(o[b][k][nt][e], alpha[nt][e & 1], acc[k][nt][e]);
             }
+        };
+#pragma unroll 1
+        for (int sub = 0; sub < TILES; sub += MT) {
+            if (at_edge) body(std::true_type{}, sub);
+            else body(std::false_type{}, sub);
         }
         __syncwarp();
         stage = stage + 1 == ST ? 0 : stage + 1;
@@ -471,9 +602,14 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
             const int col = 8 * nt + 2 * c + e;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float z = oz[b][nt][e];
+                float z;
+                if (HL) {
+                    z = oz[b % OZ][nt][e];
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+                    for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+                } else {                                               // rows b and 4 + b: of the zeros and of the scales
+                    z = __fmaf_rn(7.5f, __shfl_sync(0xffffffffu, oz[0][nt][e], 4 * (4 + b) + c), __shfl_sync(0xffffffffu, oz[0][nt][e], 4 * b + c));
+                }
                 float4 v;                                              // 2^9: the codes' unit
                 v.x = __fmaf_rn(o[b][0][nt][e], 512.0f, z);
                 v.y = __fmaf_rn(o[b][0][nt][2 + e], 512.0f, z);
