@@ -126,7 +126,7 @@ struct Kv4AttnShape {
     static constexpr int BODY = RING > MERGE ? RING : MERGE;
     static constexpr int QF = NB * 2 * NT * PARTS * 32 * 8;
     static constexpr int SMEM = BODY + QF + COLS * (NB + 4) * 4 + NT * 32 * 4;
-    static constexpr int CTAS = NT == 1 ? 16 / W : 8 / W;              // wanted on an SM
+    static constexpr int CTAS = (NT == 1 ? 16 : 8) / W;              // wanted on an SM
 };
 
 template <int D, int NT, bool HL, int W, int ST>
@@ -163,6 +163,94 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     const int steps = min((end + STEP - 1) / STEP, a.splits * a.chunk);   // no more than the call provides for
     const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;
     if (split >= active) return;
+
+    // The queries of a column: what they are made of, on its way before the tables of pages are looked at ..
+    struct Query {
+        float x[NB], y[NB], cos[NB], sin[NB];                          // the values, their partners, the angles
+        int row, h, pos;
+        bool known;
+    };
+    auto load_query = [&](int col) {
+        Query q;
+        const bool have = col < ncol;
+        const int r = have ? (col0 + col) / a.group : 0;
+        q.row = row0 + r;
+        q.h = head * a.group + (have ? col0 + col - r * a.group : 0);
+        q.pos = have ? length - nr + r : -1;
+        q.known = q.pos >= 0 && (!a.cos_tab || q.pos < a.positions);
+        if (q.pos >= 0 && !q.known && a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)seq);
+        const int64_t at = q.row * a.q_stride + (int64_t)q.h * D;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int i = 32 * b + lane;
+            q.x[b] = q.known ? kv_load(a.q, at + i, a.type) : 0.0f;
+            q.y[b] = q.cos[b] = q.sin[b] = 0.0f;
+            if (q.known && a.cos_tab) {
+                q.y[b] = kv_load(a.q, at + (i < D / 2 ? i + D / 2 : i - D / 2), a.type);
+                q.cos[b] = a.cos_tab[(int64_t)q.pos * (D / 2) + (i < D / 2 ? i : i - D / 2)];
+                q.sin[b] = a.sin_tab[(int64_t)q.pos * (D / 2) + (i < D / 2 ? i : i - D / 2)];
+            }
+        }
+        return q;
+    };
+    // .. and then: rotated, brought to the f16 range, in the B operand's order.
+    auto put_query = [&](int col, const Query &q) {
+        float v[NB];
+        uint32_t mag = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int i = 32 * b + lane;
+            v[b] = q.x[b];
+            if (a.cos_tab)
+                v[b] = i < D / 2 ? fsub(fmul(q.x[b], q.cos[b]), fmul(q.y[b], q.sin[b])) : fadd(fmul(q.x[b], q.cos[b]), fmul(q.y[b], q.sin[b]));
+            mag = max(mag, __float_as_uint(v[b]) & 0x7fffffffu);
+        }
+        mag = __reduce_max_sync(0xffffffffu, mag);
+        int e = 0;                                                     // |q| 2^e < 2^11, or 2^15 for one part
+        if (mag != 0 && mag < 0x7f800000u) e = (HL ? 10 : 14) - ((int)(mag >> 23) - 127);
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        if (lane == 0) {
+            qscale[col] = fmul(a.scale_log2e, pow2i(24 - e));
+            qrow[col] = make_int2(q.row, q.h);
+            qpos[col] = q.known ? q.pos : -1;
+        }
+        const bool bad = mag >= 0x7f800000u;                           // an infinity or a NaN: it has to show in the sums too
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float x = fmul(v[b], pow2i(e));
+            const float hi = HL ? rintf(x) : __half2float(__float2half_rn(x));
+            const float lo = HL ? rintf(fmul(x - hi, 2048.0f)) : 0.0f;
+            // The block's sum: of whole numbers, at most 2^11 and 2^10, or 2^24 for x in steps of 2^-9.
+            float sum;
+            if (HL) {
+                const int high = __reduce_add_sync(0xffffffffu, (int)hi), low = __reduce_add_sync(0xffffffffu, (int)lo);
+                sum = __fmaf_rn((float)low, 0x1p-11f, (float)high);
+            } else {
+                sum = fmul((float)__reduce_add_sync(0xffffffffu, __float2int_rn(fmul(x, 512.0f))), 0x1p-9f);
+            }
+            if (bad) sum = __uint_as_float(0x7fc00000u);
+            if (lane == 0) qsum[b * COLS + col] = fmul(sum, 0x1p-24f);
+            if (!HL && lane < 2) {                                     // k = b its f16 part, k = ZB + b the rest
+                const float z = fmul(sum, 0x1p-24f);
+                const __half part = __float2half_rn(z);
+                const int k = b + lane * ZB;
+                ((__half *)(qz + (col >> 3) * 32 + 4 * (col & 7) + (k >> 1)))[k & 1] = lane ? __float2half_rn(z - __half2float(part)) : part;
+            }
+            // dimension 8 c' + i of the block: nibble i -> k half (i >> 1) & 1, register i & 1, f16 half i >> 2
+            const int i = lane & 7, cc = lane >> 3;
+            const float unit = (i & 1) ? 0.0625f : 1.0f;
+            const int at = (((b * 2 + ((i >> 1) & 1)) * NT + (col >> 3)) * S::PARTS) * 32 + 4 * (col & 7) + cc;
+            __half *const to = (__half *)(qf + at) + (i & 1) * 2 + (i >> 2);
+            *to = __float2half_rn(fmul(hi, unit));
+            if (HL) to[32 * 4] = __float2half_rn(fmul(lo, unit));
+        }
+    };
+    constexpr int OWN = COLS / W > 0 ? COLS / W : 1;                   // columns of a warp
+    Query ahead[OWN < 2 ? OWN : 2];
+    if (warp < COLS) {
+        ahead[0] = load_query(warp);
+        if (OWN > 1) ahead[OWN > 1] = load_query(warp + W);
+    }
 
     char *const ring = smem + warp * ST * S::STAGE;
     const int step0 = split * a.chunk + warp, step_end = min(steps, split * a.chunk + a.chunk);
@@ -205,58 +293,24 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     }
     const char *from_next = tile_at(next);
 
-    if (!HL)
+    if (!HL) {                                                         // the places of no block
         for (int i = threadIdx.x; i < NT * 32; i += 32 * W) qz[i] = 0;
-    if (!HL) __syncthreads();
-    // The queries: rotated, brought to the f16 range, in the B operand's order.
-    for (int col = warp; col < COLS; col += W) {
-        const bool have = col < ncol;
-        const int r = have ? (col0 + col) / a.group : 0;
-        const int64_t row = row0 + r;
-        const int h = head * a.group + (have ? col0 + col - r * a.group : 0);
-        const int pos = have ? length - nr + r : -1;
-        const bool known = have && pos >= 0 && (!a.cos_tab || pos < a.positions);
-        if (have && pos >= 0 && !known && a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)seq);
-        float v[NB];
-        uint32_t mag = 0;
+        __syncthreads();
+    }
+    if (warp < COLS) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            v[b] = known ? kv4_rotated(a.q, row * a.q_stride + (int64_t)h * D, 32 * b + lane, D, a.type, a.cos_tab,
-                                       a.sin_tab, pos)
-                         : 0.0f;
-            mag = max(mag, __float_as_uint(v[b]) & 0x7fffffffu);
-        }
-        mag = __reduce_max_sync(0xffffffffu, mag);
-        int e = 0;                                                     // |q| 2^e < 2^11, or 2^15 for one part
-        if (mag != 0 && mag < 0x7f800000u) e = (HL ? 10 : 14) - ((int)(mag >> 23) - 127);
-        e = e < -100 ? -100 : e > 100 ? 100 : e;
-        if (lane == 0) {
-            qscale[col] = fmul(a.scale_log2e, pow2i(24 - e));
-            qrow[col] = make_int2(row0 + r, h);
-            qpos[col] = known ? pos : -1;
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float x = fmul(v[b], pow2i(e));
-            float hi = HL ? rintf(x) : __half2float(__float2half_rn(x));
-            const float lo = HL ? rintf(fmul(x - hi, 2048.0f)) : 0.0f;
-            float sum = HL ? __fmaf_rn(lo, 0x1p-11f, hi) : x;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) qsum[b * COLS + col] = fmul(sum, 0x1p-24f);
-            if (!HL && lane < 2) {                                     // k = b its f16 part, k = ZB + b the rest
-                const float z = fmul(sum, 0x1p-24f);
-                const __half part = __float2half_rn(z);
-                const int k = b + lane * ZB;
-                ((__half *)(qz + (col >> 3) * 32 + 4 * (col & 7) + (k >> 1)))[k & 1] = lane ? __float2half_rn(z - __half2float(part)) : part;
+        for (int k = 0; k < OWN; k += 2) {
+            Query more[2];
+            if (k + 2 < OWN) {
+                more[0] = load_query(warp + (k + 2) * W);
+                more[1] = load_query(warp + (k + 3) * W);
             }
-            // dimension 8 c' + i of the block: nibble i -> k half (i >> 1) & 1, register i & 1, f16 half i >> 2
-            const int i = lane & 7, cc = lane >> 3;
-            const float unit = (i & 1) ? 0.0625f : 1.0f;
-            const int64_t at = (((b * 2 + ((i >> 1) & 1)) * NT + (col >> 3)) * S::PARTS) * 32 + 4 * (col & 7) + cc;
-            __half *const to = (__half *)(qf + at) + (i & 1) * 2 + (i >> 2);
-            *to = __float2half_rn(fmul(hi, unit));
-            if (HL) to[32 * 4] = __float2half_rn(fmul(lo, unit));
+            put_query(warp + k * W, ahead[0]);
+            if (OWN > 1) put_query(warp + (k + 1) * W, ahead[OWN > 1]);
+            if (k + 2 < OWN) {
+                ahead[0] = more[0];
+                ahead[OWN > 1] = more[1];
+            }
         }
     }
     __syncthreads();
@@ -590,8 +644,10 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     __syncthreads();
 
     // The warps' parts meet: [warp][col][D] values, then [warp][col] (reference, sum).
+    const int busy = max(1, min(W, step_end - split * a.chunk));       // warps that had a step
     float *const mo = (float *)smem;
     float2 *const ml = (float2 *)(mo + W * COLS * D);
+    if (warp < busy) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -619,6 +675,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
             }
             if (g == 0) ml[warp * COLS + col] = make_float2(ref[nt][e], sum);
         }
+    }
     __syncthreads();
 
     // Four dimensions of a column to a thread; weights of the parts relative to their largest reference.
@@ -642,24 +699,21 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     };
     for (int at = threadIdx.x; at < ncol * (D / 4); at += 32 * W) {
         const int col = at / (D / 4), i = at % (D / 4) * 4;
-        float2 rl[W];
         float base = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            rl[w] = ml[w * COLS + col];
-            base = fmaxf(base, rl[w].x);
-        }
+#pragma unroll 4
+        for (int w = 0; w < busy; ++w) base = fmaxf(base, ml[w * COLS + col].x);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float x = rl[w].x == -INFINITY ? 0.0f : fast_exp2(rl[w].x - base);
+#pragma unroll 4
+        for (int w = 0; w < busy; ++w) {
+            const float2 rl = ml[w * COLS + col];
+            const float x = rl.x == -INFINITY ? 0.0f : fast_exp2(rl.x - base);
             const float4 y = *(const float4 *)(mo + (w * COLS + col) * D + i);
             v.x = __fmaf_rn(y.x, x, v.x);
             v.y = __fmaf_rn(y.y, x, v.y);
             v.z = __fmaf_rn(y.z, x, v.z);
             v.w = __fmaf_rn(y.w, x, v.w);
-            sum = __fmaf_rn(rl[w].y, x, sum);
+            sum = __fmaf_rn(rl.y, x, sum);
         }
         if (alone) {
             finish(col, i, v, sum, base);
@@ -684,18 +738,33 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
         const int col = at / (D / 4), i = at % (D / 4) * 4;
         float base = -INFINITY, sum = 0.0f;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int s = 0; s < active; ++s) {
-            const float *const p = parts + (int64_t)s * (COLS * (D + 2));
-            const float2 rl = __ldcg((const float2 *)(p + COLS * D + 2 * col));
-            const float4 y = __ldcg((const float4 *)(p + col * D + i));
-            const float to = fmaxf(base, rl.x);
-            const float x = rl.x == -INFINITY ? 0.0f : fast_exp2(rl.x - to), old = base == -INFINITY ? 0.0f : fast_exp2(base - to);
-            v.x = __fmaf_rn(v.x, old, fmul(y.x, x));
-            v.y = __fmaf_rn(v.y, old, fmul(y.y, x));
-            v.z = __fmaf_rn(v.z, old, fmul(y.z, x));
-            v.w = __fmaf_rn(v.w, old, fmul(y.w, x));
-            sum = __fmaf_rn(sum, old, fmul(rl.y, x));
+        for (int s0 = 0; s0 < active; s0 += 8) {                       // eight parts' loads at a time
+            float2 rl[8];
+            float4 y[8];
+            float to = base;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float *const p = parts + (int64_t)min(s0 + k, active - 1) * (COLS * (D + 2));
+                rl[k] = __ldcg((const float2 *)(p + COLS * D + 2 * col));
+                y[k] = __ldcg((const float4 *)(p + col * D + i));
+                if (s0 + k >= active) rl[k] = make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to = fmaxf(to, rl[k].x);
+            const float old = base == -INFINITY ? 0.0f : fast_exp2(base - to);
+            v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+            sum *= old;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float x = rl[k].x == -INFINITY ? 0.0f : fast_exp2(rl[k].x - to);
+                if (s0 + k < active) {
+                    v.x = __fmaf_rn(y[k].x, x, v.x);
+                    v.y = __fmaf_rn(y[k].y, x, v.y);
+                    v.z = __fmaf_rn(y[k].z, x, v.z);
+                    v.w = __fmaf_rn(y[k].w, x, v.w);
+                    sum = __fmaf_rn(rl[k].y, x, sum);
+                }
+            }
             base = to;
         }
         finish(col, i, v, sum, base);

@@ -85,26 +85,46 @@ float bits_to_f32(int64_t bits) {
 
 // How a call's work is cut: 8 nt columns and `chunk` steps of positions to a CTA.
 struct AttnPlan {
-    int nt, col_blocks, splits, chunk;
+    int nt, warps, col_blocks, splits, chunk;
     int64_t groups;
 };
 constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: their finish counters lead the scratch
-constexpr int KV4_WARPS = 4, KV4_STAGES = 2;
+constexpr int KV4_STAGES = 2;
 
+// Warps of a CTA and splits of the histories: the cheapest by a model of the measured times, in units of a step on an SM
+// that is full (3.3 us; 16 warps of 8 columns fill it, 8 of more): a CTA starts in about half a step, the join of
+// splits takes another half, wide CTAs lose a little to their barriers.  Few rounds of CTAs count as whole ones, as equal
+// histories take them; for long histories the last CTA's half counts instead, as lengths differ.  Measured: 64
+// sequences of 2048 positions and two heads 12.3 us in 128 CTAs of 16 warps, 14.9 in 512 of four; 128 sequences of 512
+// 8.5 us in 256 CTAs of eight, 11.3 of four, 12.0 of sixteen; 32 of 2048 and 16 heads 33 us in 512 of four, 45 of sixteen.
 AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length) {
-    AttnPlan p;
+    AttnPlan p{};
     const int64_t cols = heads / kv * max_rows;
     p.nt = cols <= 8 ? 1 : cols <= 16 || d > 64 ? 2 : 4;
     p.col_blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
     p.groups = seqs * kv * p.col_blocks;
     const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, steps = std::max<int64_t>(1, (max_length + step - 1) / step);
-    const int64_t target = 148 * 6;
-    int64_t splits = p.groups >= target || p.groups > KV4_COUNTERS || p.groups == 0 ? 1 : target / p.groups;
-    splits = std::max<int64_t>(1, std::min(splits, (steps + KV4_WARPS - 1) / KV4_WARPS));
-    int64_t chunk = (steps + splits - 1) / splits;
-    chunk = (chunk + KV4_WARPS - 1) / KV4_WARPS * KV4_WARPS;
-    p.chunk = (int)chunk;
-    p.splits = (int)((steps + chunk - 1) / chunk);
+    const int64_t most = p.groups > KV4_COUNTERS ? 1 : std::min<int64_t>(64, steps);
+    float best = 0.0f;
+    for (int64_t warps = p.nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
+        const int64_t places = 148 * (p.nt == 1 ? 16 : 8) / warps;
+        for (int64_t splits = 1; splits <= most; ++splits) {
+            const int64_t chunk = (steps + splits - 1) / splits, active = (steps + chunk - 1) / chunk;
+            if (active != splits) continue;                              // as good as fewer
+            const int64_t mine = (chunk + warps - 1) / warps;            // steps of a warp
+            const float rounds = (float)(p.groups * active) / (float)places, whole = (float)((p.groups * active + places - 1) / places);
+            const float work = whole * (float)mine <= 16.0f ? whole * (float)mine : (rounds > 1.0f ? rounds : 1.0f) * (float)mine + 0.5f * (float)mine;
+            const float start = 0.25f + 0.125f * (float)(4 * p.nt) / (float)warps;   // the more queries a warp has to bring
+            const float cost = work * (1.0f + 0.0025f * (float)warps) + start * whole + (active > 1 ? 0.5f + 0.015f * (float)active : 0.0f);
+            if (p.warps == 0 || cost < best) {
+                best = cost;
+                p.warps = (int)warps;
+                p.chunk = (int)chunk;
+                p.splits = (int)active;
+            }
+            if (p.groups * splits > 16 * places) break;
+        }
+    }
     return p;
 }
 
@@ -112,30 +132,31 @@ int64_t kv4_scratch(const AttnPlan &p, int64_t d) {
     return p.splits == 1 ? 256 : 4 * KV4_COUNTERS + p.groups * p.splits * 8 * p.nt * (d + 2) * 4;
 }
 
-template <int D, int NT, bool HL>
+template <int D, int NT, bool HL, int W>
 int32_t launch_kv4_attention_t(cudaStream_t st, const Kv4AttnArgs &a, int64_t ctas) {
-    using S = Kv4AttnShape<D, NT, HL, KV4_WARPS, KV4_STAGES>;
-    auto kernel = kv4_attention_kernel<D, NT, HL, KV4_WARPS, KV4_STAGES>;
+    using S = Kv4AttnShape<D, NT, HL, W, KV4_STAGES>;
+    auto kernel = kv4_attention_kernel<D, NT, HL, W, KV4_STAGES>;
     static std::atomic<uint64_t> allowed{0};
     NC_TRY(allow_smem_once(kernel, S::SMEM, &allowed));
-    CUDA_TRY(launch_k(kernel, (unsigned)ctas, 32 * KV4_WARPS, S::SMEM, st, a));
+    CUDA_TRY(launch_k(kernel, (unsigned)ctas, 32 * W, S::SMEM, st, a));
     return check_launch("kv4_attention_kernel");
 }
 
 template <int D, bool HL>
-int32_t launch_kv4_attention_n(cudaStream_t st, const Kv4AttnArgs &a, int nt, int64_t ctas) {
-    switch (nt) {
-        case 1: return launch_kv4_attention_t<D, 1, HL>(st, a, ctas);
-        case 2: return launch_kv4_attention_t<D, 2, HL>(st, a, ctas);
-        default:
-            if constexpr (D <= 64) return launch_kv4_attention_t<D, 4, HL>(st, a, ctas);
-            return fail(NC_ERR_ARGUMENT, "no kernel of %d columns for head dimension %d", 8 * nt, D);
+int32_t launch_kv4_attention_n(cudaStream_t st, const Kv4AttnArgs &a, const AttnPlan &p, int64_t ctas) {
+    if (p.nt == 1) {
+        if (p.warps == 4) return launch_kv4_attention_t<D, 1, HL, 4>(st, a, ctas);
+        if (p.warps == 8) return launch_kv4_attention_t<D, 1, HL, 8>(st, a, ctas);
+        return launch_kv4_attention_t<D, 1, HL, 16>(st, a, ctas);
     }
+    if (p.nt == 2) return p.warps == 4 ? launch_kv4_attention_t<D, 2, HL, 4>(st, a, ctas) : launch_kv4_attention_t<D, 2, HL, 8>(st, a, ctas);
+    if constexpr (D <= 64) return p.warps == 4 ? launch_kv4_attention_t<D, 4, HL, 4>(st, a, ctas) : launch_kv4_attention_t<D, 4, HL, 8>(st, a, ctas);
+    return fail(NC_ERR_ARGUMENT, "no kernel of %d columns for head dimension %d", 8 * p.nt, D);
 }
 
 template <int D>
-int32_t launch_kv4_attention_d(cudaStream_t st, const Kv4AttnArgs &a, int nt, int64_t ctas) {
-    return a.type != KV_BF16 ? launch_kv4_attention_n<D, true>(st, a, nt, ctas) : launch_kv4_attention_n<D, false>(st, a, nt, ctas);
+int32_t launch_kv4_attention_d(cudaStream_t st, const Kv4AttnArgs &a, const AttnPlan &p, int64_t ctas) {
+    return a.type != KV_BF16 ? launch_kv4_attention_n<D, true>(st, a, p, ctas) : launch_kv4_attention_n<D, false>(st, a, p, ctas);
 }
 
 }  // namespace
@@ -238,10 +259,10 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     if (ctas > I32 || a.at.rows * a.group > I32) return fail(NC_ERR_ARGUMENT, "%lld rows in one call", (long long)a.at.rows);
     const cudaStream_t st = (cudaStream_t)stream;
     switch (a.pool.d) {
-        case 32: return launch_kv4_attention_d<32>(st, a, plan.nt, ctas);
-        case 64: return launch_kv4_attention_d<64>(st, a, plan.nt, ctas);
-        case 96: return launch_kv4_attention_d<96>(st, a, plan.nt, ctas);
-        default: return launch_kv4_attention_d<128>(st, a, plan.nt, ctas);
+        case 32: return launch_kv4_attention_d<32>(st, a, plan, ctas);
+        case 64: return launch_kv4_attention_d<64>(st, a, plan, ctas);
+        case 96: return launch_kv4_attention_d<96>(st, a, plan, ctas);
+        default: return launch_kv4_attention_d<128>(st, a, plan, ctas);
     }
 }
 
