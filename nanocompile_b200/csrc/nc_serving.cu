@@ -113,9 +113,10 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
             if (active != splits) continue;                              // as good as fewer
             const int64_t mine = (chunk + warps - 1) / warps;            // steps of a warp
             const float rounds = (float)(p.groups * active) / (float)places, whole = (float)((p.groups * active + places - 1) / places);
-            const float work = whole * (float)mine <= 16.0f ? whole * (float)mine : (rounds > 1.0f ? rounds : 1.0f) * (float)mine + 0.5f * (float)mine;
+            const bool few = whole * (float)mine <= 16.0f;
+            const float work = few ? whole * (float)mine : (rounds > 1.0f ? rounds : 1.0f) * (float)mine + 0.5f * (float)mine;
             const float start = 0.25f + 0.125f * (float)(4 * p.nt) / (float)warps;   // the more queries a warp has to bring
-            const float cost = work * (1.0f + 0.0025f * (float)warps) + start * whole + (active > 1 ? 0.5f + 0.015f * (float)active : 0.0f);
+            const float cost = work * (1.0f + (few ? 0.0025f : 0.01f) * (float)warps) + start * whole + (active > 1 ? 0.5f + 0.015f * (float)active : 0.0f);
             if (p.warps == 0 || cost < best) {
                 best = cost;
                 p.warps = (int)warps;
