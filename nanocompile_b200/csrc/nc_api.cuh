@@ -13,6 +13,9 @@ namespace nc {
 // Records the message of nc_last_error on this thread and returns `code`.
 __attribute__((visibility("hidden"), format(printf, 2, 3))) int32_t fail(int32_t code, const char *fmt, ...);
 
+// Whether a bounded wait of the serving kernels has run out since the last call (nc_serving.cu).
+__attribute__((visibility("hidden"))) int32_t prompt_fault(bool *fault);
+
 #define CUDA_TRY(expr)                                                                           \
     do {                                                                                         \
         cudaError_t e_ = (expr);                                                                 \

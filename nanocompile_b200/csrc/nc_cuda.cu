@@ -835,7 +835,13 @@ extern "C" int32_t nc_attention_cache(void **p, const int64_t *s, void *stream) 
     return launch_attention((cudaStream_t)stream, a, rows);
 }
 
-extern "C" int32_t nc_device_faults(void) { return check_device_faults(); }
+extern "C" int32_t nc_device_faults(void) {
+    NC_TRY(check_device_faults());
+    bool prompt = false;
+    NC_TRY(prompt_fault(&prompt));
+    if (prompt) return fail(NC_ERR_KERNEL, "4-bit attention: a matrix instruction did not complete within its wait limit");
+    return NC_OK;
+}
 
 extern "C" int32_t nc_set_wait_limit(int64_t cycles) {
     const long long v = cycles > 0 ? (long long)cycles : (1ll << 31);

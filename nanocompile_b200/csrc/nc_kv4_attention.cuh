@@ -115,6 +115,64 @@ __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Four dimensions from i on of a row and head: value / sum; and the log-sum, of sums relative to 2^base.
+template <int D>
+__device__ __forceinline__ void kv4_finish(const Kv4AttnArgs &a, int2 row_head, int i, const float4 &v, float sum, float base) {
+    const float inv = sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
+    const int64_t at = row_head.x * a.out_stride + (int64_t)row_head.y * D + i;
+    if (sum == 0.0f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) kv_store(a.out, at + k, a.type, 0.0f);
+    } else {
+        kv_store(a.out, at, a.type, fmul(v.x, inv));
+        kv_store(a.out, at + 1, a.type, fmul(v.y, inv));
+        kv_store(a.out, at + 2, a.type, fmul(v.z, inv));
+        kv_store(a.out, at + 3, a.type, fmul(v.w, inv));
+    }
+    if (i == 0 && a.lse)
+        a.lse[(int64_t)row_head.x * a.heads + row_head.y] = sum == 0.0f ? -INFINITY : fmul(base + log2f(sum), 0.6931471805599453f);
+}
+
+// Joins the parts of a group's splits, in their order: [active][COLS][D] values, then [COLS] (reference, sum) in each.
+template <int COLS, int D>
+__device__ __forceinline__ void kv4_join(const Kv4AttnArgs &a, const float *parts, int active, int ncol, const int2 *rows) {
+    for (int at = threadIdx.x; at < ncol * (D / 4); at += blockDim.x) {
+        const int col = at / (D / 4), i = at % (D / 4) * 4;
+        float base = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int s0 = 0; s0 < active; s0 += 8) {                       // eight parts' loads at a time
+            float2 rl[8];
+            float4 y[8];
+            float to = base;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float *const p = parts + (int64_t)min(s0 + k, active - 1) * (COLS * (D + 2));
+                rl[k] = __ldcg((const float2 *)(p + COLS * D + 2 * col));
+                y[k] = __ldcg((const float4 *)(p + col * D + i));
+                if (s0 + k >= active) rl[k] = make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to = fmaxf(to, rl[k].x);
+            const float old = base == -INFINITY ? 0.0f : fast_exp2(base - to);
+            v.x *= old, v.y *= old, v.z *= old, v.w *= old;
+            sum *= old;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float x = rl[k].x == -INFINITY ? 0.0f : fast_exp2(rl[k].x - to);
+                if (s0 + k < active) {
+                    v.x = __fmaf_rn(y[k].x, x, v.x);
+                    v.y = __fmaf_rn(y[k].y, x, v.y);
+                    v.z = __fmaf_rn(y[k].z, x, v.z);
+                    v.w = __fmaf_rn(y[k].w, x, v.w);
+                    sum = __fmaf_rn(rl[k].y, x, sum);
+                }
+            }
+            base = to;
+        }
+        kv4_finish<D>(a, rows[col], i, v, sum, base);
+    }
+}
+
 template <int D, int NT, bool HL, int W, int ST>
 struct Kv4AttnShape {
     static constexpr int NB = D / 32, VB = kv4_vb(NB), COLS = 8 * NT, PARTS = HL ? 2 : 1;
@@ -681,22 +739,6 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     // Four dimensions of a column to a thread; weights of the parts relative to their largest reference.
     const bool alone = active == 1;
     float *const part = alone ? nullptr : a.part + ((int64_t)group * a.splits + split) * (COLS * (D + 2));
-    auto finish = [&](int col, int i, const float4 &v, float sum, float base) {
-        const int64_t row = qrow[col].x;
-        const int h = qrow[col].y;
-        const float inv = sum == 0.0f ? 0.0f : fdiv(1.0f, sum);
-        const int64_t at = row * a.out_stride + (int64_t)h * D + i;
-        if (sum == 0.0f) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) kv_store(a.out, at + k, a.type, 0.0f);
-        } else {
-            kv_store(a.out, at, a.type, fmul(v.x, inv));
-            kv_store(a.out, at + 1, a.type, fmul(v.y, inv));
-            kv_store(a.out, at + 2, a.type, fmul(v.z, inv));
-            kv_store(a.out, at + 3, a.type, fmul(v.w, inv));
-        }
-        if (i == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.0f ? -INFINITY : fmul(base + log2f(sum), 0.6931471805599453f);
-    };
     for (int at = threadIdx.x; at < ncol * (D / 4); at += 32 * W) {
         const int col = at / (D / 4), i = at % (D / 4) * 4;
         float base = -INFINITY;
@@ -716,7 +758,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
             sum = __fmaf_rn(rl.y, x, sum);
         }
         if (alone) {
-            finish(col, i, v, sum, base);
+            kv4_finish<D>(a, qrow[col], i, v, sum, base);
         } else {
             *(float4 *)(part + col * D + i) = v;
             if (i == 0) *(float2 *)(part + COLS * D + 2 * col) = make_float2(base, sum);
@@ -733,42 +775,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     if (arrived != (unsigned)active - 1) return;
     __threadfence();
     if (threadIdx.x == 0) a.counter[group] = 0;
-    const float *const parts = a.part + (int64_t)group * a.splits * (COLS * (D + 2));
-    for (int at = threadIdx.x; at < ncol * (D / 4); at += 32 * W) {
-        const int col = at / (D / 4), i = at % (D / 4) * 4;
-        float base = -INFINITY, sum = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int s0 = 0; s0 < active; s0 += 8) {                       // eight parts' loads at a time
-            float2 rl[8];
-            float4 y[8];
-            float to = base;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float *const p = parts + (int64_t)min(s0 + k, active - 1) * (COLS * (D + 2));
-                rl[k] = __ldcg((const float2 *)(p + COLS * D + 2 * col));
-                y[k] = __ldcg((const float4 *)(p + col * D + i));
-                if (s0 + k >= active) rl[k] = make_float2(-INFINITY, 0.0f);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) to = fmaxf(to, rl[k].x);
-            const float old = base == -INFINITY ? 0.0f : fast_exp2(base - to);
-            v.x *= old, v.y *= old, v.z *= old, v.w *= old;
-            sum *= old;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float x = rl[k].x == -INFINITY ? 0.0f : fast_exp2(rl[k].x - to);
-                if (s0 + k < active) {
-                    v.x = __fmaf_rn(y[k].x, x, v.x);
-                    v.y = __fmaf_rn(y[k].y, x, v.y);
-                    v.z = __fmaf_rn(y[k].z, x, v.z);
-                    v.w = __fmaf_rn(y[k].w, x, v.w);
-                    sum = __fmaf_rn(rl[k].y, x, sum);
-                }
-            }
-            base = to;
-        }
-        finish(col, i, v, sum, base);
-    }
+    kv4_join<COLS, D>(a, a.part + (int64_t)group * a.splits * (COLS * (D + 2)), active, ncol, qrow);
 }
 
 }  // namespace nc

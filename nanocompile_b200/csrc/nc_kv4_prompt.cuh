@@ -1,0 +1,540 @@
+// nc_kv4_prompt.cuh -- attention of many bfloat16 rows over a paged 4-bit cache on the tensor cores (tcgen05).
+//
+// What nc_kv4_attention.cuh computes, for prompts: 128 columns (row, head of the group) of one kv head to a CTA, 64
+// positions at a time.  Each tile's keys and values are brought from their codes to f16 in shared memory once for all
+// columns; then S = Q K^T and O += P V are tcgen05.mma kind::f16 with Q, S, P and O in tensor memory (256 columns: Q d / 2,
+// S 64 with P over it, O d), accumulated in float32.  Nothing but the values' rounding to f16 (11 bits, of quantities that
+// have 4) is lost against the products on the codes; float32 rows, which need more, stay with those.
+//
+//   keys    zero + scale * code, with scale and zero times a power of two for each tile, that the scores get back
+//   values  the same with a power of two that only grows, O rescaled when it does: no size of value leaves the f16 range
+//   p       2^(x - ref), ref a past maximum: O and the sums are rescaled only when the maximum has grown by 8
+//
+// Layouts.  An eight-value group of dimensions is held in the order 0 4 1 5 2 6 3 7 that a code word gives, by Q and K
+// alike; the positions of a tile in the order that gives a lane eight of them for one dimension: 32 positions 16 i + 8 j +
+// 2 c + h at place 8 c + 4 i + 2 j + h, by K's rows, P's columns and V alike.  K is [place][d], V [d][place], both with
+// 128-byte swizzled rows.  In writing a quarter of a warp covers all eight 16-byte units, so that it meets no bank twice.
+//
+// The CTA goes step by step -- codes of tile t + 1 on their way, keys of t decoded while O += P V of t - 1 runs, values
+// while S runs -- and a second CTA on the SM fills what is left idle.  Bound by the instruction rate (decoding 17 for eight
+// values, softmax about six a score) against a tensor pipe that would need half of that.
+#pragma once
+
+#include "nc_kv4_attention.cuh"
+
+namespace nc {
+
+constexpr int KVT_COLS = 128, KVT_STEP = 64, KVT_THREADS = 256, KVT_TMEM = 256;
+
+__device__ unsigned int g_prompt_fault;        // set when a matrix instruction's completion never came (bounded wait)
+
+template <int D>
+struct KvtShared {
+    __align__(1024) char k[KVT_STEP * D * 2];  // [d / 64][64 places][128 bytes]
+    __align__(1024) char v[KVT_STEP * D * 2];  // [d][128 bytes]
+    __align__(16) char raw[4 * 20 * D];
+    const char *src[4];                        // the next tile's cache tiles
+    uint64_t s_done, o_done;                   // mbarriers
+    float row_max[2][KVT_COLS], row_sum[2][KVT_COLS];
+    int2 row[KVT_COLS];                        // row, head
+    uint32_t tmem, top[2][4];                  // top: largest key scale, |key zero|, value scale, |value zero| of a tile (bits)
+    uint32_t nan_rows[2];
+    unsigned int arrived;
+};
+
+__device__ __forceinline__ uint32_t kvt_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void kvt_mbar_init(uint64_t *bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(kvt_smem(bar)) : "memory");
+}
+// Whether the phase completes within the bound (about a second).
+__device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity) {
+    const long long start = clock64();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(kvt_smem(bar)), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (clock64() - start > NC_DRAIN_CYCLES) return false;
+    }
+}
+// A K-major operand of 128-byte swizzled rows: eight rows are 1024 bytes.
+__device__ __forceinline__ uint64_t kvt_desc(uint32_t address) {
+    return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// D[128 x N] (+)= A[128 x 16] B[16 x N], A in tensor memory, f16 with float32 sums.
+__device__ __forceinline__ void kvt_mma(uint32_t d, uint32_t a, uint64_t b, int n, bool add) {
+    const uint32_t kind = 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void kvt_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(kvt_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void kvt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void kvt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void kvt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void kvt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void kvt_load32(uint32_t t, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(t));
+}
+__device__ __forceinline__ void kvt_store32(uint32_t t, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void kvt_store16(uint32_t t, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void kvt_store8(uint32_t t, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Pairs of codes as f16: nibbles `low` of each half-word (bits 0-3), or the next ones (4-7).
+__device__ __forceinline__ uint32_t codes_low(uint32_t w) { return add_f16x2((w & 0x000f000fu) | 0x64006400u, 0xe400e400u); }
+__device__ __forceinline__ uint32_t codes_high(uint32_t w) { return fma_f16x2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u); }
+// 2^e as a pair of f16, -14 <= e <= 15.
+__device__ __forceinline__ uint32_t pow2_f16x2(int e) { return (uint32_t)(e + 15) << 10 | (uint32_t)(e + 15) << 26; }
+// The exponent that brings zero + 15 scale below 2^15: parameters are multiplied by 2^-e.  A NaN counts as the largest number.
+__device__ __forceinline__ int kvt_exponent(uint32_t scale, uint32_t zero) {
+    const float s = __half2float(__ushort_as_half((unsigned short)min(scale, 0x7bffu)));
+    const float z = __half2float(__ushort_as_half((unsigned short)min(zero, 0x7bffu)));
+    const float most = __fmaf_rn(15.0f, s, z);
+    const int e = (int)(__float_as_uint(most) >> 23) - 127 - 14;
+    return max(-14, min(14, e));
+}
+
+template <int D>
+__global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    constexpr int NB = D / 32, VB = kv4_vb(NB);
+    static_assert(D == 64 || D == 128, "two blocks of a panel to a warp");
+    extern __shared__ __align__(1024) char kvt_raw[];
+    KvtShared<D> &sh = *reinterpret_cast<KvtShared<D> *>(kvt_raw + ((1024 - (kvt_smem(kvt_raw) & 1023)) & 1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int part = warp >> 2, col = 32 * (warp & 3) + lane;          // the thread's column and half of positions or dimensions
+
+    wait_for_producer();
+    const int split = (int)(blockIdx.x % a.splits);
+    const unsigned group = blockIdx.x / a.splits;
+    const int cb = a.col_blocks - 1 - (int)(group % a.col_blocks);     // the longest histories first
+    const int head = (int)(group / a.col_blocks % a.pool.kv);
+    const int seq = (int)(group / a.col_blocks / a.pool.kv);
+    const int length = a.at.lengths[seq];
+    const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
+    const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;
+    if (row0 < 0 || nr <= 0 || (int64_t)row0 + nr > a.at.rows) return;
+    const int cols = nr * a.group, col0 = cb * KVT_COLS;
+    if (col0 >= cols) return;
+    const int ncol = min(cols - col0, KVT_COLS);
+    const int first = length - nr + col0 / a.group, last = length - nr + (col0 + ncol - 1) / a.group;
+    const int end = last < 0 ? 0 : last + 1;
+    const int steps = min((end + KVT_STEP - 1) / KVT_STEP, a.splits * a.chunk);
+    const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;
+    if (split >= active) return;
+    const int step0 = split * a.chunk, step_end = min(steps, step0 + a.chunk);
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kvt_smem(&sh.tmem)), "n"(KVT_TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        kvt_mbar_init(&sh.s_done);
+        kvt_mbar_init(&sh.o_done);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid < 8) sh.top[tid >> 2][tid & 3] = 0;
+
+    const int tiles_per_page = a.at.page / KV4_TILE;
+    const int32_t *const table = a.at.table + (int64_t)seq * a.at.width;
+    auto find = [&](int step) {                                        // threads 0 .. 3: a cache tile each
+        const int tile = step * 4 + tid;
+        const char *src = nullptr;
+        if (step < step_end && tile * KV4_TILE < end) {
+            const int j = (int)((uint64_t)tile * a.page_magic >> 37);
+            const int page = j < a.at.width ? table[j] : -1;
+            if (page >= 0 && page < a.at.pages)
+                src = a.pool.base + page * a.pool.page_bytes + ((int64_t)head * tiles_per_page + (tile - j * tiles_per_page)) * (20 * D);
+            else if (a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+        }
+        sh.src[tid] = src;
+    };
+    auto issue = [&]() {
+        constexpr int PIECES = 20 * D / 16;
+#pragma unroll
+        for (int i = 0; i < (4 * PIECES + KVT_THREADS - 1) / KVT_THREADS; ++i) {
+            const int q = i * KVT_THREADS + tid, k = q / PIECES;
+            if (q < 4 * PIECES && sh.src[k]) copy16_async(sh.raw + q * 16, sh.src[k] + (q - k * PIECES) * 16);
+        }
+        copies_commit();
+    };
+    if (tid < 4) find(step0);
+    kvt_before();
+    __syncthreads();
+    kvt_after();
+    release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
+    issue();
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;          // the warp's quarter of tensor memory
+    const uint32_t tq = sh.tmem, ts = tq + D / 2, to = ts + KVT_STEP;
+
+    // The queries: dimensions i and i + d / 2 for a quarter of d, rotated, brought to [2^14, 2^15) and put into tensor memory.
+    const bool have = col < ncol;
+    const int r = have ? (col0 + col) / a.group : 0;
+    const int qrow = row0 + r, qhead = head * a.group + (have ? col0 + col - r * a.group : 0);
+    const int qpos = have ? length - nr + r : -1;
+    const bool known = qpos >= 0 && (!a.cos_tab || qpos < a.positions);
+    if (qpos >= 0 && !known && a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+    const int pos = known ? qpos : -1;
+    float f;                                                           // a score's factor, but for the tile's exponent
+    {
+        constexpr int Q = D / 4;
+        float lo[Q], hi[Q];
+        const int64_t at = qrow * a.q_stride + (int64_t)qhead * D + part * Q;
+        float most = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const float x = known ? kv_load(a.q, at + i, KV_BF16) : 0.0f, y = known ? kv_load(a.q, at + i + D / 2, KV_BF16) : 0.0f;
+            lo[i] = x;
+            hi[i] = y;
+            if (known && a.cos_tab) {
+                const float cs = a.cos_tab[(int64_t)qpos * (D / 2) + part * Q + i], sn = a.sin_tab[(int64_t)qpos * (D / 2) + part * Q + i];
+                lo[i] = fsub(fmul(x, cs), fmul(y, sn));
+                hi[i] = fadd(fmul(y, cs), fmul(x, sn));
+            }
+            bad = bad || !(fabsf(lo[i]) < INFINITY) || !(fabsf(hi[i]) < INFINITY);
+            most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+        }
+        sh.row_max[part][col] = bad ? INFINITY : most;
+        if (part == 0) sh.row[col] = make_int2(qrow, qhead);
+        __syncthreads();
+        most = fmaxf(sh.row_max[0][col], sh.row_max[1][col]);
+        const uint32_t bits = __float_as_uint(most);
+        int e = 0;
+        if (bits != 0 && bits < 0x7f800000u) e = 14 - ((int)(bits >> 23) - 127);
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        const float by = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : pow2i(e);     // an infinity or a NaN: all of the row
+        f = fmul(a.scale_log2e, pow2i(-e));
+        uint32_t w[Q / 2];
+        auto put = [&](const float (&x)[Q], uint32_t t) {
+#pragma unroll
+            for (int i = 0; i < Q / 8; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[4 * i + k] = pack_f16(fmul(x[8 * i + k], by), fmul(x[8 * i + k + 4], by));
+            if constexpr (Q == 32) kvt_store16(t, w);
+            else kvt_store8(t, w);
+        };
+        put(lo, tq + lanes + part * (Q / 2));
+        put(hi, tq + lanes + D / 4 + part * (Q / 2));
+        kvt_wait_st();
+    }
+
+    float ref = -INFINITY, sum = 0.0f;                                 // of the thread's half of the positions
+    int ev = -14;                                                      // the values' exponent
+    uint32_t poison = 0;                                               // blocks of dimensions that a NaN reached
+    bool ok = true;
+    unsigned parity = 0;
+    int step = step0;
+    for (; step < step_end; ++step, parity ^= 1) {
+        const int set = step & 1;
+        const bool edge = (step + 1) * KVT_STEP > first + 1;
+        // The tile's codes are here; its parameters' largest.
+        copies_wait<0>();
+        __syncthreads();
+        uint32_t there = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) there |= sh.src[k] ? 1u << k : 0;
+        {
+            uint32_t s[2] = {0, 0}, z[2] = {0, 0};
+            for (int i = tid; i < 4 * 2 * 16 * NB; i += KVT_THREADS) {
+                const int k = i / (2 * 16 * NB), j = i % (2 * 16 * NB), which = j / (16 * NB), word = j % (16 * NB);
+                uint32_t *const at = (uint32_t *)(sh.raw + k * 20 * D + which * 10 * D + 8 * D) + word;
+                const int t = step * KVT_STEP + 16 * k + word / (2 * NB) + 8 * (word & 1);
+                if (!(there >> k & 1) || t >= end) *at = 0;            // whatever was there before
+                const uint32_t w = *at;
+                s[which] = max(s[which], w & 0x7fffu);
+                z[which] = max(z[which], w >> 16 & 0x7fffu);
+            }
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                s[which] = __reduce_max_sync(0xffffffffu, s[which]);
+                z[which] = __reduce_max_sync(0xffffffffu, z[which]);
+                if (lane == 0) {
+                    atomicMax(&sh.top[set][2 * which], s[which]);
+                    atomicMax(&sh.top[set][2 * which + 1], z[which]);
+                }
+            }
+        }
+        if (tid < 4) sh.top[set ^ 1][tid] = 0;
+        __syncthreads();
+        if (tid < 4) find(step + 1);
+        const int ek = kvt_exponent(sh.top[set][0], sh.top[set][1]);
+        const int ev_now = max(ev, kvt_exponent(sh.top[set][2], sh.top[set][3]));
+        const bool nan = sh.top[set][2] > 0x7c00u || sh.top[set][3] > 0x7c00u;
+        // Keys: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half of the lanes).
+        {
+            const int k = warp & 3;
+            const char *const tile = sh.raw + k * 20 * D;
+            const uint32_t unit = pow2_f16x2(-ek);
+#pragma unroll
+            for (int n = 0; n < NB / 2; ++n) {
+                const int b = NB == 4 ? 2 * part + (n ^ (g & 1)) : part ^ (g & 1);
+                const uint2 w = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
+                const uint2 par = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, g));
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
+                    const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
+                    uint4 v;
+                    v.x = fma_f16x2(codes_low(x), s, z);
+                    v.y = fma_f16x2(codes_high(x), s, z);
+                    v.z = fma_f16x2(codes_low(x >> 8), s, z);
+                    v.w = fma_f16x2(codes_high(x >> 8), s, z);
+                    const int place = 32 * (k >> 1) + 8 * (g >> 1) + 4 * (k & 1) + 2 * j + (g & 1);
+                    *(uint4 *)(sh.k + (b >> 1) * (KVT_STEP * 128) + place * 128 + (((4 * (b & 1) + c) ^ (place & 7)) << 4)) = v;
+                }
+            }
+        }
+        // O += P V of the last tile is done: S and the values' buffer are free, and O.
+        if (step > step0) ok = kvt_mbar_wait(&sh.o_done, parity ^ 1);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        kvt_before();
+        if (__syncthreads_or(!ok)) break;
+        kvt_after();
+        if (tid == 0) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                kvt_mma(ts, tq + 8 * k, kvt_desc(kvt_smem(sh.k) + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, k > 0);
+            kvt_commit(&sh.s_done);
+        }
+        // Values: 32 positions `grp`, block b; (d = 64: two of its four dimensions of each lane).
+        {
+            const int grp = NB == 4 ? part : warp >> 1 & 1, b = NB == 4 ? warp & 3 : warp & 1;
+            const uint32_t unit = pow2_f16x2(-ev_now);
+            uint32_t s[4], z[4], w[4];                                 // by (tile, j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const char *const tile = sh.raw + (2 * grp + k) * 20 * D + 10 * D;
+                const uint2 x = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
+                uint2 even = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, 2 * c));
+                uint2 odd = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, 2 * c + 1));
+                if (nan) {                                             // dealt with row by row
+                    if (nan_params(even.x)) even.x = 0;
+                    if (nan_params(even.y)) even.y = 0;
+                    if (nan_params(odd.x)) odd.x = 0;
+                    if (nan_params(odd.y)) odd.y = 0;
+                }
+                w[2 * k] = x.x;
+                w[2 * k + 1] = x.y;
+                s[2 * k] = mul_f16x2(__byte_perm(even.x, odd.x, 0x5410), unit);
+                s[2 * k + 1] = mul_f16x2(__byte_perm(even.y, odd.y, 0x5410), unit);
+                z[2 * k] = mul_f16x2(__byte_perm(even.x, odd.x, 0x7632), unit);
+                z[2 * k + 1] = mul_f16x2(__byte_perm(even.y, odd.y, 0x7632), unit);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (NB == 2 && (i >> 1) != (warp >> 2)) continue;
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t x = i >> 1 ? w[k] >> 8 : w[k];
+                    v[k] = fma_f16x2(i & 1 ? codes_high(x) : codes_low(x), s[k], z[k]);
+                }
+                const int d = 32 * b + 4 * g + i;
+                *(uint4 *)(sh.v + d * 128 + (((4 * grp + c) ^ (d & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        if (nan) {                                                     // which of the thread's rows' positions have one
+            for (int n = 0; n < KVT_STEP; ++n) {
+                if (step * KVT_STEP + n > pos) break;
+                const uint32_t *const par = (const uint32_t *)(sh.raw + (n >> 4) * 20 * D + 18 * D);
+                for (int b = 0; b < NB; ++b)
+                    if (nan_params(par[kv4_param_word(NB, b, n & 15)])) poison |= 1u << b;
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // Softmax of the thread's 32 positions.
+        ok = kvt_mbar_wait(&sh.s_done, parity);
+        if (__syncthreads_or(!ok)) break;                              // the codes are read, too
+        issue();
+        kvt_after();
+        uint32_t x[32];
+        kvt_load32(ts + lanes + 32 * part, x);
+        kvt_wait_ld();
+        const float scale = fmul(f, pow2i(ek));
+        float most = -INFINITY;
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < 32; ++n) {
+                const int t = step * KVT_STEP + 32 * part + 16 * (n >> 2 & 1) + 8 * (n >> 1 & 1) + 2 * (n >> 3) + (n & 1);
+                if (t > pos) x[n] = 0xff800000u;
+            }
+        }
+        if (there != 15u) {
+#pragma unroll
+            for (int n = 0; n < 32; ++n)
+                if (!(there >> (2 * part + (n >> 2 & 1)) & 1)) x[n] = 0xff800000u;
+        }
+#pragma unroll
+        for (int n = 0; n < 32; ++n) most = fmaxf(most, __uint_as_float(x[n]));
+        sh.row_max[part][col] = most;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+        most = fmul(fmaxf(most, sh.row_max[part ^ 1][col]), scale);
+        // A new reference when the maximum has grown by 8, or at the first position seen; the values' exponent with it.
+        const float was = ref;
+        if (most > ref + 8.0f) ref = most;
+        const float shrink = was == ref ? 1.0f : was == -INFINITY ? 0.0f : fast_exp2(was - ref);
+        const float by = fmul(shrink, pow2i(ev - ev_now));
+        if (step > step0 && __any_sync(0xffffffffu, by != 1.0f)) {
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) {
+                uint32_t o[32];
+                kvt_load32(to + lanes + part * (D / 2) + 32 * k, o);
+                kvt_wait_ld();
+#pragma unroll
+                for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(fmul(__uint_as_float(o[n]), by));
+                kvt_store32(to + lanes + part * (D / 2) + 32 * k, o);
+            }
+        }
+        ev = ev_now;
+        sum = fmul(sum, shrink);
+        const float base = ref == -INFINITY ? 0.0f : ref;
+        uint32_t p[16];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+            const float u = fast_exp2(__fmaf_rn(__uint_as_float(x[2 * n]), scale, -base));
+            const float v = fast_exp2(__fmaf_rn(__uint_as_float(x[2 * n + 1]), scale, -base));
+            sum += u + v;
+            p[n] = pack_f16(u, v);
+        }
+        kvt_store16(ts + lanes + 16 * part, p);
+        kvt_wait_st();
+        kvt_before();
+        __syncthreads();
+        kvt_after();
+        if (tid == 0) {
+#pragma unroll
+            for (int k = 0; k < KVT_STEP / 16; ++k)
+                kvt_mma(to, ts + 8 * k, kvt_desc(kvt_smem(sh.v) + k * 32), D, step > step0 || k > 0);
+            kvt_commit(&sh.o_done);
+        }
+    }
+    copies_wait<0>();
+    const int done = step - step0;                                     // whole tiles, whose O += P V has been issued
+    if (ok && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1);
+    const bool failed = __syncthreads_or(!ok);
+    kvt_after();
+
+    // Half of the column's dimensions to a thread.
+    if (!failed) {
+        sh.row_sum[part][col] = sum;
+        __syncthreads();
+        sum += sh.row_sum[part ^ 1][col];
+        const bool alone = active == 1;
+        float *const parts = a.part + (int64_t)group * a.splits * (KVT_COLS * (D + 2)), *const mine = alone ? nullptr : parts + (int64_t)split * (KVT_COLS * (D + 2));
+        const float by = pow2i(ev), inv = sum == 0.0f ? 0.0f : fdiv(by, sum);
+        const int64_t at = qrow * a.out_stride + (int64_t)qhead * D + part * (D / 2);
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            uint32_t o[32];
+            if (done > 0) {
+                kvt_load32(to + lanes + part * (D / 2) + 32 * k, o);
+                kvt_wait_ld();
+            } else {
+#pragma unroll
+                for (int n = 0; n < 32; ++n) o[n] = 0;
+            }
+            if (poison >> (part * (D / 64) + k) & 1) {
+#pragma unroll
+                for (int n = 0; n < 32; ++n) o[n] = 0x7fc00000u;
+            }
+            if (have && alone) {
+                __nv_bfloat16 *const out = (__nv_bfloat16 *)a.out + at + 32 * k;
+                const bool none = sum == 0.0f;
+                if (((uintptr_t)out & 15) == 0) {
+#pragma unroll
+                    for (int n = 0; n < 32; n += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(none ? 0.0f : fmul(__uint_as_float(o[n + 2 * m]), inv),
+                                                                           none ? 0.0f : fmul(__uint_as_float(o[n + 2 * m + 1]), inv));
+                            w[m] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                        *(uint4 *)(out + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 32; ++n) out[n] = __float2bfloat16_rn(none ? 0.0f : fmul(__uint_as_float(o[n]), inv));
+                }
+            } else if (have) {
+#pragma unroll
+                for (int n = 0; n < 32; n += 4)
+                    *(float4 *)(mine + col * D + part * (D / 2) + 32 * k + n) =
+                        make_float4(fmul(__uint_as_float(o[n]), by), fmul(__uint_as_float(o[n + 1]), by),
+                                    fmul(__uint_as_float(o[n + 2]), by), fmul(__uint_as_float(o[n + 3]), by));
+            }
+        }
+        if (have && part == 0) {
+            if (alone) {
+                if (a.lse) a.lse[(int64_t)qrow * a.heads + qhead] = sum == 0.0f ? -INFINITY : fmul(ref + log2f(sum), 0.6931471805599453f);
+            } else {
+                *(float2 *)(mine + KVT_COLS * D + 2 * col) = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
+            }
+        }
+        if (!alone) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) sh.arrived = atomicAdd(a.counter + group, 1u);
+            __syncthreads();
+            if (sh.arrived == (unsigned)active - 1) {
+                __threadfence();
+                if (tid == 0) a.counter[group] = 0;
+                kv4_join<KVT_COLS, D>(a, parts, active, ncol, sh.row);
+            }
+        }
+    } else if (tid == 0) {
+        g_prompt_fault = 1;
+    }
+    kvt_before();
+    __syncthreads();
+    if (warp == 0) {
+        kvt_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "n"(KVT_TMEM) : "memory");
+    }
+}
+
+}  // namespace nc

@@ -5,7 +5,7 @@
 // (nanocompile/models/qwen2.py:232-271) and chooses tokens by argmax on the host
 // (nanocompile/models/qwen2.py:348-368); these operators have no counterpart there.
 #include "nc_api.cuh"
-#include "nc_kv4_attention.cuh"
+#include "nc_kv4_prompt.cuh"
 #include "nc_kv_pages.cuh"
 #include "nc_logprobs.cuh"
 
@@ -90,6 +90,7 @@ struct AttnPlan {
 };
 constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: their finish counters lead the scratch
 constexpr int KV4_STAGES = 2;
+constexpr int64_t KV4_PROMPT = 96;             // columns from which bfloat16 rows go to the tensor cores' kernel
 
 // Warps of a CTA and splits of the histories: the cheapest by a model of the measured times, in units of a step on an SM
 // that is full (3.3 us; 16 warps of 8 columns fill it, 8 of more): a CTA starts in about half a step, the join of
@@ -97,9 +98,20 @@ constexpr int KV4_STAGES = 2;
 // histories take them; for long histories the last CTA's half counts instead, as lengths differ.  Measured: 64
 // sequences of 2048 positions and two heads 12.3 us in 128 CTAs of 16 warps, 14.9 in 512 of four; 128 sequences of 512
 // 8.5 us in 256 CTAs of eight, 11.3 of four, 12.0 of sixteen; 32 of 2048 and 16 heads 33 us in 512 of four, 45 of sixteen.
-AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length) {
+AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length, bool bf16) {
     AttnPlan p{};
     const int64_t cols = heads / kv * max_rows;
+    if (bf16 && (d == 64 || d == 128) && cols >= KV4_PROMPT) {          // tensor cores: 128 columns, two CTAs to an SM
+        p.nt = KVT_COLS / 8;
+        p.col_blocks = (int)((cols + KVT_COLS - 1) / KVT_COLS);
+        p.groups = seqs * kv * p.col_blocks;
+        const int64_t steps = std::max<int64_t>(1, (max_length + KVT_STEP - 1) / KVT_STEP), places = 148 * 2;
+        int64_t splits = p.groups == 0 || p.groups > KV4_COUNTERS ? 1 : places / p.groups;
+        splits = std::max<int64_t>(1, std::min(splits, steps / 4));     // a split is worth its join from four steps on
+        p.chunk = (int)((steps + splits - 1) / splits);
+        p.splits = (int)((steps + p.chunk - 1) / p.chunk);
+        return p;
+    }
     p.nt = cols <= 8 ? 1 : cols <= 16 || d > 64 ? 2 : 4;
     p.col_blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
     p.groups = seqs * kv * p.col_blocks;
@@ -156,11 +168,32 @@ int32_t launch_kv4_attention_n(cudaStream_t st, const Kv4AttnArgs &a, const Attn
 }
 
 template <int D>
+int32_t launch_kv4_prompt(cudaStream_t st, const Kv4AttnArgs &a, int64_t ctas) {
+    constexpr size_t bytes = sizeof(KvtShared<D>) + 1024;
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(kv4_prompt_kernel<D>, bytes, &allowed));
+    CUDA_TRY(launch_k(kv4_prompt_kernel<D>, (unsigned)ctas, KVT_THREADS, bytes, st, a));
+    return check_launch("kv4_prompt_kernel");
+}
+
+template <int D>
 int32_t launch_kv4_attention_d(cudaStream_t st, const Kv4AttnArgs &a, const AttnPlan &p, int64_t ctas) {
+    if constexpr (D == 64 || D == 128)
+        if (p.nt == KVT_COLS / 8) return launch_kv4_prompt<D>(st, a, ctas);
     return a.type != KV_BF16 ? launch_kv4_attention_n<D, true>(st, a, p, ctas) : launch_kv4_attention_n<D, false>(st, a, p, ctas);
 }
 
 }  // namespace
+
+// Whether a matrix instruction's completion never came since the last call; clears it.
+int32_t nc::prompt_fault(bool *fault) {
+    unsigned int word = 0;
+    CUDA_TRY(cudaMemcpyFromSymbol(&word, g_prompt_fault, sizeof(word)));
+    *fault = word != 0;
+    word = 0;
+    if (*fault) CUDA_TRY(cudaMemcpyToSymbol(g_prompt_fault, &word, sizeof(word)));
+    return NC_OK;
+}
 
 extern "C" int32_t nc_kv4_append(void **p, const int64_t *s, void *stream) {
     Kv4AppendArgs a{};
@@ -216,7 +249,9 @@ extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {
 extern "C" int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_rows,
                                                   int64_t max_length) {
     if (seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || d <= 0 || max_rows <= 0 || max_length < 0) return 256;
-    return kv4_scratch(kv4_plan(seqs, heads, kv_heads, d, max_rows, max_length), d);
+    int64_t most = 0;
+    for (bool bf16 : {false, true}) most = std::max(most, kv4_scratch(kv4_plan(seqs, heads, kv_heads, d, max_rows, max_length, bf16), d));
+    return most;
 }
 
 extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
@@ -246,7 +281,7 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     if (a.q_stride < heads * a.pool.d || a.out_stride < heads * a.pool.d) return fail(NC_ERR_ARGUMENT, "rows of %lld values overlap", (long long)(heads * a.pool.d));
     if (max_rows <= 0 || max_rows > a.at.rows || max_length < 0 || max_length > I32 || (!a.at.row_start && max_rows != 1))
         return fail(NC_ERR_ARGUMENT, "at most %lld rows and %lld positions of a sequence", (long long)max_rows, (long long)max_length);
-    const AttnPlan plan = kv4_plan(a.at.seqs, heads, a.pool.kv, a.pool.d, max_rows, max_length);
+    const AttnPlan plan = kv4_plan(a.at.seqs, heads, a.pool.kv, a.pool.d, max_rows, max_length, a.type == KV_BF16);
     a.col_blocks = plan.col_blocks;
     a.splits = plan.splits;
     a.chunk = plan.chunk;
