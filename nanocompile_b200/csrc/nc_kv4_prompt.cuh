@@ -15,9 +15,10 @@
 // 2 c + h at place 8 c + 4 i + 2 j + h, by K's rows, P's columns and V alike.  K is [place][d], V [d][place], both with
 // 128-byte swizzled rows.  In writing a quarter of a warp covers all eight 16-byte units, so that it meets no bank twice.
 //
-// The CTA goes step by step -- codes of tile t + 1 on their way, keys of t decoded while O += P V of t - 1 runs, values
-// while S runs -- and a second CTA on the SM fills what is left idle.  Bound by the instruction rate (decoding 17 for eight
-// values, softmax about six a score) against a tensor pipe that would need half of that.
+// The CTA goes step by step -- codes arrive two tiles ahead by bulk copies, keys of tile t are decoded while O += P V of
+// t - 1 runs, values of t and the largest parameters of t + 1 while S runs -- with three barriers to a tile, and a second
+// CTA on the SM fills what is left idle.  Bound by the instruction rate (decoding 17 for eight values, softmax about five
+// a score) against a tensor pipe that would need half of that.
 #pragma once
 
 #include "nc_kv4_attention.cuh"
@@ -32,13 +33,11 @@ template <int D>
 struct KvtShared {
     __align__(1024) char k[KVT_STEP * D * 2];  // [d / 64][64 places][128 bytes]
     __align__(1024) char v[KVT_STEP * D * 2];  // [d][128 bytes]
-    __align__(16) char raw[4 * 20 * D];
-    const char *src[4];                        // the next tile's cache tiles
-    uint64_t s_done, o_done;                   // mbarriers
+    __align__(16) char raw[2][4 * 20 * D];
+    uint64_t s_done, o_done, raw_full[2];      // mbarriers
     float row_max[2][KVT_COLS], row_sum[2][KVT_COLS];
     int2 row[KVT_COLS];                        // row, head
-    uint32_t tmem, top[2][4];                  // top: largest key scale, |key zero|, value scale, |value zero| of a tile (bits)
-    uint32_t nan_rows[2];
+    uint32_t tmem, there[2], top[2][4];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits)
     unsigned int arrived;
 };
 
@@ -49,14 +48,14 @@ __device__ __forceinline__ void kvt_mbar_init(uint64_t *bar) {
 // Whether the phase completes within the bound (about a second).
 __device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity) {
     const long long start = clock64();
-    for (;;) {
+    for (;;) {                                                         // each try sleeps up to a millisecond
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
-            : "r"(kvt_smem(bar)), "r"(parity)
+            : "r"(kvt_smem(bar)), "r"(parity), "r"(1000000u)
             : "memory");
         if (done) return true;
         if (clock64() - start > NC_DRAIN_CYCLES) return false;
@@ -92,15 +91,12 @@ __device__ __forceinline__ void kvt_load32(uint32_t t, uint32_t (&r)[32]) {
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(t));
 }
-__device__ __forceinline__ void kvt_store32(uint32_t t, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void kvt_load16(uint32_t t, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-        "r"(r[31])
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(t));
 }
 __device__ __forceinline__ void kvt_store16(uint32_t t, const uint32_t *r) {
     asm volatile(
@@ -119,6 +115,11 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+__device__ __forceinline__ uint32_t max_nan_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -129,13 +130,13 @@ __device__ __forceinline__ uint32_t codes_low(uint32_t w) { return add_f16x2((w 
 __device__ __forceinline__ uint32_t codes_high(uint32_t w) { return fma_f16x2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u); }
 // 2^e as a pair of f16, -14 <= e <= 15.
 __device__ __forceinline__ uint32_t pow2_f16x2(int e) { return (uint32_t)(e + 15) << 10 | (uint32_t)(e + 15) << 26; }
-// The exponent that brings zero + 15 scale below 2^15: parameters are multiplied by 2^-e.  A NaN counts as the largest number.
+// The exponent that brings |zero| + 15 scale below 2^15 (and above 2^12): parameters are multiplied by 2^-e.  By the
+// exponent fields of the largest of each, both f16 bits: 15 s < 2^(es - 10), |z| < 2^(ez - 14).  A NaN counts as the largest.
 __device__ __forceinline__ int kvt_exponent(uint32_t scale, uint32_t zero) {
-    const float s = __half2float(__ushort_as_half((unsigned short)min(scale, 0x7bffu)));
-    const float z = __half2float(__ushort_as_half((unsigned short)min(zero, 0x7bffu)));
-    const float most = __fmaf_rn(15.0f, s, z);
-    const int e = (int)(__float_as_uint(most) >> 23) - 127 - 14;
-    return max(-14, min(14, e));
+    return max(-14, min(14, max((int)(scale >> 10) + 4, (int)(zero >> 10)) - 28));
+}
+__device__ __forceinline__ void store16_shared(uint32_t address, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
 template <int D>
@@ -174,39 +175,79 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     if (tid == 0) {
         kvt_mbar_init(&sh.s_done);
         kvt_mbar_init(&sh.o_done);
+        kvt_mbar_init(&sh.raw_full[0]);
+        kvt_mbar_init(&sh.raw_full[1]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid < 8) sh.top[tid >> 2][tid & 3] = 0;
 
+    // Lanes 0 .. 3 of the last warp: a cache tile each.  Its page is looked up a step before its copy is started.
     const int tiles_per_page = a.at.page / KV4_TILE;
     const int32_t *const table = a.at.table + (int64_t)seq * a.at.width;
-    auto find = [&](int step) {                                        // threads 0 .. 3: a cache tile each
-        const int tile = step * 4 + tid;
-        const char *src = nullptr;
-        if (step < step_end && tile * KV4_TILE < end) {
+    int page_next = -1;
+    auto look_up = [&](int step) {                                     // nothing here waits for what is read
+        const int tile = step * 4 + lane;
+        page_next = -1;
+        if (lane < 4 && step < step_end && tile * KV4_TILE < end) {
             const int j = (int)((uint64_t)tile * a.page_magic >> 37);
-            const int page = j < a.at.width ? table[j] : -1;
-            if (page >= 0 && page < a.at.pages)
-                src = a.pool.base + page * a.pool.page_bytes + ((int64_t)head * tiles_per_page + (tile - j * tiles_per_page)) * (20 * D);
-            else if (a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+            if (j < a.at.width) page_next = table[j];
         }
-        sh.src[tid] = src;
     };
-    auto issue = [&]() {
-        constexpr int PIECES = 20 * D / 16;
-#pragma unroll
-        for (int i = 0; i < (4 * PIECES + KVT_THREADS - 1) / KVT_THREADS; ++i) {
-            const int q = i * KVT_THREADS + tid, k = q / PIECES;
-            if (q < 4 * PIECES && sh.src[k]) copy16_async(sh.raw + q * 16, sh.src[k] + (q - k * PIECES) * 16);
+    auto issue = [&](int step) {                                       // by that warp, of a tile that exists, looked up before
+        const int page = page_next;
+        const int tile = step * 4 + lane, buffer = (step - step0) & 1;
+        const bool wanted = lane < 4 && tile * KV4_TILE < end, there = wanted && page >= 0 && page < a.at.pages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) {
+            sh.there[buffer] = mask;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kvt_smem(&sh.raw_full[buffer])), "r"(__popc(mask) * 20 * D) : "memory");
         }
-        copies_commit();
+        __syncwarp();
+        if (there) {
+            const int j = (int)((uint64_t)tile * a.page_magic >> 37);
+            const char *const src = a.pool.base + page * a.pool.page_bytes + ((int64_t)head * tiles_per_page + (tile - j * tiles_per_page)) * (20 * D);
+            asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(kvt_smem(sh.raw[buffer] + lane * 20 * D)),
+                         "l"(src), "n"(20 * D), "r"(kvt_smem(&sh.raw_full[buffer]))
+                         : "memory");
+        } else if (wanted && a.at.error) {
+            atomicMin(a.at.error, (unsigned long long)seq);
+        }
     };
-    if (tid < 4) find(step0);
+    // The largest parameters of a tile that is here, for its exponents; warp: cache tile warp % 4, keys or values.
+    auto look = [&](int step) {
+        const int buffer = (step - step0) & 1, k = warp & 3;
+        const bool there = sh.there[buffer] >> k & 1;
+        uint32_t most = 0;
+        if (lane < 8 * NB) {
+            uint2 *const at = (uint2 *)(sh.raw[buffer] + k * 20 * D + part * 10 * D + 8 * D) + lane;
+            const int t = step * KVT_STEP + 16 * k + lane / NB;
+            uint2 w = there ? *at : make_uint2(0, 0);
+            if (!there || t + 8 >= end) {                              // past the end: whatever was there before
+                if (t >= end) w.x = 0;
+                if (t + 8 >= end) w.y = 0;
+                *at = w;
+            }
+            most = max_nan_f16x2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+        }
+        const uint32_t s = __reduce_max_sync(0xffffffffu, most & 0xffffu), z = __reduce_max_sync(0xffffffffu, most >> 16);
+        if (lane == 0) {
+            atomicMax(&sh.top[buffer][2 * part], s);
+            atomicMax(&sh.top[buffer][2 * part + 1], z);
+        }
+    };
     kvt_before();
     __syncthreads();
     kvt_after();
     release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
-    issue();
+    int issued = min(step_end, step0 + 2), seen_raw = step0;           // tiles whose copies are started, and waited for
+    constexpr int COPIER = KVT_THREADS / 32 - 1;
+    if (warp == COPIER) {
+        for (int s = step0; s < issued; ++s) {
+            look_up(s);
+            issue(s);
+        }
+        look_up(step0 + 2);
+    }
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;          // the warp's quarter of tensor memory
     const uint32_t tq = sh.tmem, ts = tq + D / 2, to = ts + KVT_STEP;
 
@@ -265,66 +306,49 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     float ref = -INFINITY, sum = 0.0f;                                 // of the thread's half of the positions
     int ev = -14;                                                      // the values' exponent
     uint32_t poison = 0;                                               // blocks of dimensions that a NaN reached
+    // Where the thread's first key and value units go; the others differ from them in bits 4-6 and by whole rows.
+    const int key_place = 32 * (warp >> 1 & 1) + 8 * (g >> 1) + 4 * (warp & 1) + (g & 1);
+    const uint32_t key_unit = kvt_smem(sh.k) + (NB == 4 ? part : 0) * (KVT_STEP * 128) + key_place * 128 +
+                              (((4 * ((NB == 4 ? 0 : part) ^ (g & 1)) + c) ^ (key_place & 7)) << 4);
+    const int value_grp = NB == 4 ? part : warp >> 1 & 1, value_block = NB == 4 ? warp & 3 : warp & 1;
+    const uint32_t value_unit = kvt_smem(sh.v) + (32 * value_block + 4 * g) * 128 + (((4 * value_grp + c) ^ (4 * (g & 1))) << 4);
     bool ok = true;
-    unsigned parity = 0;
+    if (step0 < step_end) {
+        ok = kvt_mbar_wait(&sh.raw_full[0], 0);
+        seen_raw = step0 + 1;
+        if (ok) look(step0);
+    }
     int step = step0;
-    for (; step < step_end; ++step, parity ^= 1) {
-        const int set = step & 1;
+    bool broken = __syncthreads_or(!ok);
+    for (; step < step_end && !broken; ++step) {
+        const int set = (step - step0) & 1;
+        const unsigned parity = set;
         const bool edge = (step + 1) * KVT_STEP > first + 1;
-        // The tile's codes are here; its parameters' largest.
-        copies_wait<0>();
-        __syncthreads();
-        uint32_t there = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) there |= sh.src[k] ? 1u << k : 0;
-        {
-            uint32_t s[2] = {0, 0}, z[2] = {0, 0};
-            for (int i = tid; i < 4 * 2 * 16 * NB; i += KVT_THREADS) {
-                const int k = i / (2 * 16 * NB), j = i % (2 * 16 * NB), which = j / (16 * NB), word = j % (16 * NB);
-                uint32_t *const at = (uint32_t *)(sh.raw + k * 20 * D + which * 10 * D + 8 * D) + word;
-                const int t = step * KVT_STEP + 16 * k + word / (2 * NB) + 8 * (word & 1);
-                if (!(there >> k & 1) || t >= end) *at = 0;            // whatever was there before
-                const uint32_t w = *at;
-                s[which] = max(s[which], w & 0x7fffu);
-                z[which] = max(z[which], w >> 16 & 0x7fffu);
-            }
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                s[which] = __reduce_max_sync(0xffffffffu, s[which]);
-                z[which] = __reduce_max_sync(0xffffffffu, z[which]);
-                if (lane == 0) {
-                    atomicMax(&sh.top[set][2 * which], s[which]);
-                    atomicMax(&sh.top[set][2 * which + 1], z[which]);
-                }
-            }
-        }
-        if (tid < 4) sh.top[set ^ 1][tid] = 0;
-        __syncthreads();
-        if (tid < 4) find(step + 1);
+        const char *const raw = sh.raw[set];
+        const uint32_t there = sh.there[set];
         const int ek = kvt_exponent(sh.top[set][0], sh.top[set][1]);
         const int ev_now = max(ev, kvt_exponent(sh.top[set][2], sh.top[set][3]));
         const bool nan = sh.top[set][2] > 0x7c00u || sh.top[set][3] > 0x7c00u;
+        if (tid < 4) sh.top[set ^ 1][tid] = 0;
         // Keys: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half of the lanes).
         {
             const int k = warp & 3;
-            const char *const tile = sh.raw + k * 20 * D;
+            const char *const tile = raw + k * 20 * D;
             const uint32_t unit = pow2_f16x2(-ek);
+            const int pair = NB == 4 ? part : 0;                       // of blocks: the lane's words of both are one load
+            const uint4 codes = *(const uint4 *)((const uint32_t *)tile + kv4_code_word(VB, 2 * pair, lane, 0));
+            const uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
 #pragma unroll
             for (int n = 0; n < NB / 2; ++n) {
-                const int b = NB == 4 ? 2 * part + (n ^ (g & 1)) : part ^ (g & 1);
-                const uint2 w = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
-                const uint2 par = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, g));
+                const int v2 = (NB == 4 ? n : part) ^ (g & 1);         // odd rows take the other block first
+                const uint2 w = v2 ? make_uint2(codes.z, codes.w) : make_uint2(codes.x, codes.y);
+                const uint2 par = v2 ? make_uint2(params.z, params.w) : make_uint2(params.x, params.y);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
                     const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
-                    uint4 v;
-                    v.x = fma_f16x2(codes_low(x), s, z);
-                    v.y = fma_f16x2(codes_high(x), s, z);
-                    v.z = fma_f16x2(codes_low(x >> 8), s, z);
-                    v.w = fma_f16x2(codes_high(x >> 8), s, z);
-                    const int place = 32 * (k >> 1) + 8 * (g >> 1) + 4 * (k & 1) + 2 * j + (g & 1);
-                    *(uint4 *)(sh.k + (b >> 1) * (KVT_STEP * 128) + place * 128 + (((4 * (b & 1) + c) ^ (place & 7)) << 4)) = v;
+                    store16_shared((key_unit ^ (n << 6) ^ (j << 5)) + 256 * j, fma_f16x2(codes_low(x), s, z), fma_f16x2(codes_high(x), s, z),
+                                   fma_f16x2(codes_low(x >> 8), s, z), fma_f16x2(codes_high(x >> 8), s, z));
                 }
             }
         }
@@ -332,7 +356,8 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         if (step > step0) ok = kvt_mbar_wait(&sh.o_done, parity ^ 1);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kvt_before();
-        if (__syncthreads_or(!ok)) break;
+        broken = __syncthreads_or(!ok);
+        if (broken) break;
         kvt_after();
         if (tid == 0) {
 #pragma unroll
@@ -342,12 +367,12 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         }
         // Values: 32 positions `grp`, block b; (d = 64: two of its four dimensions of each lane).
         {
-            const int grp = NB == 4 ? part : warp >> 1 & 1, b = NB == 4 ? warp & 3 : warp & 1;
+            const int grp = value_grp, b = value_block;
             const uint32_t unit = pow2_f16x2(-ev_now);
             uint32_t s[4], z[4], w[4];                                 // by (tile, j)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const char *const tile = sh.raw + (2 * grp + k) * 20 * D + 10 * D;
+                const char *const tile = raw + (2 * grp + k) * 20 * D + 10 * D;
                 const uint2 x = *(const uint2 *)((const uint32_t *)tile + kv4_code_word(VB, b, lane, 0));
                 uint2 even = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, 2 * c));
                 uint2 odd = *(const uint2 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b, 2 * c + 1));
@@ -373,23 +398,25 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
                     const uint32_t x = i >> 1 ? w[k] >> 8 : w[k];
                     v[k] = fma_f16x2(i & 1 ? codes_high(x) : codes_low(x), s[k], z[k]);
                 }
-                const int d = 32 * b + 4 * g + i;
-                *(uint4 *)(sh.v + d * 128 + (((4 * grp + c) ^ (d & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                store16_shared((value_unit ^ (i << 4)) + 128 * i, v[0], v[1], v[2], v[3]);
             }
         }
         if (nan) {                                                     // which of the thread's rows' positions have one
             for (int n = 0; n < KVT_STEP; ++n) {
                 if (step * KVT_STEP + n > pos) break;
-                const uint32_t *const par = (const uint32_t *)(sh.raw + (n >> 4) * 20 * D + 18 * D);
+                const uint32_t *const par = (const uint32_t *)(raw + (n >> 4) * 20 * D + 18 * D);
                 for (int b = 0; b < NB; ++b)
                     if (nan_params(par[kv4_param_word(NB, b, n & 15)])) poison |= 1u << b;
             }
         }
+        if (step + 1 < step_end) {
+            ok = kvt_mbar_wait(&sh.raw_full[set ^ 1], (unsigned)((step + 1 - step0) >> 1) & 1);
+            seen_raw = step + 2;
+            if (ok) look(step + 1);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         // Softmax of the thread's 32 positions.
-        ok = kvt_mbar_wait(&sh.s_done, parity);
-        if (__syncthreads_or(!ok)) break;                              // the codes are read, too
-        issue();
+        ok = kvt_mbar_wait(&sh.s_done, parity) && ok;
         kvt_after();
         uint32_t x[32];
         kvt_load32(ts + lanes + 32 * part, x);
@@ -419,43 +446,55 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         const float shrink = was == ref ? 1.0f : was == -INFINITY ? 0.0f : fast_exp2(was - ref);
         const float by = fmul(shrink, pow2i(ev - ev_now));
         if (step > step0 && __any_sync(0xffffffffu, by != 1.0f)) {
-#pragma unroll
-            for (int k = 0; k < D / 64; ++k) {
-                uint32_t o[32];
-                kvt_load32(to + lanes + part * (D / 2) + 32 * k, o);
+#pragma unroll 1
+            for (int k = 0; k < D / 32; ++k) {                         // few at a time: the scores are in registers
+                uint32_t o[16];
+                kvt_load16(to + lanes + part * (D / 2) + 16 * k, o);
                 kvt_wait_ld();
 #pragma unroll
-                for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(fmul(__uint_as_float(o[n]), by));
-                kvt_store32(to + lanes + part * (D / 2) + 32 * k, o);
+                for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(fmul(__uint_as_float(o[n]), by));
+                kvt_store16(to + lanes + part * (D / 2) + 16 * k, o);
             }
         }
         ev = ev_now;
         sum = fmul(sum, shrink);
         const float base = ref == -INFINITY ? 0.0f : ref;
         uint32_t p[16];
+        uint64_t total = 0;                                            // two sums
+        const uint64_t scale2 = pack2(scale, scale), base2 = pack2(-base, -base);
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
-            const float u = fast_exp2(__fmaf_rn(__uint_as_float(x[2 * n]), scale, -base));
-            const float v = fast_exp2(__fmaf_rn(__uint_as_float(x[2 * n + 1]), scale, -base));
-            sum += u + v;
-            p[n] = pack_f16(u, v);
+            const float2 u = unpack2(fma2(pack2(__uint_as_float(x[2 * n]), __uint_as_float(x[2 * n + 1])), scale2, base2));
+            const float2 v = make_float2(fast_exp2(u.x), fast_exp2(u.y));
+            total = add2(total, pack2(v.x, v.y));
+            p[n] = pack_f16(v.x, v.y);
         }
+        sum += unpack2(total).x + unpack2(total).y;
         kvt_store16(ts + lanes + 16 * part, p);
         kvt_wait_st();
         kvt_before();
-        __syncthreads();
+        broken = __syncthreads_or(!ok);                                // the tile's codes are read, too
         kvt_after();
+        if (broken) break;
         if (tid == 0) {
 #pragma unroll
             for (int k = 0; k < KVT_STEP / 16; ++k)
                 kvt_mma(to, ts + 8 * k, kvt_desc(kvt_smem(sh.v) + k * 32), D, step > step0 || k > 0);
             kvt_commit(&sh.o_done);
         }
+        if (issued < step_end) {
+            if (warp == COPIER) {
+                issue(step + 2);
+                look_up(step + 3);
+            }
+            ++issued;
+        }
     }
-    copies_wait<0>();
+    // Nothing is left in flight: copies (after a wait that ran out only), matrix instructions.
+    for (; seen_raw < issued; ++seen_raw) kvt_mbar_wait(&sh.raw_full[(seen_raw - step0) & 1], (unsigned)((seen_raw - step0) >> 1) & 1);
     const int done = step - step0;                                     // whole tiles, whose O += P V has been issued
-    if (ok && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1);
-    const bool failed = __syncthreads_or(!ok);
+    if (!broken && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1);
+    const bool failed = __syncthreads_or(!ok || broken);
     kvt_after();
 
     // Half of the column's dimensions to a thread.
