@@ -15,10 +15,11 @@
 // 2 c + h at place 8 c + 4 i + 2 j + h, by K's rows, P's columns and V alike.  K is [place][d], V [d][place], both with
 // 128-byte swizzled rows.  In writing a quarter of a warp covers all eight 16-byte units, so that it meets no bank twice.
 //
-// The CTA goes step by step -- codes arrive two tiles ahead by bulk copies, keys of tile t are decoded while O += P V of
-// t - 1 runs, values of t and the largest parameters of t + 1 while S runs -- with three barriers to a tile, and a second
-// CTA on the SM fills what is left idle.  Bound by the instruction rate (decoding 17 for eight values, softmax about five
-// a score) against a tensor pipe that would need half of that.
+// Codes arrive three tiles ahead by bulk copies.  While O += P V of tile t - 1 runs, the CTA decodes the keys of t + 1; while S
+// of t runs, it looks for the largest parameters of t + 2 and decodes the values of t; then softmax and the one barrier of the
+// tile.  A second CTA on the SM fills what is left idle.  Bound by
+// the instruction rate (decoding 17 for eight values, softmax about five a score) against a tensor pipe that would need
+// half of that.
 #pragma once
 
 #include "nc_kv4_attention.cuh"
@@ -31,13 +32,13 @@ __device__ unsigned int g_prompt_fault;        // set when a matrix instruction'
 
 template <int D>
 struct KvtShared {
-    __align__(1024) char k[KVT_STEP * D * 2];  // [d / 64][64 places][128 bytes]
+    __align__(1024) char k[2][KVT_STEP * D * 2];   // [d / 64][64 places][128 bytes]
     __align__(1024) char v[KVT_STEP * D * 2];  // [d][128 bytes]
-    __align__(16) char raw[2][4 * 20 * D];
-    uint64_t s_done, o_done, raw_full[2];      // mbarriers
+    __align__(16) char raw[3][4 * 20 * D];
+    uint64_t s_done, o_done, raw_full[3];      // mbarriers
     float row_max[2][KVT_COLS], row_sum[2][KVT_COLS];
     int2 row[KVT_COLS];                        // row, head
-    uint32_t tmem, there[2], top[2][4];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits)
+    uint32_t tmem, there[4], top[4][4];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits)
     unsigned int arrived;
 };
 
@@ -177,9 +178,10 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         kvt_mbar_init(&sh.o_done);
         kvt_mbar_init(&sh.raw_full[0]);
         kvt_mbar_init(&sh.raw_full[1]);
+        kvt_mbar_init(&sh.raw_full[2]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < 8) sh.top[tid >> 2][tid & 3] = 0;
+    if (tid < 16) sh.top[tid >> 2][tid & 3] = 0;
 
     // Lanes 0 .. 3 of the last warp: a cache tile each.  Its page is looked up a step before its copy is started.
     const int tiles_per_page = a.at.page / KV4_TILE;
@@ -195,11 +197,11 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     };
     auto issue = [&](int step) {                                       // by that warp, of a tile that exists, looked up before
         const int page = page_next;
-        const int tile = step * 4 + lane, buffer = (step - step0) & 1;
+        const int tile = step * 4 + lane, buffer = (step - step0) % 3;
         const bool wanted = lane < 4 && tile * KV4_TILE < end, there = wanted && page >= 0 && page < a.at.pages;
         const uint32_t mask = __ballot_sync(0xffffffffu, there);
         if (lane == 0) {
-            sh.there[buffer] = mask;
+            sh.there[(step - step0) & 3] = mask;
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kvt_smem(&sh.raw_full[buffer])), "r"(__popc(mask) * 20 * D) : "memory");
         }
         __syncwarp();
@@ -215,8 +217,8 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     };
     // The largest parameters of a tile that is here, for its exponents; warp: cache tile warp % 4, keys or values.
     auto look = [&](int step) {
-        const int buffer = (step - step0) & 1, k = warp & 3;
-        const bool there = sh.there[buffer] >> k & 1;
+        const int buffer = (step - step0) % 3, set = (step - step0) & 3, k = warp & 3;
+        const bool there = sh.there[set] >> k & 1;
         uint32_t most = 0;
         if (lane < 8 * NB) {
             uint2 *const at = (uint2 *)(sh.raw[buffer] + k * 20 * D + part * 10 * D + 8 * D) + lane;
@@ -231,22 +233,22 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         }
         const uint32_t s = __reduce_max_sync(0xffffffffu, most & 0xffffu), z = __reduce_max_sync(0xffffffffu, most >> 16);
         if (lane == 0) {
-            atomicMax(&sh.top[buffer][2 * part], s);
-            atomicMax(&sh.top[buffer][2 * part + 1], z);
+            atomicMax(&sh.top[set][2 * part], s);
+            atomicMax(&sh.top[set][2 * part + 1], z);
         }
     };
     kvt_before();
     __syncthreads();
     kvt_after();
     release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
-    int issued = min(step_end, step0 + 2), seen_raw = step0;           // tiles whose copies are started, and waited for
+    int issued = min(step_end, step0 + 3), seen_raw = step0;           // tiles whose copies are started, and waited for
     constexpr int COPIER = KVT_THREADS / 32 - 1;
     if (warp == COPIER) {
         for (int s = step0; s < issued; ++s) {
             look_up(s);
             issue(s);
         }
-        look_up(step0 + 2);
+        look_up(step0 + 3);
     }
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;          // the warp's quarter of tensor memory
     const uint32_t tq = sh.tmem, ts = tq + D / 2, to = ts + KVT_STEP;
@@ -308,63 +310,76 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     uint32_t poison = 0;                                               // blocks of dimensions that a NaN reached
     // Where the thread's first key and value units go; the others differ from them in bits 4-6 and by whole rows.
     const int key_place = 32 * (warp >> 1 & 1) + 8 * (g >> 1) + 4 * (warp & 1) + (g & 1);
-    const uint32_t key_unit = kvt_smem(sh.k) + (NB == 4 ? part : 0) * (KVT_STEP * 128) + key_place * 128 +
+    const uint32_t key_unit = kvt_smem(sh.k[0]) + (NB == 4 ? part : 0) * (KVT_STEP * 128) + key_place * 128 +
                               (((4 * ((NB == 4 ? 0 : part) ^ (g & 1)) + c) ^ (key_place & 7)) << 4);
     const int value_grp = NB == 4 ? part : warp >> 1 & 1, value_block = NB == 4 ? warp & 3 : warp & 1;
     const uint32_t value_unit = kvt_smem(sh.v) + (32 * value_block + 4 * g) * 128 + (((4 * value_grp + c) ^ (4 * (g & 1))) << 4);
-    bool ok = true;
-    if (step0 < step_end) {
-        ok = kvt_mbar_wait(&sh.raw_full[0], 0);
-        seen_raw = step0 + 1;
-        if (ok) look(step0);
-    }
+    // Keys of a tile that is here: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half
+    // of the lanes).
+    auto decode_keys = [&](int step) {
+        const int n = step - step0, k = warp & 3, pair = NB == 4 ? part : 0;      // the lane's words of both blocks are one load
+        const char *const tile = sh.raw[n % 3] + k * 20 * D;
+        const uint32_t unit = pow2_f16x2(-kvt_exponent(sh.top[n & 3][0], sh.top[n & 3][1])), to_unit = key_unit + (n & 1) * (KVT_STEP * D * 2);
+        const uint4 codes = *(const uint4 *)((const uint32_t *)tile + kv4_code_word(VB, 2 * pair, lane, 0));
+        const uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
+#pragma unroll
+        for (int n = 0; n < NB / 2; ++n) {
+            const int v2 = (NB == 4 ? n : part) ^ (g & 1);             // odd rows take the other block first
+            const uint2 w = v2 ? make_uint2(codes.z, codes.w) : make_uint2(codes.x, codes.y);
+            const uint2 par = v2 ? make_uint2(params.z, params.w) : make_uint2(params.x, params.y);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
+                const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
+                store16_shared((to_unit ^ (n << 6) ^ (j << 5)) + 256 * j, fma_f16x2(codes_low(x), s, z), fma_f16x2(codes_high(x), s, z),
+                               fma_f16x2(codes_low(x >> 8), s, z), fma_f16x2(codes_high(x >> 8), s, z));
+            }
+        }
+    };
+    auto issue_scores = [&](int step) {                                // by one thread
+        const uint32_t keys = kvt_smem(sh.k[(step - step0) & 1]);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) kvt_mma(ts, tq + 8 * k, kvt_desc(keys + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, k > 0);
+        kvt_commit(&sh.s_done);
+    };
+    auto look_at = [&](int step) {
+        if (step >= step_end) return true;
+        seen_raw = step + 1;
+        const bool here = kvt_mbar_wait(&sh.raw_full[(step - step0) % 3], (unsigned)((step - step0) / 3) & 1);
+        if (here) look(step);
+        return here;
+    };
+    bool ok = look_at(step0);
+    ok = look_at(step0 + 1) && ok;
     int step = step0;
     bool broken = __syncthreads_or(!ok);
+    if (!broken && step0 < step_end) {
+        decode_keys(step0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        kvt_before();
+        __syncthreads();
+        kvt_after();
+        if (tid == 0) issue_scores(step0);
+    }
     for (; step < step_end && !broken; ++step) {
-        const int set = (step - step0) & 1;
-        const unsigned parity = set;
+        const int tile_no = step - step0, set = tile_no & 3;
         const bool edge = (step + 1) * KVT_STEP > first + 1;
-        const char *const raw = sh.raw[set];
+        const char *const raw = sh.raw[tile_no % 3];
         const uint32_t there = sh.there[set];
         const int ek = kvt_exponent(sh.top[set][0], sh.top[set][1]);
         const int ev_now = max(ev, kvt_exponent(sh.top[set][2], sh.top[set][3]));
         const bool nan = sh.top[set][2] > 0x7c00u || sh.top[set][3] > 0x7c00u;
-        if (tid < 4) sh.top[set ^ 1][tid] = 0;
-        // Keys: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half of the lanes).
-        {
-            const int k = warp & 3;
-            const char *const tile = raw + k * 20 * D;
-            const uint32_t unit = pow2_f16x2(-ek);
-            const int pair = NB == 4 ? part : 0;                       // of blocks: the lane's words of both are one load
-            const uint4 codes = *(const uint4 *)((const uint32_t *)tile + kv4_code_word(VB, 2 * pair, lane, 0));
-            const uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
-#pragma unroll
-            for (int n = 0; n < NB / 2; ++n) {
-                const int v2 = (NB == 4 ? n : part) ^ (g & 1);         // odd rows take the other block first
-                const uint2 w = v2 ? make_uint2(codes.z, codes.w) : make_uint2(codes.x, codes.y);
-                const uint2 par = v2 ? make_uint2(params.z, params.w) : make_uint2(params.x, params.y);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
-                    const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
-                    store16_shared((key_unit ^ (n << 6) ^ (j << 5)) + 256 * j, fma_f16x2(codes_low(x), s, z), fma_f16x2(codes_high(x), s, z),
-                                   fma_f16x2(codes_low(x >> 8), s, z), fma_f16x2(codes_high(x >> 8), s, z));
-                }
-            }
+        if (tid < 4) sh.top[(set + 3) & 3][tid] = 0;                   // of the last tile, for the look at tile step + 3
+        if (step + 1 < step_end) decode_keys(step + 1);
+        // O += P V of the last tile is done: the values' buffer and O are free, and S, whose place P had.  The keys have been in
+        // order since the last barrier.
+        ok = true;
+        if (step > step0) {
+            ok = kvt_mbar_wait(&sh.o_done, (unsigned)(tile_no - 1) & 1);
+            kvt_after();
+            if (tid == 0) issue_scores(step);
         }
-        // O += P V of the last tile is done: S and the values' buffer are free, and O.
-        if (step > step0) ok = kvt_mbar_wait(&sh.o_done, parity ^ 1);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        kvt_before();
-        broken = __syncthreads_or(!ok);
-        if (broken) break;
-        kvt_after();
-        if (tid == 0) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                kvt_mma(ts, tq + 8 * k, kvt_desc(kvt_smem(sh.k) + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, k > 0);
-            kvt_commit(&sh.s_done);
-        }
+        ok = look_at(step + 2) && ok;
         // Values: 32 positions `grp`, block b; (d = 64: two of its four dimensions of each lane).
         {
             const int grp = value_grp, b = value_block;
@@ -409,14 +424,9 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
                     if (nan_params(par[kv4_param_word(NB, b, n & 15)])) poison |= 1u << b;
             }
         }
-        if (step + 1 < step_end) {
-            ok = kvt_mbar_wait(&sh.raw_full[set ^ 1], (unsigned)((step + 1 - step0) >> 1) & 1);
-            seen_raw = step + 2;
-            if (ok) look(step + 1);
-        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         // Softmax of the thread's 32 positions.
-        ok = kvt_mbar_wait(&sh.s_done, parity) && ok;
+        ok = kvt_mbar_wait(&sh.s_done, (unsigned)tile_no & 1) && ok;
         kvt_after();
         uint32_t x[32];
         kvt_load32(ts + lanes + 32 * part, x);
@@ -484,14 +494,14 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         }
         if (issued < step_end) {
             if (warp == COPIER) {
-                issue(step + 2);
-                look_up(step + 3);
+                issue(step + 3);
+                look_up(step + 4);
             }
             ++issued;
         }
     }
     // Nothing is left in flight: copies (after a wait that ran out only), matrix instructions.
-    for (; seen_raw < issued; ++seen_raw) kvt_mbar_wait(&sh.raw_full[(seen_raw - step0) & 1], (unsigned)((seen_raw - step0) >> 1) & 1);
+    for (; seen_raw < issued; ++seen_raw) kvt_mbar_wait(&sh.raw_full[(seen_raw - step0) % 3], (unsigned)((seen_raw - step0) / 3) & 1);
     const int done = step - step0;                                     // whole tiles, whose O += P V has been issued
     if (!broken && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1);
     const bool failed = __syncthreads_or(!ok || broken);
