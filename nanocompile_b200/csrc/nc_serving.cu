@@ -90,7 +90,13 @@ struct AttnPlan {
 };
 constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: their finish counters lead the scratch
 constexpr int KV4_STAGES = 2;
-constexpr int64_t KV4_PROMPT = 96;             // columns from which bfloat16 rows go to the tensor cores' kernel
+// bfloat16 rows go to the tensor cores' kernel from this many columns of a sequence and tiles (128 columns by 64 positions)
+// of the call.  Below, its start, its wide parts and few CTAs cost more than they give.  Measured, it against the products on
+// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 70 against 157 us, 2 of
+// 300 over 300 (800) 39 against 83, 4 of 64 over 500 (512) 41 against 44, one of 64 over 2000 (512) 42 against 26; 64: 1024
+// rows of 14 heads (1792) 45 against 49, 256 over 4000 (1764) 49 against 46.
+constexpr int64_t KV4_PROMPT_COLS = 96;
+constexpr int64_t kv4_prompt_tiles(int64_t d) { return d == 128 ? 600 : 1780; }
 
 // Warps of a CTA and splits of the histories: the cheapest by a model of the measured times, in units of a step on an SM
 // that is full (3.3 us; 16 warps of 8 columns fill it, 8 of more): a CTA starts in about half a step, the join of
@@ -101,11 +107,12 @@ constexpr int64_t KV4_PROMPT = 96;             // columns from which bfloat16 ro
 AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length, bool bf16) {
     AttnPlan p{};
     const int64_t cols = heads / kv * max_rows;
-    if (bf16 && (d == 64 || d == 128) && cols >= KV4_PROMPT) {          // tensor cores: 128 columns, two CTAs to an SM
-        p.nt = KVT_COLS / 8;
-        p.col_blocks = (int)((cols + KVT_COLS - 1) / KVT_COLS);
-        p.groups = seqs * kv * p.col_blocks;
-        const int64_t steps = std::max<int64_t>(1, (max_length + KVT_STEP - 1) / KVT_STEP), places = 148 * 2;
+    const int64_t prompt_blocks = (cols + KVT_COLS - 1) / KVT_COLS, prompt_steps = std::max<int64_t>(1, (max_length + KVT_STEP - 1) / KVT_STEP);
+    if (bf16 && (d == 64 || d == 128) && cols >= KV4_PROMPT_COLS && seqs * kv * prompt_blocks * prompt_steps >= kv4_prompt_tiles(d)) {
+        p.nt = KVT_COLS / 8;                                             // 128 columns, two CTAs to an SM
+        p.col_blocks = (int)prompt_blocks;
+        p.groups = seqs * kv * prompt_blocks;
+        const int64_t steps = prompt_steps, places = 148 * 2;
         int64_t splits = p.groups == 0 || p.groups > KV4_COUNTERS ? 1 : places / p.groups;
         splits = std::max<int64_t>(1, std::min(splits, steps / 4));     // a split is worth its join from four steps on
         p.chunk = (int)((steps + splits - 1) / splits);

@@ -71,7 +71,8 @@ class Case:
         self.d_pool, self.d_table = DeviceArray.of(self.pool.bytes), DeviceArray.of(self.table)
         self.d_lengths = DeviceArray.of(self.lengths)
 
-    def attend(self, layout, q, dtype, counts=None, rope=None, scale=None, stride=None, scratch=None, max_length=None, error=None):
+    def attend(self, layout, q, dtype, counts=None, rope=None, scale=None, stride=None, scratch=None, max_length=None, error=None,
+               max_rows=None):
         """Output [rows, heads, d] and log-sums of the device's attention."""
         rows, heads, d = q.shape
         counts = [1] * len(self.lengths) if counts is None else counts
@@ -82,11 +83,12 @@ class Case:
         out = DeviceArray.zeros((rows, line), dtype)
         lse = DeviceArray.of(np.full((rows, heads), 7.0, np.float32))
         most = int(self.lengths.max()) if max_length is None else max_length
+        most_rows = max(counts) if max_rows is None else max_rows
         if scratch is None:
-            scratch = DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, rows, len(counts), most, max(counts)),), np.uint8)
-        single = all(c == 1 for c in counts)
+            scratch = DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, rows, len(counts), most, most_rows),), np.uint8)
+        single = all(c == 1 for c in counts) and most_rows == 1
         serving.kv4_attention(layout, out, given, self.d_pool, self.d_table, self.d_lengths, scratch, max_length=most,
-                              row_start=None if single else DeviceArray.of(starts_of(counts)), max_rows=max(counts),
+                              row_start=None if single else DeviceArray.of(starts_of(counts)), max_rows=most_rows,
                               rope=None if rope is None else tuple(DeviceArray.of(t) for t in rope), layer=self.layer,
                               scale=scale, lse=lse, error=error)
         return ref.decode(out.numpy(), dtype).reshape(rows, heads, d), lse.numpy()
@@ -255,6 +257,83 @@ def test_a_nan_is_seen_by_the_rows_that_see_its_position_only(cuda, dtype):
     want, _, size = ref.attention(q, [clean], [50], [0, 50], np.float32(0.125))
     bound = attention_bound(dtype, want, size, np.abs(clean[1]).max())
     assert (np.abs(got - want)[~nan] <= bound[~nan]).all()
+
+
+# bfloat16 prompts of enough work take the tensor cores' kernel. How much there is goes by the bounds that the call is
+# given, so a large bound sends small histories there: `max_length` splits them (most splits then find nothing), many
+# rows of a sequence leave them whole.
+
+
+@pytest.mark.parametrize("split", [True, False])
+@pytest.mark.parametrize("heads,kv,d,page", [(14, 2, 64, 16), (16, 4, 64, 128), (8, 1, 128, 80), (12, 3, 128, 32)])
+def test_bfloat16_prompts_on_the_tensor_cores(cuda, heads, kv, d, page, split):
+    rng = np.random.default_rng(page + split)
+    lengths, counts = [150, 5, 0, 201, 1, 40, 3, 64], [150, 2, 0, 37, 1, 40, 6, 64]
+    if not split:                                   # more blocks of columns than there are places for CTAs
+        lengths, counts = lengths * 3, counts * 3
+    case = Case(rng, lengths, kv, d, page)
+    q = rng.standard_normal((sum(counts), heads, d)).astype(np.float32)
+    bounds = dict(max_length=30000) if split else dict(max_length=640, max_rows=sum(counts))
+    error = error_word()
+    case.check(KV4Layout(heads, kv, d, page), q, "bfloat16", counts, rope=ref.rope_tables(201, d), error=error, **bounds)
+    assert error.numpy()[0] == ALL_ONES
+    case.check(KV4Layout(heads, kv, d, page), q * 20, "bfloat16", counts, stride=heads * d + 3, **bounds)      # sharp scores
+    cuda.device_faults()
+
+
+@pytest.mark.parametrize("scale_kv", [2e4, 1.0, 1e-4])
+def test_tensor_core_prompts_at_any_size_of_value(cuda, scale_kv):
+    """Values that grow by orders along the history, so that their exponent and the maximum move between tiles."""
+    rng = np.random.default_rng(13)
+    case = Case(rng, [300], 1, 128, 16)
+    keys, values = (x * np.geomspace(1e-2, 1, 300)[:, None, None].astype(np.float32) * np.float32(scale_kv) for x in case.histories[0])
+    case.pool.append(keys, values, case.table, case.lengths, [0, 300])
+    case.histories = [case.pool.history(case.table[0], 300)]
+    case.upload()
+    q = (rng.standard_normal((100, 4, 128)) * 3 / scale_kv).astype(np.float32)
+    for bounds in (dict(max_length=100000), dict(max_length=300, max_rows=100)):
+        case.check(KV4Layout(4, 1, 128, 16), q, "bfloat16", [100], **bounds)
+
+
+def test_a_nan_on_the_tensor_cores_is_seen_by_the_rows_that_see_it_only(cuda):
+    rng = np.random.default_rng(5)
+    layout, long = KV4Layout(4, 2, 128, 32), dict(max_length=50000)
+    case = Case(rng, [150], 2, 128, 32)
+    keys, values = (np.array(x) for x in case.histories[0])
+    case.pool.append(keys, values, case.table, case.lengths, [0, 150])
+    clean = case.pool.history(case.table[0], 150)
+    values[100, 0, 3] = np.nan                      # head 0, first block
+    values[20, 0, 127] = np.nan                     # head 0, last block
+    keys[137, 1, 40] = np.nan                       # head 1
+    case.pool.append(keys, values, case.table, case.lengths, [0, 150])
+    case.upload()
+    q = np.ones((150, 4, 128), np.float32)
+    got, _ = case.attend(layout, q, "bfloat16", [150], **long)
+    nan = np.isnan(got)
+    assert not nan[:100, :2, :32].any() and nan[100:, :2, :32].all() and not nan[:, :2, 32:96].any()
+    assert not nan[:20, :2].any() and nan[20:, :2, 96:].all()
+    assert not nan[:137, 2:].any() and nan[137:, 2:].all()
+    want, _, size = ref.attention(q, [clean], [150], [0, 150], np.float32(128 ** -0.5))
+    bound = attention_bound("bfloat16", want, size, np.abs(clean[1]).max())
+    assert (np.abs(got - want)[~nan] <= bound[~nan]).all()
+
+
+def test_missing_pages_on_the_tensor_cores(cuda):
+    rng = np.random.default_rng(14)
+    layout = KV4Layout(4, 1, 64, 16)
+    case = Case(rng, [100, 90], 1, 64, 16)
+    keys, values = case.histories[0]
+    gone = case.table.copy()
+    gone[0, 2] = -1
+    case.d_table = DeviceArray.of(gone)
+    error = error_word()
+    q = rng.standard_normal((60, 4, 64)).astype(np.float32)
+    q = ref.decode(ref.encode(q, "bfloat16"), "bfloat16")
+    got, _ = case.attend(layout, q, "bfloat16", [30, 30], max_length=100000, error=error)
+    assert error.numpy()[0] == 0
+    there = np.r_[0:32, 48:100]
+    want, _, size = ref.attention(q[:30], [(keys[there], values[there])], [84], [0, 30], np.float32(0.125))
+    assert (np.abs(got[:30] - want) <= attention_bound("bfloat16", want, size, np.abs(values).max())).all()
 
 
 @pytest.mark.parametrize("scale_kv,scale_q", [(1e4, 1e-3), (1e-5, 1e4), (300.0, 1e-2)])
