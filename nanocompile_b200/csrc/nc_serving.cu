@@ -83,6 +83,9 @@ float bits_to_f32(int64_t bits) {
     return f;
 }
 
+// Ways to cut that the plans weigh: every call makes its plan, so there are few of them.
+constexpr int CUTS[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 80, 96, 112, 128, 160, 192, 224, 256};
+
 // How a call's work is cut: 8 nt columns and `chunk` steps of positions to a CTA.
 struct AttnPlan {
     int nt, warps, col_blocks, splits, chunk;
@@ -125,9 +128,10 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
     const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, steps = std::max<int64_t>(1, (max_length + step - 1) / step);
     const int64_t most = p.groups > KV4_COUNTERS ? 1 : std::min<int64_t>(64, steps);
     float best = 0.0f;
-    for (int64_t warps = p.nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
+    for (int warps = p.nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
         const int64_t places = 148 * (p.nt == 1 ? 16 : 8) / warps;
-        for (int64_t splits = 1; splits <= most; ++splits) {
+        for (int splits : CUTS) {
+            if (splits > most) break;
             const int64_t chunk = (steps + splits - 1) / splits, active = (steps + chunk - 1) / chunk;
             if (active != splits) continue;                              // as good as fewer
             const int64_t mine = (chunk + warps - 1) / warps;            // steps of a warp
@@ -416,7 +420,9 @@ LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int64_t type) {
     const int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS, fewest = (vecs + longest - 1) / longest;
     int64_t best = -1;
     LogprobPlan p{0, 0};
-    for (int64_t segs = fewest; segs <= LP_SEGS && (segs == fewest || vecs / segs >= LP_THREADS); ++segs) {
+    for (int cut : CUTS) {
+        const int64_t segs = std::max<int64_t>(cut, fewest);
+        if (segs > LP_SEGS || (segs > fewest && vecs / segs < LP_THREADS)) break;
         const int64_t waves = (rows * segs + slots - 1) / slots, cost = waves * (vecs * n / segs + 4096) + 16 * segs;
         if (best >= 0 && cost >= best) continue;
         best = cost;
@@ -455,7 +461,7 @@ extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {
     if (plan.segs == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is beyond %d segments", (long long)vocab, LP_SEGS);
     if (!p[5] || (ntargets && (!p[0] || !p[6])) || (k && (!p[3] || !p[4])) || misaligned(p[5], type == KV_F32 ? 4 : 2))
         return fail(NC_ERR_ARGUMENT, "null or misaligned logits, targets or outputs");
-    if (plan.segs > 1 && (!p[7] || misaligned(p[7], 16) || scratch < nc_token_logprobs_scratch_bytes(rows, vocab, k)))
+    if (plan.segs > 1 && (!p[7] || misaligned(p[7], 16) || scratch < 4 * LP_ROWS + std::min<int64_t>(rows, LP_ROWS) * plan.segs * (16 + 8 * k)))
         return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch,
                     (long long)nc_token_logprobs_scratch_bytes(rows, vocab, k));
     a.out = (float *)p[0];

@@ -25,7 +25,6 @@ import numpy as np
 from nanocompile_b200.runtime import InterpreterError, check, library
 
 _vp, _i64 = ctypes.c_void_p, ctypes.c_int64
-_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 _SIZES = {"bfloat16": np.uint16}                        # how NumPy holds what it has no type for
 
 
@@ -130,66 +129,80 @@ class KV4Layout:
         return -(-positions // self.page_size)
 
 
-# The smallest calls take a few microseconds on the device, so the checks before them are kept short: an element type
-# is looked up by its object, and shapes are compared as the arrays give them.
-_names: dict = {}
+# The smallest calls take a few microseconds on the device, so the checks before them are kept short: every property of
+# an array is asked for once, element types are compared as small numbers, and what is wrong is looked for only
+# where something is.
+_F32, _F16, _BF16, _I32, _I64, _U8, _OTHER = range(7)
+_NAMES = {"float32": _F32, "float16": _F16, "bfloat16": _BF16, "int32": _I32, "int64": _I64, "uint8": _U8}
+
+
+class _Kinds(dict):
+    """Element types, as arrays give them, to small numbers."""
+
+    def __missing__(self, dtype) -> int:
+        kind = self[dtype] = _NAMES.get(_name(dtype), _OTHER)
+        return kind
+
+
+_kind = _Kinds()
 
 
 def _name(dtype) -> str:
-    name = _names.get(dtype)
-    if name is None:
-        name = _names[dtype] = str(dtype).removeprefix("torch.")
-    return name
+    return str(dtype).removeprefix("torch.")
 
 
-def _type_code(dtype) -> int:
-    code = _TYPES.get(_names.get(dtype) or _name(dtype))
-    if code is None:
-        raise InterpreterError(f"element type {_name(dtype)}: float32, float16 or bfloat16")
-    return code
-
-
-def _expect(what: str, array, dtype: str, shape: tuple) -> int:
-    """The address of a contiguous ``array`` of ``dtype`` and ``shape``."""
-    if array.shape != shape or (_names.get(array.dtype) or _name(array.dtype)) != dtype or not array.is_contiguous():
-        raise InterpreterError(f"{what}: {_name(array.dtype)} {tuple(array.shape)}, expected a contiguous {dtype} {shape}")
+def _expect(what: str, array, kind: int, shape: tuple) -> int:
+    """The address of a contiguous ``array`` of this kind and ``shape``."""
+    if array.shape != shape or _kind[array.dtype] != kind or not array.is_contiguous():
+        expected = next(name for name, k in _NAMES.items() if k == kind)
+        raise InterpreterError(f"{what}: {_name(array.dtype)} {tuple(array.shape)}, expected a contiguous {expected} {shape}")
     return array.data_ptr()
 
 
 def _rows(what: str, array, heads: int, d: int) -> tuple[int, int, int, int]:
-    """Address, rows, row stride and type code of ``[rows, heads * d]`` or ``[rows, heads, d]``; rows may be strided."""
-    shape, strides = array.shape, array.stride()
+    """Address, rows, row stride and kind of ``[rows, heads * d]`` or ``[rows, heads, d]``; rows may be strided."""
+    shape, strides, line, kind = array.shape, array.stride(), heads * d, _kind[array.dtype]
     if len(shape) == 2:
-        fits = shape[1] == heads * d and strides[1] == 1
+        fits = shape[1] == line and strides[1] == 1
     else:
         fits = len(shape) == 3 and shape[1] == heads and shape[2] == d and strides[2] == 1 and (heads == 1 or strides[1] == d)
     if not fits:
         raise InterpreterError(f"{what}: {tuple(shape)}, expected rows of {heads} contiguous heads of {d}")
+    if kind > _BF16:
+        raise InterpreterError(f"{what}: element type {_name(array.dtype)}: float32, float16 or bfloat16")
     rows = shape[0]
-    return array.data_ptr(), rows, strides[0] if rows > 1 else heads * d, _type_code(array.dtype)
+    return array.data_ptr(), rows, strides[0] if rows > 1 else line, kind
 
 
 def _rope(rope, d: int) -> tuple[int, int, int]:
     if rope is None:
         return 0, 0, 0
     cos, sin = rope
-    shape = (cos.shape[0], d // 2)
-    return _expect("cos", cos, "float32", shape), _expect("sin", sin, "float32", shape), shape[0]
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != d // 2 or sin.shape != shape or _kind[cos.dtype] or _kind[sin.dtype] or not (cos.is_contiguous() and sin.is_contiguous()):
+        positions = shape[0] if len(shape) else 0
+        _expect("cos", cos, _F32, (positions, d // 2))
+        _expect("sin", sin, _F32, (positions, d // 2))
+    return cos.data_ptr(), sin.data_ptr(), shape[0]
 
 
 def _cache(layout: KV4Layout, layer: int, pool, table, lengths, row_start) -> tuple:
     """Addresses of the pool, table, lengths and row starts; sequences, pages, layer offset, table width."""
-    if not 0 <= layer < layout.layers:
-        raise InterpreterError(f"layer {layer} of {layout.layers}")
-    shape = table.shape
-    if len(shape) != 2:
-        raise InterpreterError(f"table: {tuple(shape)}, expected [sequences, pages of a sequence]")
+    shape, held = table.shape, pool.shape
+    if not (len(shape) == 2 and len(held) == 2 and held[1] == layout.page_bytes and 0 <= layer < layout.layers
+            and _kind[table.dtype] == _kind[lengths.dtype] == _I32 and _kind[pool.dtype] == _U8 and lengths.shape == shape[:1]
+            and table.is_contiguous() and lengths.is_contiguous() and pool.is_contiguous()):
+        if not 0 <= layer < layout.layers:
+            raise InterpreterError(f"layer {layer} of {layout.layers}")
+        if len(shape) != 2:
+            raise InterpreterError(f"table: {tuple(shape)}, expected [sequences, pages of a sequence]")
+        _expect("table", table, _I32, tuple(shape))
+        _expect("pool", pool, _U8, (held[0] if len(held) else 0, layout.page_bytes))
+        _expect("lengths", lengths, _I32, (shape[0],))
     seqs, width = shape
-    pages = pool.shape[0]
-    return (_expect("pool", pool, "uint8", (pages, layout.page_bytes)), _expect("table", table, "int32", (seqs, width)),
-            _expect("lengths", lengths, "int32", (seqs,)),
-            0 if row_start is None else _expect("row_start", row_start, "int32", (seqs + 1,)),
-            seqs, pages, layer * layout.layer_bytes, width)
+    return (pool.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            0 if row_start is None else _expect("row_start", row_start, _I32, (seqs + 1,)),
+            seqs, held[0], layer * layout.layer_bytes, width)
 
 
 def _optional(array) -> int:
@@ -277,7 +290,7 @@ def kv4_attention(layout: KV4Layout, out, q, pool, table, lengths, scratch, *, m
     cos, sin, positions = _rope(rope, d)
     bits = layout.scale_bits if scale is None else _f32_bits(scale)
     _call("nc_kv4_attention",
-          (to, query, base, tab, lens, starts, cos, sin, 0 if lse is None else _expect("lse", lse, "float32", (rows, heads)),
+          (to, query, base, tab, lens, starts, cos, sin, 0 if lse is None else _expect("lse", lse, _F32, (rows, heads)),
            scratch.data_ptr(), _optional(error)),
           (rows, seqs, layout.kv_heads, d, layout.page_size, pages, layout.page_bytes, offset, width, heads, q_stride,
            out_stride, kind, positions, bits, max_rows, max_length, scratch.shape[0]), stream)
@@ -289,11 +302,13 @@ def kv_pages_scratch_bytes(seqs: int, width: int, pages: int) -> int:
 
 
 def _pages(new_table, table, lengths, pool, status, scratch, page_size: int) -> tuple[tuple, tuple]:
-    seqs, width = table.shape
-    pages, page_bytes = pool.shape
-    return ((_expect("new_table", new_table, "int32", (seqs, width)), _expect("table", table, "int32", (seqs, width)),
-             _expect("lengths", lengths, "int32", (seqs,)), _expect("status", status, "int64", (4,)),
-             _expect("pool", pool, "uint8", (pages, page_bytes)), scratch.data_ptr()),
+    shape, held = table.shape, pool.shape
+    if len(shape) != 2 or len(held) != 2:
+        raise InterpreterError(f"table {tuple(shape)} and pool {tuple(held)}: expected [sequences, pages] and [pages, bytes]")
+    (seqs, width), (pages, page_bytes) = shape, held
+    return ((_expect("new_table", new_table, _I32, shape), _expect("table", table, _I32, shape),
+             _expect("lengths", lengths, _I32, (seqs,)), _expect("status", status, _I64, (4,)),
+             _expect("pool", pool, _U8, held), scratch.data_ptr()),
             (seqs, width, pages, page_size, page_bytes, scratch.shape[0]))
 
 
@@ -307,9 +322,9 @@ def kv_pages_update(new_table, new_lengths, table, lengths, pool, status, scratc
     (new, old, lens, state, base, work), sizes = _pages(new_table, table, lengths, pool, status, scratch, page_size)
     n = (sizes[0],)
     _call("nc_kv_pages_update",
-          (new, _expect("new_lengths", new_lengths, "int32", n), old, lens, state, base, work,
-           0 if parent is None else _expect("parent", parent, "int32", n),
-           0 if grow is None else _expect("grow", grow, "int32", n)), sizes, stream)
+          (new, _expect("new_lengths", new_lengths, _I32, n), old, lens, state, base, work,
+           0 if parent is None else _expect("parent", parent, _I32, n),
+           0 if grow is None else _expect("grow", grow, _I32, n)), sizes, stream)
 
 
 def kv_pages_compact(new_table, table, lengths, pool, status, scratch, *, page_size: int, stream: int = 0) -> None:
@@ -334,15 +349,18 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
     if len(shape) != 2 or strides[1] != 1:
         raise InterpreterError(f"logits: {tuple(shape)}, expected [rows, vocabulary] with contiguous rows")
     rows, vocab = shape
+    kind = _kind[logits.dtype]
+    if kind > _BF16:
+        raise InterpreterError(f"logits: element type {_name(logits.dtype)}: float32, float16 or bfloat16")
     n = targets.shape[-1] if targets is not None else 0
     k = top.shape[-1] if top is not None else 0
     _call("nc_token_logprobs",
-          (_expect("out", out, "float32", (rows, n)) if n else 0,
-           0 if entropy is None else _expect("entropy", entropy, "float32", (rows,)),
-           0 if lse is None else _expect("lse", lse, "float32", (rows,)),
-           _expect("top", top, "int64", (rows, k)) if k else 0,
-           _expect("top_logprobs", top_logprobs, "float32", (rows, k)) if k else 0,
-           logits.data_ptr(), _expect("targets", targets, "int64", (rows, n)) if n else 0,
+          (_expect("out", out, _F32, (rows, n)) if n else 0,
+           0 if entropy is None else _expect("entropy", entropy, _F32, (rows,)),
+           0 if lse is None else _expect("lse", lse, _F32, (rows,)),
+           _expect("top", top, _I64, (rows, k)) if k else 0,
+           _expect("top_logprobs", top_logprobs, _F32, (rows, k)) if k else 0,
+           logits.data_ptr(), _expect("targets", targets, _I64, (rows, n)) if n else 0,
            _optional(scratch), _optional(error)),
-          (rows, vocab, strides[0] if rows > 1 else vocab, _type_code(logits.dtype), n, k,
+          (rows, vocab, strides[0] if rows > 1 else vocab, kind, n, k,
            0 if scratch is None else scratch.shape[0]), stream)
