@@ -314,14 +314,23 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     const int step0 = split * a.chunk + warp, step_end = min(steps, split * a.chunk + a.chunk);
     const int tiles_per_page = a.at.page / KV4_TILE;
     const int32_t *const table = a.at.table + (int64_t)seq * a.at.width;
-    // Where the lane's tile (lane % TILES) of a step lies; null past the end or where the table names no page.
-    auto tile_at = [&](int step) -> const char * {
+    // The page of the lane's tile (lane % TILES) of a step, by the table alone: nothing here waits for what is read.  -2: no
+    // such tile.
+    auto page_of = [&](int step) {
         const int tile = step * TILES + lane % TILES;
-        if (step >= step_end || tile * KV4_TILE >= end) return nullptr;
-        const int j = (int)((uint64_t)tile * a.page_magic >> 37);
-        const int page = j < a.at.width ? table[j] : -1;
+        int page = -2;
+        if (step < step_end && tile * KV4_TILE < end) {
+            const int j = (int)((uint64_t)tile * a.page_magic >> 37);
+            page = -1;
+            if (j < a.at.width) page = table[j];
+        }
+        return page;
+    };
+    // Where it lies; null where there is none (reported).
+    auto tile_at = [&](int step, int page) -> const char * {
+        const int tile = step * TILES + lane % TILES, j = (int)((uint64_t)tile * a.page_magic >> 37);
         if (page < 0 || page >= a.at.pages) {
-            if (a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+            if (page != -2 && a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
             return nullptr;
         }
         return a.pool.base + page * a.pool.page_bytes + ((int64_t)head * tiles_per_page + (tile - j * tiles_per_page)) * (20 * D);
@@ -341,15 +350,18 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     };
     uint32_t held[ST];                                                 // which tiles of the steps in flight are there
     int next = step0;
+    int pages[ST];
+#pragma unroll
+    for (int s = 0; s < ST; ++s) pages[s] = page_of(step0 + s * W);
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) {
-        const char *const from = tile_at(next);
+        const char *const from = tile_at(next, pages[s]);
         held[s] = __ballot_sync(0xffffffffu, from != nullptr);
         issue(s, from);
         copies_commit();
         next += W;
     }
-    const char *from_next = tile_at(next);
+    int page_next = pages[ST - 1];
 
     if (!HL) {                                                         // the places of no block
         for (int i = threadIdx.x; i < NT * 32; i += 32 * W) qz[i] = 0;
@@ -404,11 +416,12 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
 #pragma unroll 1
     for (int step = step0; step < step_end; step += W) {
         // Start the copies ST - 1 steps ahead, into the stage that the last step read.
-        issue(stage == 0 ? ST - 1 : stage - 1, from_next);
+        const char *const from = tile_at(next, page_next);
+        issue(stage == 0 ? ST - 1 : stage - 1, from);
         copies_commit();
-        held[ST - 1] = __ballot_sync(0xffffffffu, from_next != nullptr);
+        held[ST - 1] = __ballot_sync(0xffffffffu, from != nullptr);
         next += W;
-        from_next = tile_at(next);
+        page_next = page_of(next);
         copies_wait<ST - 1>();
         __syncwarp();
         const uint32_t whole = held[0];
