@@ -20,6 +20,11 @@
 //                32 b + 4 g + i
 //   parameters   u32 word [g][b][j]: scale low, zero high
 // Words and half-words belong to one position each, so positions are appended without reading.
+//
+// Both kernels read and write each byte once; memory's floor for 4 x 2048 rows of 8 heads of 128 (bfloat16 in, 44 MB for
+// the append; float32 out, 78 MB for the read) is 6.7 and 11.9 us.  They take 22 us, bound by the instructions of the
+// rounding (about 90 for eight values, the rotation included) and by 2.8 rounds of CTAs, and 17 us (4.5 TB/s).  One row of
+// each of 256 sequences takes 5.3 and 5.8 us: the start and the chain from a row's sequence over its page to its bytes.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -115,6 +120,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // Two floats to an instruction.  A packed multiplication and a packed addition after it may become one FMA (seen, with
 // -fmad=false and .rn too): where both roundings count, one of the two is not packed.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -143,19 +158,21 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t add2_rz(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // A block of 32 values in four neighbouring lanes, eight each: the lane's eight codes in a word, the block's parameters.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t *params) {
-    float low = x[0], high = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        low = min_nan(low, x[i]);
-        high = max_nan(high, x[i]);
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-    }
+    float low = min_nan(x[0], x[1], x[2]), high = max_nan(x[0], x[1], x[2]);
+    low = min_nan(low, x[3], x[4]), high = max_nan(high, x[3], x[4]);
+    low = min_nan(low, x[5], x[6]), high = max_nan(high, x[5], x[6]);
+    low = min_nan(low, x[7], __shfl_xor_sync(0xffffffffu, min_nan(low, x[7]), 1));
+    high = max_nan(high, x[7], __shfl_xor_sync(0xffffffffu, max_nan(high, x[7]), 1));
+    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, 2));
+    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, 2));
     const float limit = 65504.0f;
     const float z = min_nan(max_nan(low, -limit), limit);
     // An infinite range, or none between infinities of one sign, counts as the largest; a NaN among the values stays one.
@@ -166,16 +183,26 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t *
     if (!(s > 0.0f)) return 0;
     const float inv = fdiv(1.0f, s);
     const uint64_t from2 = pack2(-from, -from), inv2 = pack2(inv, inv);
+    uint64_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(mul2(add2(pack2(x[2 * i], x[2 * i + 1]), from2), inv2));
+        q[i] = pack2(fadd(v.x, 0.5f), fadd(v.y, 0.5f));
+    }
+    // The extremes' codes bound the others': seldom (a scale that f16 rounds far, infinities) is there anything to clamp.
+    if (!(fadd(fmul(fsub(low, from), inv), 0.5f) >= 0.0f && fadd(fmul(fsub(high, from), inv), 0.5f) < 16.0f)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = unpack2(q[i]);
+            q[i] = pack2(fminf(fmaxf(v.x, 0.0f), 15.0f), fminf(fmaxf(v.y, 0.0f), 15.0f));
+        }
+    }
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 6; i >= 0; i -= 2) {
-        float2 q = unpack2(mul2(add2(pack2(x[i], x[i + 1]), from2), inv2));
-        q.x = fadd(q.x, 0.5f);
-        q.y = fadd(q.y, 0.5f);
-        // 2^23 + the clamped code, rounded towards zero: floor, as it is not negative.  The code is in the low bits.
-        const uint32_t a = __float_as_uint(__fadd_rz(fminf(fmaxf(q.x, 0.0f), 15.0f), 8388608.0f));
-        const uint32_t b = __float_as_uint(__fadd_rz(fminf(fmaxf(q.y, 0.0f), 15.0f), 8388608.0f));
-        word = (word * 16 + b) * 16 + a;
+    for (int i = 3; i >= 0; --i) {
+        // 2^23 + the code, rounded towards zero: floor, as it is not negative.  The code is in the low bits.
+        const float2 c = unpack2(add2_rz(q[i], pack2(8388608.0f, 8388608.0f)));
+        word = (word * 16 + __float_as_uint(c.y)) * 16 + __float_as_uint(c.x);
     }
     return word - 0x4b000000u * 0x11111111u;       // what the eight 2^23 have added, modulo 2^32
 }
@@ -227,10 +254,10 @@ __device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bo
     }
 }
 
-// The append and the read go by tiles: the rows of a call that fall into one tile are one piece of work for a warp
-// and head, keys or values, with lane 4 g + c at dimensions 32 b + 8 c .. of positions g and 8 + g: for keys the
+// The append of many rows and the read go by tiles: the rows of a call that fall into one tile are one piece of work for a
+// warp and head, keys or values, with lane 4 g + c at dimensions 32 b + 8 c .. of positions g and 8 + g: for keys the
 // lane's words are the ones it writes, for values two shuffles turn them.  A CTA looks through `window` rows for
-// the first rows of tiles.  One row of each sequence (a decode step) is the same with tiles of one row.
+// the first rows of tiles.
 struct Kv4TileRows {
     char *tile;                    // of the first head, or null: no page
     int64_t row, position;         // of the first row
@@ -280,9 +307,65 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Rows &at, const Kv4Pool &pool
 }
 constexpr int KV4_TILE_WARPS = 4;
 
+// The append of few rows, or of one to a sequence: four lanes to a block of a row, eight blocks to a warp (six of d = 96).
 template <int NB>
-__global__ void __launch_bounds__(32 * KV4_TILE_WARPS, 6) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, int window, bool vectors) {
-    constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2;
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_append_rows_kernel(const __grid_constant__ Kv4AppendArgs a, bool vectors) {
+    constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2, SHARE = NB == 3 ? 4 : NB;
+    release_dependents();
+    wait_for_producer();
+    const int lane = threadIdx.x & 31, c = lane & 3, b = (lane >> 2) % SHARE;
+    const int64_t line = ((int64_t)blockIdx.x * (32 * KV4_TILE_WARPS) + threadIdx.x) / (4 * SHARE);   // row, 2 head + (0 keys, 1 values)
+    const int64_t row = line / (2 * a.pool.kv);
+    const int job = (int)(line % (2 * a.pool.kv)), head = job >> 1, which = job & 1;
+    char *tile = nullptr;
+    int t = 0;
+    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < a.at.rows && b < NB) {
+        const void *const p = which ? a.values : a.keys;
+        const int64_t from = row * (which ? a.value_stride : a.key_stride) + (int64_t)head * D;
+        const int i0 = 32 * b + 8 * c, k = i0 < HALF ? i0 : i0 - HALF;
+        const bool low = i0 < HALF, rotate = which == 0 && a.cos_tab;
+        float y[8];
+        kv_load8(p, from + i0, a.type, vectors, x);
+        if (rotate) kv_load8(p, from + (low ? i0 + HALF : k), a.type, vectors, y);
+        const int seq = kv4_sequence(a.at, row);
+        const int64_t position = a.at.lengths[seq] - (a.at.row_start ? a.at.row_start[seq + 1] - row : 1);
+        if (position >= 0 && position < a.at.lengths[seq]) {
+            const int page = kv4_page(a.at, seq, (int)position);
+            if (page >= 0 && a.cos_tab && position >= a.positions) {
+                if (a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
+            } else if (page >= 0) {
+                const int place = (int)position % a.at.page;
+                t = place % KV4_TILE;
+                tile = a.pool.base + page * a.pool.page_bytes + ((int64_t)head * (a.at.page / KV4_TILE) + place / KV4_TILE) * (20 * D) + which * 10 * D;
+                if (rotate) {
+                    float cs[8], sn[8];
+                    kv_load8(a.cos_tab, position * HALF + k, KV_F32, vectors, cs);
+                    kv_load8(a.sin_tab, position * HALF + k, KV_F32, vectors, sn);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        x[i] = low ? fsub(fmul(x[i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[i], cs[i]), fmul(y[i], sn[i]));
+                }
+            }
+        }
+    }
+    uint32_t params;
+    const uint32_t word = kv4_quantise(x, &params);
+    if (!tile) return;
+    const int g = t & 7, j = t >> 3;
+    if (which) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+            ((uint16_t *)tile)[2 * kv4_code_word(VB, b, 4 * (2 * c + half) + (g >> 1), j) + (g & 1)] = (uint16_t)(word >> (16 * half));
+    } else {
+        ((uint32_t *)tile)[kv4_code_word(VB, b, 4 * g + c, j)] = word;
+    }
+    if (c == 0) ((uint32_t *)(tile + 8 * D))[kv4_param_word(NB, b, t)] = params;
+}
+
+template <int NB>
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS, NB > 2 ? 5 : 6) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, bool vectors) {
+    constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2, window = KV4_TILE;
     release_dependents();
     wait_for_producer();
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -311,60 +394,83 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS, 6) kv4_append_kernel(cons
         bool in[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) in[j] = 8 * j + g >= rows.t0 && 8 * j + g < rows.t0 + count;
+        const bool rotate = which == 0 && a.cos_tab;
+        uint32_t words[NB][2], params[NB][2];
 #pragma unroll
-        for (int b0 = 0; b0 < NB; b0 += VB) {
-            uint32_t words[VB][2], params[VB][2];
+        for (int j = 0; j < 2; ++j) {
+            const int t = 8 * j + g;
+            const int64_t at = (rows.row + t - rows.t0) * stride + (int64_t)head * D + 8 * c;
+            float x[NB][8];
 #pragma unroll
-            for (int v = 0; v < VB; ++v)
+            for (int b = 0; b < NB; ++b) {
+                if (in[j]) kv_load8(p, at + 32 * b, a.type, vectors, x[b]);
+                else
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int t = 8 * j + g, i0 = 32 * (b0 + v) + 8 * c;
-                    const int64_t at = (rows.row + t - rows.t0) * stride + (int64_t)head * D;
-                    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    if (in[j]) {
-                        kv_load8(p, at + i0, a.type, vectors, x);
-                        if (which == 0 && a.cos_tab) {                // as kv4_rotated, eight at a time
-                            const bool low = i0 < HALF;
-                            const int k = low ? i0 : i0 - HALF;
-                            const int64_t angle = (rows.position + t - rows.t0) * HALF + k;
-                            float y[8], cs[8], sn[8];
-                            kv_load8(p, at + (low ? i0 + HALF : k), a.type, vectors, y);
-                            kv_load8(a.cos_tab, angle, KV_F32, vectors, cs);
-                            kv_load8(a.sin_tab, angle, KV_F32, vectors, sn);
+                    for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
+            }
+            if (rotate && in[j]) {                                    // as kv4_rotated, eight at a time
+                const int64_t angle = (rows.position + t - rows.t0) * HALF;
+                if constexpr (NB % 2 == 0) {                          // a lane has both of a pair
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                x[i] = low ? fsub(fmul(x[i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[i], cs[i]), fmul(y[i], sn[i]));
+                    for (int b = 0; b < NB / 2; ++b) {
+                        float cs[8], sn[8];
+                        kv_load8(a.cos_tab, angle + 32 * b + 8 * c, KV_F32, vectors, cs);
+                        kv_load8(a.sin_tab, angle + 32 * b + 8 * c, KV_F32, vectors, sn);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float u = x[b][i], v = x[b + NB / 2][i];
+                            x[b][i] = fsub(fmul(u, cs[i]), fmul(v, sn[i]));
+                            x[b + NB / 2][i] = fadd(fmul(v, cs[i]), fmul(u, sn[i]));
                         }
                     }
-                    words[v][j] = kv4_quantise(x, &params[v][j]);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int i0 = 32 * b + 8 * c;
+                        const bool low = i0 < HALF;
+                        const int k = low ? i0 : i0 - HALF;
+                        float y[8], cs[8], sn[8];
+                        kv_load8(p, at - 8 * c + (low ? i0 + HALF : k), a.type, vectors, y);
+                        kv_load8(a.cos_tab, angle + k, KV_F32, vectors, cs);
+                        kv_load8(a.sin_tab, angle + k, KV_F32, vectors, sn);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            x[b][i] = low ? fsub(fmul(x[b][i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[b][i], cs[i]), fmul(y[i], sn[i]));
+                    }
                 }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) words[b][j] = kv4_quantise(x[b], &params[b][j]);
+        }
+#pragma unroll
+        for (int b0 = 0; b0 < NB; b0 += VB) {
             if (which) {
                 // Value words: lane 4 g' + c' takes dimension group g' of positions 2 c' and 2 c' + 1.
 #pragma unroll
                 for (int v = 0; v < VB; ++v)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const uint32_t even = __shfl_sync(0xffffffffu, words[v][j], 8 * c + (g >> 1));
-                        const uint32_t odd = __shfl_sync(0xffffffffu, words[v][j], 8 * c + 4 + (g >> 1));
-                        words[v][j] = __byte_perm(even, odd, g & 1 ? 0x7632 : 0x5410);
+                        const uint32_t even = __shfl_sync(0xffffffffu, words[b0 + v][j], 8 * c + (g >> 1));
+                        const uint32_t odd = __shfl_sync(0xffffffffu, words[b0 + v][j], 8 * c + 4 + (g >> 1));
+                        words[b0 + v][j] = __byte_perm(even, odd, g & 1 ? 0x7632 : 0x5410);
                     }
             }
             uint32_t *const codes = (uint32_t *)tile + kv4_code_word(VB, b0, lane, 0);
             if (full) {
-                if constexpr (VB == 2) *(uint4 *)codes = make_uint4(words[0][0], words[0][1], words[1][0], words[1][1]);
-                else *(uint2 *)codes = make_uint2(words[0][0], words[0][1]);
+                if constexpr (VB == 2) *(uint4 *)codes = make_uint4(words[b0][0], words[b0][1], words[b0 + 1][0], words[b0 + 1][1]);
+                else *(uint2 *)codes = make_uint2(words[b0][0], words[b0][1]);
             } else {
 #pragma unroll
                 for (int v = 0; v < VB; ++v)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         if (which == 0) {
-                            if (in[j]) codes[2 * v + j] = words[v][j];
+                            if (in[j]) codes[2 * v + j] = words[b0 + v][j];
                         } else {
                             const int t = 8 * j + 2 * c;
                             uint16_t *const shorts = (uint16_t *)(codes + 2 * v + j);
-                            if (t >= rows.t0 && t < rows.t0 + count) shorts[0] = (uint16_t)words[v][j];
-                            if (t + 1 >= rows.t0 && t + 1 < rows.t0 + count) shorts[1] = (uint16_t)(words[v][j] >> 16);
+                            if (t >= rows.t0 && t < rows.t0 + count) shorts[0] = (uint16_t)words[b0 + v][j];
+                            if (t + 1 >= rows.t0 && t + 1 < rows.t0 + count) shorts[1] = (uint16_t)(words[b0 + v][j] >> 16);
                         }
                     }
             }
@@ -373,10 +479,10 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS, 6) kv4_append_kernel(cons
                 if (c == v) {
                     uint32_t *const to = (uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b0 + v, g);
                     if (full) {
-                        *(uint2 *)to = make_uint2(params[v][0], params[v][1]);
+                        *(uint2 *)to = make_uint2(params[b0 + v][0], params[b0 + v][1]);
                     } else {
-                        if (in[0]) to[0] = params[v][0];
-                        if (in[1]) to[1] = params[v][1];
+                        if (in[0]) to[0] = params[b0 + v][0];
+                        if (in[1]) to[1] = params[b0 + v][1];
                     }
                 }
         }
@@ -425,7 +531,13 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_read_kernel(const __g
                 const float2 sz = __half22float2(*reinterpret_cast<const __half2 *>(j ? &params[b].y : &params[b].x));
                 float x[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = tile ? fadd(sz.y, fmul(sz.x, (float)(word >> (4 * i) & 15u))) : 0.0f;
+                for (int i = 0; i < 8; i += 2) {             // a code times an f16 is exact, so that the FMA rounds as the sum does
+                    const uint64_t code = add2(pack2(__uint_as_float(0x4b000000u | (word >> (4 * i) & 15u)), __uint_as_float(0x4b000000u | (word >> (4 * i + 4) & 15u))),
+                                               pack2(-8388608.0f, -8388608.0f));
+                    const float2 v = unpack2(fma2(code, pack2(sz.x, sz.x), pack2(sz.y, sz.y)));
+                    x[i] = v.x;
+                    x[i + 1] = v.y;
+                }
                 float *const to = out + ((rows.row + t - rows.t0) * a.pool.kv + head) * D + 32 * b + 8 * c;
                 if (vectors) {
                     *(float4 *)to = make_float4(x[0], x[1], x[2], x[3]);

@@ -76,6 +76,20 @@ dim3 kv4_tile_grid(const Kv4Rows &at, const Kv4Pool &pool, int window) {
     return dim3((unsigned)((at.rows + window - 1) / window), (unsigned)((2 * pool.kv + KV4_TILE_WARPS - 1) / KV4_TILE_WARPS));
 }
 
+// Many rows of each sequence go by tiles, the others row by row.  Measured (us, by rows / by tiles), bfloat16 keys and values:
+// 256 sequences' single rows of 8 heads of 128 5.3 / 12.7; one sequence's 512 rows 4.8 / 9.1, 1024 6.7 / 7.8; 4 sequences'
+// 2048 rows each 36 / 22, of 96 37 / 20; float32 of 2 heads of 64, 8 of 1024 6.9 / 5.8.
+template <int NB>
+int32_t launch_kv4_append(cudaStream_t st, const Kv4AppendArgs &a, bool vectors) {
+    if (!a.at.row_start || a.at.rows < 16 * (int64_t)a.at.seqs || a.at.rows < 2048) {
+        const int64_t threads = a.at.rows * 2 * a.pool.kv * 4 * (NB == 3 ? 4 : NB), cta = 32 * KV4_TILE_WARPS;
+        CUDA_TRY(launch_k(kv4_append_rows_kernel<NB>, (unsigned)((threads + cta - 1) / cta), (unsigned)cta, 0, st, a, vectors));
+        return check_launch("kv4_append_rows_kernel");
+    }
+    CUDA_TRY(launch_k(kv4_append_kernel<NB>, kv4_tile_grid(a.at, a.pool, KV4_TILE), 32 * KV4_TILE_WARPS, 0, st, a, vectors));
+    return check_launch("kv4_append_kernel");
+}
+
 float bits_to_f32(int64_t bits) {
     const uint32_t u = (uint32_t)bits;
     float f;
@@ -225,16 +239,13 @@ extern "C" int32_t nc_kv4_append(void **p, const int64_t *s, void *stream) {
     const int64_t bytes = a.type == KV_F32 ? 4 : 2;
     const bool vectors = !misaligned(a.keys, 16) && !misaligned(a.values, 16) && a.key_stride * bytes % 16 == 0 &&
                          a.value_stride * bytes % 16 == 0 && !misaligned(a.cos_tab, 16) && !misaligned(a.sin_tab, 16);
-    const int window = kv4_window(a.at);
-    const dim3 grid = kv4_tile_grid(a.at, a.pool, window);
     const cudaStream_t st = (cudaStream_t)stream;
     switch (a.pool.d) {
-        case 32: CUDA_TRY(launch_k(kv4_append_kernel<1>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
-        case 64: CUDA_TRY(launch_k(kv4_append_kernel<2>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
-        case 96: CUDA_TRY(launch_k(kv4_append_kernel<3>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
-        default: CUDA_TRY(launch_k(kv4_append_kernel<4>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
+        case 32: return launch_kv4_append<1>(st, a, vectors);
+        case 64: return launch_kv4_append<2>(st, a, vectors);
+        case 96: return launch_kv4_append<3>(st, a, vectors);
+        default: return launch_kv4_append<4>(st, a, vectors);
     }
-    return check_launch("kv4_append_kernel");
 }
 
 extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {

@@ -168,6 +168,67 @@ def test_append_writes_the_reference_bytes_and_no_others(cuda, dtype, kv, d, pag
                 assert np.array_equal(got[r], want)
 
 
+@pytest.mark.parametrize("rows_of", ["few", "many"])
+@pytest.mark.parametrize("dtype,kv,d,page,rotated,odd", [("float32", 2, 64, 32, True, 0), ("bfloat16", 3, 128, 64, True, 0), ("bfloat16", 1, 96, 16, True, 8),
+                                                         ("float16", 2, 32, 16, True, 1), ("float16", 1, 128, 48, False, 3), ("float32", 1, 32, 16, False, 0)])
+def test_appends_of_few_and_many_rows_write_the_reference_bytes(cuda, rows_of, dtype, kv, d, page, rotated, odd):
+    """Both kernels of the append: ragged sequences, rows before position 0, a missing page, an end of the angles, and blocks
+    that f16 parameters hold badly (far from nought, tiny, huge, with infinities)."""
+    rng = np.random.default_rng(d + kv)
+    counts, before = ([1500, 0, 33, 700], [5, 9, -20, 31]) if rows_of == "many" else ([21, 0, 5, 33, 1], [30, 9, -3, 0, 15])
+    lengths = np.array([b + c for b, c in zip(before, counts)], np.int32)
+    table, pages = table_of(rng, np.maximum(lengths, 0), page)
+    missing = (0, (before[0] + 20) // page)                                       # a page of sequence 0
+    layout, pool = KV4Layout(kv, kv, d, page), ref.Pool(pages, kv, d, page, fill=0xA5)
+    starts, line = starts_of(counts), kv * d
+    rows = int(starts[-1])
+    host = rng.standard_normal((rows, 2, line)).astype(np.float32) * 3
+    kind = rng.integers(0, 12, rows)
+    host[kind == 0] = host[kind == 0] * 1e-3 + 1000
+    host[kind == 1] *= 1e-6
+    host[kind == 2] *= 1e4
+    if not rotated:
+        host[kind == 3, :, 7] = np.inf
+        host[kind == 4, :, 3] = -np.inf
+        host[kind == 5] = -2.5
+    x = np.zeros((rows, 2 * line + odd), np.float32)
+    x[:, :line], x[:, line: 2 * line] = host[:, 0], host[:, 1]
+    x = ref.encode(x, dtype)
+    keys, values = (ref.decode(np.ascontiguousarray(v), dtype).reshape(rows, kv, d) for v in (x[:, :line], x[:, line: 2 * line]))
+    angles = int(lengths.max()) - 3
+    rope = ref.rope_tables(angles, d) if rotated else None
+    d_pool, d_x, error = DeviceArray.of(pool.bytes), DeviceArray.of(x, dtype), error_word()
+
+    class Part(Rows):
+        def data_ptr(self):
+            return self.array.data_ptr() + line * x.itemsize
+
+    holed = table.copy()
+    holed[missing] = -1
+    serving.kv4_append(layout, d_pool, Rows(d_x, line), Part(d_x, line), DeviceArray.of(holed), DeviceArray.of(lengths),
+                       row_start=DeviceArray.of(starts), error=error, rope=None if rope is None else tuple(DeviceArray.of(t) for t in rope))
+    got = ref.Pool(pages, kv, d, page)
+    got.bytes = d_pool.numpy()
+    for i, n in enumerate(lengths):
+        first = int(n) - counts[i]
+        for r in range(counts[i]):
+            t = first + r
+            if t < 0 or (rotated and t >= angles) or (i, t // page) == missing:
+                continue
+            at = slice(starts[i] + r, starts[i] + r + 1)
+            pool.append(keys[at], values[at], table[i: i + 1], np.array([t + 1], np.int32), [0, 1], rope)
+            for h in range(kv):
+                for which in range(2):
+                    place = (table[i, t // page], 0, h, t % page, which)
+                    want = pool.get(*place)
+                    if np.isnan(want).any():                                     # of infinities that were rotated: any NaN will do
+                        assert np.array_equal(got.get(*place), want, equal_nan=True)
+                        for p in (got, pool):
+                            p.put(*place, np.zeros((d // 32, 32), np.uint8), np.zeros(d // 32, np.float16), np.zeros(d // 32, np.float16))
+    assert np.array_equal(got.bytes, pool.bytes)
+    assert error.numpy()[0] == 0
+
+
 def test_append_of_values_at_the_edge_of_the_types(cuda):
     rows, d = 8, 64
     x = np.random.default_rng(1).standard_normal((rows, d)).astype(np.float32)
