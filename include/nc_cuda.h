@@ -170,7 +170,8 @@ int32_t nc_attention(void **p, const int64_t *s, void *stream);
 int32_t nc_attention_cache(void **p, const int64_t *s, void *stream);
 
 /* NC_ERR_KERNEL if a kernel recorded a device-side fault since the last call (a TMA stage of
- * the grouped attention kernel that did not arrive within its bounded wait); clears it. */
+ * the grouped attention kernel that did not arrive within its bounded wait, or a matrix instruction of
+ * nc_kv4_attention's prompts); clears it. */
 int32_t nc_device_faults(void);
 
 /* Bounds the library's abandonable device-side waits (pipeline stages of the tensor-core
@@ -213,7 +214,7 @@ int32_t nc_selfcheck_div127(int64_t *mismatches);
  * one needs.
  *
  * The cache.  A pool of `pages` pages of `page bytes` each.  A layer's part of a page begins at `layer offset`
- * and takes kv_heads * page * d * 5 / 4 bytes: `page` positions (a multiple of 16) of every head, keys and
+ * and takes kv_heads * page * d * 5 / 4 bytes: `page` positions (a multiple of 16, 1024 at most) of every head, keys and
  * values, in blocks of 32 along the head dimension (d: 32, 64, 96 or 128), each block with an f16 scale and
  * zero and sixteen levels (layout and rounding: nanocompile_b200/csrc/nc_kv4.cuh).  Sequence i's position t
  * is in page table[i][t / page].  Rows of a call: row_start[i] .. row_start[i + 1] - 1 are sequence i's last
@@ -237,8 +238,10 @@ int32_t nc_kv4_append(void **p, const int64_t *s, void *stream);
 int32_t nc_kv4_read(void **p, const int64_t *s, void *stream);
 
 /* Attention of rows over the cache: row r at position t sees positions 0..t of its sequence; a row that sees
- * nothing gets zeros and a log-sum of -inf.  Queries are rotated where there is a table.  float32 calls
- * keep float32 accuracy (queries and probabilities as two f16 parts); 16-bit calls round each to one.
+ * nothing gets zeros and a log-sum of -inf.  Queries are rotated where there is a table.  float32 and
+ * float16 calls keep float32 accuracy (queries and probabilities in two parts); bfloat16 calls round each to
+ * one f16 part.  The scale is positive.  Rows of a sequence past `the most rows` get no output, and positions
+ * past `the most positions` no share.
  * p: [0] out [rows, heads, d]  [1] q [rows, heads, d]  [2] pool  [3] table  [4] lengths
  *    [5] row_start (nullable)  [6] cos  [7] sin (nullable)  [8] log-sums f32[rows, heads] (nullable)
  *    [9] scratch (device, >= nc_kv4_attention_scratch_bytes)  [10] error word (nullable)

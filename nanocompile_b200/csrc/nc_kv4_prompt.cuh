@@ -17,9 +17,11 @@
 //
 // Codes arrive three tiles ahead by bulk copies.  While O += P V of tile t - 1 runs, the CTA decodes the keys of t + 1; while S
 // of t runs, it looks for the largest parameters of t + 2 and decodes the values of t; then softmax and the one barrier of the
-// tile.  A second CTA on the SM fills what is left idle.  Bound by
-// the instruction rate (decoding 17 for eight values, softmax about five a score) against a tensor pipe that would need
-// half of that.
+// tile.  A second CTA on the SM fills what is left idle.
+//
+// Bound by the instruction rate: decoding takes 17 for eight values and the softmax about five a score.  Measured: 2
+// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 476 us, 0.38 PFLOP/s (the matrix pipe is busy for a
+// fifth of it, an instruction issues in half of the cycles); the products on the codes take 1.1 ms there.
 #pragma once
 
 #include "nc_kv4_attention.cuh"

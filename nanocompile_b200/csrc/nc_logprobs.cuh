@@ -14,6 +14,10 @@
 // many blocks as k reach: they are read again and their values from there up ranked.  Where that is more blocks than are
 // read at once, T is found among them, or bit by bit; where more end in T than are read at once, the first k of its equals
 // in the row's order are taken.  The last CTA of a row joins the segments, in their order.
+//
+// Measured, 151936 logits to a row, 20 best of each: 512 float32 rows 71 us (4.4 TB/s; 59 with no best asked for, 48 at the
+// rate of a copy), 512 bfloat16 rows 45 us, where unpacking and exponentials bound it; one row 8.9 us, five of them the
+// start, the join and the ranking.  A running list of the best inside the loop took 298 us for the first of these.
 #pragma once
 
 #include "nc_kv4.cuh"

@@ -70,15 +70,16 @@ int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, co
     return NC_OK;
 }
 
-// Rows that a CTA looks through for tiles: a tile's worth, or one where there are few rows or each is a sequence's only one.
-int kv4_window(const Kv4Rows &at) { return at.row_start && at.rows >= 16 * at.seqs && at.rows >= 1024 ? KV4_TILE : 1; }
+// Rows that a CTA looks through for tiles: a tile's worth, or one where tiles have few.  Measured, the read of 8 heads of 128 with
+// sixteen / one: 4 x 2048 rows 17 / 37 us, 1 x 1024 4.8 / 6.9, 1 x 256 3.2 / 4.6, one of each of 256 sequences 20 / 5.8.
+int kv4_window(const Kv4Rows &at) { return at.row_start && at.rows >= 16 * (int64_t)at.seqs ? KV4_TILE : 1; }
 dim3 kv4_tile_grid(const Kv4Rows &at, const Kv4Pool &pool, int window) {
     return dim3((unsigned)((at.rows + window - 1) / window), (unsigned)((2 * pool.kv + KV4_TILE_WARPS - 1) / KV4_TILE_WARPS));
 }
 
-// Many rows of each sequence go by tiles, the others row by row.  Measured (us, by rows / by tiles), bfloat16 keys and values:
-// 256 sequences' single rows of 8 heads of 128 5.3 / 12.7; one sequence's 512 rows 4.8 / 9.1, 1024 6.7 / 7.8; 4 sequences'
-// 2048 rows each 36 / 22, of 96 37 / 20; float32 of 2 heads of 64, 8 of 1024 6.9 / 5.8.
+// Many rows of each sequence go by tiles, the others row by row.  Measured (us, by rows / by tiles), bfloat16 keys and values of
+// 8 heads of 128: one sequence's 512 rows 4.9 / 7.2, 1024 6.9 / 7.8, 2048 10.3 / 8.9, 4 of 2048 36 / 22 (96: 37 / 20), one of
+// each of 256 sequences 5.3 / 12.7; of 2 heads of 64 1024 rows 3.4 / 5.1, 2048 4.2 / 5.1, 8 of 1024 7.1 / 6.1.
 template <int NB>
 int32_t launch_kv4_append(cudaStream_t st, const Kv4AppendArgs &a, bool vectors) {
     if (!a.at.row_start || a.at.rows < 16 * (int64_t)a.at.seqs || a.at.rows < 2048) {

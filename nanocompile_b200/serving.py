@@ -95,7 +95,7 @@ def _f32_bits(value: float) -> int:
 
 @dataclass(frozen=True)
 class KV4Layout:
-    """The sizes of a 4-bit paged cache: ``page_size`` positions (a multiple of 16) of ``layers`` layers to a page."""
+    """The sizes of a 4-bit paged cache: ``page_size`` positions (a multiple of 16, at most 1024) of ``layers`` layers to a page."""
 
     heads: int
     kv_heads: int
@@ -277,7 +277,8 @@ def kv4_attention(layout: KV4Layout, out, q, pool, table, lengths, scratch, *, m
     """Attention of the rows ``q`` over the cache, to ``out`` (``nc_kv4_attention``).
 
     Each row sees its sequence's positions up to its own (rows as in :func:`kv4_append`). ``max_length`` and ``max_rows``
-    bound the sequences' lengths and rows; what lies past them is left out. ``scale`` defaults to ``head_dim ** -0.5``.
+    bound the sequences' lengths and rows; what lies past them is left out. ``scale`` (positive) defaults to
+    ``head_dim ** -0.5``. float32 and float16 rows keep float32 accuracy; bfloat16 rows are rounded once to an f16 part.
     ``lse``: float32 ``[rows, heads]`` for the log-sums of the scores.
     """
     base, tab, lens, starts, seqs, pages, offset, width = _cache(layout, layer, pool, table, lengths, row_start)
