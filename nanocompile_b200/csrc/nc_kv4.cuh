@@ -22,8 +22,8 @@
 // Words and half-words belong to one position each, so positions are appended without reading.
 //
 // Both kernels read and write each byte once; memory's floor for 4 x 2048 rows of 8 heads of 128 (bfloat16 in, 44 MB for
-// the append; float32 out, 78 MB for the read) is 6.7 and 11.9 us.  They take 22 us, bound by the instructions of the
-// rounding (about 90 for eight values, the rotation included) and by 2.8 rounds of CTAs, and 17 us (4.5 TB/s).  One row of
+// the append; float32 out, 78 MB for the read) is 6.7 and 11.9 us.  They take 21 us, bound by the instructions of the
+// rounding (about 90 for eight values, the rotation included) and the chain before them, and 17 us (4.5 TB/s).  One row of
 // each of 256 sequences takes 5.3 and 5.8 us: the start and the chain from a row's sequence over its page to its bytes.
 #pragma once
 
@@ -254,8 +254,8 @@ __device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bo
     }
 }
 
-// The append of many rows and the read go by tiles: the rows of a call that fall into one tile are one piece of work for a
-// warp and head, keys or values, with lane 4 g + c at dimensions 32 b + 8 c .. of positions g and 8 + g: for keys the
+// The append of many rows and the read go by tiles: the rows of a call that fall into one tile are one piece of work (two for
+// the append) for a warp and head, keys or values, with lane 4 g + c at dimensions 32 b + 8 c .. of positions g and 8 + g: for keys the
 // lane's words are the ones it writes, for values two shuffles turn them.  A CTA looks through `window` rows for
 // the first rows of tiles.
 struct Kv4TileRows {
@@ -363,18 +363,19 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_append_rows_kernel(co
     if (c == 0) ((uint32_t *)(tile + 8 * D))[kv4_param_word(NB, b, t)] = params;
 }
 
+// A warp takes the positions 8 j .. 8 j + 7 of a tile: with both halves to a warp, 4 x 2048 rows took 22 us instead of 21, 2048 rows 8.9 instead of 7.2.
 template <int NB>
-__global__ void __launch_bounds__(32 * KV4_TILE_WARPS, NB > 2 ? 5 : 6) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, bool vectors) {
+__global__ void __launch_bounds__(32 * KV4_TILE_WARPS, NB == 3 ? 6 : 8) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a, bool vectors) {
     constexpr int D = 32 * NB, VB = kv4_vb(NB), HALF = D / 2, window = KV4_TILE;
     release_dependents();
     wait_for_producer();
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int job = blockIdx.y * KV4_TILE_WARPS + (threadIdx.x >> 5);     // 2 head + (0 keys, 1 values)
-    const int head = job >> 1, which = job & 1;
+    const int job = blockIdx.y * KV4_TILE_WARPS + (threadIdx.x >> 5);     // 4 head + 2 (0 keys, 1 values) + j
+    const int head = job >> 2, which = job >> 1 & 1, j = job & 1;
     if (head < a.pool.kv) {                                          // the rows are on their way while their tiles are looked up
         const int size = a.type == KV_F32 ? 4 : 2, lines = (D * size + 127) / 128;
-        for (int i = lane; i < window * lines; i += 32) {
-            const int64_t r = (int64_t)blockIdx.x * window + i / lines;
+        for (int i = lane; i < window / 2 * lines; i += 32) {
+            const int64_t r = (int64_t)blockIdx.x * window + i / lines * 2 + j;
             if (r < a.at.rows)
                 asm volatile("prefetch.global.L2 [%0];" ::"l"((const char *)(which ? a.values : a.keys) +
                              (r * (which ? a.value_stride : a.key_stride) + (int64_t)head * D) * size + min(i % lines * 128, D * size - 1)));
@@ -387,104 +388,69 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS, NB > 2 ? 5 : 6) kv4_appen
             if (a.at.error && lane == 0) atomicMin(a.at.error, (unsigned long long)rows.seq);
             count = (int)(a.positions - rows.position);
         }
+        if (rows.t0 >= 8 * j + 8 || rows.t0 + count <= 8 * j) return;
         char *const tile = rows.tile + (int64_t)head * (a.at.page / KV4_TILE) * (20 * D) + which * 10 * D;
         const void *const p = which ? a.values : a.keys;
-        const int64_t stride = which ? a.value_stride : a.key_stride;
-        const bool full = count == KV4_TILE;
-        bool in[2];
+        const int t = 8 * j + g;
+        const bool in = t >= rows.t0 && t < rows.t0 + count, rotate = which == 0 && a.cos_tab;
+        const int64_t at = (rows.row + t - rows.t0) * (which ? a.value_stride : a.key_stride) + (int64_t)head * D + 8 * c;
+        float x[NB][8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) in[j] = 8 * j + g >= rows.t0 && 8 * j + g < rows.t0 + count;
-        const bool rotate = which == 0 && a.cos_tab;
-        uint32_t words[NB][2], params[NB][2];
+        for (int b = 0; b < NB; ++b) {
+            if (in) kv_load8(p, at + 32 * b, a.type, vectors, x[b]);
+            else
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int t = 8 * j + g;
-            const int64_t at = (rows.row + t - rows.t0) * stride + (int64_t)head * D + 8 * c;
-            float x[NB][8];
+                for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
+        }
+        if (rotate && in) {                                           // as kv4_rotated, eight at a time
+            const int64_t angle = (rows.position + t - rows.t0) * HALF;
+            if constexpr (NB % 2 == 0) {                              // a lane has both of a pair
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (in[j]) kv_load8(p, at + 32 * b, a.type, vectors, x[b]);
-                else
+                for (int b = 0; b < NB / 2; ++b) {
+                    float cs[8], sn[8];
+                    kv_load8(a.cos_tab, angle + 32 * b + 8 * c, KV_F32, vectors, cs);
+                    kv_load8(a.sin_tab, angle + 32 * b + 8 * c, KV_F32, vectors, sn);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
-            }
-            if (rotate && in[j]) {                                    // as kv4_rotated, eight at a time
-                const int64_t angle = (rows.position + t - rows.t0) * HALF;
-                if constexpr (NB % 2 == 0) {                          // a lane has both of a pair
-#pragma unroll
-                    for (int b = 0; b < NB / 2; ++b) {
-                        float cs[8], sn[8];
-                        kv_load8(a.cos_tab, angle + 32 * b + 8 * c, KV_F32, vectors, cs);
-                        kv_load8(a.sin_tab, angle + 32 * b + 8 * c, KV_F32, vectors, sn);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float u = x[b][i], v = x[b + NB / 2][i];
-                            x[b][i] = fsub(fmul(u, cs[i]), fmul(v, sn[i]));
-                            x[b + NB / 2][i] = fadd(fmul(v, cs[i]), fmul(u, sn[i]));
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const int i0 = 32 * b + 8 * c;
-                        const bool low = i0 < HALF;
-                        const int k = low ? i0 : i0 - HALF;
-                        float y[8], cs[8], sn[8];
-                        kv_load8(p, at - 8 * c + (low ? i0 + HALF : k), a.type, vectors, y);
-                        kv_load8(a.cos_tab, angle + k, KV_F32, vectors, cs);
-                        kv_load8(a.sin_tab, angle + k, KV_F32, vectors, sn);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            x[b][i] = low ? fsub(fmul(x[b][i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[b][i], cs[i]), fmul(y[i], sn[i]));
+                    for (int i = 0; i < 8; ++i) {
+                        const float u = x[b][i], v = x[b + NB / 2][i];
+                        x[b][i] = fsub(fmul(u, cs[i]), fmul(v, sn[i]));
+                        x[b + NB / 2][i] = fadd(fmul(v, cs[i]), fmul(u, sn[i]));
                     }
                 }
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) words[b][j] = kv4_quantise(x[b], &params[b][j]);
-        }
-#pragma unroll
-        for (int b0 = 0; b0 < NB; b0 += VB) {
-            if (which) {
-                // Value words: lane 4 g' + c' takes dimension group g' of positions 2 c' and 2 c' + 1.
-#pragma unroll
-                for (int v = 0; v < VB; ++v)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t even = __shfl_sync(0xffffffffu, words[b0 + v][j], 8 * c + (g >> 1));
-                        const uint32_t odd = __shfl_sync(0xffffffffu, words[b0 + v][j], 8 * c + 4 + (g >> 1));
-                        words[b0 + v][j] = __byte_perm(even, odd, g & 1 ? 0x7632 : 0x5410);
-                    }
-            }
-            uint32_t *const codes = (uint32_t *)tile + kv4_code_word(VB, b0, lane, 0);
-            if (full) {
-                if constexpr (VB == 2) *(uint4 *)codes = make_uint4(words[b0][0], words[b0][1], words[b0 + 1][0], words[b0 + 1][1]);
-                else *(uint2 *)codes = make_uint2(words[b0][0], words[b0][1]);
             } else {
 #pragma unroll
-                for (int v = 0; v < VB; ++v)
+                for (int b = 0; b < NB; ++b) {
+                    const int i0 = 32 * b + 8 * c;
+                    const bool low = i0 < HALF;
+                    const int k = low ? i0 : i0 - HALF;
+                    float y[8], cs[8], sn[8];
+                    kv_load8(p, at - 8 * c + (low ? i0 + HALF : k), a.type, vectors, y);
+                    kv_load8(a.cos_tab, angle + k, KV_F32, vectors, cs);
+                    kv_load8(a.sin_tab, angle + k, KV_F32, vectors, sn);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (which == 0) {
-                            if (in[j]) codes[2 * v + j] = words[b0 + v][j];
-                        } else {
-                            const int t = 8 * j + 2 * c;
-                            uint16_t *const shorts = (uint16_t *)(codes + 2 * v + j);
-                            if (t >= rows.t0 && t < rows.t0 + count) shorts[0] = (uint16_t)words[b0 + v][j];
-                            if (t + 1 >= rows.t0 && t + 1 < rows.t0 + count) shorts[1] = (uint16_t)(words[b0 + v][j] >> 16);
-                        }
-                    }
-            }
-#pragma unroll
-            for (int v = 0; v < VB; ++v)
-                if (c == v) {
-                    uint32_t *const to = (uint32_t *)(tile + 8 * D) + kv4_param_word(NB, b0 + v, g);
-                    if (full) {
-                        *(uint2 *)to = make_uint2(params[b0 + v][0], params[b0 + v][1]);
-                    } else {
-                        if (in[0]) to[0] = params[b0 + v][0];
-                        if (in[1]) to[1] = params[b0 + v][1];
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        x[b][i] = low ? fsub(fmul(x[b][i], cs[i]), fmul(y[i], sn[i])) : fadd(fmul(x[b][i], cs[i]), fmul(y[i], sn[i]));
                 }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t params, word = kv4_quantise(x[b], &params);
+            uint32_t *const code = (uint32_t *)tile + kv4_code_word(VB, b, lane, j);
+            if (which) {
+                // Value words: lane 4 g' + c' takes dimension group g' of positions 2 c' and 2 c' + 1.
+                const uint32_t even = __shfl_sync(0xffffffffu, word, 8 * c + (g >> 1));
+                const uint32_t odd = __shfl_sync(0xffffffffu, word, 8 * c + 4 + (g >> 1));
+                word = __byte_perm(even, odd, g & 1 ? 0x7632 : 0x5410);
+                const int t2 = 8 * j + 2 * c;
+                const bool first = t2 >= rows.t0 && t2 < rows.t0 + count, second = t2 + 1 >= rows.t0 && t2 + 1 < rows.t0 + count;
+                if (first && second) *code = word;
+                else if (first) ((uint16_t *)code)[0] = (uint16_t)word;
+                else if (second) ((uint16_t *)code)[1] = (uint16_t)(word >> 16);
+            } else if (in) {
+                *code = word;
+            }
+            if (in && c == (b & 3)) ((uint32_t *)(tile + 8 * D))[kv4_param_word(NB, b, t)] = params;
         }
     });
 }

@@ -73,13 +73,13 @@ int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, co
 // Rows that a CTA looks through for tiles: a tile's worth, or one where tiles have few.  Measured, the read of 8 heads of 128 with
 // sixteen / one: 4 x 2048 rows 17 / 37 us, 1 x 1024 4.8 / 6.9, 1 x 256 3.2 / 4.6, one of each of 256 sequences 20 / 5.8.
 int kv4_window(const Kv4Rows &at) { return at.row_start && at.rows >= 16 * (int64_t)at.seqs ? KV4_TILE : 1; }
-dim3 kv4_tile_grid(const Kv4Rows &at, const Kv4Pool &pool, int window) {
-    return dim3((unsigned)((at.rows + window - 1) / window), (unsigned)((2 * pool.kv + KV4_TILE_WARPS - 1) / KV4_TILE_WARPS));
+dim3 kv4_tile_grid(const Kv4Rows &at, const Kv4Pool &pool, int window, int jobs) {       // jobs: warps to a tile and head
+    return dim3((unsigned)((at.rows + window - 1) / window), (unsigned)((jobs * pool.kv + KV4_TILE_WARPS - 1) / KV4_TILE_WARPS));
 }
 
 // Many rows of each sequence go by tiles, the others row by row.  Measured (us, by rows / by tiles), bfloat16 keys and values of
-// 8 heads of 128: one sequence's 512 rows 4.9 / 7.2, 1024 6.9 / 7.8, 2048 10.3 / 8.9, 4 of 2048 36 / 22 (96: 37 / 20), one of
-// each of 256 sequences 5.3 / 12.7; of 2 heads of 64 1024 rows 3.4 / 5.1, 2048 4.2 / 5.1, 8 of 1024 7.1 / 6.1.
+// 8 heads of 128: one sequence's 512 rows 4.7 / 5.3, 1024 6.7 / 6.6, 2048 10.3 / 7.2, 4 of 2048 36 / 21 (96: 36 / 23), one of
+// each of 256 sequences 5.3 / 12.7; of 2 heads of 64 1024 rows 3.4 / 3.9, 2048 4.1 / 4.1, 8 of 1024 7.1 / 5.6.
 template <int NB>
 int32_t launch_kv4_append(cudaStream_t st, const Kv4AppendArgs &a, bool vectors) {
     if (!a.at.row_start || a.at.rows < 16 * (int64_t)a.at.seqs || a.at.rows < 2048) {
@@ -87,7 +87,7 @@ int32_t launch_kv4_append(cudaStream_t st, const Kv4AppendArgs &a, bool vectors)
         CUDA_TRY(launch_k(kv4_append_rows_kernel<NB>, (unsigned)((threads + cta - 1) / cta), (unsigned)cta, 0, st, a, vectors));
         return check_launch("kv4_append_rows_kernel");
     }
-    CUDA_TRY(launch_k(kv4_append_kernel<NB>, kv4_tile_grid(a.at, a.pool, KV4_TILE), 32 * KV4_TILE_WARPS, 0, st, a, vectors));
+    CUDA_TRY(launch_k(kv4_append_kernel<NB>, kv4_tile_grid(a.at, a.pool, KV4_TILE, 4), 32 * KV4_TILE_WARPS, 0, st, a, vectors));
     return check_launch("kv4_append_kernel");
 }
 
@@ -258,7 +258,7 @@ extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {
     if (!a.keys || !a.values) return fail(NC_ERR_ARGUMENT, "null keys or values");
     const bool vectors = !misaligned(a.keys, 16) && !misaligned(a.values, 16);
     const int window = kv4_window(a.at);
-    const dim3 grid = kv4_tile_grid(a.at, a.pool, window);
+    const dim3 grid = kv4_tile_grid(a.at, a.pool, window, 2);
     const cudaStream_t st = (cudaStream_t)stream;
     switch (a.pool.d) {
         case 32: CUDA_TRY(launch_k(kv4_read_kernel<1>, grid, 32 * KV4_TILE_WARPS, 0, st, a, window, vectors)); break;
