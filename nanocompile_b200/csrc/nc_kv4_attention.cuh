@@ -34,7 +34,7 @@
 // Measured (us; memory's floor for the cache in brackets): one sequence of 97 positions and 14 heads on 2 of 64 5.8, the
 // start and two steps; 64 of 2048 12.2 (3.3), the latency of the two steps that each of 2048 warps makes; bfloat16, 24
 // sequences of up to 16384 and 32 heads on 8 of 128 85 (43), the instruction rate, with lengths that differ; 512 rows of a
-// prompt 23 (0.6).
+// prompt 17.8 (0.6).
 #pragma once
 
 #include <type_traits>

@@ -110,18 +110,22 @@ constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: thei
 constexpr int KV4_STAGES = 2;
 // bfloat16 rows go to the tensor cores' kernel from this many columns of a sequence and tiles (128 columns by 64 positions)
 // of the call.  Below, its start, its wide parts and few CTAs cost more than they give.  Measured, it against the products on
-// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 70 against 157 us, 2 of
-// 300 over 300 (800) 39 against 83, 4 of 64 over 500 (512) 41 against 44, one of 64 over 2000 (512) 42 against 26; 64: 1024
-// rows of 14 heads (1792) 45 against 49, 256 over 4000 (1764) 49 against 46.
+// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 71 against 93 us, 2 of
+// 300 over 300 (800) 41 against 58, 4 of 64 over 500 (512) 41 against 38, one of 64 over 2000 (512) 41 against 25, of 512 over
+// 512 (1024) 59 against 57; 64: 4 of 512 rows of 14 heads (1792) 34 against 70, 1024 rows (1792) 45 against 45, 256 over 4000
+// (1764) 49 against 47.
 constexpr int64_t KV4_PROMPT_COLS = 96;
 constexpr int64_t kv4_prompt_tiles(int64_t d) { return d == 128 ? 600 : 1780; }
 
-// Warps of a CTA and splits of the histories: the cheapest by a model of the measured times, in units of a step on an SM
-// that is full (3.3 us; 16 warps of 8 columns fill it, 8 of more): a CTA starts in about half a step, the join of
-// splits takes another half, wide CTAs lose a little to their barriers.  Few rounds of CTAs count as whole ones, as equal
-// histories take them; for long histories the last CTA's half counts instead, as lengths differ.  Measured: 64
-// sequences of 2048 positions and two heads 12.3 us in 128 CTAs of 16 warps, 14.9 in 512 of four; 128 sequences of 512
-// 8.5 us in 256 CTAs of eight, 11.3 of four, 12.0 of sixteen; 32 of 2048 and 16 heads 33 us in 512 of four, 45 of sixteen.
+// Columns and warps of a CTA, and splits of the histories: the cheapest by a model of the measured times, in units of a step on
+// an SM that is full (3.3 us; 16 warps of 8 columns fill it, or 8 of 16, which share the codes' way to operands): a CTA
+// starts in about half a step, the join of splits takes another half in every round, wide CTAs lose a little to their
+// barriers.  Few rounds of CTAs count as whole ones, as equal histories take them; for long histories the last CTA's half
+// counts instead, as lengths differ, and for prompts the mean over their rows.  Measured: 64 sequences of 2048 positions and
+// two heads 12.3 us in 128 CTAs of 16 warps, 14.9 in 512 of four; 128 sequences of 512 8.5 us in 256 CTAs of eight, 11.3 of
+// four, 12.0 of sixteen; 32 of 2048 and 16 heads 33 us in 512 of four, 45 of sixteen; a float32 prompt of 512 rows of 7 heads a
+// key head 17.8 us by 8 columns and four warps, 23 of eight, 21 by 16 columns and four; of 1024 rows 41.6 by 8, 44.7 by 16;
+// bfloat16, 8 sequences of 16 rows of 4 heads over 2000 41 us by 16, 48 by 8.
 AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length, bool bf16) {
     AttnPlan p{};
     const int64_t cols = heads / kv * max_rows;
@@ -137,31 +141,46 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
         p.splits = (int)((steps + p.chunk - 1) / p.chunk);
         return p;
     }
-    p.nt = cols <= 8 ? 1 : cols <= 16 || d > 64 ? 2 : 4;
-    p.col_blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
-    p.groups = seqs * kv * p.col_blocks;
     const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, steps = std::max<int64_t>(1, (max_length + step - 1) / step);
-    const int64_t most = p.groups > KV4_COUNTERS ? 1 : std::min<int64_t>(64, steps);
+    const int64_t first = std::max<int64_t>(1, (max_length - max_rows + step) / step);       // of the first row
     float best = 0.0f;
-    for (int warps = p.nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
-        const int64_t places = 148 * (p.nt == 1 ? 16 : 8) / warps;
-        for (int splits : CUTS) {
-            if (splits > most) break;
-            const int64_t chunk = (steps + splits - 1) / splits, active = (steps + chunk - 1) / chunk;
-            if (active != splits) continue;                              // as good as fewer
-            const int64_t mine = (chunk + warps - 1) / warps;            // steps of a warp
-            const float rounds = (float)(p.groups * active) / (float)places, whole = (float)((p.groups * active + places - 1) / places);
-            const bool few = whole * (float)mine <= 16.0f;
-            const float work = few ? whole * (float)mine : (rounds > 1.0f ? rounds : 1.0f) * (float)mine + 0.5f * (float)mine;
-            const float start = 0.25f + 0.125f * (float)(4 * p.nt) / (float)warps;   // the more queries a warp has to bring
-            const float cost = work * (1.0f + (few ? 0.0025f : 0.01f) * (float)warps) + start * whole + (active > 1 ? 0.5f + 0.015f * (float)active : 0.0f);
-            if (p.warps == 0 || cost < best) {
-                best = cost;
-                p.warps = (int)warps;
-                p.chunk = (int)chunk;
-                p.splits = (int)active;
+    for (int nt = 1; nt <= (cols <= 8 ? 1 : 2); ++nt) {
+        const int64_t col_blocks = (cols + 8 * nt - 1) / (8 * nt), groups = seqs * kv * col_blocks;
+        const int64_t most = groups > KV4_COUNTERS ? 1 : std::min<int64_t>(64, steps);
+        for (int warps = nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
+            const int64_t places = 148 * (nt == 1 ? 16 : 8) / warps;
+            for (int splits : CUTS) {
+                if (splits > most) break;
+                const int64_t chunk = (steps + splits - 1) / splits, active = (steps + chunk - 1) / chunk;
+                if (active != splits) continue;                          // as good as fewer
+                const int64_t mine = (chunk + warps - 1) / warps;        // steps of a warp
+                const float rounds = (float)(groups * active) / (float)places, whole = (float)((groups * active + places - 1) / places);
+                const bool few = whole * (float)mine <= 16.0f, grows = steps - first >= warps && rounds > 1.0f;
+                const float turns = rounds > 1.0f ? rounds : 1.0f;
+                float mean = (float)mine;                                // of a warp's steps, over a prompt's rows
+                if (grows) {
+                    mean = 0.0f;
+                    for (int i = 1; i < 8; i += 2) {
+                        const int64_t sees = first + (steps - first) * i / 8, rest = sees % chunk;
+                        mean += 0.25f / (float)active * (float)(sees / chunk * mine + (rest + warps - 1) / warps);
+                    }
+                }
+                float work = few && !grows ? whole * (float)mine : turns * mean + 0.5f * (float)mine;
+                if (nt > 1) work *= 0.98f;
+                const float start = 0.25f + 0.125f * (float)(4 * nt) / (float)warps;   // the more queries a warp has to bring
+                const float cost = work * (1.0f + (few ? 0.0025f : 0.01f) * (float)warps) + start * (grows ? turns + 0.5f : whole) +
+                                   (active > 1 ? (0.5f + 0.015f * (float)active) * turns : 0.0f);
+                if (p.warps == 0 || cost < best) {
+                    best = cost;
+                    p.nt = nt;
+                    p.col_blocks = (int)col_blocks;
+                    p.groups = groups;
+                    p.warps = warps;
+                    p.chunk = (int)chunk;
+                    p.splits = (int)active;
+                }
+                if (groups * splits > 16 * places) break;
             }
-            if (p.groups * splits > 16 * places) break;
         }
     }
     return p;
@@ -188,9 +207,7 @@ int32_t launch_kv4_attention_n(cudaStream_t st, const Kv4AttnArgs &a, const Attn
         if (p.warps == 8) return launch_kv4_attention_t<D, 1, HL, 8>(st, a, ctas);
         return launch_kv4_attention_t<D, 1, HL, 16>(st, a, ctas);
     }
-    if (p.nt == 2) return p.warps == 4 ? launch_kv4_attention_t<D, 2, HL, 4>(st, a, ctas) : launch_kv4_attention_t<D, 2, HL, 8>(st, a, ctas);
-    if constexpr (D <= 64) return p.warps == 4 ? launch_kv4_attention_t<D, 4, HL, 4>(st, a, ctas) : launch_kv4_attention_t<D, 4, HL, 8>(st, a, ctas);
-    return fail(NC_ERR_ARGUMENT, "no kernel of %d columns for head dimension %d", 8 * p.nt, D);
+    return p.warps == 4 ? launch_kv4_attention_t<D, 2, HL, 4>(st, a, ctas) : launch_kv4_attention_t<D, 2, HL, 8>(st, a, ctas);
 }
 
 template <int D>
