@@ -33,7 +33,7 @@
 //
 // Measured (us; memory's floor for the cache in brackets): one sequence of 97 positions and 14 heads on 2 of 64 5.8, the
 // start and two steps; 64 of 2048 12.2 (3.3), the latency of the two steps that each of 2048 warps makes; bfloat16, 24
-// sequences of up to 16384 and 32 heads on 8 of 128 85 (43), the instruction rate, with lengths that differ; 512 rows of a
+// sequences of up to 16384 and 32 heads on 8 of 128 87 (43), the instruction rate, with lengths that differ; 512 rows of a
 // prompt 17.8 (0.6).
 #pragma once
 
@@ -210,9 +210,9 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     wait_for_producer();
     const int split = (int)(blockIdx.x % a.splits);
     const unsigned group = blockIdx.x / a.splits;
-    const int cb = a.col_blocks - 1 - (int)(group % a.col_blocks);     // the longest histories first
-    const int head = (int)(group / a.col_blocks % a.pool.kv);
-    const int seq = (int)(group / a.col_blocks / a.pool.kv);
+    const int cb = a.col_blocks - 1 - (int)(group / a.pool.kv / a.at.seqs);   // the rows that see most first
+    const int head = (int)(group % a.pool.kv);
+    const int seq = (int)(group / a.pool.kv % a.at.seqs);
     const int length = a.at.lengths[seq];
     const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
     const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;

@@ -20,7 +20,7 @@
 // tile.  A second CTA on the SM fills what is left idle.
 //
 // Bound by the instruction rate: decoding takes 17 for eight values and the softmax about five a score.  Measured: 2
-// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 476 us, 0.38 PFLOP/s (the matrix pipe is busy for a
+// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 458 us, 0.39 PFLOP/s (the matrix pipe is busy for a
 // fifth of it, an instruction issues in half of the cycles); the products on the codes take 1.1 ms there.
 #pragma once
 
@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     wait_for_producer();
     const int split = (int)(blockIdx.x % a.splits);
     const unsigned group = blockIdx.x / a.splits;
-    const int cb = a.col_blocks - 1 - (int)(group % a.col_blocks);     // the longest histories first
-    const int head = (int)(group / a.col_blocks % a.pool.kv);
-    const int seq = (int)(group / a.col_blocks / a.pool.kv);
+    const unsigned histories = (unsigned)(a.at.seqs * a.pool.kv), history = group % histories;
+    const int cb = a.col_blocks - 1 - (int)(group / histories);        // the rows that see most first, of all sequences and heads: 479 -> 458 us, a 1024-row prompt 65 -> 58
+    const int head = (int)(history % a.pool.kv), seq = (int)(history / a.pool.kv);
     const int length = a.at.lengths[seq];
     const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
     const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;

@@ -110,9 +110,9 @@ constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: thei
 constexpr int KV4_STAGES = 2;
 // bfloat16 rows go to the tensor cores' kernel from this many columns of a sequence and tiles (128 columns by 64 positions)
 // of the call.  Below, its start, its wide parts and few CTAs cost more than they give.  Measured, it against the products on
-// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 71 against 93 us, 2 of
-// 300 over 300 (800) 41 against 58, 4 of 64 over 500 (512) 41 against 38, one of 64 over 2000 (512) 41 against 25, of 512 over
-// 512 (1024) 59 against 57; 64: 4 of 512 rows of 14 heads (1792) 34 against 70, 1024 rows (1792) 45 against 45, 256 over 4000
+// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 70 against 93 us, 2 of
+// 300 over 300 (800) 36 against 58, 4 of 64 over 500 (512) 41 against 38, one of 64 over 2000 (512) 41 against 25, of 512 over
+// 512 (1024) 59 against 57; 64: 4 of 512 rows of 14 heads (1792) 29 against 70, 1024 rows (1792) 40 against 45, 256 over 4000
 // (1764) 49 against 47.
 constexpr int64_t KV4_PROMPT_COLS = 96;
 constexpr int64_t kv4_prompt_tiles(int64_t d) { return d == 128 ? 600 : 1780; }
