@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(const __g
 #pragma unroll
         for (int i = 1; i < LP_VECS; ++i) top = max_nan(top, lp_vector_max<TYPE>(raw[i]));
         if (a.k) sh.block[batches][tid] = lp_order(top);
-        if (!(top <= sum.m)) {                                   // a larger value, or a NaN
+        if (top > sum.m || top != top) {                         // a larger value, or a NaN, which then stays the maximum
             const float s = pair.x + pair.y, e = epair.x + epair.y;
             const float d = max_nan(sum.m - top, LP_LEAST), w = lp_exp2(d * LP_LOG2E);
             pair = make_float2(s * w, 0.0f);

@@ -716,3 +716,20 @@ def test_more_rows_than_a_launch_and_scratch_from_shape_to_shape(cuda):
         check_scores(long, targets[1], 32, scratch=scratch)
         check_scores(many, targets[0], 3, scratch=scratch)
         check_scores(rng.standard_normal((9, 151936)), rng.integers(0, 151936, (9, 1)), 32, scratch=scratch)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(64, 151936), (592, 40001)])             # several segments of several batches, and one
+def test_a_nan_anywhere_in_a_long_row_comes_first(cuda, dtype, rows, vocab):
+    x = np.zeros((rows, vocab), np.float32)
+    x[:8] = np.random.default_rng(vocab).standard_normal((8, vocab)) * 3
+    for r, at in enumerate(([100], [vocab // 2], [vocab - 1], [vocab - 1, vocab // 3], [7], list(range(40, 80)))):
+        x[r, at] = np.nan
+    x[4, 8:] = -np.inf                                # nothing after the NaN
+    targets = np.tile(np.array([[0, vocab - 2]]), (rows, 1))
+    x = ref.decode(ref.encode(x, dtype), dtype)
+    got = scores(x, targets, 20, dtype)
+    want = ref.logprobs(x[:8], targets[:8], 20)
+    assert np.array_equal(got[3][:8], want[3])
+    for i in (0, 1, 2, 4):
+        assert np.isnan(got[i][:6]).all() and np.isfinite(got[i][6:]).all()
