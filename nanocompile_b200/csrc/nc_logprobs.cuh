@@ -298,15 +298,25 @@ __device__ __forceinline__ void lp_segment_top(const LogprobArgs &a, LpShared &s
     }
     __syncthreads();
     if (!all) {                                                    // the first k equals, in the row's order
+        static_assert((LP_MAX_TOP - 1) * SIZE + LP_MAX_TOP <= LP_CAND, "values of fewer than k blocks, and k equals");
         int found = 0;
         for (int64_t e0 = max((int64_t)0, seg0 * N - skew); found < a.k && e0 < min(a.vocab, v_end * N - skew); e0 += LP_THREADS) {
             const int64_t e = e0 + tid;
             const unsigned long long key = e < min(a.vocab, v_end * N - skew) ? lp_key(kv_load(base, e, TYPE), (uint32_t)e) : 0;
             const bool is = key != 0 && (uint32_t)(key >> 32) == kth;
-            if (is) sh.cand[atomicAdd(&sh.count, 1)] = key;
-            found += __syncthreads_count(is);
+            const uint32_t equals = __ballot_sync(0xffffffffu, is);
+            if (lane == 0) sh.round[warp] = __popc(equals);
+            __syncthreads();
+            int rank = found + __popc(equals & ((1u << lane) - 1));
+#pragma unroll
+            for (int w = 0; w < LP_THREADS / 32; ++w) {
+                const int n = (int)sh.round[w];
+                if (w < warp) rank += n;
+                found += n;
+            }
+            if (is && rank < a.k) sh.cand[atomicAdd(&sh.count, 1)] = key;
+            __syncthreads();
         }
-        __syncthreads();
     }
     lp_rank(sh.cand, sh.count, a.k, sh.best);
     __syncthreads();

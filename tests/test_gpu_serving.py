@@ -733,3 +733,38 @@ def test_a_nan_anywhere_in_a_long_row_comes_first(cuda, dtype, rows, vocab):
     assert np.array_equal(got[3][:8], want[3])
     for i in (0, 1, 2, 4):
         assert np.isnan(got[i][:6]).all() and np.isfinite(got[i][6:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 592])                                       # several segments of a row, and one
+def test_equals_below_many_better_logits(cuda, dtype, rows):
+    """Whole blocks above the k-th best, and masses of equals from there down: no more of them than are wanted are taken."""
+    vocab, rng = 8192, np.random.default_rng(rows)
+    x = np.zeros((rows, vocab), np.float32)
+    x[0] = -np.inf
+    for u in range(4):                                # with vectors of eight, these are all of the first 31 threads' blocks
+        x[0, 2048 * u: 2048 * u + 248] = rng.permutation(248) + 1000 * (u == 2)
+        x[1, 2048 * u: 2048 * u + 248] = 5
+        if rows > 2:
+            x[2, 2048 * u: 2048 * u + 248] = 5 + (np.arange(248) % 8 == 0)
+            x[3, 1024 * u: 1024 * u + 124] = rng.permutation(124) + 1        # the same with vectors of four
+    if rows > 4:
+        x[4] = np.round(rng.standard_normal(vocab))
+        x[5, ::50] = 1                                # more equals at the top than are wanted
+        x[6, 8100:] = 1
+    for k in (25, 31, 32):
+        check_scores(x, rng.integers(0, vocab, (rows, 1)), k, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("vocab", [257, 5000, 151936])
+def test_equal_logits_of_16_bits_go_by_their_index(cuda, dtype, vocab):
+    rng = np.random.default_rng(vocab)
+    x = np.zeros((6, vocab))
+    x[1] = np.round(rng.standard_normal(vocab))
+    x[2, rng.integers(0, vocab, 40)] = 1
+    x[3] = -np.inf
+    x[3, vocab // 2:] = 2
+    x[4] = np.arange(vocab) // 50
+    x[5, ::2] = -0.0
+    check_scores(x, rng.integers(0, vocab, (6, 2)), 32, dtype)
