@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     const int cols = nr * a.group, col0 = cb * COLS;                   // the entry point bounds rows * group
     if (col0 >= cols) return;
     const int ncol = min(cols - col0, COLS);
-    // Positions 0 .. end - 1 are seen by the block's last row, all of 0 .. first by every row of it.
-    const int first = length - nr + col0 / a.group, last = length - nr + (col0 + ncol - 1) / a.group;
+    // Positions 0 .. end - 1 are seen by the block's last row, all of 0 .. first by every row of it: none where a row has no angle.
+    const int last = length - nr + (col0 + ncol - 1) / a.group;
+    const int first = a.cos_tab && last >= a.positions ? -1 : length - nr + col0 / a.group;
     const int end = last < 0 ? 0 : last + 1;
     const int steps = min((end + STEP - 1) / STEP, a.splits * a.chunk);   // no more than the call provides for
     const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;

@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const int cols = nr * a.group, col0 = cb * KVT_COLS;
     if (col0 >= cols) return;
     const int ncol = min(cols - col0, KVT_COLS);
-    const int first = length - nr + col0 / a.group, last = length - nr + (col0 + ncol - 1) / a.group;
+    const int last = length - nr + (col0 + ncol - 1) / a.group;
+    const int first = a.cos_tab && last >= a.positions ? -1 : length - nr + col0 / a.group;      // as there
     const int end = last < 0 ? 0 : last + 1;
     const int steps = min((end + KVT_STEP - 1) / KVT_STEP, a.splits * a.chunk);
     const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;

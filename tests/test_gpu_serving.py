@@ -768,3 +768,26 @@ def test_equal_logits_of_16_bits_go_by_their_index(cuda, dtype, vocab):
     x[4] = np.arange(vocab) // 50
     x[5, ::2] = -0.0
     check_scores(x, rng.integers(0, vocab, (6, 2)), 32, dtype)
+
+
+@pytest.mark.parametrize("dtype,d,bounds", [("float32", 64, {}), ("float16", 128, {}), ("bfloat16", 96, {}), ("bfloat16", 64, dict(max_length=100000)),
+                                            ("bfloat16", 128, dict(max_length=100000))])
+def test_rows_without_an_angle_see_nothing_of_a_long_history(cuda, dtype, d, bounds):
+    """Rows past the table's end get zeros and -inf, whole steps before them or not; the others of their block what they see."""
+    rng = np.random.default_rng(d)
+    layout, angles = KV4Layout(4, 1, d, 16), 250
+    case = Case(rng, [300, 200], 1, d, 16)
+    counts = [100, 30]                                # positions 200 .. 299, and 170 .. 199
+    q = ref.decode(ref.encode(rng.standard_normal((130, 4, d)).astype(np.float32), dtype), dtype)
+    rope, error = ref.rope_tables(300, d), error_word()
+    got, lse = case.attend(layout, q, dtype, counts, tuple(t[:angles].copy() for t in rope), error=error, **bounds)
+    assert error.numpy()[0] == 0
+    want, want_lse, size = ref.attention(q, case.histories, case.lengths, starts_of(counts), np.float32(d ** -0.5), rope)
+    none = np.arange(130) // 50 == 1
+    none[100:] = False
+    assert not got[none].any() and np.isneginf(lse[none]).all()
+    most = max(np.abs(v).max() for _, v in case.histories)
+    assert (np.abs(got - want) <= attention_bound(dtype, want, size, most))[~none].all()
+    assert np.isfinite(lse[~none]).all()
+    alone, lse = case.attend(layout, q[:2], dtype, [1, 1], tuple(t[:180].copy() for t in rope))       # single tokens, both past the end
+    assert not alone.any() and np.isneginf(lse).all()
