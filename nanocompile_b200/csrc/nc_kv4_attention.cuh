@@ -58,7 +58,8 @@ struct Kv4AttnArgs {
     int64_t q_stride, out_stride, positions;
     uint64_t page_magic;               // ceil(2^37 / tiles of a page): the tile's page by a multiplication
     float scale_log2e;
-    int type, heads, group, col_blocks, splits, chunk;   // chunk: steps of a split
+    int type, heads, group, col_blocks, splits, chunk;   // chunk: steps of a split; splits * chunk steps hold max_length
+    int max_rows, max_length;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint2 &b) {
@@ -217,14 +218,14 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
     const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
     const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;
     if (row0 < 0 || nr <= 0 || (int64_t)row0 + nr > a.at.rows) return;
-    const int cols = nr * a.group, col0 = cb * COLS;                   // the entry point bounds rows * group
+    const int cols = min(nr, a.max_rows) * a.group, col0 = cb * COLS;  // the entry point bounds rows * group
     if (col0 >= cols) return;
     const int ncol = min(cols - col0, COLS);
     // Positions 0 .. end - 1 are seen by the block's last row, all of 0 .. first by every row of it: none where a row has no angle.
     const int last = length - nr + (col0 + ncol - 1) / a.group;
-    const int first = a.cos_tab && last >= a.positions ? -1 : length - nr + col0 / a.group;
-    const int end = last < 0 ? 0 : last + 1;
-    const int steps = min((end + STEP - 1) / STEP, a.splits * a.chunk);   // no more than the call provides for
+    const int first = a.cos_tab && last >= a.positions ? -1 : min(length - nr + col0 / a.group, a.max_length - 1);
+    const int end = min(last < 0 ? 0 : last + 1, a.max_length);
+    const int steps = (end + STEP - 1) / STEP;
     const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;
     if (split >= active) return;
 
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(32 * W, (Kv4AttnShape<D, NT, HL, W, ST>::CTAS)
         if (lane == 0) {
             qscale[col] = fmul(a.scale_log2e, pow2i(24 - e));
             qrow[col] = make_int2(q.row, q.h);
-            qpos[col] = q.known ? q.pos : -1;
+            qpos[col] = q.known ? min(q.pos, a.max_length - 1) : -1;   // the last position that the row sees
         }
         const bool bad = mag >= 0x7f800000u;                           // an infinity or a NaN: it has to show in the sums too
 #pragma unroll

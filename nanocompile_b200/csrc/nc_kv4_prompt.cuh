@@ -161,13 +161,13 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const int row0 = a.at.row_start ? a.at.row_start[seq] : seq;
     const int nr = a.at.row_start ? a.at.row_start[seq + 1] - row0 : 1;
     if (row0 < 0 || nr <= 0 || (int64_t)row0 + nr > a.at.rows) return;
-    const int cols = nr * a.group, col0 = cb * KVT_COLS;
+    const int cols = min(nr, a.max_rows) * a.group, col0 = cb * KVT_COLS;
     if (col0 >= cols) return;
     const int ncol = min(cols - col0, KVT_COLS);
     const int last = length - nr + (col0 + ncol - 1) / a.group;
-    const int first = a.cos_tab && last >= a.positions ? -1 : length - nr + col0 / a.group;      // as there
-    const int end = last < 0 ? 0 : last + 1;
-    const int steps = min((end + KVT_STEP - 1) / KVT_STEP, a.splits * a.chunk);
+    const int first = a.cos_tab && last >= a.positions ? -1 : min(length - nr + col0 / a.group, a.max_length - 1);   // as there
+    const int end = min(last < 0 ? 0 : last + 1, a.max_length);
+    const int steps = (end + KVT_STEP - 1) / KVT_STEP;
     const int active = steps <= a.chunk ? 1 : (steps + a.chunk - 1) / a.chunk;
     if (split >= active) return;
     const int step0 = split * a.chunk, step_end = min(steps, step0 + a.chunk);
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const int qpos = have ? length - nr + r : -1;
     const bool known = qpos >= 0 && (!a.cos_tab || qpos < a.positions);
     if (qpos >= 0 && !known && a.at.error) atomicMin(a.at.error, (unsigned long long)seq);
-    const int pos = known ? qpos : -1;
+    const int pos = known ? min(qpos, a.max_length - 1) : -1;          // the last position that the row sees
     float f;                                                           // a score's factor, but for the tile's exponent
     {
         constexpr int Q = D / 4;

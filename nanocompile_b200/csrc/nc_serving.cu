@@ -325,6 +325,8 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     a.col_blocks = plan.col_blocks;
     a.splits = plan.splits;
     a.chunk = plan.chunk;
+    a.max_rows = (int)max_rows;
+    a.max_length = (int)max_length;
     if (plan.splits > 1) {
         if (!p[9] || misaligned(p[9], 16) || scratch < kv4_scratch(plan, a.pool.d))
             return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch, (long long)kv4_scratch(plan, a.pool.d));

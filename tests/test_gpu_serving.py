@@ -791,3 +791,43 @@ def test_rows_without_an_angle_see_nothing_of_a_long_history(cuda, dtype, d, bou
     assert np.isfinite(lse[~none]).all()
     alone, lse = case.attend(layout, q[:2], dtype, [1, 1], tuple(t[:180].copy() for t in rope))       # single tokens, both past the end
     assert not alone.any() and np.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype,d", [("float32", 64), ("float16", 32), ("bfloat16", 96), ("bfloat16", 128), ("bfloat16", 64)])
+@pytest.mark.parametrize("longest", [0, 1, 100, 128])
+def test_positions_past_the_longest_length_have_no_share(cuda, dtype, d, longest):
+    rng = np.random.default_rng(d + longest)
+    times = 8 if dtype == "bfloat16" and d != 96 else 1
+    lengths, counts = [128, 300, 40] * times, [30, 2, 30] * times
+    case = Case(rng, lengths, 3, d, 16)
+    q = rng.standard_normal((sum(counts), 12, d)).astype(np.float32)
+    rope = ref.rope_tables(300, d)
+    cut = [(k[:longest], v[:longest]) for k, v in case.histories]
+    q = ref.decode(ref.encode(q, dtype), dtype)
+    for rows, most_rows in ((counts, sum(counts)), ([1] * len(lengths), 1)):
+        x = q[: sum(rows)]
+        got, lse = case.attend(KV4Layout(12, 3, d, 16), x, dtype, rows, rope, max_length=longest, max_rows=most_rows)
+        if longest == 0:
+            assert not got.any() and np.isneginf(lse).all()
+            continue
+        want, want_lse, size = ref.attention(x, cut, case.lengths, starts_of(rows), np.float32(d ** -0.5), rope)
+        most = max(np.abs(v).max() for _, v in cut)
+        assert (np.abs(got - want) <= attention_bound(dtype, want, size, most)).all()
+        slack = (2.0 ** -18 if dtype != "bfloat16" else 2.0 ** -11) * (size + 4)
+        assert (np.abs(lse - want_lse) <= slack + 2.0 ** -22 * np.abs(want_lse)).all()
+
+
+@pytest.mark.parametrize("dtype,heads,d,bounds", [("float32", 7, 64, {}), ("bfloat16", 7, 128, {}), ("bfloat16", 30, 128, dict(max_length=50000)),
+                                                  ("bfloat16", 30, 64, dict(max_length=100000))])
+def test_rows_past_the_most_rows_get_no_output(cuda, dtype, heads, d, bounds):
+    rng = np.random.default_rng(heads + d)
+    counts, most_rows = [5, 40, 3, 4], 4
+    case = Case(rng, [70, 90, 3, 150], 1, d, 16)
+    q = ref.decode(ref.encode(rng.standard_normal((sum(counts), heads, d)).astype(np.float32), dtype), dtype)
+    got, lse = case.attend(KV4Layout(heads, 1, d, 16), q, dtype, counts, max_rows=most_rows, **bounds)
+    want, want_lse, size = ref.attention(q, case.histories, case.lengths, starts_of(counts), np.float32(d ** -0.5))
+    past = np.concatenate([np.arange(c) >= most_rows for c in counts])
+    assert not got[past].any() and (lse[past] == 7.0).all()
+    most = max(np.abs(v).max() for _, v in case.histories)
+    assert (np.abs(got - want) <= attention_bound(dtype, want, size, most))[~past].all()
+    assert (np.abs(lse - want_lse) <= 2.0 ** -11 * (size + 4))[~past].all()
