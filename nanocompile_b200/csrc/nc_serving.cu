@@ -298,7 +298,8 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     Kv4AttnArgs a{};
     NC_TRY(kv4_common(&a.at, &a.pool, p[2], p[3], p[4], p[5], p[10], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8]));
     NC_TRY(check_type(s[12]));
-    const int64_t heads = s[9], max_rows = s[15], max_length = s[16], scratch = s[17];
+    const int64_t heads = s[9], max_length = s[16], scratch = s[17];
+    int64_t max_rows = s[15];
     if (heads <= 0 || heads % a.pool.kv) return fail(NC_ERR_ARGUMENT, "%lld query heads do not share %d KV heads evenly", (long long)heads, a.pool.kv);
     if (a.at.rows == 0 || a.at.seqs == 0) return NC_OK;
     a.out = p[0];
@@ -319,8 +320,9 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     a.group = (int)(heads / a.pool.kv);
     if (!a.out || !a.q || !a.cos_tab != !a.sin_tab) return fail(NC_ERR_ARGUMENT, "null output or queries, or half a rotation table");
     if (a.q_stride < heads * a.pool.d || a.out_stride < heads * a.pool.d) return fail(NC_ERR_ARGUMENT, "rows of %lld values overlap", (long long)(heads * a.pool.d));
-    if (max_rows <= 0 || max_rows > a.at.rows || max_length < 0 || max_length > I32 || (!a.at.row_start && max_rows != 1))
+    if (max_rows <= 0 || max_length < 0 || max_length > I32 || (!a.at.row_start && max_rows != 1))
         return fail(NC_ERR_ARGUMENT, "at most %lld rows and %lld positions of a sequence", (long long)max_rows, (long long)max_length);
+    max_rows = std::min(max_rows, a.at.rows);
     const AttnPlan plan = kv4_plan(a.at.seqs, heads, a.pool.kv, a.pool.d, max_rows, max_length, a.type == KV_BF16);
     a.col_blocks = plan.col_blocks;
     a.splits = plan.splits;

@@ -831,3 +831,11 @@ def test_rows_past_the_most_rows_get_no_output(cuda, dtype, heads, d, bounds):
     most = max(np.abs(v).max() for _, v in case.histories)
     assert (np.abs(got - want) <= attention_bound(dtype, want, size, most))[~past].all()
     assert (np.abs(lse - want_lse) <= 2.0 ** -11 * (size + 4))[~past].all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_bound_of_rows_above_the_calls_rows(cuda, dtype):
+    rng = np.random.default_rng(21)
+    case = Case(rng, [40, 9], 1, 64, 16)
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    case.check(KV4Layout(4, 1, 64, 16), q, dtype, [3, 2], max_rows=512)
