@@ -249,6 +249,7 @@ int32_t nc_kv4_read(void **p, const int64_t *s, void *stream);
  *    stride, element type of q and out, positions, scale as float32 bits, the most rows of a sequence,
  *    the most positions of a sequence, scratch bytes */
 int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream);
+/* Enough for every call of these heads with up to so many sequences, rows of a sequence and positions. */
 int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_rows,
                                        int64_t max_length);
 

@@ -107,6 +107,8 @@ struct AttnPlan {
     int64_t groups;
 };
 constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: their finish counters lead the scratch
+constexpr int64_t KV4_PARTS = 1 << 17;         // columns of all parts of a split call at most: bounds the scratch of every smaller call
+constexpr int64_t KV4_SPLITS = 64, KVT_PLACES = 148 * 2;
 constexpr int KV4_STAGES = 2;
 // bfloat16 rows go to the tensor cores' kernel from this many columns of a sequence and tiles (128 columns by 64 positions)
 // of the call.  Below, its start, its wide parts and few CTAs cost more than they give.  Measured, it against the products on
@@ -134,8 +136,8 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
         p.nt = KVT_COLS / 8;                                             // 128 columns, two CTAs to an SM
         p.col_blocks = (int)prompt_blocks;
         p.groups = seqs * kv * prompt_blocks;
-        const int64_t steps = prompt_steps, places = 148 * 2;
-        int64_t splits = p.groups == 0 || p.groups > KV4_COUNTERS ? 1 : places / p.groups;
+        const int64_t steps = prompt_steps;
+        int64_t splits = p.groups == 0 || p.groups > KV4_COUNTERS ? 1 : KVT_PLACES / p.groups;
         splits = std::max<int64_t>(1, std::min(splits, steps / 4));     // a split is worth its join from four steps on
         p.chunk = (int)((steps + splits - 1) / splits);
         p.splits = (int)((steps + p.chunk - 1) / p.chunk);
@@ -146,7 +148,7 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
     float best = 0.0f;
     for (int nt = 1; nt <= (cols <= 8 ? 1 : 2); ++nt) {
         const int64_t col_blocks = (cols + 8 * nt - 1) / (8 * nt), groups = seqs * kv * col_blocks;
-        const int64_t most = groups > KV4_COUNTERS ? 1 : std::min<int64_t>(64, steps);
+        const int64_t most = groups > KV4_COUNTERS ? 1 : std::min({KV4_SPLITS, steps, std::max<int64_t>(1, KV4_PARTS / (groups * 8 * nt))});
         for (int warps = nt == 1 ? 16 : 8; warps >= 4; warps /= 2) {
             const int64_t places = 148 * (nt == 1 ? 16 : 8) / warps;
             for (int splits : CUTS) {
@@ -289,9 +291,16 @@ extern "C" int32_t nc_kv4_read(void **p, const int64_t *s, void *stream) {
 extern "C" int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_rows,
                                                   int64_t max_length) {
     if (seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || d <= 0 || max_rows <= 0 || max_length < 0) return 256;
+    // Not what the plan for these sizes needs, which may be nothing where one for fewer sequences or rows has splits, but a bound
+    // that grows with each of them: the columns of all groups times the most splits, within what the plans keep to.
+    const int64_t cols = heads / kv_heads * std::min(max_rows, I32), histories = std::min(KV4_PARTS, std::min(seqs, I32) * std::min(kv_heads, KV4_PARTS));
+    auto padded = [&](int64_t n) { return std::min(KV4_PARTS, (cols + n - 1) / n * n); };
+    const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, splits = std::min(KV4_SPLITS, (max_length + step - 1) / step);
     int64_t most = 0;
-    for (bool bf16 : {false, true}) most = std::max(most, kv4_scratch(kv4_plan(seqs, heads, kv_heads, d, max_rows, max_length, bf16), d));
-    return most;
+    if (splits > 1) most = std::min(KV4_PARTS, histories * padded(cols <= 8 ? 8 : 16) * splits);
+    if (const int64_t wide = max_length / KVT_STEP / 4; wide > 0 && cols >= KV4_PROMPT_COLS)
+        most = std::max(most, std::min(KVT_PLACES * KVT_COLS, histories * padded(KVT_COLS) * (wide + 1)));
+    return most == 0 ? 256 : 4 * KV4_COUNTERS + most * (d + 2) * 4;
 }
 
 extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {

@@ -267,7 +267,7 @@ def kv4_read(layout: KV4Layout, keys, values, pool, table, lengths, *, row_start
 
 
 def kv4_attention_scratch_bytes(layout: KV4Layout, rows: int, seqs: int, max_length: int, max_rows: int = 1) -> int:
-    """Scratch for :func:`kv4_attention` calls of these sizes (``rows`` is not needed; a sequence has ``max_rows`` at most)."""
+    """Scratch for :func:`kv4_attention` calls of up to these sizes (``rows`` is not needed; a sequence has ``max_rows`` at most)."""
     return int(library().nc_kv4_attention_scratch_bytes(seqs, layout.heads, layout.kv_heads, layout.head_dim, max_rows, max_length))
 
 

@@ -839,3 +839,15 @@ def test_a_bound_of_rows_above_the_calls_rows(cuda, dtype):
     case = Case(rng, [40, 9], 1, 64, 16)
     q = rng.standard_normal((5, 4, 64)).astype(np.float32)
     case.check(KV4Layout(4, 1, 64, 16), q, dtype, [3, 2], max_rows=512)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,d", [(14, 2, 64), (8, 2, 128)])
+def test_one_attention_scratch_for_a_batch_that_shrinks(cuda, dtype, heads, kv, d):
+    rng = np.random.default_rng(22)
+    layout, most = KV4Layout(heads, kv, d, 16), 2048
+    scratch = DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, 64 * 40, 64, most, 40),), np.uint8)
+    for lengths, rows in (([300, 30, 7, 200] * 8, 1), ([300, 30, 7, 200], 1), ([300, 200], 40), ([2048], 1), ([100], 100)):
+        case = Case(rng, lengths, kv, d, 16)
+        q = rng.standard_normal((rows * len(lengths), heads, d)).astype(np.float32)
+        case.check(layout, q, dtype, [rows] * len(lengths), scratch=scratch, max_length=most, max_rows=rows)

@@ -172,3 +172,23 @@ def test_quantisation_error_is_half_a_step():
     # Half a step, and what the ends lose to parameters rounded to f16: half a unit of the zero, 15 of the scale's.
     slack = np.abs(x).max() * 2.0 ** -11 + 15 * step * 2.0 ** -11
     assert (np.abs(ref.stands_for(code, scale, zero) - x) <= step / 2 + slack).all()
+
+
+@pytest.mark.parametrize("heads,kv,d", [(14, 2, 64), (32, 8, 128), (12, 4, 96), (4, 2, 32)])
+def test_attention_scratch_covers_smaller_calls(heads, kv, d):
+    """Sequences leave a batch, steps have fewer rows, histories are shorter: the size for the largest call is enough."""
+    layout = serving.KV4Layout(heads, kv, d)
+
+    def size(seqs, length, rows):
+        return serving.kv4_attention_scratch_bytes(layout, seqs * rows, seqs, length, rows)
+
+    assert size(32, 2048, 1) <= size(64, 2048, 1)
+    seqs, rows, lengths = [1, 2, 3, 5, 8, 13, 24, 32, 48, 64, 100, 256, 700], [1, 2, 3, 5, 16, 33, 64, 200, 512, 1000], [1, 16, 64, 100, 257, 700, 2048, 6001, 32768]
+    for sizes in ((seqs, [1], lengths), (seqs[:7], rows, lengths)):
+        for a in range(1, len(sizes[0])):
+            for r in range(len(sizes[1])):
+                for n in range(1, len(sizes[2])):
+                    here = size(sizes[0][a], sizes[2][n], sizes[1][r])
+                    assert size(sizes[0][a - 1], sizes[2][n], sizes[1][r]) <= here
+                    assert size(sizes[0][a], sizes[2][n - 1], sizes[1][r]) <= here
+                    assert r == 0 or size(sizes[0][a], sizes[2][n], sizes[1][r - 1]) <= here
