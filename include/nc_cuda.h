@@ -280,6 +280,7 @@ int64_t nc_kv_pages_scratch_bytes(int64_t seqs, int64_t width, int64_t pages);
  *    [8] error word (device u64, nullable)
  * s: rows, vocab, logit row stride (elements), element type, targets, k (0..32), scratch bytes */
 int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream);
+/* Enough for every call of this vocabulary, of any type, with up to so many rows and alternatives. */
 int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
 
 /* ---- 2. the model runtime ---------------------------------------------------------------- */

@@ -454,17 +454,28 @@ struct LogprobPlan {
     int64_t seg_vecs;
 };
 
+constexpr int64_t LP_PARTS = 1 << 14;          // segments of a launch at most, where rows are cut for speed: bounds the scratch
+
+int64_t logprob_vecs(int64_t vocab, int64_t type) {               // of a row at any alignment
+    const int n = type == KV_F32 ? 4 : 8;
+    return (vocab + 2 * (n - 1)) / n;
+}
+// As many segments as a row has to have.
+int64_t logprob_fewest(int64_t vocab, int64_t type) {
+    constexpr int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS;
+    return (logprob_vecs(vocab, type) + longest - 1) / longest;
+}
+
 // Segments to a row: the fewest elements' time over the waves of CTAs that the card holds at once, a segment's
 // start and end counted as 4096 elements and its share of the join as 16.
 LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int64_t type) {
     const int n = type == KV_F32 ? 4 : 8;
-    const int64_t vecs = (vocab + 2 * (n - 1)) / n, slots = 148 * LP_CTAS;      // at any alignment
-    const int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS, fewest = (vecs + longest - 1) / longest;
+    const int64_t vecs = logprob_vecs(vocab, type), slots = 148 * LP_CTAS, fewest = logprob_fewest(vocab, type);
     int64_t best = -1;
     LogprobPlan p{0, 0};
     for (int cut : CUTS) {
         const int64_t segs = std::max<int64_t>(cut, fewest);
-        if (segs > LP_SEGS || (segs > fewest && vecs / segs < LP_THREADS)) break;
+        if (segs > LP_SEGS || (segs > fewest && (vecs / segs < LP_THREADS || rows * segs > LP_PARTS))) break;
         const int64_t waves = (rows * segs + slots - 1) / slots, cost = waves * (vecs * n / segs + 4096) + 16 * segs;
         if (best >= 0 && cost >= best) continue;
         best = cost;
@@ -484,9 +495,14 @@ int32_t launch_logprobs(cudaStream_t st, const LogprobArgs &a, int64_t rows) {
 
 extern "C" int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k) {
     if (rows <= 0 || vocab <= 0 || k < 0) return 4 * LP_ROWS;
+    // A bound that grows with the rows: fewer of them are cut into more segments.
     int64_t most = 0;
-    for (int type : {KV_F32, KV_F16}) most = std::max<int64_t>(most, logprob_plan(std::min<int64_t>(rows, LP_ROWS), vocab, type).segs);
-    return 4 * LP_ROWS + std::min<int64_t>(rows, LP_ROWS) * most * (16 + 8 * k);
+    rows = std::min<int64_t>(rows, LP_ROWS);
+    for (int type : {KV_F32, KV_F16}) {
+        const int64_t fewest = logprob_fewest(vocab, type), cut = std::min<int64_t>(LP_SEGS, logprob_vecs(vocab, type) / LP_THREADS);
+        most = std::max({most, rows * fewest, std::min(LP_PARTS, rows * cut)});
+    }
+    return 4 * LP_ROWS + most * (16 + 8 * k);
 }
 
 extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {

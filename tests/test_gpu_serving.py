@@ -851,3 +851,13 @@ def test_one_attention_scratch_for_a_batch_that_shrinks(cuda, dtype, heads, kv, 
         case = Case(rng, lengths, kv, d, 16)
         q = rng.standard_normal((rows * len(lengths), heads, d)).astype(np.float32)
         case.check(layout, q, dtype, [rows] * len(lengths), scratch=scratch, max_length=most, max_rows=rows)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_scratch_for_fewer_rows_of_logits(cuda, dtype):
+    rng, vocab = np.random.default_rng(23), 151936
+    x = rng.standard_normal((64, vocab)).astype(np.float32)
+    scratch = DeviceArray.zeros((serving.token_logprobs_scratch_bytes(64, vocab, 20),), np.uint8)
+    for rows in (64, 50, 12, 6, 1):
+        scores(x[:rows], rng.integers(0, vocab, (rows, 1)), 20, dtype, scratch=scratch)
+    check_scores(x[:6], rng.integers(0, vocab, (6, 1)), 20, dtype, scratch=scratch)

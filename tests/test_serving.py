@@ -192,3 +192,12 @@ def test_attention_scratch_covers_smaller_calls(heads, kv, d):
                     assert size(sizes[0][a - 1], sizes[2][n], sizes[1][r]) <= here
                     assert size(sizes[0][a], sizes[2][n - 1], sizes[1][r]) <= here
                     assert r == 0 or size(sizes[0][a], sizes[2][n], sizes[1][r - 1]) <= here
+
+
+@pytest.mark.parametrize("vocab", [300, 32000, 50257, 128256, 151936, 2000000])
+def test_log_probability_scratch_covers_fewer_rows(vocab):
+    rows = [1, 2, 3, 5, 6, 8, 12, 16, 24, 32, 50, 64, 100, 128, 200, 253, 256, 300, 507, 512, 592, 1000, 4095, 4096, 4097, 9000]
+    for k in (0, 1, 20, 32):
+        sizes = [serving.token_logprobs_scratch_bytes(n, vocab, k) for n in rows]
+        assert sizes == sorted(sizes)
+        assert k == 0 or all(serving.token_logprobs_scratch_bytes(n, vocab, k - 1) <= size for n, size in zip(rows, sizes))
