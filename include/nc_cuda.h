@@ -170,8 +170,8 @@ int32_t nc_attention(void **p, const int64_t *s, void *stream);
 int32_t nc_attention_cache(void **p, const int64_t *s, void *stream);
 
 /* NC_ERR_KERNEL if a kernel recorded a device-side fault since the last call (a TMA stage of
- * the grouped attention kernel that did not arrive within its bounded wait, or a matrix instruction of
- * nc_kv4_attention's prompts); clears it. */
+ * the grouped attention kernel that did not arrive within its bounded wait, or a copy or a matrix
+ * instruction of nc_kv4_attention's prompts, whose output is then missing in part); clears it. */
 int32_t nc_device_faults(void);
 
 /* Bounds the library's abandonable device-side waits (pipeline stages of the tensor-core

@@ -15,6 +15,8 @@ __attribute__((visibility("hidden"), format(printf, 2, 3))) int32_t fail(int32_t
 
 // Whether a bounded wait of the serving kernels has run out since the last call (nc_serving.cu).
 __attribute__((visibility("hidden"))) int32_t prompt_fault(bool *fault);
+// Their g_wait_cycles: each source file has its own.
+__attribute__((visibility("hidden"))) int32_t set_prompt_wait_limit(long long cycles);
 
 #define CUDA_TRY(expr)                                                                           \
     do {                                                                                         \

@@ -839,14 +839,14 @@ extern "C" int32_t nc_device_faults(void) {
     NC_TRY(check_device_faults());
     bool prompt = false;
     NC_TRY(prompt_fault(&prompt));
-    if (prompt) return fail(NC_ERR_KERNEL, "4-bit attention: a matrix instruction did not complete within its wait limit");
+    if (prompt) return fail(NC_ERR_KERNEL, "4-bit attention: a copy or a matrix instruction did not complete within its wait limit");
     return NC_OK;
 }
 
 extern "C" int32_t nc_set_wait_limit(int64_t cycles) {
     const long long v = cycles > 0 ? (long long)cycles : (1ll << 31);
     CUDA_TRY(cudaMemcpyToSymbol(g_wait_cycles, &v, sizeof(v)));
-    return NC_OK;
+    return set_prompt_wait_limit(v);
 }
 
 extern "C" int32_t nc_selftest_wait(int32_t kind) {

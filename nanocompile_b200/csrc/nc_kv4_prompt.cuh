@@ -30,7 +30,8 @@ namespace nc {
 
 constexpr int KVT_COLS = 128, KVT_STEP = 64, KVT_THREADS = 256, KVT_TMEM = 256;
 
-__device__ unsigned int g_prompt_fault;        // set when a matrix instruction's completion never came (bounded wait)
+__device__ unsigned int g_prompt_fault;        // set when a copy or a matrix instruction did not come to its end within the wait limit
+constexpr unsigned int KVT_FAILED = 0x10000;   // added to a group's finish counter by a CTA whose part is not there
 
 template <int D>
 struct KvtShared {
@@ -48,11 +49,20 @@ __device__ __forceinline__ uint32_t kvt_smem(const void *p) { return (uint32_t)_
 __device__ __forceinline__ void kvt_mbar_init(uint64_t *bar) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(kvt_smem(bar)) : "memory");
 }
-// Whether the phase completes within the bound (about a second).
-__device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity) {
+// Whether the phase is complete, or becomes so within `limit` cycles (g_wait_cycles where the kernel can stop, NC_DRAIN_CYCLES for
+// what is in flight).  No clock is read for a phase that is: with it first, 476 us instead of 454 for the largest prompt below.
+__device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity, long long limit) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(kvt_smem(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
     const long long start = clock64();
-    for (;;) {                                                         // each try sleeps up to a millisecond
-        uint32_t done;
+    while (clock64() - start < limit) {                                // each try sleeps up to a millisecond
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -61,8 +71,8 @@ __device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity) {
             : "r"(kvt_smem(bar)), "r"(parity), "r"(1000000u)
             : "memory");
         if (done) return true;
-        if (clock64() - start > NC_DRAIN_CYCLES) return false;
     }
+    return false;
 }
 // A K-major operand of 128-byte swizzled rows: eight rows are 1024 bytes.
 __device__ __forceinline__ uint64_t kvt_desc(uint32_t address) {
@@ -152,6 +162,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const int part = warp >> 2, col = 32 * (warp & 3) + lane;          // the thread's column and half of positions or dimensions
 
     wait_for_producer();
+    const long long limit = g_wait_cycles;
     const int split = (int)(blockIdx.x % a.splits);
     const unsigned group = blockIdx.x / a.splits;
     const unsigned histories = (unsigned)(a.at.seqs * a.pool.kv), history = group % histories;
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     __syncthreads();
     kvt_after();
     release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
-    int issued = min(step_end, step0 + 3), seen_raw = step0;           // tiles whose copies are started, and waited for
+    int issued = min(step_end, step0 + 3);                             // tiles whose copies are started
     constexpr int COPIER = KVT_THREADS / 32 - 1;
     if (warp == COPIER) {
         for (int s = step0; s < issued; ++s) {
@@ -347,8 +358,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     };
     auto look_at = [&](int step) {
         if (step >= step_end) return true;
-        seen_raw = step + 1;
-        const bool here = kvt_mbar_wait(&sh.raw_full[(step - step0) % 3], (unsigned)((step - step0) / 3) & 1);
+        const bool here = kvt_mbar_wait(&sh.raw_full[(step - step0) % 3], (unsigned)((step - step0) / 3) & 1, limit);
         if (here) look(step);
         return here;
     };
@@ -356,7 +366,8 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     ok = look_at(step0 + 1) && ok;
     int step = step0;
     bool broken = __syncthreads_or(!ok);
-    if (!broken && step0 < step_end) {
+    const bool begun = !broken && step0 < step_end;                    // scores have been asked for
+    if (begun) {
         decode_keys(step0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kvt_before();
@@ -378,7 +389,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         // order since the last barrier.
         ok = true;
         if (step > step0) {
-            ok = kvt_mbar_wait(&sh.o_done, (unsigned)(tile_no - 1) & 1);
+            ok = kvt_mbar_wait(&sh.o_done, (unsigned)(tile_no - 1) & 1, limit);
             kvt_after();
             if (tid == 0) issue_scores(step);
         }
@@ -429,7 +440,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         // Softmax of the thread's 32 positions.
-        ok = kvt_mbar_wait(&sh.s_done, (unsigned)tile_no & 1) && ok;
+        ok = kvt_mbar_wait(&sh.s_done, (unsigned)tile_no & 1, limit) && ok;
         kvt_after();
         uint32_t x[32];
         kvt_load32(ts + lanes + 32 * part, x);
@@ -503,20 +514,23 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
             ++issued;
         }
     }
-    // Nothing is left in flight: copies (after a wait that ran out only), matrix instructions.
-    for (; seen_raw < issued; ++seen_raw) kvt_mbar_wait(&sh.raw_full[(seen_raw - step0) % 3], (unsigned)((seen_raw - step0) / 3) & 1);
+    // Nothing is left in flight. After a wait that ran out: the copies of the last three tiles, and the scores of the tile that was not
+    // finished, behind which no matrix instruction has been issued; else the last O += P V.
+    for (int s = max(step0, issued - 3); broken && s < issued; ++s)
+        kvt_mbar_wait(&sh.raw_full[(s - step0) % 3], (unsigned)((s - step0) / 3) & 1, NC_DRAIN_CYCLES);
     const int done = step - step0;                                     // whole tiles, whose O += P V has been issued
-    if (!broken && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1);
+    if (broken && begun) kvt_mbar_wait(&sh.s_done, (unsigned)done & 1, NC_DRAIN_CYCLES);
+    if (!broken && done > 0) ok = kvt_mbar_wait(&sh.o_done, (unsigned)(done - 1) & 1, NC_DRAIN_CYCLES);
     const bool failed = __syncthreads_or(!ok || broken);
     kvt_after();
 
     // Half of the column's dimensions to a thread.
+    const bool alone = active == 1;
+    float *const parts = a.part + (int64_t)group * a.splits * (KVT_COLS * (D + 2)), *const mine = alone ? nullptr : parts + (int64_t)split * (KVT_COLS * (D + 2));
     if (!failed) {
         sh.row_sum[part][col] = sum;
         __syncthreads();
         sum += sh.row_sum[part ^ 1][col];
-        const bool alone = active == 1;
-        float *const parts = a.part + (int64_t)group * a.splits * (KVT_COLS * (D + 2)), *const mine = alone ? nullptr : parts + (int64_t)split * (KVT_COLS * (D + 2));
         const float by = pow2i(ev), inv = sum == 0.0f ? 0.0f : fdiv(by, sum);
         const int64_t at = qrow * a.out_stride + (int64_t)qhead * D + part * (D / 2);
 #pragma unroll
@@ -567,19 +581,19 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
                 *(float2 *)(mine + KVT_COLS * D + 2 * col) = make_float2(sum == 0.0f ? -INFINITY : ref, sum);
             }
         }
-        if (!alone) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) sh.arrived = atomicAdd(a.counter + group, 1u);
-            __syncthreads();
-            if (sh.arrived == (unsigned)active - 1) {
-                __threadfence();
-                if (tid == 0) a.counter[group] = 0;
-                kv4_join<KVT_COLS, D>(a, parts, active, ncol, sh.row);
-            }
-        }
     } else if (tid == 0) {
         g_prompt_fault = 1;
+    }
+    if (!alone) {                                                      // a part that is not there counts too: the last one leaves the counter at zero
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) sh.arrived = atomicAdd(a.counter + group, failed ? 1u + KVT_FAILED : 1u);
+        __syncthreads();
+        if ((sh.arrived & (KVT_FAILED - 1)) == (unsigned)active - 1) {
+            __threadfence();
+            if (tid == 0) a.counter[group] = 0;
+            if (!failed && sh.arrived < KVT_FAILED) kv4_join<KVT_COLS, D>(a, parts, active, ncol, sh.row);
+        }
     }
     kvt_before();
     __syncthreads();

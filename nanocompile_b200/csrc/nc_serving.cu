@@ -230,7 +230,12 @@ int32_t launch_kv4_attention_d(cudaStream_t st, const Kv4AttnArgs &a, const Attn
 
 }  // namespace
 
-// Whether a matrix instruction's completion never came since the last call; clears it.
+int32_t nc::set_prompt_wait_limit(long long cycles) {
+    CUDA_TRY(cudaMemcpyToSymbol(g_wait_cycles, &cycles, sizeof(cycles)));
+    return NC_OK;
+}
+
+// Whether a wait has run out since the last call; clears it.
 int32_t nc::prompt_fault(bool *fault) {
     unsigned int word = 0;
     CUDA_TRY(cudaMemcpyFromSymbol(&word, g_prompt_fault, sizeof(word)));

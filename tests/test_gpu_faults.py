@@ -103,3 +103,28 @@ def test_device_cache_capacity_overflow_is_refused(cuda, reference):
     with pytest.raises(cuda.InterpreterError, match="capacity"):
         cuda.new_device_cache(model, 64)
     assert cache.length == 10                          # the refused step changed nothing
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_4_bit_prompt_stops_on_a_short_wait_and_its_scratch_stays_good(short_waits, d):
+    """Waits cut short end the tensor cores' attention; the next call on the same scratch is right."""
+    from nanocompile_b200 import serving
+    from tests.test_gpu_serving import Case
+
+    cuda, rng = short_waits, np.random.default_rng(d)
+    layout, case = serving.KV4Layout(4, 1, d, 16), Case(rng, [700, 150], 1, d, 16)
+    query, counts = rng.standard_normal((80, 4, d)).astype(np.float32), [50, 30]
+    scratch = serving.DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, 80, 2, 20000, 80),), np.uint8)
+    # Enough work, by its bounds, for that kernel, in chunks of 448 positions: two of the longer history.
+    bounds = dict(max_length=20000, max_rows=80, scratch=scratch)
+    want = case.check(layout, query, "bfloat16", counts, **bounds)
+    cuda.set_wait_limit(1)
+    for _ in range(2):
+        case.attend(layout, query, "bfloat16", counts, **bounds)
+    with pytest.raises(cuda.KernelError, match="4-bit attention.*wait limit"):
+        cuda.device_faults()
+    cuda.set_wait_limit(0)
+    for _ in range(2):
+        got = case.check(layout, query, "bfloat16", counts, **bounds)
+        assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(got, want))
+    cuda.device_faults()
