@@ -54,6 +54,7 @@ int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, co
                     (long long)layer, (long long)offset, (long long)page_bytes);
     if (!row_start && rows != seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of %lld sequences need row_start", (long long)rows, (long long)seqs);
     if (rows && (!base || !table || !lengths)) return fail(NC_ERR_ARGUMENT, "null pool, table or lengths");
+    if (misaligned(error, 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
     at->table = (const int32_t *)table;
     at->lengths = (const int32_t *)lengths;
     at->row_start = (const int32_t *)row_start;
@@ -524,6 +525,7 @@ extern "C" int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream) {
     if (plan.segs == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is beyond %d segments", (long long)vocab, LP_SEGS);
     if (!p[5] || (ntargets && (!p[0] || !p[6])) || (k && (!p[3] || !p[4])) || misaligned(p[5], type == KV_F32 ? 4 : 2))
         return fail(NC_ERR_ARGUMENT, "null or misaligned logits, targets or outputs");
+    if (misaligned(p[8], 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
     if (plan.segs > 1 && (!p[7] || misaligned(p[7], 16) || scratch < 4 * LP_ROWS + std::min<int64_t>(rows, LP_ROWS) * plan.segs * (16 + 8 * k)))
         return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch,
                     (long long)nc_token_logprobs_scratch_bytes(rows, vocab, k));

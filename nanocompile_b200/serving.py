@@ -132,8 +132,8 @@ class KV4Layout:
 # The smallest calls take a few microseconds on the device, so the checks before them are kept short: every property of
 # an array is asked for once, element types are compared as small numbers, and what is wrong is looked for only
 # where something is.
-_F32, _F16, _BF16, _I32, _I64, _U8, _OTHER = range(7)
-_NAMES = {"float32": _F32, "float16": _F16, "bfloat16": _BF16, "int32": _I32, "int64": _I64, "uint8": _U8}
+_F32, _F16, _BF16, _I32, _I64, _U64, _U8, _OTHER = range(8)
+_NAMES = {"float32": _F32, "float16": _F16, "bfloat16": _BF16, "int32": _I32, "int64": _I64, "uint64": _U64, "uint8": _U8}
 
 
 class _Kinds(dict):
@@ -205,8 +205,22 @@ def _cache(layout: KV4Layout, layer: int, pool, table, lengths, row_start) -> tu
             seqs, held[0], layer * layout.layer_bytes, width)
 
 
-def _optional(array) -> int:
-    return 0 if array is None else array.data_ptr()
+def _error(array) -> int:
+    """The address of an error word, which is written with eight bytes; 0 for none."""
+    if array is None:
+        return 0
+    kind = _kind[array.dtype]
+    if kind != _U64 and kind != _I64 or 0 in array.shape:
+        raise InterpreterError(f"error: {_name(array.dtype)} {tuple(array.shape)}, expected a word of 64 bits")
+    return array.data_ptr()
+
+
+def _scratch(array) -> tuple[int, int]:
+    """Address and bytes of scratch."""
+    shape = array.shape
+    if len(shape) != 1 or not array.is_contiguous():
+        raise InterpreterError(f"scratch: {_name(array.dtype)} {tuple(shape)}, expected contiguous bytes")
+    return array.data_ptr(), shape[0]
 
 
 _entries: dict = {}
@@ -247,7 +261,7 @@ def kv4_append(layout: KV4Layout, pool, keys, values, table, lengths, *, row_sta
     if v_kind != kind:
         raise InterpreterError("keys and values of different types")
     cos, sin, positions = _rope(rope, d)
-    _call("nc_kv4_append", (base, k, v, tab, lens, starts, cos, sin, _optional(error)),
+    _call("nc_kv4_append", (base, k, v, tab, lens, starts, cos, sin, _error(error)),
           (rows, seqs, kv, d, layout.page_size, pages, layout.page_bytes, offset, width, k_stride, v_stride, kind, positions),
           stream)
 
@@ -262,7 +276,7 @@ def kv4_read(layout: KV4Layout, keys, values, pool, table, lengths, *, row_start
     _same_rows("values", v_rows, rows)
     if kind or v_kind or k_stride != kv * d or v_stride != kv * d:
         raise InterpreterError("keys and values: contiguous float32 rows")
-    _call("nc_kv4_read", (k, v, base, tab, lens, starts, _optional(error)),
+    _call("nc_kv4_read", (k, v, base, tab, lens, starts, _error(error)),
           (rows, seqs, kv, d, layout.page_size, pages, layout.page_bytes, offset, width), stream)
 
 
@@ -290,11 +304,12 @@ def kv4_attention(layout: KV4Layout, out, q, pool, table, lengths, scratch, *, m
         raise InterpreterError("q and out of different types")
     cos, sin, positions = _rope(rope, d)
     bits = layout.scale_bits if scale is None else _f32_bits(scale)
+    work, work_bytes = _scratch(scratch)
     _call("nc_kv4_attention",
           (to, query, base, tab, lens, starts, cos, sin, 0 if lse is None else _expect("lse", lse, _F32, (rows, heads)),
-           scratch.data_ptr(), _optional(error)),
+           work, _error(error)),
           (rows, seqs, layout.kv_heads, d, layout.page_size, pages, layout.page_bytes, offset, width, heads, q_stride,
-           out_stride, kind, positions, bits, max_rows, max_length, scratch.shape[0]), stream)
+           out_stride, kind, positions, bits, max_rows, max_length, work_bytes), stream)
 
 
 def kv_pages_scratch_bytes(seqs: int, width: int, pages: int) -> int:
@@ -307,10 +322,11 @@ def _pages(new_table, table, lengths, pool, status, scratch, page_size: int) -> 
     if len(shape) != 2 or len(held) != 2:
         raise InterpreterError(f"table {tuple(shape)} and pool {tuple(held)}: expected [sequences, pages] and [pages, bytes]")
     (seqs, width), (pages, page_bytes) = shape, held
+    work, work_bytes = _scratch(scratch)
     return ((_expect("new_table", new_table, _I32, shape), _expect("table", table, _I32, shape),
              _expect("lengths", lengths, _I32, (seqs,)), _expect("status", status, _I64, (4,)),
-             _expect("pool", pool, _U8, held), scratch.data_ptr()),
-            (seqs, width, pages, page_size, page_bytes, scratch.shape[0]))
+             _expect("pool", pool, _U8, held), work),
+            (seqs, width, pages, page_size, page_bytes, work_bytes))
 
 
 def kv_pages_update(new_table, new_lengths, table, lengths, pool, status, scratch, *, page_size: int, parent=None,
@@ -355,6 +371,7 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
         raise InterpreterError(f"logits: element type {_name(logits.dtype)}: float32, float16 or bfloat16")
     n = targets.shape[-1] if targets is not None else 0
     k = top.shape[-1] if top is not None else 0
+    work, work_bytes = (0, 0) if scratch is None else _scratch(scratch)
     _call("nc_token_logprobs",
           (_expect("out", out, _F32, (rows, n)) if n else 0,
            0 if entropy is None else _expect("entropy", entropy, _F32, (rows,)),
@@ -362,6 +379,5 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
            _expect("top", top, _I64, (rows, k)) if k else 0,
            _expect("top_logprobs", top_logprobs, _F32, (rows, k)) if k else 0,
            logits.data_ptr(), _expect("targets", targets, _I64, (rows, n)) if n else 0,
-           _optional(scratch), _optional(error)),
-          (rows, vocab, strides[0] if rows > 1 else vocab, kind, n, k,
-           0 if scratch is None else scratch.shape[0]), stream)
+           work, _error(error)),
+          (rows, vocab, strides[0] if rows > 1 else vocab, kind, n, k, work_bytes), stream)

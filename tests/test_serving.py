@@ -201,3 +201,31 @@ def test_log_probability_scratch_covers_fewer_rows(vocab):
         sizes = [serving.token_logprobs_scratch_bytes(n, vocab, k) for n in rows]
         assert sizes == sorted(sizes)
         assert k == 0 or all(serving.token_logprobs_scratch_bytes(n, vocab, k - 1) <= size for n, size in zip(rows, sizes))
+
+
+ROWS = Fake((2, 128), np.float32)
+
+
+@pytest.mark.parametrize("error,what", [(Fake((1,), np.int32), "error: int32"), (Fake((2,), np.float32), "error: float32"), (Fake((0,), np.uint64), "error: uint64"),
+                                        (Fake((1,), np.uint64, address=4100), "8-byte boundary"), (Fake((1,), np.int64, address=4092), "8-byte boundary")])
+def test_an_error_word_has_64_bits(error, what):
+    pool, table, lengths = cache(LAYOUT)
+    for call in (lambda: attend(LAYOUT, error=error),
+                 lambda: serving.kv4_append(LAYOUT, pool, ROWS, ROWS, table, lengths, error=error),
+                 lambda: serving.kv4_read(LAYOUT, ROWS, ROWS, pool, table, lengths, error=error),
+                 lambda: serving.token_logprobs(Fake((2, 50), np.float32), Fake((2, 1), np.int64), Fake((2, 1), np.float32), error=error)):
+        with pytest.raises(runtime.InterpreterError, match=what):
+            call()
+
+
+@pytest.mark.parametrize("scratch", [Fake((1 << 22,), np.uint8, strides=(0,)), Fake((1 << 22, 2), np.uint8), Fake((), np.uint8)])
+def test_scratch_is_contiguous_bytes(scratch):
+    two = Fake((2, 3), np.int32)
+    for call in (lambda: attend(LAYOUT, scratch=scratch),
+                 lambda: serving.token_logprobs(Fake((2, 50), np.float32), Fake((2, 1), np.int64), Fake((2, 1), np.float32), scratch=scratch),
+                 lambda: serving.kv_pages_update(two, Fake((2,), np.int32), Fake((2, 3), np.int32, address=8192), Fake((2,), np.int32, address=8192),
+                                                 Fake((5, 64), np.uint8), Fake((4,), np.int64), scratch, page_size=16),
+                 lambda: serving.kv_pages_compact(two, Fake((2, 3), np.int32, address=8192), Fake((2,), np.int32), Fake((5, 64), np.uint8),
+                                                  Fake((4,), np.int64), scratch, page_size=16)):
+        with pytest.raises(runtime.InterpreterError, match="scratch: uint8"):
+            call()
