@@ -359,8 +359,8 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
                    stream: int = 0) -> None:
     """Log probabilities of ``targets`` (int64 ``[rows, n]``) under rows of ``logits``, to ``out`` (``nc_token_logprobs``).
 
-    ``entropy`` and ``lse``: float32 ``[rows]``. ``top`` (int64) and ``top_logprobs`` (float32), ``[rows, k]`` with ``k`` up
-    to 32: the best tokens, in order.
+    ``entropy`` and ``lse``: float32 ``[rows]``. ``top`` (int64) and ``top_logprobs`` (float32), both or neither, ``[rows, k]``
+    with ``k`` up to 32: the best tokens, in order.
     """
     shape, strides = logits.shape, logits.stride()
     if len(shape) != 2 or strides[1] != 1:
@@ -369,6 +369,8 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
     kind = _kind[logits.dtype]
     if kind > _BF16:
         raise InterpreterError(f"logits: element type {_name(logits.dtype)}: float32, float16 or bfloat16")
+    if (top is None) != (top_logprobs is None) or (targets is not None and out is None):
+        raise InterpreterError("targets go with out, and top with top_logprobs")
     n = targets.shape[-1] if targets is not None else 0
     k = top.shape[-1] if top is not None else 0
     work, work_bytes = (0, 0) if scratch is None else _scratch(scratch)

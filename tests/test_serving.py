@@ -229,3 +229,11 @@ def test_scratch_is_contiguous_bytes(scratch):
                                                   Fake((4,), np.int64), scratch, page_size=16)):
         with pytest.raises(runtime.InterpreterError, match="scratch: uint8"):
             call()
+
+
+@pytest.mark.parametrize("change", [dict(top=None), dict(top_logprobs=None), dict(out=None)])
+def test_outputs_of_log_probabilities_come_in_pairs(change):
+    given = {"logits": Fake((2, 50), np.float32), "targets": Fake((2, 1), np.int64), "out": Fake((2, 1), np.float32),
+             "top": Fake((2, 5), np.int64), "top_logprobs": Fake((2, 5), np.float32), "scratch": Fake((1 << 22,), np.uint8), **change}
+    with pytest.raises(runtime.InterpreterError, match="top with top_logprobs"):
+        serving.token_logprobs(**given)
