@@ -282,7 +282,7 @@ __device__ __forceinline__ void kv4_tiles(const Kv4Rows &at, const Kv4Pool &pool
             count = 1;
         } else if (after > 0) {
             starts = r == begin || position % KV4_TILE == 0;
-            count = (int)min(after, (int64_t)(KV4_TILE - position % KV4_TILE));
+            count = (int)min(min(after, at.rows - r), (int64_t)(KV4_TILE - position % KV4_TILE));   // row_start may end past the call's rows
         } else {                                                     // belongs to no sequence
             starts = true;
             count = 1;

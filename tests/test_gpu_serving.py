@@ -861,3 +861,29 @@ def test_one_scratch_for_fewer_rows_of_logits(cuda, dtype):
     for rows in (64, 50, 12, 6, 1):
         scores(x[:rows], rng.integers(0, vocab, (rows, 1)), 20, dtype, scratch=scratch)
     check_scores(x[:6], rng.integers(0, vocab, (6, 1)), 20, dtype, scratch=scratch)
+
+
+@pytest.mark.parametrize("rows", [20, 2059])                                     # appended row by row, and by tiles
+def test_row_starts_that_end_past_the_rows_reach_no_others(cuda, rows):
+    rng, kv, d, page, more = np.random.default_rng(rows), 2, 64, 32, 40
+    layout, line, length = KV4Layout(kv, kv, d, page), kv * d, rows + 37         # the last of 37 positions that have no row here
+    table, pages = table_of(rng, [length], page)
+    pool = ref.Pool(pages, kv, d, page, fill=0xA5)
+    x = rng.standard_normal((rows + more, line)).astype(np.float32)
+    d_pool, d_x = DeviceArray.of(pool.bytes), DeviceArray.of(x)
+
+    class First(Rows):
+        def __init__(self, array):
+            self.array, self.shape, self.dtype = array, (rows, line), array.dtype
+
+    args = DeviceArray.of(table), DeviceArray.of(np.array([length], np.int32))
+    starts = DeviceArray.of(np.array([0, length], np.int32))
+    serving.kv4_append(layout, d_pool, First(d_x), First(d_x), *args, row_start=starts)
+    held = x[:rows].reshape(rows, kv, d)
+    pool.append(held, held, table, [rows], [0, rows])
+    assert np.array_equal(d_pool.numpy(), pool.bytes)
+    back = [DeviceArray.of(np.full(x.shape, 5, np.float32)) for _ in range(2)]
+    serving.kv4_read(layout, First(back[0]), First(back[1]), d_pool, *args, row_start=starts)
+    want = ref.stands_for(*ref.quantise(held)).reshape(rows, line)
+    for got in back:
+        assert np.array_equal(got.numpy()[:rows], want) and (got.numpy()[rows:] == 5).all()
