@@ -52,6 +52,7 @@ int32_t kv4_common(Kv4Rows *at, Kv4Pool *pool, void *base, const void *table, co
     if (offset < 0 || offset % 16 || page_bytes % 16 || offset + layer > page_bytes || misaligned(base, 16))
         return fail(NC_ERR_ARGUMENT, "a layer takes %lld bytes of a page at a 16-byte boundary; offset %lld in pages of %lld bytes",
                     (long long)layer, (long long)offset, (long long)page_bytes);
+    if (rows && !seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of no sequence", (long long)rows);
     if (!row_start && rows != seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of %lld sequences need row_start", (long long)rows, (long long)seqs);
     if (rows && (!base || !table || !lengths)) return fail(NC_ERR_ARGUMENT, "null pool, table or lengths");
     if (misaligned(error, 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
@@ -316,7 +317,7 @@ extern "C" int32_t nc_kv4_attention(void **p, const int64_t *s, void *stream) {
     const int64_t heads = s[9], max_length = s[16], scratch = s[17];
     int64_t max_rows = s[15];
     if (heads <= 0 || heads % a.pool.kv) return fail(NC_ERR_ARGUMENT, "%lld query heads do not share %d KV heads evenly", (long long)heads, a.pool.kv);
-    if (a.at.rows == 0 || a.at.seqs == 0) return NC_OK;
+    if (a.at.rows == 0) return NC_OK;
     a.out = p[0];
     a.q = p[1];
     a.cos_tab = (const float *)p[6];

@@ -237,3 +237,13 @@ def test_outputs_of_log_probabilities_come_in_pairs(change):
              "top": Fake((2, 5), np.int64), "top_logprobs": Fake((2, 5), np.float32), "scratch": Fake((1 << 22,), np.uint8), **change}
     with pytest.raises(runtime.InterpreterError, match="top with top_logprobs"):
         serving.token_logprobs(**given)
+
+
+def test_rows_of_no_sequence_are_refused():
+    pool, table, lengths = cache(LAYOUT, seqs=0)
+    start = Fake((1,), np.int32)
+    for call in (lambda: attend(LAYOUT, table=table, lengths=lengths, row_start=start),
+                 lambda: serving.kv4_append(LAYOUT, pool, ROWS, ROWS, table, lengths, row_start=start),
+                 lambda: serving.kv4_read(LAYOUT, ROWS, ROWS, pool, table, lengths, row_start=start)):
+        with pytest.raises(runtime.InterpreterError, match="2 rows of no sequence"):
+            call()
