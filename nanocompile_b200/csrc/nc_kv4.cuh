@@ -216,18 +216,6 @@ struct Kv4AppendArgs {
     int type;
 };
 
-// The value of dimension i of a head's row, rotated where there is a table: the reference's
-// t * cos + rot(t) * sin (nanocompile/nn.py:97-106), each product and sum rounded by itself.
-__device__ __forceinline__ float kv4_rotated(const void *p, int64_t base, int i, int d, int type, const float *cos_tab,
-                                             const float *sin_tab, int64_t position) {
-    const float x = kv_load(p, base + i, type);
-    if (!cos_tab) return x;
-    const int half = d >> 1, k = i < half ? i : i - half;
-    const float y = kv_load(p, base + (i < half ? i + half : i - half), type);
-    const float c = cos_tab[position * half + k], s = sin_tab[position * half + k];
-    return i < half ? fsub(fmul(x, c), fmul(y, s)) : fadd(fmul(x, c), fmul(y, s));
-}
-
 // Eight values from element `at` (of 16-byte aligned memory where `vectors`).
 __device__ __forceinline__ void kv_load8(const void *p, int64_t at, int type, bool vectors, float (&x)[8]) {
     if (!vectors) {
@@ -338,7 +326,7 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS) kv4_append_rows_kernel(co
                 const int place = (int)position % a.at.page;
                 t = place % KV4_TILE;
                 tile = a.pool.base + page * a.pool.page_bytes + ((int64_t)head * (a.at.page / KV4_TILE) + place / KV4_TILE) * (20 * D) + which * 10 * D;
-                if (rotate) {
+                if (rotate) {                          // the reference's t * cos + rot(t) * sin (nanocompile/nn.py:97-106), every step rounded
                     float cs[8], sn[8];
                     kv_load8(a.cos_tab, position * HALF + k, KV_F32, vectors, cs);
                     kv_load8(a.sin_tab, position * HALF + k, KV_F32, vectors, sn);
@@ -402,7 +390,7 @@ __global__ void __launch_bounds__(32 * KV4_TILE_WARPS, NB == 3 ? 6 : 8) kv4_appe
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
         }
-        if (rotate && in) {                                           // as kv4_rotated, eight at a time
+        if (rotate && in) {                                           // as row by row
             const int64_t angle = (rows.position + t - rows.t0) * HALF;
             if constexpr (NB % 2 == 0) {                              // a lane has both of a pair
 #pragma unroll
