@@ -887,3 +887,22 @@ def test_row_starts_that_end_past_the_rows_reach_no_others(cuda, rows):
     want = ref.stands_for(*ref.quantise(held)).reshape(rows, line)
     for got in back:
         assert np.array_equal(got.numpy()[:rows], want) and (got.numpy()[rows:] == 5).all()
+
+
+@pytest.mark.parametrize("seqs", [2, 700])                                       # one CTA's bookkeeping, and a cluster's
+def test_a_shortage_of_pages_changes_nothing(cuda, seqs):
+    rng = np.random.default_rng(seqs)
+    if seqs == 2:                                     # both continue the second: a copy of page 2 and a page behind each, of pages 0 and 1
+        pages, missing, used = 3, 1, 3
+        table, lengths = np.array([[0, 1], [2, -1]], np.int32), np.array([32, 5], np.int32)
+        parent, grow = [1, 1], [16, 17]
+    else:                                             # a hundred more continue the first, whose last page is not full, and 50 pages are free
+        width, live, pages, missing, used = 9, 600, 5450, 50, 5400
+        table = np.full((seqs, width), -1, np.int32)
+        table[:live] = rng.permutation(pages)[: live * width].reshape(live, width)
+        lengths = np.where(np.arange(seqs) < live, 16 * (width - 1) + 5, 0).astype(np.int32)
+        parent, grow = np.where(np.arange(seqs) < live, np.arange(seqs), 0), np.where(np.arange(seqs) < live, 0, 200)
+    pool = rng.integers(0, 256, (pages, 32), np.uint8)
+    new, n, status, same = update(table, lengths, 16, pool, parent, grow)
+    assert status == [missing, used, 0, 0]
+    assert np.array_equal(new, table) and np.array_equal(n, lengths) and np.array_equal(same, pool)
