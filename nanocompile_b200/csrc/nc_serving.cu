@@ -112,14 +112,41 @@ constexpr int64_t KV4_COUNTERS = 4096;         // groups that can be split: thei
 constexpr int64_t KV4_PARTS = 1 << 17;         // columns of all parts of a split call at most: bounds the scratch of every smaller call
 constexpr int64_t KV4_SPLITS = 64, KVT_PLACES = 148 * 2;
 constexpr int KV4_STAGES = 2;
-// bfloat16 rows go to the tensor cores' kernel from this many columns of a sequence and tiles (128 columns by 64 positions)
-// of the call.  Below, its start, its wide parts and few CTAs cost more than they give.  Measured, it against the products on
-// the codes, head dimension 128: 8 sequences of 32 rows of 4 heads over 2000 positions (2048 tiles) 70 against 93 us, 2 of
-// 300 over 300 (800) 36 against 58, 4 of 64 over 500 (512) 41 against 38, one of 64 over 2000 (512) 41 against 25, of 512 over
-// 512 (1024) 59 against 57; 64: 4 of 512 rows of 14 heads (1792) 29 against 70, 1024 rows (1792) 40 against 45, 256 over 4000
-// (1764) 49 against 47.
-constexpr int64_t KV4_PROMPT_COLS = 96;
-constexpr int64_t kv4_prompt_tiles(int64_t d) { return d == 128 ? 600 : 1780; }
+// bfloat16 rows of this many columns of a sequence and more may go to the tensor cores' kernel: half of its 128 are idle then.
+constexpr int64_t KV4_PROMPT_COLS = 64;
+
+// Its splits, and what they take by a model of the measured times, in us: the start with the queries, a chunk of tiles (128 columns by
+// 64 positions) in a CTA that has an SM to itself or shares it, more of both in rounds of CTAs, the join of split histories.  The call
+// goes there where this is less than what the products on the codes take by their model.  Both timed for 546 calls (1 to 128
+// sequences, 1 to 2,000 rows, histories to 16,000, fourteen layouts of heads; 250 of them drawn after the model was fitted), the choice
+// costs 1% against the better of the two in the mean, 40% at most (16 heads of 64, 2 sequences of 256 rows over 756: 43 us, 31 by
+// the codes).  In us, there and by the codes: 14 heads on 2 of 64, 4 sequences of 480 rows 27 and 61, one of 1024 38 and 47; 32 on 8 of
+// 128, 480 rows 31 and 53, 128 rows over 3128 59 (in four splits; 108 whole, 99 in ten) and 94; 128 rows alone 20 and 14.
+struct PromptPlan {
+    int splits, chunk;
+    float cost;
+};
+PromptPlan kv4_prompt_plan(int64_t groups, int64_t group, int64_t d, int64_t max_rows, int64_t max_length) {
+    const bool wide = d == 128;
+    const float start = wide ? 16.0f : 10.5f, alone = wide ? 1.8f : 1.7f, shared = wide ? 2.8f : 2.7f, round = wide ? 30.0f : 20.0f;
+    const float join = wide ? 19.0f : 9.0f, part = wide ? 1.7f : 0.6f;
+    const int64_t steps = std::max<int64_t>(1, (max_length + KVT_STEP - 1) / KVT_STEP);
+    const int64_t block_rows = std::min(max_rows, std::max<int64_t>(1, KVT_COLS / group));       // the first block's last row sees `first` tiles
+    const int64_t first = std::max<int64_t>(1, (max_length - max_rows + block_rows + KVT_STEP - 1) / KVT_STEP);
+    const float mean = 0.5f * (float)(std::min(first, steps) + steps);
+    PromptPlan best{};
+    for (int splits : CUTS) {
+        if (splits > 1 && (splits > std::min(KV4_SPLITS, steps) || groups * splits > KVT_PLACES)) break;
+        const int64_t chunk = (steps + splits - 1) / splits;
+        if ((steps + chunk - 1) / chunk != splits) continue;            // as good as fewer
+        const float ctas = (float)groups * (splits == 1 ? 1.0f : std::min((float)splits, mean / (float)chunk + 0.5f));
+        float cost = start + (splits > 1 ? join + part * (float)splits : 0.0f);
+        if (ctas <= (float)KVT_PLACES) cost += (ctas <= (float)(KVT_PLACES / 2) ? alone : shared) * (float)chunk;
+        else cost += shared * (float)groups * mean / (float)KVT_PLACES + 1.2f * (float)chunk + round * (ctas / (float)KVT_PLACES - 1.0f);
+        if (best.splits == 0 || cost < best.cost) best = PromptPlan{splits, (int)chunk, cost};
+    }
+    return best;
+}
 
 // Columns and warps of a CTA, and splits of the histories: the cheapest by a model of the measured times, in units of a step on
 // an SM that is full (3.3 us; 16 warps of 8 columns fill it, or 8 of 16, which share the codes' way to operands): a CTA
@@ -133,18 +160,6 @@ constexpr int64_t kv4_prompt_tiles(int64_t d) { return d == 128 ? 600 : 1780; }
 AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t max_rows, int64_t max_length, bool bf16) {
     AttnPlan p{};
     const int64_t cols = heads / kv * max_rows;
-    const int64_t prompt_blocks = (cols + KVT_COLS - 1) / KVT_COLS, prompt_steps = std::max<int64_t>(1, (max_length + KVT_STEP - 1) / KVT_STEP);
-    if (bf16 && (d == 64 || d == 128) && cols >= KV4_PROMPT_COLS && seqs * kv * prompt_blocks * prompt_steps >= kv4_prompt_tiles(d)) {
-        p.nt = KVT_COLS / 8;                                             // 128 columns, two CTAs to an SM
-        p.col_blocks = (int)prompt_blocks;
-        p.groups = seqs * kv * prompt_blocks;
-        const int64_t steps = prompt_steps;
-        int64_t splits = p.groups == 0 || p.groups > KV4_COUNTERS ? 1 : KVT_PLACES / p.groups;
-        splits = std::max<int64_t>(1, std::min(splits, steps / 4));     // a split is worth its join from four steps on
-        p.chunk = (int)((steps + splits - 1) / splits);
-        p.splits = (int)((steps + p.chunk - 1) / p.chunk);
-        return p;
-    }
     const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, steps = std::max<int64_t>(1, (max_length + step - 1) / step);
     const int64_t first = std::max<int64_t>(1, (max_length - max_rows + step) / step);       // of the first row
     float best = 0.0f;
@@ -185,6 +200,17 @@ AttnPlan kv4_plan(int64_t seqs, int64_t heads, int64_t kv, int64_t d, int64_t ma
                 }
                 if (groups * splits > 16 * places) break;
             }
+        }
+    }
+    if (bf16 && (d == 64 || d == 128) && cols >= KV4_PROMPT_COLS) {
+        const int64_t blocks = (cols + KVT_COLS - 1) / KVT_COLS, groups = seqs * kv * blocks;
+        const PromptPlan t = kv4_prompt_plan(groups, heads / kv, d, max_rows, max_length);
+        if (t.cost < (p.nt == 1 ? 3.7f + 4.2f * best : 6.8f + 2.6f * best)) {     // the model's units as us, fitted to the same calls
+            p.nt = KVT_COLS / 8;                                         // 128 columns, two CTAs to an SM
+            p.col_blocks = (int)blocks;
+            p.groups = groups;
+            p.splits = t.splits;
+            p.chunk = t.chunk;
         }
     }
     return p;
@@ -305,8 +331,8 @@ extern "C" int64_t nc_kv4_attention_scratch_bytes(int64_t seqs, int64_t heads, i
     const int64_t step = kv4_step_tiles((int)d) * KV4_TILE, splits = std::min(KV4_SPLITS, (max_length + step - 1) / step);
     int64_t most = 0;
     if (splits > 1) most = std::min(KV4_PARTS, histories * padded(cols <= 8 ? 8 : 16) * splits);
-    if (const int64_t wide = max_length / KVT_STEP / 4; wide > 0 && cols >= KV4_PROMPT_COLS)
-        most = std::max(most, std::min(KVT_PLACES * KVT_COLS, histories * padded(KVT_COLS) * (wide + 1)));
+    if (const int64_t prompt = std::min(KV4_SPLITS, (max_length + KVT_STEP - 1) / KVT_STEP); prompt > 1 && cols >= KV4_PROMPT_COLS)
+        most = std::max(most, std::min(KVT_PLACES * KVT_COLS, histories * padded(KVT_COLS) * prompt));
     return most == 0 ? 256 : 4 * KV4_COUNTERS + most * (d + 2) * 4;
 }
 

@@ -112,11 +112,11 @@ def test_a_4_bit_prompt_stops_on_a_short_wait_and_its_scratch_stays_good(short_w
     from tests.test_gpu_serving import Case
 
     cuda, rng = short_waits, np.random.default_rng(d)
-    layout, case = serving.KV4Layout(4, 1, d, 16), Case(rng, [700, 150], 1, d, 16)
-    query, counts = rng.standard_normal((80, 4, d)).astype(np.float32), [50, 30]
-    scratch = serving.DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, 80, 2, 20000, 80),), np.uint8)
-    # Enough work, by its bounds, for that kernel, in chunks of 448 positions: two of the longer history.
-    bounds = dict(max_length=20000, max_rows=80, scratch=scratch)
+    layout, case = serving.KV4Layout(16, 1, d, 16), Case(rng, [700, 150], 1, d, 16)
+    query, counts = rng.standard_normal((80, 16, d)).astype(np.float32), [50, 30]
+    scratch = serving.DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, 80, 2, 2000, 80),), np.uint8)
+    # Enough work, by its bounds, for that kernel, in chunks of 320 positions: three of the longer history.
+    bounds = dict(max_length=2000, max_rows=80, scratch=scratch)
     want = case.check(layout, query, "bfloat16", counts, **bounds)
     cuda.set_wait_limit(1)
     for _ in range(2):

@@ -906,3 +906,27 @@ def test_a_shortage_of_pages_changes_nothing(cuda, seqs):
     new, n, status, same = update(table, lengths, 16, pool, parent, grow)
     assert status == [missing, used, 0, 0]
     assert np.array_equal(new, table) and np.array_equal(n, lengths) and np.array_equal(same, pool)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_split_histories_on_the_tensor_cores(cuda, d):
+    """Sixteen heads of one key head and a bound of 2000 positions: chunks of 320, several to the longer histories."""
+    rng = np.random.default_rng(d)
+    case, counts = Case(rng, [1500, 330, 70, 0], 1, d, 32), [50, 80, 70, 3]
+    layout, bounds = KV4Layout(16, 1, d, 32), dict(max_length=2000, max_rows=80)
+    q, rope = rng.standard_normal((sum(counts), 16, d)).astype(np.float32), ref.rope_tables(1500, d)
+    scratch = DeviceArray.zeros((serving.kv4_attention_scratch_bytes(layout, sum(counts), 4, 2000, 80),), np.uint8)
+    want = case.check(layout, q, "bfloat16", counts, rope=rope, scratch=scratch, **bounds)
+    case.check(layout, q * 20, "bfloat16", counts, scratch=scratch, **bounds)
+    q = ref.decode(ref.encode(q, "bfloat16"), "bfloat16")
+    again = case.attend(layout, q, "bfloat16", counts, rope, scratch=scratch, **bounds)
+    assert all(np.array_equal(a.view(np.uint32), b.view(np.uint32)) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("heads,kv,d,rows", [(14, 2, 64, 480), (8, 2, 64, 128), (8, 2, 128, 64), (128, 1, 128, 1), (100, 1, 64, 3)])
+def test_bfloat16_prompts_on_either_side_of_the_choice(cuda, heads, kv, d, rows):
+    rng = np.random.default_rng(rows)
+    for seqs in (1, 4):
+        case = Case(rng, [rows + 5 * i for i in range(seqs)], kv, d, 64)
+        q = rng.standard_normal((seqs * rows, heads, d)).astype(np.float32)
+        case.check(KV4Layout(heads, kv, d, 64), q, "bfloat16", [rows] * seqs)
