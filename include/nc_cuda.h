@@ -240,7 +240,7 @@ int32_t nc_kv4_read(void **p, const int64_t *s, void *stream);
 /* Attention of rows over the cache: row r at position t sees positions 0..t of its sequence; a row that sees
  * nothing gets zeros and a log-sum of -inf.  Queries are rotated where there is a table.  float32 and
  * float16 calls keep float32 accuracy (queries and probabilities in two parts); bfloat16 calls round each to
- * one f16 part.  The scale is positive.  Rows of a sequence past `the most rows` get no output, and positions
+ * one f16 part, and with many rows the decoded values and scale x code of the keys too.  The scale is positive.  Rows of a sequence past `the most rows` get no output, and positions
  * past `the most positions` no share.
  * p: [0] out [rows, heads, d]  [1] q [rows, heads, d]  [2] pool  [3] table  [4] lengths
  *    [5] row_start (nullable)  [6] cos  [7] sin (nullable)  [8] log-sums f32[rows, heads] (nullable)

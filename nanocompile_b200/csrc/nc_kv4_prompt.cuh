@@ -3,12 +3,16 @@
 // What nc_kv4_attention.cuh computes, for prompts: 128 columns (row, head of the group) of one kv head to a CTA, 64
 // positions at a time.  Each tile's keys and values are brought from their codes to f16 in shared memory once for all
 // columns; then S = Q K^T and O += P V are tcgen05.mma kind::f16 with Q, S, P and O in tensor memory (256 columns: Q d / 2,
-// S 64 with P over it, O d), accumulated in float32.  Nothing but the values' rounding to f16 (11 bits, of quantities that
-// have 4) is lost against the products on the codes; float32 rows, which need more, stay with those.
+// S 64 with P over it, O d), accumulated in float32.
 //
-//   keys    zero + scale * code, with scale and zero times a power of two for each tile, that the scores get back
-//   values  the same with a power of two that only grows, O rescaled when it does: no size of value leaves the f16 range
+//   keys    scale * code, with scale and zero times a power of two for each tile, that the scores get back; the zeros go into S
+//           by one more instruction, as 16 more dimensions: the blocks' sums of q in two f16 parts times the zeros
+//   values  zero + scale * code times a power of two that only grows, O rescaled when it does: no size of value leaves the f16 range
 //   p       2^(x - ref), ref a past maximum: O and the sums are rescaled only when the maximum has grown by 8
+//
+// Accuracy.  q, p, scale * code of the keys and the decoded values are each rounded once to f16's 11 bits; the products on the codes
+// round q, p and p * scale.  Keys far from nought lose nothing by it, as their zeros are not rounded (with zero + scale * code in f16
+// as keys, a log-sum over keys N(100, 0.3) was off by up to 3.5e-2, now by 3.8e-4).  float32 rows, which need more, stay with the codes.
 //
 // Layouts.  An eight-value group of dimensions is held in the order 0 4 1 5 2 6 3 7 that a code word gives, by Q and K
 // alike; the positions of a tile in the order that gives a lane eight of them for one dimension: 32 positions 16 i + 8 j +
@@ -20,7 +24,7 @@
 // tile.  A second CTA on the SM fills what is left idle.
 //
 // Bound by the instruction rate: decoding takes 17 for eight values and the softmax about five a score.  Measured: 2
-// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 458 us, 0.39 PFLOP/s (the matrix pipe is busy for a
+// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 463 us, 0.39 PFLOP/s (the matrix pipe is busy for a
 // fifth of it, an instruction issues in half of the cycles); the products on the codes take 1.1 ms there.
 #pragma once
 
@@ -37,9 +41,11 @@ template <int D>
 struct KvtShared {
     __align__(1024) char k[2][KVT_STEP * D * 2];   // [d / 64][64 places][128 bytes]
     __align__(1024) char v[KVT_STEP * D * 2];  // [d][128 bytes]
+    __align__(1024) char kz[2][KVT_STEP * 32]; // [64 places][16 f16]: the blocks' zeros, twice, then nothing
+    __align__(1024) char qz[KVT_COLS * 32];    // [128 columns][16 f16]: the blocks' sums of q in two parts, then nothing
     __align__(16) char raw[3][4 * 20 * D];
     uint64_t s_done, o_done, raw_full[3];      // mbarriers
-    float row_max[2][KVT_COLS], row_sum[2][KVT_COLS];
+    float row_max[2][KVT_COLS], row_sum[2][KVT_COLS], block_sum[2][2][KVT_COLS];
     int2 row[KVT_COLS];                        // row, head
     uint32_t tmem, there[4], top[4][4];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits)
     unsigned int arrived;
@@ -78,7 +84,20 @@ __device__ __forceinline__ bool kvt_mbar_wait(uint64_t *bar, unsigned parity, lo
 __device__ __forceinline__ uint64_t kvt_desc(uint32_t address) {
     return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// D[128 x N] (+)= A[128 x 16] B[16 x N], A in tensor memory, f16 with float32 sums.
+// The same of 32-byte swizzled rows: eight rows are 256 bytes, and bit 4 of an address is flipped by its bit 7.
+__device__ __forceinline__ uint64_t kvt_desc32(uint32_t address) {
+    return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)6 << 61;
+}
+// D[128 x N] = A[128 x 16] B[16 x N], both in shared memory, f16 with float32 sums.
+__device__ __forceinline__ void kvt_mma_shared(uint32_t d, uint64_t a, uint64_t b, int n) {
+    const uint32_t kind = 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(kind), "r"(0u)
+        : "memory");
+}
+// D[128 x N] (+)= A[128 x 16] B[16 x N], A in tensor memory.
 __device__ __forceinline__ void kvt_mma(uint32_t d, uint32_t a, uint64_t b, int n, bool add) {
     const uint32_t kind = 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
     asm volatile(
@@ -267,7 +286,8 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;          // the warp's quarter of tensor memory
     const uint32_t tq = sh.tmem, ts = tq + D / 2, to = ts + KVT_STEP;
 
-    // The queries: dimensions i and i + d / 2 for a quarter of d, rotated, brought to [2^14, 2^15) and put into tensor memory.
+    // The queries: dimensions i and i + d / 2 for a quarter of d, rotated, brought to [2^9, 2^10), that a block's sum stays in f16's
+    // range, and put into tensor memory; the blocks' sums, of what is not rounded yet, go to shared memory.
     const bool have = col < ncol;
     const int r = have ? (col0 + col) / a.group : 0;
     const int qrow = row0 + r, qhead = head * a.group + (have ? col0 + col - r * a.group : 0);
@@ -301,7 +321,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         most = fmaxf(sh.row_max[0][col], sh.row_max[1][col]);
         const uint32_t bits = __float_as_uint(most);
         int e = 0;
-        if (bits != 0 && bits < 0x7f800000u) e = 14 - ((int)(bits >> 23) - 127);
+        if (bits != 0 && bits < 0x7f800000u) e = 9 - ((int)(bits >> 23) - 127);
         e = e < -100 ? -100 : e > 100 ? 100 : e;
         const float by = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : pow2i(e);     // an infinity or a NaN: all of the row
         f = fmul(a.scale_log2e, pow2i(-e));
@@ -317,6 +337,33 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         put(lo, tq + lanes + part * (Q / 2));
         put(hi, tq + lanes + D / 4 + part * (Q / 2));
         kvt_wait_st();
+        float first_half = 0.0f, second_half = 0.0f;                   // of blocks `part` and 2 + part, or halves of blocks 0 and 1 (d = 64)
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            first_half = __fmaf_rn(lo[i], by, first_half);
+            second_half = __fmaf_rn(hi[i], by, second_half);
+        }
+        sh.block_sum[part][0][col] = first_half;
+        sh.block_sum[part][1][col] = second_half;
+        __syncthreads();
+        if (part == 0) {
+            float sums[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) sums[b] = NB == 4 ? sh.block_sum[b & 1][b >> 1][col] : sh.block_sum[0][b][col] + sh.block_sum[1][b][col];
+            uint32_t z[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                z[b / 2] = pack_f16(sums[b], sums[b + 1]);
+                const float2 high = unpack_f16(z[b / 2]);
+                z[(NB + b) / 2] = pack_f16(sums[b] - high.x, sums[b + 1] - high.y);
+            }
+            const uint32_t to_row = kvt_smem(sh.qz) + col * 32, flip = col >> 2 & 1;
+            store16_shared(to_row + 16 * flip, z[0], z[1], z[2], z[3]);
+            store16_shared(to_row + 16 * (flip ^ 1), 0, 0, 0, 0);
+        } else {
+            store16_shared(kvt_smem(sh.kz[0]) + col * 32, 0, 0, 0, 0);  // both buffers' 128 rows
+            store16_shared(kvt_smem(sh.kz[0]) + col * 32 + 16, 0, 0, 0, 0);
+        }
     }
 
     float ref = -INFINITY, sum = 0.0f;                                 // of the thread's half of the positions
@@ -326,9 +373,10 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const int key_place = 32 * (warp >> 1 & 1) + 8 * (g >> 1) + 4 * (warp & 1) + (g & 1);
     const uint32_t key_unit = kvt_smem(sh.k[0]) + (NB == 4 ? part : 0) * (KVT_STEP * 128) + key_place * 128 +
                               (((4 * ((NB == 4 ? 0 : part) ^ (g & 1)) + c) ^ (key_place & 7)) << 4);
+    const uint32_t zero_row = kvt_smem(sh.kz[0]) + (key_place + 2 * c) * 32 + 16 * (key_place >> 2 & 1) + (NB == 4 ? 4 * part : 0);   // of lanes c < 2
     const int value_grp = NB == 4 ? part : warp >> 1 & 1, value_block = NB == 4 ? warp & 3 : warp & 1;
     const uint32_t value_unit = kvt_smem(sh.v) + (32 * value_block + 4 * g) * 128 + (((4 * value_grp + c) ^ (4 * (g & 1))) << 4);
-    // Keys of a tile that is here: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half
+    // Keys of a tile that is here, and their zeros: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half
     // of the lanes).
     auto decode_keys = [&](int step) {
         const int n = step - step0, k = warp & 3, pair = NB == 4 ? part : 0;      // the lane's words of both blocks are one load
@@ -336,6 +384,10 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         const uint32_t unit = pow2_f16x2(-kvt_exponent(sh.top[n & 3][0], sh.top[n & 3][1])), to_unit = key_unit + (n & 1) * (KVT_STEP * D * 2);
         const uint4 codes = *(const uint4 *)((const uint32_t *)tile + kv4_code_word(VB, 2 * pair, lane, 0));
         const uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
+        if (c < 2 && (NB == 4 || part == 0)) {                         // the zeros of position 8 c + g, for both parts of the sums
+            const uint32_t z = mul_f16x2(__byte_perm(c ? params.y : params.x, c ? params.w : params.z, 0x7632), unit), row = zero_row + (n & 1) * (KVT_STEP * 32);
+            asm volatile("st.shared.b32 [%0], %1;\n\tst.shared.b32 [%0 + %2], %1;" ::"r"(row), "r"(z), "n"(2 * NB) : "memory");
+        }
 #pragma unroll
         for (int n = 0; n < NB / 2; ++n) {
             const int v2 = (NB == 4 ? n : part) ^ (g & 1);             // odd rows take the other block first
@@ -344,16 +396,17 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
-                const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
-                store16_shared((to_unit ^ (n << 6) ^ (j << 5)) + 256 * j, fma_f16x2(codes_low(x), s, z), fma_f16x2(codes_high(x), s, z),
-                               fma_f16x2(codes_low(x >> 8), s, z), fma_f16x2(codes_high(x >> 8), s, z));
+                const uint32_t s = __byte_perm(p, p, 0x1010);
+                store16_shared((to_unit ^ (n << 6) ^ (j << 5)) + 256 * j, mul_f16x2(codes_low(x), s), mul_f16x2(codes_high(x), s),
+                               mul_f16x2(codes_low(x >> 8), s), mul_f16x2(codes_high(x >> 8), s));
             }
         }
     };
     auto issue_scores = [&](int step) {                                // by one thread
         const uint32_t keys = kvt_smem(sh.k[(step - step0) & 1]);
+        kvt_mma_shared(ts, kvt_desc32(kvt_smem(sh.qz)), kvt_desc32(kvt_smem(sh.kz[(step - step0) & 1])), KVT_STEP);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) kvt_mma(ts, tq + 8 * k, kvt_desc(keys + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, k > 0);
+        for (int k = 0; k < D / 16; ++k) kvt_mma(ts, tq + 8 * k, kvt_desc(keys + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, true);
         kvt_commit(&sh.s_done);
     };
     auto look_at = [&](int step) {

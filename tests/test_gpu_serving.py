@@ -930,3 +930,37 @@ def test_bfloat16_prompts_on_either_side_of_the_choice(cuda, heads, kv, d, rows)
         case = Case(rng, [rows + 5 * i for i in range(seqs)], kv, d, 64)
         q = rng.standard_normal((seqs * rows, heads, d)).astype(np.float32)
         case.check(KV4Layout(heads, kv, d, 64), q, "bfloat16", [rows] * seqs)
+
+
+@pytest.mark.parametrize("heads,d,bounds", [(16, 128, dict(max_length=2000, max_rows=80)), (16, 64, dict(max_length=2000, max_rows=80)), (2, 128, {}), (4, 96, {})])
+@pytest.mark.parametrize("centre,spread", [(100.0, 0.3), (-30.0, 1.0), (0.0, 1.0)])
+def test_bfloat16_scores_of_keys_far_from_nought(cuda, heads, d, bounds, centre, spread):
+    """Blocks stand for zero + scale * code, and only the second part is rounded, with the queries.
+
+    A score is off by 2^-12 of R = sum_i |q_i| scale_i code_i for the queries and as much again for the keys, and by 2^-20 of
+    S = sum_i |q_i k_i| as for the other types; a log-sum by no more than the scores that are in it, and 2^-18.
+    """
+    rng = np.random.default_rng(d)
+    case, counts = Case(rng, [64, 300], 1, d, 16), [64, 80]
+    if not bounds:
+        counts = [3, 5]
+    starts, page = starts_of(case.lengths), 16
+    keys = (rng.standard_normal((starts[-1], 1, d)) * spread + centre * np.where(np.arange(d) // 32 % 2, -1, 1)).astype(np.float32)
+    case.pool.append(keys, keys / max(1.0, abs(centre)), case.table, case.lengths, starts)
+    case.histories = [case.pool.history(case.table[i], n) for i, n in enumerate(case.lengths)]
+    case.upload()
+    q = ref.decode(ref.encode(rng.standard_normal((sum(counts), heads, d)).astype(np.float32), "bfloat16"), "bfloat16")
+    got, lse = case.attend(KV4Layout(heads, 1, d, page), q, "bfloat16", counts, **bounds)
+    want, want_lse, size = ref.attention(q, case.histories, case.lengths, starts_of(counts), np.float32(d ** -0.5))
+    ranges = np.zeros_like(size)
+    for i, (k, _) in enumerate(case.histories):
+        offset = k.reshape(len(k), d // 32, 32)
+        offset = (offset - offset.min(-1, keepdims=True)).astype(np.float64).reshape(len(k), d)
+        rows = slice(starts_of(counts)[i], starts_of(counts)[i + 1])
+        for r in range(rows.start, rows.stop):
+            seen = int(case.lengths[i]) - (rows.stop - r) + 1
+            ranges[r] = (offset[:seen] @ np.abs(q[r]).T).max(0) * d ** -0.5
+    assert (np.abs(lse - want_lse) <= 2.0 ** -11 * ranges + 2.0 ** -20 * size + 2.0 ** -18 + 2.0 ** -22 * np.abs(want_lse)).all()
+    most = max(np.abs(v).max() for _, v in case.histories)
+    bound = (2 * (2.0 ** -11 * ranges + 2.0 ** -20 * size) + 2.0 ** -10)[..., None] * most + ROUNDING["bfloat16"] * np.abs(want) * 1.001
+    assert (np.abs(got - want) <= bound).all()
