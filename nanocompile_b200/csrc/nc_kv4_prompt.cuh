@@ -5,14 +5,15 @@
 // columns; then S = Q K^T and O += P V are tcgen05.mma kind::f16 with Q, S, P and O in tensor memory (256 columns: Q d / 2,
 // S 64 with P over it, O d), accumulated in float32.
 //
-//   keys    scale * code, with scale and zero times a power of two for each tile, that the scores get back; the zeros go into S
-//           by one more instruction, as 16 more dimensions: the blocks' sums of q in two f16 parts times the zeros
+//   keys    zero + scale * code, with scale and zero times a power of two for each tile, that the scores get back; of blocks far from
+//           nought (|zero| above 16 scales) scale * code alone, and their zeros go into S by one more instruction, as 16 more
+//           dimensions: the blocks' sums of q in two f16 parts times the zeros
 //   values  zero + scale * code times a power of two that only grows, O rescaled when it does: no size of value leaves the f16 range
 //   p       2^(x - ref), ref a past maximum: O and the sums are rescaled only when the maximum has grown by 8
 //
-// Accuracy.  q, p, scale * code of the keys and the decoded values are each rounded once to f16's 11 bits; the products on the codes
-// round q, p and p * scale.  Keys far from nought lose nothing by it, as their zeros are not rounded (with zero + scale * code in f16
-// as keys, a log-sum over keys N(100, 0.3) was off by up to 3.5e-2, now by 3.8e-4).  float32 rows, which need more, stay with the codes.
+// Accuracy.  q, p, the decoded keys (far zeros apart) and values are each rounded once to f16's 11 bits, the keys so by 1/64 of a
+// scale at most; the products on the codes round q, p and p * scale.  With far zeros in the keys a log-sum over keys N(100, 0.3) was
+// off by up to 3.5e-2, now by 3.8e-4.  float32 rows, which need more, stay with the codes.
 //
 // Layouts.  An eight-value group of dimensions is held in the order 0 4 1 5 2 6 3 7 that a code word gives, by Q and K
 // alike; the positions of a tile in the order that gives a lane eight of them for one dimension: 32 positions 16 i + 8 j +
@@ -24,7 +25,7 @@
 // tile.  A second CTA on the SM fills what is left idle.
 //
 // Bound by the instruction rate: decoding takes 17 for eight values and the softmax about five a score.  Measured: 2
-// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 463 us, 0.39 PFLOP/s (the matrix pipe is busy for a
+// sequences' last 1000 of 6001 positions, 32 heads on 8 of dimension 128, 462 us, 0.39 PFLOP/s (the matrix pipe is busy for a
 // fifth of it, an instruction issues in half of the cycles); the products on the codes take 1.1 ms there.
 #pragma once
 
@@ -41,13 +42,13 @@ template <int D>
 struct KvtShared {
     __align__(1024) char k[2][KVT_STEP * D * 2];   // [d / 64][64 places][128 bytes]
     __align__(1024) char v[KVT_STEP * D * 2];  // [d][128 bytes]
-    __align__(1024) char kz[2][KVT_STEP * 32]; // [64 places][16 f16]: the blocks' zeros, twice, then nothing
+    __align__(1024) char kz[2][KVT_STEP * 32]; // [64 places][16 f16]: the far blocks' zeros, twice, then nothing
     __align__(1024) char qz[KVT_COLS * 32];    // [128 columns][16 f16]: the blocks' sums of q in two parts, then nothing
     __align__(16) char raw[3][4 * 20 * D];
     uint64_t s_done, o_done, raw_full[3];      // mbarriers
     float row_max[2][KVT_COLS], row_sum[2][KVT_COLS], block_sum[2][2][KVT_COLS];
     int2 row[KVT_COLS];                        // row, head
-    uint32_t tmem, there[4], top[4][4];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits)
+    uint32_t tmem, there[4], top[4][8];                  // there: the tile's cache tiles; top: its largest key scale, |key zero|, value scale, |value zero| (bits); whether there are far blocks
     unsigned int arrived;
 };
 
@@ -152,6 +153,14 @@ __device__ __forceinline__ uint32_t max_nan_f16x2(uint32_t a, uint32_t b) {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// Whether either half of `a` is above that of `b`.
+__device__ __forceinline__ bool any_above_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("{\n\t.reg .pred p, q;\n\tsetp.gt.f16x2 p|q, %1, %2;\n\tor.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+    return r != 0;
+}
+// A block's parameters with a zero of 0 where it is far from nought: |zero| above 16 scales, 4 more in the exponent.
+__device__ __forceinline__ uint32_t kvt_near(uint32_t w) { return (w >> 16 & 0x7fffu) > (w & 0xffffu) + 0x1000u ? w & 0xffffu : w; }
 __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         kvt_mbar_init(&sh.raw_full[2]);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < 16) sh.top[tid >> 2][tid & 3] = 0;
+    if (tid < 32) sh.top[tid >> 3][tid & 7] = 0;
 
     // Lanes 0 .. 3 of the last warp: a cache tile each.  Its page is looked up a step before its copy is started.
     const int tiles_per_page = a.at.page / KV4_TILE;
@@ -253,6 +262,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         const int buffer = (step - step0) % 3, set = (step - step0) & 3, k = warp & 3;
         const bool there = sh.there[set] >> k & 1;
         uint32_t most = 0;
+        bool far = false;                                              // a block further from nought than 16 scales, hence all on one side
         if (lane < 8 * NB) {
             uint2 *const at = (uint2 *)(sh.raw[buffer] + k * 20 * D + part * 10 * D + 8 * D) + lane;
             const int t = step * KVT_STEP + 16 * k + lane / NB;
@@ -263,7 +273,9 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
                 *at = w;
             }
             most = max_nan_f16x2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+            far = part == 0 && any_above_f16x2(__byte_perm(w.x, w.y, 0x7632) & 0x7fff7fffu, mul_f16x2(__byte_perm(w.x, w.y, 0x5410), 0x4c004c00u));
         }
+        if (__any_sync(0xffffffffu, far) && lane == 0) sh.top[set][4] = 1;
         const uint32_t s = __reduce_max_sync(0xffffffffu, most & 0xffffu), z = __reduce_max_sync(0xffffffffu, most >> 16);
         if (lane == 0) {
             atomicMax(&sh.top[set][2 * part], s);
@@ -376,17 +388,22 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
     const uint32_t zero_row = kvt_smem(sh.kz[0]) + (key_place + 2 * c) * 32 + 16 * (key_place >> 2 & 1) + (NB == 4 ? 4 * part : 0);   // of lanes c < 2
     const int value_grp = NB == 4 ? part : warp >> 1 & 1, value_block = NB == 4 ? warp & 3 : warp & 1;
     const uint32_t value_unit = kvt_smem(sh.v) + (32 * value_block + 4 * g) * 128 + (((4 * value_grp + c) ^ (4 * (g & 1))) << 4);
-    // Keys of a tile that is here, and their zeros: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half
+    // Keys of a tile that is here: cache tile warp % 4, the blocks of panel `part` (d = 64: one of the panel's two for each half
     // of the lanes).
     auto decode_keys = [&](int step) {
         const int n = step - step0, k = warp & 3, pair = NB == 4 ? part : 0;      // the lane's words of both blocks are one load
         const char *const tile = sh.raw[n % 3] + k * 20 * D;
         const uint32_t unit = pow2_f16x2(-kvt_exponent(sh.top[n & 3][0], sh.top[n & 3][1])), to_unit = key_unit + (n & 1) * (KVT_STEP * D * 2);
         const uint4 codes = *(const uint4 *)((const uint32_t *)tile + kv4_code_word(VB, 2 * pair, lane, 0));
-        const uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
-        if (c < 2 && (NB == 4 || part == 0)) {                         // the zeros of position 8 c + g, for both parts of the sums
-            const uint32_t z = mul_f16x2(__byte_perm(c ? params.y : params.x, c ? params.w : params.z, 0x7632), unit), row = zero_row + (n & 1) * (KVT_STEP * 32);
-            asm volatile("st.shared.b32 [%0], %1;\n\tst.shared.b32 [%0 + %2], %1;" ::"r"(row), "r"(z), "n"(2 * NB) : "memory");
+        uint4 params = *(const uint4 *)((const uint32_t *)(tile + 8 * D) + kv4_param_word(NB, 2 * pair, g));
+        if (sh.top[n & 3][4]) {                                        // far blocks' zeros go apart
+            const uint4 near = make_uint4(kvt_near(params.x), kvt_near(params.y), kvt_near(params.z), kvt_near(params.w));
+            if (c < 2 && (NB == 4 || part == 0)) {                     // of position 8 c + g
+                const uint32_t row = zero_row + (n & 1) * (KVT_STEP * 32);
+                const uint32_t z = mul_f16x2(__byte_perm(c ? params.y ^ near.y : params.x ^ near.x, c ? params.w ^ near.w : params.z ^ near.z, 0x7632), unit);
+                asm volatile("st.shared.b32 [%0], %1;\n\tst.shared.b32 [%0 + %2], %1;" ::"r"(row), "r"(z), "n"(2 * NB) : "memory");
+            }
+            params = near;
         }
 #pragma unroll
         for (int n = 0; n < NB / 2; ++n) {
@@ -396,17 +413,18 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t x = j ? w.y : w.x, p = mul_f16x2(j ? par.y : par.x, unit);
-                const uint32_t s = __byte_perm(p, p, 0x1010);
-                store16_shared((to_unit ^ (n << 6) ^ (j << 5)) + 256 * j, mul_f16x2(codes_low(x), s), mul_f16x2(codes_high(x), s),
-                               mul_f16x2(codes_low(x >> 8), s), mul_f16x2(codes_high(x >> 8), s));
+                const uint32_t s = __byte_perm(p, p, 0x1010), z = __byte_perm(p, p, 0x3232);
+                store16_shared((to_unit ^ (n << 6) ^ (j << 5)) + 256 * j, fma_f16x2(codes_low(x), s, z), fma_f16x2(codes_high(x), s, z),
+                               fma_f16x2(codes_low(x >> 8), s, z), fma_f16x2(codes_high(x >> 8), s, z));
             }
         }
     };
     auto issue_scores = [&](int step) {                                // by one thread
         const uint32_t keys = kvt_smem(sh.k[(step - step0) & 1]);
-        kvt_mma_shared(ts, kvt_desc32(kvt_smem(sh.qz)), kvt_desc32(kvt_smem(sh.kz[(step - step0) & 1])), KVT_STEP);
+        const bool far = sh.top[(step - step0) & 3][4] != 0;
+        if (far) kvt_mma_shared(ts, kvt_desc32(kvt_smem(sh.qz)), kvt_desc32(kvt_smem(sh.kz[(step - step0) & 1])), KVT_STEP);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) kvt_mma(ts, tq + 8 * k, kvt_desc(keys + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, true);
+        for (int k = 0; k < D / 16; ++k) kvt_mma(ts, tq + 8 * k, kvt_desc(keys + (k >> 2) * (KVT_STEP * 128) + (k & 3) * 32), KVT_STEP, k > 0 || far);
         kvt_commit(&sh.s_done);
     };
     auto look_at = [&](int step) {
@@ -436,7 +454,7 @@ __global__ void __launch_bounds__(KVT_THREADS, 2) kv4_prompt_kernel(const __grid
         const int ek = kvt_exponent(sh.top[set][0], sh.top[set][1]);
         const int ev_now = max(ev, kvt_exponent(sh.top[set][2], sh.top[set][3]));
         const bool nan = sh.top[set][2] > 0x7c00u || sh.top[set][3] > 0x7c00u;
-        if (tid < 4) sh.top[(set + 3) & 3][tid] = 0;                   // of the last tile, for the look at tile step + 3
+        if (tid < 8) sh.top[(set + 3) & 3][tid] = 0;                   // of the last tile, for the look at tile step + 3
         if (step + 1 < step_end) decode_keys(step + 1);
         // O += P V of the last tile is done: the values' buffer and O are free, and S, whose place P had.  The keys have been in
         // order since the last barrier.

@@ -933,34 +933,38 @@ def test_bfloat16_prompts_on_either_side_of_the_choice(cuda, heads, kv, d, rows)
 
 
 @pytest.mark.parametrize("heads,d,bounds", [(16, 128, dict(max_length=2000, max_rows=80)), (16, 64, dict(max_length=2000, max_rows=80)), (2, 128, {}), (4, 96, {})])
-@pytest.mark.parametrize("centre,spread", [(100.0, 0.3), (-30.0, 1.0), (0.0, 1.0)])
-def test_bfloat16_scores_of_keys_far_from_nought(cuda, heads, d, bounds, centre, spread):
-    """Blocks stand for zero + scale * code, and only the second part is rounded, with the queries.
+@pytest.mark.parametrize("centre,spread,share", [(100.0, 0.3, 1.0), (-30.0, 1.0, 1.0), (0.0, 1.0, 1.0), (200.0, 0.2, 0.02), (60.0, 1.0, 0.5)])
+def test_bfloat16_scores_of_keys_far_from_nought(cuda, heads, d, bounds, centre, spread, share):
+    """Of keys far from nought only what lies above their block's zero is rounded, with the queries; `share` of the blocks are far.
 
-    A score is off by 2^-12 of R = sum_i |q_i| scale_i code_i for the queries and as much again for the keys, and by 2^-20 of
-    S = sum_i |q_i k_i| as for the other types; a log-sum by no more than the scores that are in it, and 2^-18.
+    f16 rounds by 2^-11 at most: a score is off by 2^-11 of R = sum_i |q_i r_i| for the queries and as much again for the keys, r_i what
+    is rounded of a key or stands beside its query, and by 2^-20 of S = sum_i |q_i k_i| as for the other types; a log-sum by no more than
+    the scores that are in it, and 2^-18.
     """
     rng = np.random.default_rng(d)
-    case, counts = Case(rng, [64, 300], 1, d, 16), [64, 80]
-    if not bounds:
-        counts = [3, 5]
-    starts, page = starts_of(case.lengths), 16
-    keys = (rng.standard_normal((starts[-1], 1, d)) * spread + centre * np.where(np.arange(d) // 32 % 2, -1, 1)).astype(np.float32)
+    case, counts = Case(rng, [64, 300], 1, d, 16), [64, 80] if bounds else [3, 5]
+    starts, blocks = starts_of(case.lengths), d // 32
+    keys = rng.standard_normal((starts[-1], blocks, 32)) * spread
+    keys += (centre * np.where(np.arange(blocks) % 2, -1, 1) * (rng.random((starts[-1], blocks)) < share))[..., None]
+    keys = keys.reshape(-1, 1, d).astype(np.float32)
     case.pool.append(keys, keys / max(1.0, abs(centre)), case.table, case.lengths, starts)
     case.histories = [case.pool.history(case.table[i], n) for i, n in enumerate(case.lengths)]
     case.upload()
     q = ref.decode(ref.encode(rng.standard_normal((sum(counts), heads, d)).astype(np.float32), "bfloat16"), "bfloat16")
-    got, lse = case.attend(KV4Layout(heads, 1, d, page), q, "bfloat16", counts, **bounds)
+    got, lse = case.attend(KV4Layout(heads, 1, d, 16), q, "bfloat16", counts, **bounds)
     want, want_lse, size = ref.attention(q, case.histories, case.lengths, starts_of(counts), np.float32(d ** -0.5))
-    ranges = np.zeros_like(size)
+    rounded, rows = np.zeros_like(size), starts_of(counts)
     for i, (k, _) in enumerate(case.histories):
-        offset = k.reshape(len(k), d // 32, 32)
-        offset = (offset - offset.min(-1, keepdims=True)).astype(np.float64).reshape(len(k), d)
-        rows = slice(starts_of(counts)[i], starts_of(counts)[i + 1])
-        for r in range(rows.start, rows.stop):
-            seen = int(case.lengths[i]) - (rows.stop - r) + 1
-            ranges[r] = (offset[:seen] @ np.abs(q[r]).T).max(0) * d ** -0.5
-    assert (np.abs(lse - want_lse) <= 2.0 ** -11 * ranges + 2.0 ** -20 * size + 2.0 ** -18 + 2.0 ** -22 * np.abs(want_lse)).all()
+        k = k.reshape(len(k), blocks, 32).astype(np.float64)
+        zero = k.min(-1, keepdims=True)
+        far = np.abs(zero) > 16 / 15 * (k.max(-1, keepdims=True) - zero)
+        r = np.maximum(k - zero, np.where(far, 0, np.abs(k))).reshape(len(k), d)
+        for row in range(rows[i], rows[i + 1]):
+            seen = int(case.lengths[i]) - (rows[i + 1] - row) + 1
+            rounded[row] = (r[:seen] @ np.abs(q[row]).T).max(0) * d ** -0.5
+    off = 2.0 ** -10 * rounded + 2.0 ** -20 * size
+    assert (np.abs(lse - want_lse) <= off + 2.0 ** -18 + 2.0 ** -22 * np.abs(want_lse)).all()
+    # The output: probabilities by a factor 1 +- 2 off, themselves and the values by 2^-11 each.
     most = max(np.abs(v).max() for _, v in case.histories)
-    bound = (2 * (2.0 ** -11 * ranges + 2.0 ** -20 * size) + 2.0 ** -10)[..., None] * most + ROUNDING["bfloat16"] * np.abs(want) * 1.001
+    bound = (2 * off + 2.0 ** -10)[..., None] * most + ROUNDING["bfloat16"] * np.abs(want) * 1.001
     assert (np.abs(got - want) <= bound).all()
