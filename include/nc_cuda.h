@@ -220,7 +220,8 @@ int32_t nc_selfcheck_div127(int64_t *mismatches);
  * is in page table[i][t / page].  Rows of a call: row_start[i] .. row_start[i + 1] - 1 are sequence i's last
  * positions before lengths[i] (row_start null: one row of each sequence); row_start[0] = 0, ascending.
  * A position whose page is not in 0..pages-1 (or that has no rotation angle) is left out, and the smallest
- * such sequence is put into the error word (device u64, set to all ones before; nullable). */
+ * such sequence is put into the error word (device u64 at an 8-byte boundary, set to all ones before; nullable).
+ * Rows of no sequence are refused. */
 
 /* Quantises rows of keys and values into the cache; keys are rotated first (RoPE, as nc_attention does)
  * where there is a table.  Rows before position 0 are left out.
@@ -240,7 +241,7 @@ int32_t nc_kv4_read(void **p, const int64_t *s, void *stream);
 /* Attention of rows over the cache: row r at position t sees positions 0..t of its sequence; a row that sees
  * nothing gets zeros and a log-sum of -inf.  Queries are rotated where there is a table.  float32 and
  * float16 calls keep float32 accuracy (queries and probabilities in two parts); bfloat16 calls round each to
- * one f16 part, and with many rows the decoded values and scale x code of the keys too.  The scale is positive.  Rows of a sequence past `the most rows` get no output, and positions
+ * one f16 part, and with many rows the decoded keys (zeros above 16 scales apart) and values too.  The scale is positive.  Rows of a sequence past `the most rows` get no output, and positions
  * past `the most positions` no share.
  * p: [0] out [rows, heads, d]  [1] q [rows, heads, d]  [2] pool  [3] table  [4] lengths
  *    [5] row_start (nullable)  [6] cos  [7] sin (nullable)  [8] log-sums f32[rows, heads] (nullable)

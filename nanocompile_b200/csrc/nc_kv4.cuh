@@ -22,9 +22,11 @@
 // Words and half-words belong to one position each, so positions are appended without reading.
 //
 // Both kernels read and write each byte once; memory's floor for 4 x 2048 rows of 8 heads of 128 (bfloat16 in, 44 MB for
-// the append; float32 out, 78 MB for the read) is 6.7 and 11.9 us.  They take 21 us, bound by the instructions of the
-// rounding (about 90 for eight values, the rotation included) and the chain before them, and 17 us (4.5 TB/s).  One row of
-// each of 256 sequences takes 5.3 and 5.8 us: the start and the chain from a row's sequence over its page to its bytes.
+// the append; float32 out, 78 MB for the read) is 6.7 and 11.9 us.  The append takes 21 us, bound by instructions and the latency
+// between them (one issues in 61% of the cycles): a warp makes 236 for eight values a lane, of which rounding and rotation are about 90;
+// the others find the rows' sequences, pages and tiles, once in every warp, and the angles, once for every head.  The read takes
+// 17 us (4.5 TB/s), bound by the latency of the same chain (10 of a warp's 20 cycles an instruction wait for loads, issue 34%).
+// One row of each of 256 sequences takes 5.3 and 5.8 us: the start and the chain from a row's sequence over its page to its bytes.
 #pragma once
 
 #include <cuda_bf16.h>

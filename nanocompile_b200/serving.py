@@ -72,6 +72,7 @@ class DeviceArray:
             check(library().nc_copy_to_device(self._pointer, host.ctypes.data, self.nbytes))
 
     def numpy(self) -> np.ndarray:
+        """A host copy, after what the default stream has been given; calls on other streams are to be waited for first."""
         out = np.empty(self.shape, self.host_type)
         if self.nbytes:
             check(library().nc_copy_to_host(out.ctypes.data, self._pointer, self.nbytes))
