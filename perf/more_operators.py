@@ -289,7 +289,7 @@ def plain_lora(state):
     """An adapter at a time, its rows gathered; everything in 32 bits."""
     case, widths = state["case"], widths_of(state["case"])
     rank, ranks = case["rank"], state["host"][2]
-    out = state["base"].float()
+    out = state["base"].to(torch.float32, copy=True)
     for s, rows in state["where"].items():
         x, r = state["x"][rows].float(), ranks[s]
         parts, at = [], 0
