@@ -284,6 +284,58 @@ int32_t nc_token_logprobs(void **p, const int64_t *s, void *stream);
 /* Enough for every call of this vocabulary, of any type, with up to so many rows and alternatives. */
 int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
 
+/* What the requests of a batch have of their own: adapters and beams.  As above: p[] / s[], nothing allocated or synchronized, scratch
+ * zeroed once, element types 0 float32, 1 float16, 2 bfloat16.
+ *
+ * Low-rank adapters beside a shared projection.  Slot a of the adapters holds A_a [targets * rank][inputs] and B_a
+ * [outputs][rank] (16-bit, contiguous); the targets share x (q, k and v, say) and their outputs follow one another.  Row r of
+ * a sequence with adapter a, output n of target t:
+ *   out[r, n] = base[r, n] + scales[a] * sum_{j < ranks[a]} B_a[n, j] * sum_k A_a[t * rank + j, k] * x[r, k]
+ * What a slot holds past ranks[a] is not read.  Rows of sequences without an adapter are base's (nought without base).
+ *
+ * The plan: the rows of a call grouped by adapter, made once for all projections and layers of a batch.  Adapters outside
+ * 0 .. slots - 1 are none; the smallest sequence with one from `slots` on is put into the error word.  Rows outside
+ * row_start[0] .. row_start[seqs] - 1 are left as they are by the projections.
+ * p: [0] plan (>= nc_lora_plan_bytes)  [1] adapters i32[seqs]  [2] row_start i32[seqs + 1] (null: one row each)
+ *    [3] error word (nullable)
+ * s: rows, seqs (8192 at most), slots, plan bytes */
+int32_t nc_lora_plan(void **p, const int64_t *s, void *stream);
+int64_t nc_lora_plan_bytes(int64_t rows, int64_t seqs, int64_t slots);
+
+/* Adds the adapters' shares to projections' outputs; the plan was made for the same rows, seqs and slots.
+ * p: [0] out [rows, outputs] (may be base)  [1] x [rows, inputs]  [2] base (nullable)  [3] A  [4] B  [5] plan
+ *    [6] ranks i32[slots] (null: rank)  [7] scales f32[slots] (null: 1)
+ * s: rows, seqs, slots, inputs, rank (both multiples of 8; rank 128 at most), targets (8 at most), element type of x, base
+ *    and out, element type of A and B (1 or 2), plan bytes, x row stride (elements), base row stride, out row stride,
+ *    outputs of each target */
+int32_t nc_lora_project(void **p, const int64_t *s, void *stream);
+
+/* Beam search's choice.  Rows g * beams .. (g + 1) * beams - 1 are request g's.  scores[r]: the sum of the log
+ * probabilities of beam r's tokens; -inf: there is no such beam.  A live beam's candidates are its score plus the log
+ * probability of each token; one that has finished has itself, with the token `end`.  The `beams` best go on, by their total (over
+ * norms[r], which is positive, where given), among equals the lower row's, then the lower token's.  Rows that have no beam or have finished are not
+ * read.  A beam with a NaN or +inf among its logits, or a NaN for a score, has no candidates, and the smallest such row is put into the
+ * error word.
+ * New beam i: parent (a row; -1 and score -inf where there are too few candidates), token, score, whether it has finished (its token
+ * is `end`, or its parent had finished, or there is none), grow (1 where its parent was live), and history (its parent, -1 where it
+ * has finished: the parent for nc_kv_pages_update, as a finished beam needs no history).
+ * p: [0] parent i32[rows]  [1] tokens i64[rows]  [2] new scores f32[rows]  [3] new finished i32[rows] (nullable)
+ *    [4] grow i32[rows] (nullable)  [5] history i32[rows] (nullable)  [6] logits [rows, vocab]  [7] scores f32[rows]
+ *    [8] finished i32[rows] (nullable)  [9] norms f32[rows] (nullable)  [10] scratch (device, >= nc_beam_select_scratch_bytes)
+ *    [11] error word (nullable)
+ * s: rows, vocab, logit row stride (elements), element type, beams (32 at most), end (-1: none), scratch bytes */
+int32_t nc_beam_select(void **p, const int64_t *s, void *stream);
+/* Enough for every call of this vocabulary, of any type, with up to so many rows and beams. */
+int64_t nc_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int64_t beams);
+
+/* States reordered by parents: lines 0 .. lengths[parent[i]] - 1 (every line without lengths) of each plane of row parent[i] to
+ * row i, then one line of `append` (where grow[i] is not 0, and there is room).  Other lines are left as they were, and so are rows
+ * with a parent outside 0 .. rows - 1 (new length 0).  The new states do not overlap the old ones.
+ * p: [0] new states [rows][planes][capacity][line]  [1] old states  [2] parent i32[rows]  [3] lengths i32[rows] (nullable)
+ *    [4] new lengths i32[rows] (nullable)  [5] append [rows][planes][line] (nullable)  [6] grow i32[rows] (null: 1)
+ * s: rows, planes, capacity, bytes of a line, row stride of the new states (bytes), of the old ones */
+int32_t nc_beam_reorder(void **p, const int64_t *s, void *stream);
+
 /* ---- 2. the model runtime ---------------------------------------------------------------- */
 
 typedef struct nc_model nc_model;

@@ -1,0 +1,349 @@
+// nc_requests.cu -- entry points of what the requests of a batch have of their own: low-rank adapters beside the shared
+// projections, and beam search's selection and reordering of states.
+//
+// nanocompile runs one sequence with one set of weights and chooses its tokens by argmax on the host
+// (nanocompile/models/qwen2.py:348-368); these operators have no counterpart there.
+#include "nc_api.cuh"
+#include "nc_beams.cuh"
+#include "nc_lora.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+using namespace nc;
+
+namespace {
+
+constexpr int64_t I32 = (int64_t(1) << 31) - 1;
+
+bool misaligned(const void *p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) != 0; }
+bool misaligned(int64_t v, int64_t n) { return (v & (n - 1)) != 0; }
+
+// Raises a kernel's limit of shared memory, once on each device (`allowed`: a bit for each).
+template <typename K>
+int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) {
+    int device = 0;
+    CUDA_TRY(cudaGetDevice(&device));
+    if (device < 64 && (allowed->load(std::memory_order_relaxed) >> device & 1)) return NC_OK;
+    CUDA_TRY(allow_smem(kernel, bytes));
+    if (device < 64) allowed->fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    return NC_OK;
+}
+
+int32_t check_type(int64_t type) {
+    if (type < KV_F32 || type > KV_BF16) return fail(NC_ERR_ARGUMENT, "element type %lld: 0 float32, 1 float16, 2 bfloat16", (long long)type);
+    return NC_OK;
+}
+int64_t type_bytes(int64_t type) { return type == KV_F32 ? 4 : 2; }
+
+// ---- adapters -----------------------------------------------------------------------------------
+
+int32_t lora_batch(int64_t rows, int64_t seqs, int64_t slots) {
+    if (rows < 0 || rows > I32 / 2 || seqs < 0 || seqs > LORA_SEQS || slots <= 0 || slots > I32 / 2)
+        return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows of %lld sequences (%d at most), %lld adapters", (long long)rows, (long long)seqs,
+                    LORA_SEQS, (long long)slots);
+    if (rows && !seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of no sequence", (long long)rows);
+    return NC_OK;
+}
+int64_t lora_groups(int64_t seqs, int64_t slots) { return std::min(seqs, slots + 1); }
+// Rows of an item: by the mean of the largest number of groups, as only the device knows how many there are.
+int64_t lora_tile(int64_t rows, int64_t seqs, int64_t slots) {
+    const int64_t mean = rows / std::max<int64_t>(1, lora_groups(seqs, slots));
+    return mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+}
+int64_t lora_places(int64_t rows, int64_t seqs, int64_t slots) {
+    const int64_t tile = lora_tile(rows, seqs, slots);
+    return (rows + tile - 1) / tile + lora_groups(seqs, slots);
+}
+
+template <int TX, int TW, int NT>
+int32_t launch_lora(cudaStream_t st, const LoraArgs &a, int passes) {
+    auto kernel = lora_rows_kernel<TX, TW, NT>;
+    constexpr size_t bytes = LoraShape<NT>::SMEM;
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(kernel, bytes, &allowed));
+    const int64_t subs = (a.tile + 8 * NT - 1) / (8 * NT), clusters = (int64_t)a.items * passes * subs;
+    int ctas = 8;                              // as many CTAs to an item as leave room for all items at once, two on an SM
+    while (ctas > 1 && clusters * ctas > 2 * 148) ctas /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * ctas), (unsigned)passes, (unsigned)subs);
+    cfg.blockDim = LORA_THREADS;
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+    return check_launch("lora_rows_kernel");
+}
+template <int TX, int TW>
+int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes) {
+    return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : a.tile == 16 ? launch_lora<TX, TW, 2>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
+}
+template <int TX>
+int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes) {
+    return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes) : launch_lora_n<TX, KV_BF16>(st, a, passes);
+}
+
+}  // namespace
+
+extern "C" int64_t nc_lora_plan_bytes(int64_t rows, int64_t seqs, int64_t slots) {
+    if (rows < 0 || rows > I32 / 2 || seqs < 0 || seqs > LORA_SEQS || slots <= 0 || slots > I32 / 2) return 0;
+    return 4 * (LORA_HEAD + 4 * lora_places(rows, seqs, slots) + rows);
+}
+
+extern "C" int32_t nc_lora_plan(void **p, const int64_t *s, void *stream) {
+    const int64_t rows = s[0], seqs = s[1], slots = s[2];
+    NC_TRY(lora_batch(rows, seqs, slots));
+    if (!p[2] && rows != seqs) return fail(NC_ERR_ARGUMENT, "%lld rows of %lld sequences need row_start", (long long)rows, (long long)seqs);
+    if (!p[0] || misaligned(p[0], 16) || s[3] < nc_lora_plan_bytes(rows, seqs, slots))
+        return fail(NC_ERR_ARGUMENT, "a plan of %lld bytes, %lld needed at a 16-byte boundary", (long long)s[3], (long long)nc_lora_plan_bytes(rows, seqs, slots));
+    if (seqs && !p[1]) return fail(NC_ERR_ARGUMENT, "null adapters");
+    if (misaligned(p[3], 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
+    LoraPlanArgs a{};
+    a.plan = (int32_t *)p[0];
+    a.adapters = (const int32_t *)p[1];
+    a.row_start = (const int32_t *)p[2];
+    a.error = (unsigned long long *)p[3];
+    a.rows = (int)rows;
+    a.seqs = (int)seqs;
+    a.slots = (int)slots;
+    a.tile = (int)lora_tile(rows, seqs, slots);
+    a.items = (int)lora_places(rows, seqs, slots);
+    a.size = 2;
+    while (a.size < a.seqs) a.size *= 2;
+    // Threads for the longer of the sort's pairs, the items and the rows, as barriers of fewer warps are cheaper.
+    const int64_t work = std::max<int64_t>({a.size / 2, a.items, rows / 4});
+    const unsigned threads = work <= 128 ? 128 : work <= 256 ? 256 : work <= 512 ? 512 : 1024;
+    const size_t bytes = (size_t)a.size * 8 + (size_t)3 * 4 * (a.size + 1);
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(lora_plan_kernel, (size_t)LORA_SEQS * 8 + (size_t)3 * 4 * (LORA_SEQS + 1), &allowed));
+    CUDA_TRY(launch_k(lora_plan_kernel, 1, threads, bytes, (cudaStream_t)stream, a));
+    return check_launch("lora_plan_kernel");
+}
+
+extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
+    LoraArgs a{};
+    const int64_t rows = s[0], seqs = s[1], slots = s[2], inputs = s[3], rank = s[4], targets = s[5], type = s[6], wtype = s[7];
+    NC_TRY(lora_batch(rows, seqs, slots));
+    NC_TRY(check_type(type));
+    if (wtype != KV_F16 && wtype != KV_BF16) return fail(NC_ERR_ARGUMENT, "adapters of element type %lld: 1 float16 or 2 bfloat16", (long long)wtype);
+    if (inputs <= 0 || inputs % 8 || inputs > I32 || rank <= 0 || rank % 8 || rank > LORA_RANK)
+        return fail(NC_ERR_ARGUMENT, "%lld inputs, rank %lld: multiples of 8, the rank %d at most", (long long)inputs, (long long)rank, LORA_RANK);
+    if (targets <= 0 || targets > LORA_TARGETS) return fail(NC_ERR_ARGUMENT, "%lld targets: 1 to %d", (long long)targets, LORA_TARGETS);
+    int64_t outputs = 0;
+    bool even = true;
+    for (int t = 0; t < targets; ++t) {
+        const int64_t width = s[12 + t];
+        if (width <= 0 || width > I32 / LORA_TARGETS) return fail(NC_ERR_ARGUMENT, "a target of %lld outputs", (long long)width);
+        even = even && outputs % 2 == 0;
+        a.width[t] = (int)width;
+        outputs += width;
+    }
+    if (s[8] < nc_lora_plan_bytes(rows, seqs, slots) || !p[5] || misaligned(p[5], 16))
+        return fail(NC_ERR_ARGUMENT, "a plan of %lld bytes, %lld needed at a 16-byte boundary", (long long)s[8], (long long)nc_lora_plan_bytes(rows, seqs, slots));
+    if (rows == 0) return NC_OK;
+    const int64_t bytes = type_bytes(type);
+    a.out = p[0];
+    a.x = p[1];
+    a.base = p[2];
+    a.a = p[3];
+    a.b = p[4];
+    a.plan = (const int32_t *)p[5];
+    a.ranks = (const int32_t *)p[6];
+    a.scales = (const float *)p[7];
+    a.x_stride = s[9];
+    a.base_stride = s[10];
+    a.out_stride = s[11];
+    if (!a.out || !a.x || !a.a || !a.b) return fail(NC_ERR_ARGUMENT, "null output, rows or adapters");
+    if (misaligned(a.a, 16) || misaligned(a.b, 16)) return fail(NC_ERR_ARGUMENT, "adapters are not at a 16-byte boundary");
+    if (misaligned(a.x, bytes) || misaligned(a.out, bytes) || misaligned(a.base, bytes)) return fail(NC_ERR_ARGUMENT, "misaligned rows");
+    if (a.x_stride < inputs || a.out_stride < outputs || (a.base && a.base_stride < outputs))
+        return fail(NC_ERR_ARGUMENT, "rows of %lld inputs or %lld outputs overlap", (long long)inputs, (long long)outputs);
+    a.rows = (int)rows;
+    a.items = (int)lora_places(rows, seqs, slots);
+    a.tile = (int)lora_tile(rows, seqs, slots);
+    a.inputs = (int)inputs;
+    a.outputs = (int)outputs;
+    a.rank = (int)rank;
+    a.slots = (int)slots;
+    a.targets = (int)targets;
+    a.type = (int)type;
+    a.wtype = (int)wtype;
+    a.x_vectors = !misaligned(a.x, 16) && !misaligned(a.x_stride * bytes, 16);
+    a.pairs = even && !misaligned(a.out, 2 * bytes) && !misaligned(a.base, 2 * bytes) && a.out_stride % 2 == 0 && (!a.base || a.base_stride % 2 == 0);
+    a.pass_targets = (int)std::min<int64_t>(targets, std::max<int64_t>(1, LORA_PASS / ((rank + 31) / 32 * 32)));
+    const int passes = (int)((targets + a.pass_targets - 1) / a.pass_targets);
+    const cudaStream_t st = (cudaStream_t)stream;
+    return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes) : launch_lora_w<KV_BF16>(st, a, passes);
+}
+
+// ---- beams --------------------------------------------------------------------------------------
+
+namespace {
+
+constexpr int64_t BEAM_COUNTERS = 2 * LP_ROWS;
+constexpr int64_t BEAM_PARTS = 1 << 14;        // segments of a launch at most, where rows are cut for speed: bounds the scratch
+constexpr int BEAM_CUTS[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 80, 96, 112, 128, 160, 192, 224, 256};
+
+int64_t beam_vecs(int64_t vocab, int64_t type) {                  // of a row at any alignment
+    const int64_t n = 16 / type_bytes(type);
+    return (vocab + 2 * (n - 1)) / n;
+}
+int64_t beam_fewest(int64_t vocab, int64_t type) {                // segments that a row has to have
+    constexpr int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS;
+    return (beam_vecs(vocab, type) + longest - 1) / longest;
+}
+struct BeamPlan {
+    int segs;
+    int64_t seg_vecs;
+};
+// Segments to a row: the fewest elements' time over the waves of CTAs that the card holds at once, a segment's start and end
+// counted as 4096 elements and its share of the join as 16.
+BeamPlan beam_plan(int64_t rows, int64_t vocab, int64_t type) {
+    const int64_t n = 16 / type_bytes(type), vecs = beam_vecs(vocab, type), slots = 148 * 2, fewest = beam_fewest(vocab, type);
+    int64_t best = -1;
+    BeamPlan p{0, 0};
+    for (int cut : BEAM_CUTS) {
+        const int64_t segs = std::max<int64_t>(cut, fewest);
+        if (segs > LP_SEGS || (segs > fewest && (vecs / segs < LP_THREADS || rows * segs > BEAM_PARTS))) break;
+        const int64_t waves = (rows * segs + slots - 1) / slots, cost = waves * (vecs * n / segs + 4096) + 16 * segs;
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        p.seg_vecs = (vecs + segs - 1) / segs;
+        p.segs = (int)((vecs + p.seg_vecs - 1) / p.seg_vecs);
+    }
+    return p;
+}
+int64_t beam_launch_rows(int64_t rows, int64_t beams) { return std::min<int64_t>(rows, LP_ROWS / beams * beams); }
+
+template <int TYPE>
+int32_t launch_beams(cudaStream_t st, const BeamArgs &a, int64_t rows) {
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(beam_select_kernel<TYPE>, sizeof(BeamShared), &allowed));
+    CUDA_TRY(launch_k(beam_select_kernel<TYPE>, (unsigned)(rows * a.segs), LP_THREADS, sizeof(BeamShared), st, a));
+    return check_launch("beam_select_kernel");
+}
+
+}  // namespace
+
+extern "C" int64_t nc_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int64_t beams) {
+    if (rows <= 0 || vocab <= 0 || beams <= 0 || beams > LP_MAX_TOP) return 4 * BEAM_COUNTERS;
+    // A bound that grows with the rows: fewer of them are cut into more segments.
+    int64_t most = 0;
+    rows = std::min<int64_t>(rows, LP_ROWS);
+    for (int type : {KV_F32, KV_F16}) {
+        const int64_t fewest = beam_fewest(vocab, type), cut = std::min<int64_t>(LP_SEGS, beam_vecs(vocab, type) / LP_THREADS);
+        most = std::max({most, rows * fewest, std::min(BEAM_PARTS, rows * cut)});
+    }
+    return 4 * BEAM_COUNTERS + (most + rows) * 8 * (1 + beams);
+}
+
+extern "C" int32_t nc_beam_select(void **p, const int64_t *s, void *stream) {
+    const int64_t rows = s[0], vocab = s[1], type = s[3], beams = s[4], scratch = s[6];
+    BeamArgs a{};
+    NC_TRY(check_type(type));
+    if (rows < 0 || rows > I32 || vocab <= 0 || vocab >= (int64_t(1) << 32) - 1)
+        return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows of %lld logits", (long long)rows, (long long)vocab);
+    if (beams <= 0 || beams > LP_MAX_TOP || rows % beams)
+        return fail(NC_ERR_ARGUMENT, "%lld beams: at most %d, and the %lld rows are those of whole requests", (long long)beams, LP_MAX_TOP, (long long)rows);
+    if (s[2] < vocab) return fail(NC_ERR_ARGUMENT, "rows of %lld logits overlap at a stride of %lld", (long long)vocab, (long long)s[2]);
+    if (s[5] >= vocab) return fail(NC_ERR_ARGUMENT, "the end token %lld is outside the vocabulary", (long long)s[5]);
+    if (s[5] < 0 && p[8]) return fail(NC_ERR_ARGUMENT, "finished beams without an end token");
+    if (rows == 0) return NC_OK;
+    const int64_t at_once = beam_launch_rows(rows, beams), k = std::min(beams, vocab);
+    const BeamPlan plan = beam_plan(at_once, vocab, type);
+    if (plan.segs == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is beyond %d segments", (long long)vocab, LP_SEGS);
+    if (!p[0] || !p[1] || !p[2] || !p[6] || !p[7] || misaligned(p[6], type_bytes(type)))
+        return fail(NC_ERR_ARGUMENT, "null or misaligned logits, scores or outputs");
+    if (p[7] == p[2] || (p[8] && p[8] == p[3])) return fail(NC_ERR_ARGUMENT, "the new scores or flags are the old ones");
+    if (misaligned(p[11], 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
+    const int64_t need = 4 * BEAM_COUNTERS + at_once * (plan.segs * (8 + 8 * k) + 8 + 8 * k);
+    if (!p[10] || misaligned(p[10], 16) || scratch < need)
+        return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch, (long long)nc_beam_select_scratch_bytes(rows, vocab, beams));
+    a.parent = (int32_t *)p[0];
+    a.tokens = (int64_t *)p[1];
+    a.new_scores = (float *)p[2];
+    a.new_finished = (int32_t *)p[3];
+    a.grow = (int32_t *)p[4];
+    a.history = (int32_t *)p[5];
+    a.logits = (const char *)p[6];
+    a.scores = (const float *)p[7];
+    a.finished = (const int32_t *)p[8];
+    a.norms = (const float *)p[9];
+    a.error = (unsigned long long *)p[11];
+    a.stride = s[2];
+    a.vocab = vocab;
+    a.beams = (int)beams;
+    a.end = s[5];
+    a.k = (int)k;
+    a.segs = plan.segs;
+    a.seg_vecs = plan.seg_vecs;
+    a.counter = (unsigned int *)p[10];
+    a.lse = (double *)((char *)p[10] + 4 * BEAM_COUNTERS);
+    a.best = (unsigned long long *)(a.lse + at_once);
+    a.part_top = a.best + at_once * k;
+    a.part = (float2 *)(a.part_top + at_once * plan.segs * k);
+    const cudaStream_t st = (cudaStream_t)stream;
+    for (int64_t first = 0; first < rows; first += at_once) {
+        const int64_t n = std::min(rows - first, at_once);
+        a.row_first = first;
+        NC_TRY(type == KV_F32 ? launch_beams<KV_F32>(st, a, n) : type == KV_F16 ? launch_beams<KV_F16>(st, a, n) : launch_beams<KV_BF16>(st, a, n));
+    }
+    return NC_OK;
+}
+
+namespace {
+
+template <typename V>
+int32_t launch_reorder(cudaStream_t st, ReorderArgs a) {
+    const int64_t chunk = (int64_t)sizeof(V) * BEAM_COPY_THREADS * BEAM_COPY_VECS;
+    a.chunks = std::max<int64_t>(1, (a.capacity * a.line + chunk - 1) / chunk);
+    const int64_t ctas = (int64_t)a.rows * a.planes * a.chunks;
+    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%d rows of %d planes of %lld bytes in one call", a.rows, a.planes, (long long)(a.capacity * a.line));
+    CUDA_TRY(launch_k(beam_reorder_kernel<V>, (unsigned)ctas, BEAM_COPY_THREADS, 0, st, a));
+    return check_launch("beam_reorder_kernel");
+}
+
+}  // namespace
+
+extern "C" int32_t nc_beam_reorder(void **p, const int64_t *s, void *stream) {
+    const int64_t rows = s[0], planes = s[1], capacity = s[2], line = s[3], to_stride = s[4], from_stride = s[5];
+    if (rows < 0 || rows > I32 || planes <= 0 || planes > I32 || capacity < 0 || capacity >= I32 || line <= 0 || line > (int64_t(1) << 40) / std::max<int64_t>(1, capacity))
+        return fail(NC_ERR_ARGUMENT, "bad sizes: %lld rows of %lld planes of %lld lines of %lld bytes", (long long)rows, (long long)planes, (long long)capacity,
+                    (long long)line);
+    if (planes * (long double)capacity * line > 4e18L || to_stride < planes * capacity * line || from_stride < planes * capacity * line)
+        return fail(NC_ERR_ARGUMENT, "rows of %lld planes of %lld lines of %lld bytes overlap", (long long)planes, (long long)capacity, (long long)line);
+    if (rows == 0) return NC_OK;
+    if (!p[2] || (capacity && (!p[0] || !p[1]))) return fail(NC_ERR_ARGUMENT, "null states or parents");
+    if (p[0] == p[1] && capacity) return fail(NC_ERR_ARGUMENT, "the new states are the old ones");
+    if (p[3] && p[3] == p[4]) return fail(NC_ERR_ARGUMENT, "the new lengths are the old ones");
+    if (!p[3] && (p[4] || p[5] || p[6])) return fail(NC_ERR_ARGUMENT, "new lengths, a line to append or grow without lengths");
+    if (p[6] && !p[5]) return fail(NC_ERR_ARGUMENT, "grow without a line to append");
+    ReorderArgs a{};
+    a.to = (char *)p[0];
+    a.from = (const char *)p[1];
+    a.parent = (const int32_t *)p[2];
+    a.lengths = (const int32_t *)p[3];
+    a.new_lengths = (int32_t *)p[4];
+    a.append = (const char *)p[5];
+    a.grow = (const int32_t *)p[6];
+    a.to_stride = to_stride;
+    a.from_stride = from_stride;
+    a.line = line;
+    a.rows = (int)rows;
+    a.planes = (int)planes;
+    a.capacity = (int)capacity;
+    // The widest vectors that every plane of every row begins at.
+    const int64_t at = (int64_t)(uintptr_t)p[0] | (int64_t)(uintptr_t)p[1] | to_stride | from_stride | capacity * line;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (!misaligned(at, 16)) return launch_reorder<uint4>(st, a);
+    if (!misaligned(at, 8)) return launch_reorder<uint2>(st, a);
+    if (!misaligned(at, 4)) return launch_reorder<uint32_t>(st, a);
+    return !misaligned(at, 2) ? launch_reorder<uint16_t>(st, a) : launch_reorder<uint8_t>(st, a);
+}

@@ -69,7 +69,7 @@ GROUP_ENTRY_POINTS = ("nc_gather_rows", "nc_rms_norm_quantize", "nc_quantize_blo
                       "nc_lm_head_argmax_noalloc", "nc_attention", "nc_attention_cache", "nc_expf_exact",
                       "nc_lm_head_q8_prepare", "nc_lm_head_q8_argmax", "nc_quantize_int8_rows",
                       "nc_kv4_append", "nc_kv4_read", "nc_kv4_attention", "nc_kv_pages_update", "nc_kv_pages_compact",
-                      "nc_token_logprobs")
+                      "nc_token_logprobs", "nc_lora_plan", "nc_lora_project", "nc_beam_select", "nc_beam_reorder")
 
 
 def library() -> ctypes.CDLL:
@@ -96,6 +96,8 @@ def library() -> ctypes.CDLL:
             "nc_kv4_attention_scratch_bytes": ([_i64] * 6, _i64),
             "nc_kv_pages_scratch_bytes": ([_i64] * 3, _i64),
             "nc_token_logprobs_scratch_bytes": ([_i64] * 3, _i64),
+            "nc_lora_plan_bytes": ([_i64] * 3, _i64),
+            "nc_beam_select_scratch_bytes": ([_i64] * 3, _i64),
             "nc_device_count": ([_P32], _i32),
             "nc_set_device": ([_i32], _i32),
             "nc_device_alloc": ([_i64, ctypes.POINTER(_vp)], _i32),

@@ -1,11 +1,13 @@
-"""Serving operators next to the Qwen2 step: a paged key/value cache held in 4 bits, and token log probabilities.
+"""Serving operators next to the Qwen2 step: a paged key/value cache held in 4 bits, token log probabilities, beams and adapters.
 
 The reference keeps one sequence's history as float32 arrays (``nanocompile/models/qwen2.py:232-271``) and
 picks tokens by ``np.argmax`` (``nanocompile/models/qwen2.py:348-368``). Sampling several continuations of a
 prompt, or searching with beams, needs more: histories that share their pages (:func:`kv_pages_update` forks,
 reorders, grows, cuts and frees sequences, :func:`kv_pages_compact` packs them), at 5 bits a value
 (:func:`kv4_append`, :func:`kv4_attention`, :func:`kv4_read`), and the scores of a step's tokens
-(:func:`token_logprobs`). Each function is one entry point of ``libnc_cuda.so`` (``include/nc_cuda.h``).
+(:func:`token_logprobs`). The beams of a batch of requests are chosen on the device (:func:`beam_select`), dense states follow
+them (:func:`beam_reorder`), and each request may have a low-rank adapter of its own beside the shared projections
+(:func:`lora_plan`, :func:`lora_project`). Each function is one entry point of ``libnc_cuda.so`` (``include/nc_cuda.h``).
 
 Arguments are device arrays: anything with ``data_ptr()``, ``shape``, ``stride()``, ``is_contiguous()`` and ``dtype`` --
 this module's :class:`DeviceArray`, a PyTorch tensor -- on the current device. Calls are asynchronous on ``stream`` (a CUDA stream
@@ -384,3 +386,173 @@ def token_logprobs(logits, targets, out, entropy=None, top=None, top_logprobs=No
            logits.data_ptr(), _expect("targets", targets, _I64, (rows, n)) if n else 0,
            work, _error(error)),
           (rows, vocab, strides[0] if rows > 1 else vocab, kind, n, k, work_bytes), stream)
+
+
+@dataclass(frozen=True)
+class LoraBatch:
+    """The sizes of a batch: ``rows`` of ``seqs`` sequences (8192 at most), whose adapters are among ``slots``."""
+
+    rows: int
+    seqs: int
+    slots: int
+
+    def __post_init__(self) -> None:
+        if min(self.rows, self.seqs) < 0 or self.slots <= 0 or self.seqs > 8192:
+            raise InterpreterError(f"{self.rows} rows of {self.seqs} sequences (8192 at most), {self.slots} adapters")
+
+    @cached_property
+    def plan_bytes(self) -> int:
+        """The bytes of a plan (at a 16-byte boundary) for :func:`lora_plan`."""
+        return int(library().nc_lora_plan_bytes(self.rows, self.seqs, self.slots))
+
+
+@dataclass(frozen=True)
+class LoraLayout:
+    """Adapters of up to ``rank`` (a multiple of 8, at most 128) on projections of ``inputs`` (a multiple of 8) that share their rows:
+    ``widths`` are their outputs (eight projections at most)."""
+
+    inputs: int
+    widths: tuple[int, ...]
+    rank: int
+
+    def __post_init__(self) -> None:
+        object.__setattr__(self, "widths", tuple(int(w) for w in self.widths))
+        if self.inputs <= 0 or self.inputs % 8 or not 0 < self.rank <= 128 or self.rank % 8:
+            raise InterpreterError(f"{self.inputs} inputs, rank {self.rank}: multiples of 8, the rank at most 128")
+        if not 0 < len(self.widths) <= 8 or min(self.widths) <= 0:
+            raise InterpreterError(f"outputs {self.widths}: of one to eight projections")
+
+    @cached_property
+    def outputs(self) -> int:
+        return sum(self.widths)
+
+    def a_shape(self, slots: int) -> tuple[int, int, int]:
+        """The adapters' first factors: ``[slots, projections * rank, inputs]``."""
+        return slots, len(self.widths) * self.rank, self.inputs
+
+    def b_shape(self, slots: int) -> tuple[int, int, int]:
+        """Their second factors: ``[slots, outputs, rank]``."""
+        return slots, self.outputs, self.rank
+
+
+def lora_plan(batch: LoraBatch, plan, adapters, *, row_start=None, error=None, stream: int = 0) -> None:
+    """Group the rows of a batch by adapter, to ``plan`` (uint8), for every :func:`lora_project` of the batch (``nc_lora_plan``).
+
+    ``adapters``: int32 ``[seqs]``, each sequence's slot, -1 for none. ``row_start``: int32 ``[seqs + 1]`` (default: one row each).
+    """
+    work, work_bytes = _scratch(plan)
+    seqs = batch.seqs
+    _call("nc_lora_plan", (work, _expect("adapters", adapters, _I32, (seqs,)),
+                           0 if row_start is None else _expect("row_start", row_start, _I32, (seqs + 1,)), _error(error)),
+          (batch.rows, seqs, batch.slots, work_bytes), stream)
+
+
+def _lora_rows(what: str, array, rows: int, line: int) -> tuple[int, int, int]:
+    """Address, row stride and kind of ``[rows, line]`` with contiguous rows."""
+    shape, strides, kind = array.shape, array.stride(), _kind[array.dtype]
+    if len(shape) != 2 or shape[0] != rows or shape[1] != line or strides[1] != 1 and line > 1:
+        raise InterpreterError(f"{what}: {tuple(shape)}, expected {rows} contiguous rows of {line}")
+    if kind > _BF16:
+        raise InterpreterError(f"{what}: element type {_name(array.dtype)}: float32, float16 or bfloat16")
+    return array.data_ptr(), strides[0] if rows > 1 else line, kind
+
+
+def lora_project(layout: LoraLayout, batch: LoraBatch, out, x, a, b, plan, *, base=None, ranks=None, scales=None,
+                 stream: int = 0) -> None:
+    """Add the adapters' shares to the outputs of projections of ``x`` (``nc_lora_project``).
+
+    ``out`` = ``base`` (default: nought; may be ``out`` itself) + ``scales`` * B (A x), each row with its sequence's adapter.
+    ``a`` and ``b``: float16 or bfloat16, as :meth:`LoraLayout.a_shape` and ``b_shape`` say. ``ranks`` (int32 ``[slots]``): the adapters' own
+    ranks, where lower; ``scales``: float32 ``[slots]``. float32 rows keep float32 accuracy.
+    """
+    rows, slots = batch.rows, batch.slots
+    to, out_stride, kind = _lora_rows("out", out, rows, layout.outputs)
+    source, x_stride, x_kind = _lora_rows("x", x, rows, layout.inputs)
+    was, base_stride, base_kind = (0, 0, kind) if base is None else _lora_rows("base", base, rows, layout.outputs)
+    if x_kind != kind or base_kind != kind:
+        raise InterpreterError("x, base and out of different types")
+    weights = _kind[a.dtype]
+    if weights != _F16 and weights != _BF16:
+        raise InterpreterError(f"a: element type {_name(a.dtype)}: float16 or bfloat16")
+    work, work_bytes = _scratch(plan)
+    widths = layout.widths + (0,) * (8 - len(layout.widths))
+    _call("nc_lora_project",
+          (to, source, was, _expect("a", a, weights, layout.a_shape(slots)), _expect("b", b, weights, layout.b_shape(slots)), work,
+           0 if ranks is None else _expect("ranks", ranks, _I32, (slots,)),
+           0 if scales is None else _expect("scales", scales, _F32, (slots,))),
+          (rows, batch.seqs, slots, layout.inputs, layout.rank, len(layout.widths), kind, weights, work_bytes, x_stride, base_stride,
+           out_stride, *widths), stream)
+
+
+def beam_select_scratch_bytes(rows: int, vocab: int, beams: int) -> int:
+    """Scratch for :func:`beam_select` calls of up to ``rows`` rows and ``beams`` beams."""
+    return int(library().nc_beam_select_scratch_bytes(rows, vocab, beams))
+
+
+def beam_select(parent, tokens, new_scores, logits, scores, scratch, *, beams: int, end: int = -1, finished=None, new_finished=None,
+                grow=None, history=None, norms=None, error=None, stream: int = 0) -> None:
+    """The ``beams`` (32 at most) best continuations of each request's beams (``nc_beam_select``).
+
+    Rows ``g * beams ..`` of ``logits`` and ``scores`` (float32 ``[rows]``, -inf: no beam) are request ``g``'s. A beam for which
+    ``finished`` (int32) is not 0 goes on as itself, with the token ``end``. Totals are compared over ``norms`` (float32, positive),
+    where given. Out: ``parent`` (int32: rows, -1 for none), ``tokens`` (int64), ``new_scores``, and where wanted ``new_finished``, ``grow``
+    (1 where the parent was live) and ``history`` (the parent, -1 where the beam has finished: :func:`kv_pages_update`'s parent), all int32.
+    """
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) != 2 or strides[1] != 1 and shape[1] > 1:
+        raise InterpreterError(f"logits: {tuple(shape)}, expected [rows, vocabulary] with contiguous rows")
+    rows, vocab = shape
+    kind, n = _kind[logits.dtype], (rows,)
+    if kind > _BF16:
+        raise InterpreterError(f"logits: element type {_name(logits.dtype)}: float32, float16 or bfloat16")
+    work, work_bytes = _scratch(scratch)
+    _call("nc_beam_select",
+          (_expect("parent", parent, _I32, n), _expect("tokens", tokens, _I64, n), _expect("new_scores", new_scores, _F32, n),
+           0 if new_finished is None else _expect("new_finished", new_finished, _I32, n),
+           0 if grow is None else _expect("grow", grow, _I32, n),
+           0 if history is None else _expect("history", history, _I32, n),
+           logits.data_ptr(), _expect("scores", scores, _F32, n),
+           0 if finished is None else _expect("finished", finished, _I32, n),
+           0 if norms is None else _expect("norms", norms, _F32, n), work, _error(error)),
+          (rows, vocab, strides[0] if rows > 1 else vocab, kind, beams, end, work_bytes), stream)
+
+
+_ITEM_BYTES = {_F32: 4, _F16: 2, _BF16: 2, _I32: 4, _I64: 8, _U64: 8, _U8: 1}
+
+
+def _states(what: str, array) -> tuple[tuple, int, int]:
+    """Shape ``(rows, planes, capacity, line)``, row stride and bytes of an element of states; rows may be strided."""
+    shape, strides = tuple(array.shape), tuple(array.stride())
+    if len(shape) == 2:
+        shape, strides = (shape[0], 1, shape[1], 1), (strides[0], shape[1], strides[1], 1)
+    size = _ITEM_BYTES.get(_kind[array.dtype])
+    if len(shape) != 4 or size is None:
+        raise InterpreterError(f"{what}: {_name(array.dtype)} {shape}, expected [rows, planes, positions, values] or [rows, positions]")
+    rows, planes, capacity, line = shape
+    for n, stride, expected in ((line, strides[3], 1), (capacity, strides[2], line), (planes, strides[1], capacity * line)):
+        if n > 1 and stride != expected:
+            raise InterpreterError(f"{what}: strides {strides}, expected contiguous rows")
+    return shape, strides[0] if rows > 1 else planes * capacity * line, size
+
+
+def beam_reorder(new, old, parent, *, lengths=None, new_lengths=None, append=None, grow=None, stream: int = 0) -> None:
+    """States ``new[i] = old[parent[i]]``, up to the parent's length, and one position more from ``append`` (``nc_beam_reorder``).
+
+    ``new`` and ``old``: ``[rows, planes, positions, values]`` or ``[rows, positions]`` of one type, not overlapping. ``lengths``
+    (int32 ``[rows]``): the old rows' positions (default: all). ``append``: ``[rows, planes, values]`` or ``[rows]``, put at the end where
+    ``grow`` (int32, default 1) is not 0. Rows with a parent outside ``0 .. rows - 1`` are left as they are.
+    """
+    shape, to_stride, size = _states("new", new)
+    from_shape, from_stride, _ = _states("old", old)
+    if from_shape != shape or _kind[old.dtype] != _kind[new.dtype]:
+        raise InterpreterError(f"old: {_name(old.dtype)} {tuple(old.shape)}, expected new's {_name(new.dtype)} {tuple(new.shape)}")
+    rows, planes, capacity, line = shape
+    n = (rows,)
+    tail = n if len(new.shape) == 2 else (rows, planes, line)
+    _call("nc_beam_reorder",
+          (new.data_ptr(), old.data_ptr(), _expect("parent", parent, _I32, n),
+           0 if lengths is None else _expect("lengths", lengths, _I32, n),
+           0 if new_lengths is None else _expect("new_lengths", new_lengths, _I32, n),
+           0 if append is None else _expect("append", append, _kind[new.dtype], tail),
+           0 if grow is None else _expect("grow", grow, _I32, n)),
+          (rows, planes, capacity, line * size, to_stride * size, from_stride * size), stream)
