@@ -840,13 +840,17 @@ extern "C" int32_t nc_device_faults(void) {
     bool prompt = false;
     NC_TRY(prompt_fault(&prompt));
     if (prompt) return fail(NC_ERR_KERNEL, "4-bit attention: a copy or a matrix instruction did not complete within its wait limit");
+    bool adapters = false;
+    NC_TRY(requests_fault(&adapters));
+    if (adapters) return fail(NC_ERR_KERNEL, "adapters: a matrix instruction did not complete within its wait limit");
     return NC_OK;
 }
 
 extern "C" int32_t nc_set_wait_limit(int64_t cycles) {
     const long long v = cycles > 0 ? (long long)cycles : (1ll << 31);
     CUDA_TRY(cudaMemcpyToSymbol(g_wait_cycles, &v, sizeof(v)));
-    return set_prompt_wait_limit(v);
+    NC_TRY(set_prompt_wait_limit(v));
+    return set_requests_wait_limit(v);
 }
 
 extern "C" int32_t nc_selftest_wait(int32_t kind) {

@@ -159,7 +159,7 @@ struct LoraArgs {
     const float *scales;                       // [slots] or null
     int64_t x_stride, base_stride, out_stride;
     int rows, items, tile, inputs, outputs, rank, slots, targets, pass_targets, type, wtype;
-    int x_vectors, pairs;                      // 16-byte loads of x; two outputs to an access
+    int x_vectors, pairs, wide;                // 16-byte loads of x; two outputs to an access; 16 bytes of them
     int width[LORA_TARGETS];
 };
 

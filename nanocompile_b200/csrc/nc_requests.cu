@@ -5,7 +5,7 @@
 // (nanocompile/models/qwen2.py:348-368); these operators have no counterpart there.
 #include "nc_api.cuh"
 #include "nc_beams.cuh"
-#include "nc_lora.cuh"
+#include "nc_lora_tiles.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -85,12 +85,57 @@ template <int TX, int TW>
 int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes) {
     return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : a.tile == 16 ? launch_lora<TX, TW, 2>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
 }
+// For items of 128 rows.
+template <int TX>
+int32_t launch_lora_tiles(cudaStream_t st, LoraArgs a) {
+    using S = LoraTiles<TX>;
+    auto kernel = lora_tiles_kernel<TX>;
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(kernel, 221 * 1024, &allowed));
+    a.pass_targets = std::min(a.targets, std::max(1, LORA_PASS / ((a.rank + 15) / 16 * 16)));
+    const int passes = (a.targets + a.pass_targets - 1) / a.pass_targets;
+    const LoraTilesPlan plan = lora_tiles_plan(a.pass_targets, a.rank, S::PH, S::COLS);
+    const size_t bytes = (size_t)plan.bytes + 1024;
+    const int64_t places = 148 * (bytes <= 112 * 1024 ? 2 : 1);
+    int ctas = 8;
+    while (ctas > 1 && (int64_t)a.items * passes * ctas > places) ctas /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * ctas), (unsigned)passes);
+    cfg.blockDim = LT_THREADS;
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, plan));
+    return check_launch("lora_tiles_kernel");
+}
 template <int TX>
 int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes) {
     return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes) : launch_lora_n<TX, KV_BF16>(st, a, passes);
 }
 
 }  // namespace
+
+int32_t nc::set_requests_wait_limit(long long cycles) {
+    CUDA_TRY(cudaMemcpyToSymbol(g_wait_cycles, &cycles, sizeof(cycles)));
+    return NC_OK;
+}
+
+// Whether a wait has run out since the last call; clears it.
+int32_t nc::requests_fault(bool *fault) {
+    unsigned int word = 0;
+    CUDA_TRY(cudaMemcpyFromSymbol(&word, g_lora_fault, sizeof(word)));
+    *fault = word != 0;
+    word = 0;
+    if (*fault) CUDA_TRY(cudaMemcpyToSymbol(g_lora_fault, &word, sizeof(word)));
+    return NC_OK;
+}
 
 extern "C" int64_t nc_lora_plan_bytes(int64_t rows, int64_t seqs, int64_t slots) {
     if (rows < 0 || rows > I32 / 2 || seqs < 0 || seqs > LORA_SEQS || slots <= 0 || slots > I32 / 2) return 0;
@@ -177,9 +222,15 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     a.wtype = (int)wtype;
     a.x_vectors = !misaligned(a.x, 16) && !misaligned(a.x_stride * bytes, 16);
     a.pairs = even && !misaligned(a.out, 2 * bytes) && !misaligned(a.base, 2 * bytes) && a.out_stride % 2 == 0 && (!a.base || a.base_stride % 2 == 0);
+    bool wide = !misaligned(a.out, 16) && !misaligned(a.base, 16) && !misaligned(a.out_stride * bytes, 16) && (!a.base || !misaligned(a.base_stride * bytes, 16));
+    for (int t = 0; t + 1 < targets; ++t) wide = wide && !misaligned(a.width[t] * bytes, 16);
+    a.wide = wide;
     a.pass_targets = (int)std::min<int64_t>(targets, std::max<int64_t>(1, LORA_PASS / ((rank + 31) / 32 * 32)));
     const int passes = (int)((targets + a.pass_targets - 1) / a.pass_targets);
     const cudaStream_t st = (cudaStream_t)stream;
+    const bool tiles = a.tile == LT_ROWS && a.x_vectors && targets * rank * inputs <= I32;
+    if (tiles && type == KV_BF16 && wtype == KV_BF16) return launch_lora_tiles<KV_BF16>(st, a);
+    if (tiles && type == KV_F16 && wtype == KV_F16) return launch_lora_tiles<KV_F16>(st, a);
     return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes) : launch_lora_w<KV_BF16>(st, a, passes);
 }
 
