@@ -391,8 +391,13 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
     for (int i = tid; i < rp * (t1 - t0) * COLS; i += LORA_THREADS) {
         const int col = i % COLS, at = i / COLS, t = at / rp, j = at - t * rp;
         float v = 0.0f;
-        if (j < r)
-            for (int k = 0; k < ctas; ++k) v = fadd(v, lora_peer(sum + (t * per * 16 + j) * COLS + col, k));
+        if (j < r) {
+            float p[8];                                            // asked for all at once
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = k < ctas ? lora_peer(sum + (t * per * 16 + j) * COLS + col, k) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v = fadd(v, p[k]);
+        }
         h[col * S::HS + at] = v;
     }
     lora_cluster_arrive();                                         // the peers' sums are read; they may go once all CTAs are here

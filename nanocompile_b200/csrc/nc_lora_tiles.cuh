@@ -19,7 +19,9 @@ namespace nc {
 
 constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_THREADS = LT_WORKERS + 32, LT_TMEM = 256;
 constexpr int LT_BLOCK = LT_ROWS * 128;        // 128 rows of 128 bytes
+constexpr int LT_HALF = LT_ROWS * 64;          // 128 rows of 64 bytes
 constexpr int LT_STAGES = 6;                   // of the first products at most
+constexpr int LT_TWICE = 110 * 1024, LT_ONCE = 200 * 1024;             // bytes of tiles with two CTAs on an SM, with one
 constexpr int LT_LINE = 36;                    // floats from a row to the next of a warp's 32 x 32: no bank twice in a quarter
 
 __device__ unsigned int g_lora_fault;          // set when a matrix instruction did not come to its end within the wait limit
@@ -32,28 +34,27 @@ struct LoraTiles {
     static constexpr int SIZE = TX == KV_F32 ? 4 : 2;
 };
 
-// How shared memory is laid out, by the most rows of h in a pass: the stages of the first products lie over all of the rest.
+// How shared memory is laid out, by the most rows of h in a pass: h's operand, then the sums of h; over these B and the warps'
+// lines; over all of it the stages of the first products.
 struct LoraTilesPlan {
     int wide;                                  // rows of h in whole 16s
     int stages, a_bytes;                       // of a stage: LT_BLOCK for rows, a_bytes for A
-    int h_blocks, b_blocks;                    // blocks of 64 for a part of h, for B
-    int b_at, sum_at, line_at, early, bytes;   // early: B's first tiles do not lie where the sums do
+    int h_blocks, b_blocks;                    // blocks of 32 for a part of h, for B
+    int sum_at, line_at, bytes;
 };
 inline LoraTilesPlan lora_tiles_plan(int targets, int rank, int parts, int cols) {
     LoraTilesPlan p{};
     p.wide = targets * ((rank + 15) / 16 * 16);
     p.a_bytes = p.wide * 128;
-    p.h_blocks = (p.wide + 63) / 64;
-    p.b_blocks = (rank + 63) / 64;
-    p.b_at = parts * p.h_blocks * LT_BLOCK;
-    p.line_at = p.b_at + 2 * p.b_blocks * cols * 128;
+    p.h_blocks = (p.wide + 31) / 32;
+    p.b_blocks = (rank + 31) / 32;
+    p.sum_at = parts * p.h_blocks * LT_HALF;
+    p.line_at = p.sum_at + 2 * p.b_blocks * cols * 64;
     const int sums = LT_ROWS * (p.wide + 4) * 4, lines = LT_WARPS * 32 * LT_LINE * 4;
-    p.early = p.line_at + sums <= 200 * 1024;
-    p.sum_at = p.early ? p.line_at : p.b_at;
     p.bytes = p.line_at + lines > p.sum_at + sums ? p.line_at + lines : p.sum_at + sums;
-    for (p.stages = LT_STAGES; p.stages > 2 && p.stages * (LT_BLOCK + p.a_bytes) > (p.bytes > 110 * 1024 ? 200 * 1024 : 110 * 1024); --p.stages) {}
-    const int ring = p.stages * (LT_BLOCK + p.a_bytes);
-    if (ring > p.bytes) p.bytes = ring;
+    const int stage = LT_BLOCK + p.a_bytes, most = p.bytes > LT_TWICE ? LT_ONCE : LT_TWICE;       // room for two CTAs on an SM, or one
+    p.stages = most / stage < LT_STAGES ? most / stage : LT_STAGES;
+    if (p.stages * stage > p.bytes) p.bytes = p.stages * stage;
     return p;
 }
 
@@ -82,6 +83,10 @@ __device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, int n
         "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
         : "memory");
 }
+// A K-major operand of 64-byte swizzled rows: eight rows are 512 bytes, and bits 4 and 5 of an address are flipped by its bits 7 and 8.
+__device__ __forceinline__ uint64_t lt_desc64(uint32_t address) {
+    return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
 __device__ __forceinline__ void lt_async_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
 // 16 bytes from `from`, of which `bytes` are there: the others become nought.
 __device__ __forceinline__ void lt_copy16(uint32_t to, const void *from, int bytes) {
@@ -92,16 +97,14 @@ template <int N>
 __device__ __forceinline__ void lt_wait_copies() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t rank, uint32_t v) {
-    asm volatile("{\n\t.reg .u32 to;\n\tmapa.shared::cluster.u32 to, %0, %1;\n\tst.shared::cluster.u32 [to], %2;\n\t}" ::"r"(at), "r"(rank), "r"(v) : "memory");
+__device__ __forceinline__ uint32_t lt_peer(uint32_t at, uint32_t rank) {                        // of another CTA's shared memory
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
 }
-__device__ __forceinline__ float2 lt_load_peer2(uint32_t at, uint32_t rank) {
-    float2 v;
-    asm volatile("{\n\t.reg .u32 from;\n\tmapa.shared::cluster.u32 from, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [from];\n\t}"
-                 : "=f"(v.x), "=f"(v.y)
-                 : "r"(at), "r"(rank)
-                 : "memory");
-    return v;
+__device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 // Two values rounded to 16 bits, and what that leaves.
 template <int TW>
@@ -215,6 +218,12 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
             const int row = sh.row[line + 32 * i];
             x[i] = row < 0 ? nullptr : (const char *)a.x + (int64_t)row * a.x_stride * 2;
         }
+        int from[LORA_PASS / 32];                                      // of A's rows; -1: none there
+#pragma unroll
+        for (int i = 0; i < LORA_PASS / 32; ++i) {
+            const int j = line + 32 * i, t = j / rp;
+            from[i] = j < wide && j - t * rp < r ? (t * a.rank + j - t * rp) * a.inputs : -1;
+        }
         const uint32_t swizzled = (uint32_t)line * 128 + (uint32_t)((c ^ (line & 7)) << 4);
         auto issue = [&](int k) {
             const uint32_t to = base_at + (uint32_t)(k % plan.stages) * stage_bytes + swizzled;
@@ -222,13 +231,12 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
             const bool in = e < a.inputs;
 #pragma unroll
             for (int i = 0; i < 4; ++i) lt_copy16(to + i * 4096, in && x[i] ? x[i] + e * 2 : a.x, in && x[i] ? 16 : 0);
-            for (int i = 0, j = line; j < wide; ++i, j += 32) {
-                const int t = j / rp, jr = j - t * rp;
-                const bool there = in && jr < r;
-                lt_copy16(to + LT_BLOCK + i * 4096, there ? wa + ((int64_t)(t * a.rank + jr) * a.inputs + e) * 2 : wa, there ? 16 : 0);
-            }
+#pragma unroll
+            for (int i = 0; i < LORA_PASS / 32; ++i)
+                if (line + 32 * i < wide) lt_copy16(to + LT_BLOCK + i * 4096, in && from[i] >= 0 ? wa + (int64_t)(from[i] + e) * 2 : wa, in && from[i] >= 0 ? 16 : 0);
         };
-        const int ahead = plan.stages - 1;
+        // A stage is asked for again when the products two blocks back are done with it, not those just begun.
+        const int ahead = max(1, plan.stages - 2);
         for (int k = 0; k < ahead; ++k) {
             if (k < k_blocks) issue(k);
             lt_commit();
@@ -244,8 +252,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
                 case 1: lt_wait_copies<1>(); break;
                 case 2: lt_wait_copies<2>(); break;
                 case 3: lt_wait_copies<3>(); break;
-                case 4: lt_wait_copies<4>(); break;
-                default: lt_wait_copies<5>(); break;
+                default: lt_wait_copies<4>(); break;
             }
             lt_async_fence();
             lt_arrive(&sh.full[k % plan.stages]);
@@ -266,8 +273,8 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
     __syncwarp();
     wait(&sh.d1_done, 0);
     kvt_after();
-    // B's tiles: outputs' rows of up to 128 bytes in blocks of 64.
-    const int b_bytes = plan.b_blocks * S::COLS * 128;
+    // B's tiles: outputs' rows in blocks of 32, 64 bytes each; a worker has 16 bytes of every 64th row.
+    const int b_bytes = plan.b_blocks * S::COLS * 64, bc = tid & 3, bl = tid >> 2;
     int target = t0, tile0 = 0, n_target = n_first;                    // of the tile that is asked for next
     auto issue_b = [&](int i) {
         const int tile = tile_low + i;
@@ -277,10 +284,11 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
             ++target;
         }
         const int n0 = (tile - tile0) * S::COLS;
-        const uint32_t to = base_at + plan.b_at + (uint32_t)(i & 1) * b_bytes;
-        for (int n = line; n < S::COLS; n += 32)
-            for (int j = 8 * c; j < rp; j += 64) {
-                const uint32_t at = to + (uint32_t)(j >> 6) * (S::COLS * 128) + (uint32_t)n * 128 + (uint32_t)((c ^ (n & 7)) << 4);
+        const uint32_t to = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
+#pragma unroll
+        for (int n = bl; n < S::COLS; n += 64)
+            for (int j = 8 * bc; j < rp; j += 32) {
+                const uint32_t at = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
                 const char *const from = wb + (((int64_t)n_target + n0 + n) * a.rank + j) * 2;
                 const bool there = n0 + n < a.width[target];
                 if (j + 8 <= r || j >= r || !there) {
@@ -294,12 +302,13 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
                 }
             }
     };
+    lora_cluster_arrive();                     // every CTA is done with its stages: sums may lie over them
+    lora_cluster_wait();
+    const int mine = LT_ROWS / ctas, pitch = plan.wide + 4;            // rows that a CTA adds up
     if (worker) {
-        if (plan.early)
-            for (int i = 0; i < min(2, my_tiles); ++i) issue_b(i);
-        // The CTA's sums to where its peers can read them: a row to a thread, 16 columns at a time, a half of them to a warp.
-        const uint32_t sums = base_at + plan.sum_at;
+        // The CTA's sums go to the CTAs that add them up: a row to a thread, 16 columns at a time, a half of them to a warp.
         const int row = 32 * (warp & 3) + lane;
+        const uint32_t to = lt_peer(base_at + plan.sum_at + (uint32_t)((cta * mine + row % mine) * pitch) * 4, row / mine);
         for (int j = 16 * (warp >> 2); j < wide; j += 32) {
             uint32_t v[16];
             kvt_load16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + j, v);
@@ -308,7 +317,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = 0;
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) store16_shared(sums + (uint32_t)(row * (plan.wide + 4) + j + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 16; e += 4) lt_store_peer(to + (j + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
         }
     }
     kvt_before();
@@ -316,47 +325,55 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
     lora_cluster_wait();
     kvt_after();
     if (worker) {
-        const int mine = LT_ROWS / ctas;                               // rows that this CTA adds up
+        // A row to a warp, two columns of every 64 to a lane.
+        const float *const sums = (const float *)(tiles + plan.sum_at) + 2 * lane;
+        uint32_t keep = 0;                                             // columns that are h's
+#pragma unroll
+        for (int m = 0; m < LORA_PASS / 64; ++m) {
+            const int col = 64 * m + 2 * lane, j = col % rp;
+            if (col < wide) keep |= (uint32_t)((j < r) | (j + 1 < r) << 1 | 4) << (4 * m);
+        }
         for (int i = warp; i < mine; i += LT_WARPS) {
             const int row = cta * mine + i;
-            float2 v[4];
+            float2 v[LORA_PASS / 64];
             float most = 0.0f;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int col = 64 * m + 2 * lane, j = col % rp;
+            for (int m = 0; m < LORA_PASS / 64; ++m) {
                 v[m] = make_float2(0.0f, 0.0f);
-                if (col >= wide) continue;
+                if (!(keep >> (4 * m) & 4)) continue;
                 for (int k = 0; k < ctas; ++k) {
-                    const float2 p = lt_load_peer2(base_at + plan.sum_at + (uint32_t)(row * (plan.wide + 4) + col) * 4, k);
+                    const float2 p = *(const float2 *)(sums + (k * mine + i) * pitch + 64 * m);
                     v[m].x = fadd(v[m].x, p.x);
                     v[m].y = fadd(v[m].y, p.y);
                 }
-                if (j >= r) v[m].x = 0.0f;
-                if (j + 1 >= r) v[m].y = 0.0f;
+                if (!(keep >> (4 * m) & 1)) v[m].x = 0.0f;
+                if (!(keep >> (4 * m) & 2)) v[m].y = 0.0f;
                 most = fmaxf(most, fmaxf(fabsf(v[m].x), fabsf(v[m].y)));
             }
-            float back = 1.0f;
             if constexpr (TX == KV_F16) {
                 const uint32_t exponent = __reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23;
+                float back = 1.0f;
                 if (exponent > 20 && exponent < 255) {                 // 2^14 <= most * 2^(141 - exponent) < 2^15
                     const float to = __uint_as_float((268 - exponent) << 23);
                     back = __uint_as_float((exponent - 14) << 23);
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) v[m].x = fmul(v[m].x, to), v[m].y = fmul(v[m].y, to);
+                    for (int m = 0; m < LORA_PASS / 64; ++m) v[m].x = fmul(v[m].x, to), v[m].y = fmul(v[m].y, to);
                 }
-                if (lane == 0)
-                    for (int k = 0; k < ctas; ++k) lt_store_peer(kvt_smem(&sh.row_scale[row]), k, __float_as_uint(back));
+                if (lane < ctas) lt_store_peer(lt_peer(kvt_smem(&sh.row_scale[row]), lane), __float_as_uint(back));
             }
+            uint32_t w[LORA_PASS / 64][S::PH];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int col = 64 * m + 2 * lane;
-                if (col >= wide) continue;
-                const uint32_t at = base_at + (uint32_t)m * LT_BLOCK + (uint32_t)row * 128 + (uint32_t)(((lane >> 2) ^ (row & 7)) << 4) + (uint32_t)(lane & 3) * 4;
+            for (int m = 0; m < LORA_PASS / 64; ++m)
 #pragma unroll
-                for (int p = 0; p < S::PH; ++p) {
-                    const uint32_t w = lt_part<TX>(v[m]);
-                    for (int k = 0; k < ctas; ++k) lt_store_peer(at + (uint32_t)(p * plan.h_blocks) * LT_BLOCK, k, w);
-                }
+                for (int p = 0; p < S::PH; ++p) w[m][p] = lt_part<TX>(v[m]);
+            const uint32_t at = base_at + (uint32_t)(lane >> 4) * LT_HALF + (uint32_t)row * 64 + (uint32_t)(((lane >> 2 & 3) ^ ((row >> 1) & 3)) << 4) + (uint32_t)(lane & 3) * 4;
+            for (int k = 0; k < ctas; ++k) {
+                const uint32_t to = lt_peer(at, k);
+#pragma unroll
+                for (int m = 0; m < LORA_PASS / 64; ++m)
+                    if (keep >> (4 * m) & 4)
+#pragma unroll
+                        for (int p = 0; p < S::PH; ++p) lt_store_peer(to + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF, w[m][p]);
             }
         }
     }
@@ -365,8 +382,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
     lora_cluster_wait();                       // nothing of a peer's shared memory is read or written from here on
     lt_async_fence();
     if (worker) {
-        if (!plan.early)
-            for (int i = 0; i < min(2, my_tiles); ++i) issue_b(i);
+        for (int i = 0; i < min(2, my_tiles); ++i) issue_b(i);
         lt_commit();
         lt_wait_copies<0>();
         lt_async_fence();
@@ -382,13 +398,13 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
                 if (!wait(&sh.b_full[i & 1], (i >> 1) & 1)) break;
                 if (i >= 2 && !wait(&sh.d2_free[i & 1], ((i >> 1) - 1) & 1)) break;
                 kvt_after();
-                const uint32_t b = base_at + plan.b_at + (uint32_t)(i & 1) * b_bytes;
+                const uint32_t b = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
                 bool add = false;
                 for (int p = 0; p < S::PH; ++p)
                     for (int j = 0; j < rp; j += 16, add = true) {
                         const int at = (mt - t0) * rp + j;
-                        lt_mma<TX>(tmem + (uint32_t)(i & 1) * 128, kvt_desc(base_at + (uint32_t)(p * plan.h_blocks + (at >> 6)) * LT_BLOCK + (uint32_t)(at & 63) * 2),
-                                   kvt_desc(b + (uint32_t)(j >> 6) * (S::COLS * 128) + (uint32_t)(j & 63) * 2), S::COLS, add);
+                        lt_mma<TX>(tmem + (uint32_t)(i & 1) * 128, lt_desc64(base_at + (uint32_t)(p * plan.h_blocks + (at >> 5)) * LT_HALF + (uint32_t)(at & 31) * 2),
+                                   lt_desc64(b + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)(j & 31) * 2), S::COLS, add);
                     }
                 kvt_commit(&sh.d2_done[i & 1]);
             }

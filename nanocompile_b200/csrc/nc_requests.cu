@@ -96,7 +96,7 @@ int32_t launch_lora_tiles(cudaStream_t st, LoraArgs a) {
     const int passes = (a.targets + a.pass_targets - 1) / a.pass_targets;
     const LoraTilesPlan plan = lora_tiles_plan(a.pass_targets, a.rank, S::PH, S::COLS);
     const size_t bytes = (size_t)plan.bytes + 1024;
-    const int64_t places = 148 * (bytes <= 112 * 1024 ? 2 : 1);
+    const int64_t places = 148 * (plan.bytes <= LT_TWICE ? 2 : 1);
     int ctas = 8;
     while (ctas > 1 && (int64_t)a.items * passes * ctas > places) ctas /= 2;
     cudaLaunchConfig_t cfg = {};
