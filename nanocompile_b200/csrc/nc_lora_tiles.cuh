@@ -2,10 +2,11 @@
 //
 // An item to a cluster.  First each CTA multiplies its share of the inputs, 64 at a time: D1 [128 rows][h] += x A^T, tcgen05.mma with the
 // rows and the adapter's A copied asynchronously into 128-byte swizzled tiles, D1 in tensor memory.  The CTAs' sums of h are added
-// through distributed shared memory, each CTA taking 128 / CTAs rows and giving them to all, already split into the operand's
-// parts.  Then each CTA expands its share of the outputs, 256 bytes of a row at a time: D2 [128][outputs] = h B^T in two halves of
-// tensor memory, while the warps add the last tile to base: base is asked for a tile ahead, and goes by way of a warp's own
-// shared memory from a row to a thread to whole lines of rows.  The targets' h lie side by side, whole 16s to each.
+// through distributed shared memory: each CTA is sent its share of the rows, and copies them, added up and split into the
+// operand's parts, to all.  Then each CTA expands its share of the outputs, 256 bytes of a row at a time: D2 [128][outputs] = h B^T in two
+// halves of tensor memory.  Four warps ask for B and, up to four tiles ahead, for base; four warps add a tile's D2 to its base in shared
+// memory, a row to a thread, and store it, whole rows to half a warp; four others have the next tile.  The targets' h lie side by side,
+// whole 16s to each.
 //
 // Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (16 bits and the next 16: bfloat16 2^-17 of it is
 // lost, float16 2^-22; float16's h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its
@@ -17,12 +18,14 @@
 
 namespace nc {
 
-constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_THREADS = LT_WORKERS + 32, LT_TMEM = 256;
+constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_LOADERS = 128, LT_TMEM = 256;
+constexpr int LT_MMA = LT_WARPS, LT_THREADS = LT_WORKERS + 32 + LT_LOADERS;            // the warp after the workers', then those that load
 constexpr int LT_BLOCK = LT_ROWS * 128;        // 128 rows of 128 bytes
 constexpr int LT_HALF = LT_ROWS * 64;          // 128 rows of 64 bytes
 constexpr int LT_STAGES = 6;                   // of the first products at most
-constexpr int LT_TWICE = 110 * 1024, LT_ONCE = 200 * 1024;             // bytes of tiles with two CTAs on an SM, with one
-constexpr int LT_LINE = 36;                    // floats from a row to the next of a warp's 32 x 32: no bank twice in a quarter
+constexpr int LT_BYTES = 216 * 1024;           // of tiles at most
+constexpr int LT_LINE = 272, LT_SLOT = LT_ROWS * LT_LINE;              // bytes from a row to the next of a tile of base: no bank twice in a quarter
+constexpr int LT_SLOTS = 4;                    // tiles of base on their way or in work, at most
 
 __device__ unsigned int g_lora_fault;          // set when a matrix instruction did not come to its end within the wait limit
 
@@ -30,17 +33,16 @@ template <int TX>
 struct LoraTiles {
     static constexpr int PH = 2;                                       // parts of h
     static constexpr int COLS = TX == KV_F32 ? 64 : 128;               // outputs of a tile
-    static constexpr int CHUNKS = COLS / 64;                           // of 32 outputs, for each warp
     static constexpr int SIZE = TX == KV_F32 ? 4 : 2;
 };
 
-// How shared memory is laid out, by the most rows of h in a pass: h's operand, then the sums of h; over these B and the warps'
-// lines; over all of it the stages of the first products.
+// How shared memory is laid out, by the most rows of h in a pass: h's operand, then the sums of h; over these two tiles of B and the
+// slots of base; over all of it the stages of the first products.
 struct LoraTilesPlan {
     int wide;                                  // rows of h in whole 16s
     int stages, a_bytes;                       // of a stage: LT_BLOCK for rows, a_bytes for A
     int h_blocks, b_blocks;                    // blocks of 32 for a part of h, for B
-    int sum_at, line_at, bytes;
+    int sum_at, slot_at, slots, bytes;
 };
 inline LoraTilesPlan lora_tiles_plan(int targets, int rank, int parts, int cols) {
     LoraTilesPlan p{};
@@ -49,18 +51,19 @@ inline LoraTilesPlan lora_tiles_plan(int targets, int rank, int parts, int cols)
     p.h_blocks = (p.wide + 31) / 32;
     p.b_blocks = (rank + 31) / 32;
     p.sum_at = parts * p.h_blocks * LT_HALF;
-    p.line_at = p.sum_at + 2 * p.b_blocks * cols * 64;
-    const int sums = LT_ROWS * (p.wide + 4) * 4, lines = LT_WARPS * 32 * LT_LINE * 4;
-    p.bytes = p.line_at + lines > p.sum_at + sums ? p.line_at + lines : p.sum_at + sums;
-    const int stage = LT_BLOCK + p.a_bytes, most = p.bytes > LT_TWICE ? LT_ONCE : LT_TWICE;       // room for two CTAs on an SM, or one
-    p.stages = most / stage < LT_STAGES ? most / stage : LT_STAGES;
+    p.slot_at = p.sum_at + 2 * p.b_blocks * cols * 64;
+    p.slots = (LT_BYTES - p.slot_at) / LT_SLOT < LT_SLOTS ? (LT_BYTES - p.slot_at) / LT_SLOT : LT_SLOTS;
+    p.bytes = p.slot_at + p.slots * LT_SLOT;
+    const int sums = p.sum_at + (LT_ROWS + 12) * (p.wide + 4) * 4, stage = LT_BLOCK + p.a_bytes;  // the last CTA's share may be shorter
+    if (sums > p.bytes) p.bytes = sums;
+    p.stages = LT_BYTES / stage < LT_STAGES ? LT_BYTES / stage : LT_STAGES;
     if (p.stages * stage > p.bytes) p.bytes = p.stages * stage;
     return p;
 }
 
 struct LoraTilesShared {                       // before the tiles
-    uint64_t full[LT_STAGES], empty[LT_STAGES], d1_done, b_full[2], d2_done[2], d2_free[2], drained;
-    float row_scale[LT_ROWS];
+    uint64_t full[LT_STAGES], empty[LT_STAGES], d1_done, b_full[2], d2_done[2], d2_free[2], slot_full[LT_SLOTS], slot_free[LT_SLOTS], h_full, drained;
+    __align__(16) float row_scale[LT_ROWS];
     int row[LT_ROWS];
     uint32_t tmem;
     int failed;
@@ -87,7 +90,8 @@ __device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, int n
 __device__ __forceinline__ uint64_t lt_desc64(uint32_t address) {
     return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
 }
-__device__ __forceinline__ void lt_async_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void lt_async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void lt_async_fence_cluster() { asm volatile("fence.proxy.async.shared::cluster;" ::: "memory"); }
 // 16 bytes from `from`, of which `bytes` are there: the others become nought.
 __device__ __forceinline__ void lt_copy16(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -146,7 +150,7 @@ __device__ __forceinline__ uint4 lt_add(const uint4 &was, const float (&v)[8], f
 }
 
 template <int TX>
-__global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraTilesPlan plan) {
+__global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraTilesPlan plan) {
     using S = LoraTiles<TX>;
     extern __shared__ __align__(1024) char lt_raw[];
     char *const tiles = lt_raw + ((1024 - (kvt_smem(lt_raw) & 1023)) & 1023);
@@ -182,7 +186,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
         for (int64_t at = low + tid * 4096; at < high; at += LT_THREADS * 4096)
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(wb + at), "r"((uint32_t)min((int64_t)4096, high - at)) : "memory");
     }
-    if (warp == LT_WARPS) {
+    if (warp == LT_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kvt_smem(&sh.tmem)), "n"(LT_TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -190,7 +194,9 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
         for (int i = 0; i < plan.stages; ++i) lt_init(&sh.full[i], LT_WORKERS), lt_init(&sh.empty[i], 1);
         lt_init(&sh.d1_done, 1);
         lt_init(&sh.drained, 1);
-        for (int i = 0; i < 2; ++i) lt_init(&sh.b_full[i], LT_WORKERS), lt_init(&sh.d2_done[i], 1), lt_init(&sh.d2_free[i], LT_WORKERS);
+        for (int i = 0; i < 2; ++i) lt_init(&sh.b_full[i], LT_LOADERS), lt_init(&sh.d2_done[i], 1), lt_init(&sh.d2_free[i], LT_ROWS);
+        for (int i = 0; i < LT_SLOTS; ++i) lt_init(&sh.slot_full[i], LT_LOADERS), lt_init(&sh.slot_free[i], LT_ROWS);
+        lt_init(&sh.h_full, 1);
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
             lt_arrive(&sh.full[k % plan.stages]);
         }
         lt_wait_copies<0>();
-    } else if (lane == 0) {
+    } else if (warp == LT_MMA && lane == 0) {
         for (int k = 0; k < k_blocks; ++k) {
             const int stage = k % plan.stages;
             if (!wait(&sh.full[stage], (k / plan.stages) & 1)) break;
@@ -273,42 +279,14 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
     __syncwarp();
     wait(&sh.d1_done, 0);
     kvt_after();
-    // B's tiles: outputs' rows in blocks of 32, 64 bytes each; a worker has 16 bytes of every 64th row.
-    const int b_bytes = plan.b_blocks * S::COLS * 64, bc = tid & 3, bl = tid >> 2;
-    int target = t0, tile0 = 0, n_target = n_first;                    // of the tile that is asked for next
-    auto issue_b = [&](int i) {
-        const int tile = tile_low + i;
-        while (tile - tile0 >= (a.width[target] + S::COLS - 1) / S::COLS) {
-            tile0 += (a.width[target] + S::COLS - 1) / S::COLS;
-            n_target += a.width[target];
-            ++target;
-        }
-        const int n0 = (tile - tile0) * S::COLS;
-        const uint32_t to = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
-#pragma unroll
-        for (int n = bl; n < S::COLS; n += 64)
-            for (int j = 8 * bc; j < rp; j += 32) {
-                const uint32_t at = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
-                const char *const from = wb + (((int64_t)n_target + n0 + n) * a.rank + j) * 2;
-                const bool there = n0 + n < a.width[target];
-                if (j + 8 <= r || j >= r || !there) {
-                    lt_copy16(at, there && j < r ? from : wb, there && j < r ? 16 : 0);
-                } else {                                               // what lies past the adapter's own rank may be anything
-                    const uint4 w = __ldg((const uint4 *)from);
-                    uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[e] = j + 2 * e >= r ? 0u : j + 2 * e + 1 >= r ? u[e] & 0xffffu : u[e];
-                    store16_shared(at, u[0], u[1], u[2], u[3]);
-                }
-            }
-    };
     lora_cluster_arrive();                     // every CTA is done with its stages: sums may lie over them
     lora_cluster_wait();
-    const int mine = LT_ROWS / ctas, pitch = plan.wide + 4;            // rows that a CTA adds up
+    const int mine = (LT_ROWS / 4 + ctas - 1) / ctas * 4, pitch = plan.wide + 4;     // rows that a CTA adds up; the last one's may be fewer
     if (worker) {
         // The CTA's sums go to the CTAs that add them up: a row to a thread, 16 columns at a time, a half of them to a warp.
         const int row = 32 * (warp & 3) + lane;
-        const uint32_t to = lt_peer(base_at + plan.sum_at + (uint32_t)((cta * mine + row % mine) * pitch) * 4, row / mine);
+        const bool here = row / mine == cta;
+        const uint32_t at = base_at + plan.sum_at + (uint32_t)((cta * mine + row % mine) * pitch) * 4, to = lt_peer(at, row / mine);
         for (int j = 16 * (warp >> 2); j < wide; j += 32) {
             uint32_t v[16];
             kvt_load16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + j, v);
@@ -317,7 +295,9 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = 0;
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) lt_store_peer(to + (j + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 16; e += 4)
+                if (here) store16_shared(at + (j + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
+                else lt_store_peer(to + (j + e) * 4, v[e], v[e + 1], v[e + 2], v[e + 3]);
         }
     }
     kvt_before();
@@ -333,7 +313,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
             const int col = 64 * m + 2 * lane, j = col % rp;
             if (col < wide) keep |= (uint32_t)((j < r) | (j + 1 < r) << 1 | 4) << (4 * m);
         }
-        for (int i = warp; i < mine; i += LT_WARPS) {
+        for (int i = warp; i < min(mine, LT_ROWS - cta * mine); i += LT_WARPS) {
             const int row = cta * mine + i;
             float2 v[LORA_PASS / 64];
             float most = 0.0f;
@@ -359,42 +339,108 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
 #pragma unroll
                     for (int m = 0; m < LORA_PASS / 64; ++m) v[m].x = fmul(v[m].x, to), v[m].y = fmul(v[m].y, to);
                 }
-                if (lane < ctas) lt_store_peer(lt_peer(kvt_smem(&sh.row_scale[row]), lane), __float_as_uint(back));
+                if (lane == 0) sh.row_scale[row] = back;
             }
-            uint32_t w[LORA_PASS / 64][S::PH];
-#pragma unroll
-            for (int m = 0; m < LORA_PASS / 64; ++m)
-#pragma unroll
-                for (int p = 0; p < S::PH; ++p) w[m][p] = lt_part<TX>(v[m]);
             const uint32_t at = base_at + (uint32_t)(lane >> 4) * LT_HALF + (uint32_t)row * 64 + (uint32_t)(((lane >> 2 & 3) ^ ((row >> 1) & 3)) << 4) + (uint32_t)(lane & 3) * 4;
-            for (int k = 0; k < ctas; ++k) {
-                const uint32_t to = lt_peer(at, k);
 #pragma unroll
-                for (int m = 0; m < LORA_PASS / 64; ++m)
-                    if (keep >> (4 * m) & 4)
+            for (int m = 0; m < LORA_PASS / 64; ++m) {
+                if (!(keep >> (4 * m) & 4)) continue;
 #pragma unroll
-                        for (int p = 0; p < S::PH; ++p) lt_store_peer(to + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF, w[m][p]);
+                for (int p = 0; p < S::PH; ++p)
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<TX>(v[m])) : "memory");
             }
         }
-    }
-    lt_async_fence();
-    lora_cluster_arrive();
-    lora_cluster_wait();                       // nothing of a peer's shared memory is read or written from here on
-    lt_async_fence();
-    if (worker) {
-        for (int i = 0; i < min(2, my_tiles); ++i) issue_b(i);
-        lt_commit();
-        lt_wait_copies<0>();
         lt_async_fence();
-        lt_arrive(&sh.b_full[0]);
-        lt_arrive(&sh.b_full[1]);
+    }
+    if (warp != LT_MMA) asm volatile("bar.sync 1, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");       // h's rows of this CTA are there, the sums read
+    if (warp == 0) {
+        // To each peer this CTA's rows of every block, 64 bytes each, and their scales: one bulk copy a lane.
+        const int from_row = cta * mine, rows = min(mine, LT_ROWS - from_row), used = (wide + 31) / 32, per = S::PH * used + (TX == KV_F16);
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kvt_smem(&sh.h_full)),
+                         "r"((LT_ROWS - rows) * (S::PH * used * 64 + (TX == KV_F16 ? 4 : 0)))
+                         : "memory");
+        __syncwarp();
+        for (int i = lane; i < per * (ctas - 1); i += 32) {
+            const int k = i / per, peer = k + (k >= cta), which = i - k * per;
+            const bool scales = which == S::PH * used;
+            const uint32_t at = scales ? kvt_smem(&sh.row_scale[from_row]) : base_at + (uint32_t)(which / used * plan.h_blocks + which % used) * LT_HALF + (uint32_t)from_row * 64;
+            asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(lt_peer(at, peer)), "r"(at),
+                         "r"(rows * (scales ? 4 : 64)), "r"(lt_peer(kvt_smem(&sh.h_full), peer))
+                         : "memory");
+        }
+        __syncwarp();
     }
 
-    if (!worker) {
+    // Tiles: `look_up` goes on to tile i of this CTA, in ascending order.
+    int target = t0, tile0 = 0, n_target = n_first;
+    auto look_up = [&](int i) {
+        while (tile_low + i - tile0 >= (a.width[target] + S::COLS - 1) / S::COLS) {
+            tile0 += (a.width[target] + S::COLS - 1) / S::COLS;
+            n_target += a.width[target];
+            ++target;
+        }
+        return (tile_low + i - tile0) * S::COLS;                       // the tile's first output of its target
+    };
+    const int b_bytes = plan.b_blocks * S::COLS * 64;
+    const bool staged = a.wide != 0;
+    if (warp > LT_MMA) {
+        // B's rows in blocks of 32, 64 bytes each, 16 of every 32nd row to a thread; base's rows, 16 bytes of every eighth to a thread.
+        const int at = tid - LT_WORKERS - 32, bc = at & 3, bl = at >> 2, cc = at & 15, cl = at >> 4;
+        auto issue_b = [&](int i, int n0) {
+            const uint32_t to = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
+            for (int n = bl; n < S::COLS; n += LT_LOADERS / 4)
+                for (int j = 8 * bc; j < rp; j += 32) {
+                    const uint32_t dst = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
+                    const char *const from = wb + (((int64_t)n_target + n0 + n) * a.rank + j) * 2;
+                    const bool there = n0 + n < a.width[target];
+                    if (j + 8 <= r || j >= r || !there) {
+                        lt_copy16(dst, there && j < r ? from : wb, there && j < r ? 16 : 0);
+                    } else {                                           // what lies past the adapter's own rank may be anything
+                        const uint4 w = __ldg((const uint4 *)from);
+                        uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[e] = j + 2 * e >= r ? 0u : j + 2 * e + 1 >= r ? u[e] & 0xffffu : u[e];
+                        store16_shared(dst, u[0], u[1], u[2], u[3]);
+                    }
+                }
+            lt_commit();
+        };
+        // Tile i's B is waited for once the next one's is asked for; base is asked for as slots become free, and its copies
+        // report to the slot's barrier themselves.
+        for (int i = 0; i <= my_tiles; ++i) {
+            int n0 = 0;
+            if (i < my_tiles) {
+                if (i >= 2) wait(&sh.d2_done[i & 1], ((i >> 1) - 1) & 1);
+                n0 = look_up(i);
+                issue_b(i, n0);
+            }
+            if (i > 0) {
+                if (i < my_tiles) lt_wait_copies<1>();
+                else lt_wait_copies<0>();
+                lt_async_fence();
+                lt_arrive(&sh.b_full[(i - 1) & 1]);
+            }
+            if (i == my_tiles || !staged || !a.base) continue;
+            const int slot_i = i % plan.slots, left = a.width[target] - n0;
+            if (i >= plan.slots) wait(&sh.slot_free[slot_i], (i / plan.slots - 1) & 1);
+            const uint32_t to = base_at + plan.slot_at + (uint32_t)(slot_i * LT_SLOT + cc * 16);
+            const char *const from = (const char *)a.base + ((int64_t)n_target + n0) * S::SIZE + cc * 16;
+            if ((cc + 1) * (16 / S::SIZE) <= left)
+#pragma unroll 4
+                for (int k = cl; k < LT_ROWS; k += LT_LOADERS / 16) {
+                    const int row = sh.row[k];
+                    if (row >= 0) lt_copy16(to + k * LT_LINE, from + (int64_t)row * a.base_stride * S::SIZE, 16);
+                }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(kvt_smem(&sh.slot_full[slot_i])) : "memory");
+        }
+        lt_wait_copies<0>();
+    } else if (warp == LT_MMA) {
         if (lane == 0) {
-            int mt = t0, mt0 = 0;
-            for (int i = 0; i < my_tiles; ++i) {
-                while (tile_low + i - mt0 >= (a.width[mt] + S::COLS - 1) / S::COLS) mt0 += (a.width[mt] + S::COLS - 1) / S::COLS, ++mt;
+            const bool ready = wait(&sh.h_full, 0);
+            lt_async_fence();
+            for (int i = 0; i < my_tiles && ready; ++i) {
+                look_up(i);
                 if (!wait(&sh.b_full[i & 1], (i >> 1) & 1)) break;
                 if (i >= 2 && !wait(&sh.d2_free[i & 1], ((i >> 1) - 1) & 1)) break;
                 kvt_after();
@@ -402,7 +448,7 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
                 bool add = false;
                 for (int p = 0; p < S::PH; ++p)
                     for (int j = 0; j < rp; j += 16, add = true) {
-                        const int at = (mt - t0) * rp + j;
+                        const int at = (target - t0) * rp + j;
                         lt_mma<TX>(tmem + (uint32_t)(i & 1) * 128, lt_desc64(base_at + (uint32_t)(p * plan.h_blocks + (at >> 5)) * LT_HALF + (uint32_t)(at & 31) * 2),
                                    lt_desc64(b + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)(j & 31) * 2), S::COLS, add);
                     }
@@ -412,91 +458,66 @@ __global__ void __launch_bounds__(LT_THREADS, 2) lora_tiles_kernel(const __grid_
         }
         __syncwarp();
     } else {
-        // A warp: 32 rows, a half of the tile's outputs in chunks of 32.  For base and out lane l has 16 bytes of row 8 i + l / 4.
-        const int q = warp & 3, half = warp >> 2, rl = lane >> 2, cl = (lane & 3) * 8;
-        float *const lines = (float *)(tiles + plan.line_at) + warp * 32 * LT_LINE;
-        int et = t0, et0 = 0, en = n_first;                            // of the tile whose base is asked for
-        uint4 was[S::CHUNKS][4];
-        int n_of = 0, left_of = 0;                                     // of that tile: the first output, those of its target from there on
-        auto look_up = [&](int i) {
-            const int tile = tile_low + i;
-            while (tile - et0 >= (a.width[et] + S::COLS - 1) / S::COLS) {
-                et0 += (a.width[et] + S::COLS - 1) / S::COLS;
-                en += a.width[et];
-                ++et;
-            }
-            n_of = en + (tile - et0) * S::COLS;
-            left_of = a.width[et] - (tile - et0) * S::COLS;
-        };
-        auto ask = [&](int m) {
-            if (!a.base || !a.wide) return;
-            const int col = half * (S::COLS / 2) + 32 * m + cl;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = sh.row[32 * q + 8 * k + rl];
-                if (row >= 0 && col + 8 <= left_of) was[m][k] = __ldcs((const uint4 *)((const char *)a.base + ((int64_t)row * a.base_stride + n_of + col) * 2));
-            }
-        };
-        if (!a.base)
-#pragma unroll
-            for (int m = 0; m < S::CHUNKS; ++m)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) was[m][k] = make_uint4(0, 0, 0, 0);
-        if (my_tiles > 0) {
-            look_up(0);
-#pragma unroll
-            for (int m = 0; m < S::CHUNKS; ++m) ask(m);
-        }
-        for (int i = 0; i < my_tiles; ++i) {
-            const int n = n_of, left = left_of;
-            if (i + 1 < my_tiles) look_up(i + 1);
-            wait(&sh.d2_done[i & 1], (i >> 1) & 1);
+        // Every other tile, a row to a thread.
+        if constexpr (TX == KV_F16) wait(&sh.h_full, 0);               // the rows' scales
+        const int at = 32 * (warp & 3) + lane, row = sh.row[at], half = warp >> 2, cc = lane & 15, cl = lane >> 4;
+        const float by = TX == KV_F16 ? scale * sh.row_scale[at] : scale;
+        const uint32_t d2 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)half * 128;
+        for (int i = half; i < my_tiles; i += 2) {
+            const int n0 = look_up(i), left = min(S::COLS, a.width[target] - n0), n = n_target + n0, slot_i = i % plan.slots;
+            char *const slot_line = tiles + plan.slot_at + slot_i * LT_SLOT + at * LT_LINE;
+            wait(&sh.d2_done[half], (i >> 1) & 1);
             kvt_after();
-            if (i + 2 < my_tiles) issue_b(i + 2);
-            lt_commit();
-#pragma unroll
-            for (int m = 0; m < S::CHUNKS; ++m) {
+            if (staged && a.base) wait(&sh.slot_full[slot_i], (i / plan.slots) & 1);
+#pragma unroll 1
+            for (int m = 0; m < S::COLS; m += 32) {
                 uint32_t v[32];
-                kvt_load32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(i & 1) * 128 + half * (S::COLS / 2) + 32 * m, v);
+                __syncwarp();
+                kvt_load32(d2 + m, v);
                 kvt_wait_ld();
-                if (m == S::CHUNKS - 1) {
+                if (m + 32 == S::COLS) {
                     kvt_before();
-                    lt_arrive(&sh.d2_free[i & 1]);
+                    lt_arrive(&sh.d2_free[half]);
                 }
-                __syncwarp();
+                if (row < 0 || m >= left) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *(float4 *)(lines + lane * LT_LINE + e) = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-                __syncwarp();
-                const int col = half * (S::COLS / 2) + 32 * m + cl;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int at = 8 * k + rl, row = sh.row[32 * q + at];
-                    if (row < 0 || col >= left) continue;
-                    const float4 s0 = *(const float4 *)(lines + at * LT_LINE + cl), s1 = *(const float4 *)(lines + at * LT_LINE + cl + 4);
-                    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-                    const float by = TX == KV_F16 ? scale * sh.row_scale[32 * q + at] : scale;
-                    const int64_t to = (int64_t)row * a.out_stride + n + col;
-                    if (a.wide && col + 8 <= left) {
-                        __stcs((uint4 *)((char *)a.out + to * 2), lt_add<TX>(was[m][k], s, by));
+                for (int e = 0; e < 32; e += 8) {
+                    const float f[8] = {__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]),
+                                        __uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]), __uint_as_float(v[e + 6]), __uint_as_float(v[e + 7])};
+                    if (staged && m + e + 8 <= left) {
+                        uint4 *const was = (uint4 *)(slot_line + (m + e) * S::SIZE);
+                        *was = lt_add<TX>(a.base ? *was : make_uint4(0, 0, 0, 0), f, by);
                     } else {
-                        for (int e = 0; e < min(8, left - col); ++e)
-                            kv_store(a.out, to + e, TX, __fmaf_rn(by, s[e], a.base ? kv_load(a.base, (int64_t)row * a.base_stride + n + col + e, TX) : 0.0f));
+                        const int64_t to = (int64_t)row * a.out_stride + n + m + e, was = (int64_t)row * a.base_stride + n + m + e;
+                        for (int k = 0; k < min(8, left - m - e); ++k)
+                            kv_store(a.out, to + k, TX, __fmaf_rn(by, f[k], a.base ? kv_load(a.base, was + k, TX) : 0.0f));
                     }
                 }
-                if (i + 1 < my_tiles) ask(m);                          // of the next tile
             }
-            lt_wait_copies<0>();
-            lt_async_fence();
-            if (i + 2 < my_tiles) lt_arrive(&sh.b_full[i & 1]);
+            if (!staged) continue;
+            __syncwarp();
+            const char *const from = tiles + plan.slot_at + slot_i * LT_SLOT + (32 * (warp & 3)) * LT_LINE + cc * 16;
+            char *const to = (char *)a.out + (int64_t)n * S::SIZE + cc * 16;
+            if ((cc + 1) * (16 / S::SIZE) <= left)
+#pragma unroll 4
+                for (int k = cl; k < 32; k += 2) {
+                    const int to_row = sh.row[32 * (warp & 3) + k];
+                    if (to_row >= 0) __stcs((uint4 *)(to + (int64_t)to_row * a.out_stride * S::SIZE), *(const uint4 *)(from + k * LT_LINE));
+                }
+            __syncwarp();
+            lt_arrive(&sh.slot_free[slot_i]);
         }
     }
+    __syncwarp();
+    // What this CTA has sent is there once every CTA has come here.
+    lora_cluster_arrive();
     // Nothing reads or writes tensor memory any more once the last matrix instruction has come to its end.
     kvt_mbar_wait(&sh.drained, 0, NC_DRAIN_CYCLES);
     kvt_before();
     __syncthreads();
     kvt_after();
-    if (warp == LT_WARPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(LT_TMEM) : "memory");
+    if (warp == LT_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(LT_TMEM) : "memory");
+    lora_cluster_wait();
 }
 
 }  // namespace nc

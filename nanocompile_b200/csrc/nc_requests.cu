@@ -91,14 +91,13 @@ int32_t launch_lora_tiles(cudaStream_t st, LoraArgs a) {
     using S = LoraTiles<TX>;
     auto kernel = lora_tiles_kernel<TX>;
     static std::atomic<uint64_t> allowed{0};
-    NC_TRY(allow_smem_once(kernel, 221 * 1024, &allowed));
+    NC_TRY(allow_smem_once(kernel, LT_BYTES + 1024, &allowed));
     a.pass_targets = std::min(a.targets, std::max(1, LORA_PASS / ((a.rank + 15) / 16 * 16)));
+    LoraTilesPlan plan = lora_tiles_plan(a.pass_targets, a.rank, S::PH, S::COLS);
+    while (plan.slots < 2 && a.pass_targets > 1) plan = lora_tiles_plan(--a.pass_targets, a.rank, S::PH, S::COLS);
     const int passes = (a.targets + a.pass_targets - 1) / a.pass_targets;
-    const LoraTilesPlan plan = lora_tiles_plan(a.pass_targets, a.rank, S::PH, S::COLS);
     const size_t bytes = (size_t)plan.bytes + 1024;
-    const int64_t places = 148 * (plan.bytes <= LT_TWICE ? 2 : 1);
-    int ctas = 8;
-    while (ctas > 1 && (int64_t)a.items * passes * ctas > places) ctas /= 2;
+    const int ctas = (int)std::clamp<int64_t>(148 / ((int64_t)a.items * passes), 1, 8);          // one on an SM
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * ctas), (unsigned)passes);
     cfg.blockDim = LT_THREADS;
