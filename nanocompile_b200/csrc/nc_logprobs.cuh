@@ -206,9 +206,9 @@ __device__ __forceinline__ unsigned long long lp_block_max(unsigned long long v,
 }
 
 // The k best keys of a segment, in order, to sh.best (0 past its end); `mine`: the largest of the thread's blocks.  A: arguments with
-// the row's `vocab` and the wanted `k`.
-template <int TYPE, typename A>
-__device__ __forceinline__ void lp_segment_top(const A &a, LpShared &sh, const char *base, int skew, int64_t seg0,
+// the row's `vocab` and the wanted `k`; SH: LpShared, or the same with room for other batches.
+template <int TYPE, typename A, typename SH>
+__device__ __forceinline__ void lp_segment_top(const A &a, SH &sh, const char *base, int skew, int64_t seg0,
                                                int64_t v_end, int batches, uint32_t mine) {
     constexpr int N = LpVec<TYPE>::N, SIZE = LP_VECS * N, MOST = LP_CAND / SIZE;      // values of a block; blocks to read again
     constexpr int64_t BATCH = LP_THREADS * LP_VECS;

@@ -237,46 +237,30 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
 
 namespace {
 
-constexpr int64_t BEAM_COUNTERS = 2 * LP_ROWS;
-constexpr int64_t BEAM_PARTS = 1 << 14;        // segments of a launch at most, where rows are cut for speed: bounds the scratch
-constexpr int BEAM_CUTS[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 80, 96, 112, 128, 160, 192, 224, 256};
+constexpr int64_t BEAM_COUNTERS = BEAM_ROWS;
 
-int64_t beam_vecs(int64_t vocab, int64_t type) {                  // of a row at any alignment
-    const int64_t n = 16 / type_bytes(type);
-    return (vocab + 2 * (n - 1)) / n;
+int64_t beam_batches(int64_t vocab, int64_t type) {               // of a row at any alignment
+    const int64_t n = 16 / type_bytes(type), vecs = (vocab + 2 * (n - 1)) / n;
+    return (vecs + BEAM_BATCH - 1) / BEAM_BATCH;
 }
-int64_t beam_fewest(int64_t vocab, int64_t type) {                // segments that a row has to have
-    constexpr int64_t longest = (int64_t)LP_BATCHES * LP_THREADS * LP_VECS;
-    return (beam_vecs(vocab, type) + longest - 1) / longest;
-}
+// Batches of a CTA's share at least, that a request has no more than BEAM_LISTS segments (0: it has more), and segments of a row at most:
+// it is cut where shares end, and after every 16 batches.
 struct BeamPlan {
-    int segs;
-    int64_t seg_vecs;
+    int64_t least, lists;
 };
-// Segments to a row: the fewest elements' time over the waves of CTAs that the card holds at once, a segment's start and end
-// counted as 4096 elements and its share of the join as 16.
-BeamPlan beam_plan(int64_t rows, int64_t vocab, int64_t type) {
-    const int64_t n = 16 / type_bytes(type), vecs = beam_vecs(vocab, type), slots = 148 * 2, fewest = beam_fewest(vocab, type);
-    int64_t best = -1;
-    BeamPlan p{0, 0};
-    for (int cut : BEAM_CUTS) {
-        const int64_t segs = std::max<int64_t>(cut, fewest);
-        if (segs > LP_SEGS || (segs > fewest && (vecs / segs < LP_THREADS || rows * segs > BEAM_PARTS))) break;
-        const int64_t waves = (rows * segs + slots - 1) / slots, cost = waves * (vecs * n / segs + 4096) + 16 * segs;
-        if (best >= 0 && cost >= best) continue;
-        best = cost;
-        p.seg_vecs = (vecs + segs - 1) / segs;
-        p.segs = (int)((vecs + p.seg_vecs - 1) / p.seg_vecs);
-    }
-    return p;
+BeamPlan beam_plan(int64_t batches, int64_t beams) {
+    auto lists = [&](int64_t least) { return std::min(batches, (std::max<int64_t>(batches - 2, 0)) / least + 2 + batches / BEAM_BATCHES); };
+    int64_t least = std::max<int64_t>(1, batches * beams / BEAM_LISTS);
+    // Two batches where that leaves half of the candidates that are taken at once: 4 beams of 151936 float32 logits 13.2 us, 14.7 with one.
+    if (least == 1 && batches > 1 && lists(1) * beams * beams > 512 && lists(2) * beams * beams <= 512) least = 2;
+    while (least < batches && lists(least) * beams > BEAM_LISTS) ++least;
+    return lists(least) * beams > BEAM_LISTS ? BeamPlan{0, 0} : BeamPlan{least, lists(least)};
 }
-int64_t beam_launch_rows(int64_t rows, int64_t beams) { return std::min<int64_t>(rows, LP_ROWS / beams * beams); }
+int64_t beam_launch_rows(int64_t rows, int64_t beams) { return std::min<int64_t>(rows, BEAM_ROWS / beams * beams); }
 
 template <int TYPE>
 int32_t launch_beams(cudaStream_t st, const BeamArgs &a, int64_t rows) {
-    static std::atomic<uint64_t> allowed{0};
-    NC_TRY(allow_smem_once(beam_select_kernel<TYPE>, sizeof(BeamShared), &allowed));
-    CUDA_TRY(launch_k(beam_select_kernel<TYPE>, (unsigned)(rows * a.segs), LP_THREADS, sizeof(BeamShared), st, a));
+    CUDA_TRY(launch_k(beam_select_kernel<TYPE>, (unsigned)std::min<int64_t>(rows * a.batches, BEAM_CTAS), LP_THREADS, 0, st, a));
     return check_launch("beam_select_kernel");
 }
 
@@ -284,14 +268,10 @@ int32_t launch_beams(cudaStream_t st, const BeamArgs &a, int64_t rows) {
 
 extern "C" int64_t nc_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int64_t beams) {
     if (rows <= 0 || vocab <= 0 || beams <= 0 || beams > LP_MAX_TOP) return 4 * BEAM_COUNTERS;
-    // A bound that grows with the rows: fewer of them are cut into more segments.
-    int64_t most = 0;
-    rows = std::min<int64_t>(rows, LP_ROWS);
-    for (int type : {KV_F32, KV_F16}) {
-        const int64_t fewest = beam_fewest(vocab, type), cut = std::min<int64_t>(LP_SEGS, beam_vecs(vocab, type) / LP_THREADS);
-        most = std::max({most, rows * fewest, std::min(BEAM_PARTS, rows * cut)});
-    }
-    return 4 * BEAM_COUNTERS + (most + rows) * 8 * (1 + beams);
+    int64_t row = 0;                           // fewer beams may have more segments
+    for (int type : {KV_F32, KV_F16})
+        for (int64_t n = 1; n <= beams; ++n) row = std::max(row, beam_plan(beam_batches(vocab, type), n).lists * 8 * (1 + n));
+    return 4 * BEAM_COUNTERS + std::min<int64_t>(rows, BEAM_ROWS) * row;
 }
 
 extern "C" int32_t nc_beam_select(void **p, const int64_t *s, void *stream) {
@@ -307,13 +287,13 @@ extern "C" int32_t nc_beam_select(void **p, const int64_t *s, void *stream) {
     if (s[5] < 0 && p[8]) return fail(NC_ERR_ARGUMENT, "finished beams without an end token");
     if (rows == 0) return NC_OK;
     const int64_t at_once = beam_launch_rows(rows, beams), k = std::min(beams, vocab);
-    const BeamPlan plan = beam_plan(at_once, vocab, type);
-    if (plan.segs == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is beyond %d segments", (long long)vocab, LP_SEGS);
+    const BeamPlan plan = beam_plan(beam_batches(vocab, type), beams);
+    if (plan.least == 0) return fail(NC_ERR_ARGUMENT, "a vocabulary of %lld is too large for %lld beams", (long long)vocab, (long long)beams);
     if (!p[0] || !p[1] || !p[2] || !p[6] || !p[7] || misaligned(p[6], type_bytes(type)))
         return fail(NC_ERR_ARGUMENT, "null or misaligned logits, scores or outputs");
     if (p[7] == p[2] || (p[8] && p[8] == p[3])) return fail(NC_ERR_ARGUMENT, "the new scores or flags are the old ones");
     if (misaligned(p[11], 8)) return fail(NC_ERR_ARGUMENT, "the error word is not at an 8-byte boundary");
-    const int64_t need = 4 * BEAM_COUNTERS + at_once * (plan.segs * (8 + 8 * k) + 8 + 8 * k);
+    const int64_t need = 4 * BEAM_COUNTERS + at_once * plan.lists * (8 + 8 * k);
     if (!p[10] || misaligned(p[10], 16) || scratch < need)
         return fail(NC_ERR_ARGUMENT, "scratch of %lld bytes, %lld needed", (long long)scratch, (long long)nc_beam_select_scratch_bytes(rows, vocab, beams));
     a.parent = (int32_t *)p[0];
@@ -332,17 +312,17 @@ extern "C" int32_t nc_beam_select(void **p, const int64_t *s, void *stream) {
     a.beams = (int)beams;
     a.end = s[5];
     a.k = (int)k;
-    a.segs = plan.segs;
-    a.seg_vecs = plan.seg_vecs;
+    a.batches = (int)beam_batches(vocab, type);
+    a.least = (int)plan.least;
+    a.lists = (int)plan.lists;
     a.counter = (unsigned int *)p[10];
-    a.lse = (double *)((char *)p[10] + 4 * BEAM_COUNTERS);
-    a.best = (unsigned long long *)(a.lse + at_once);
-    a.part_top = a.best + at_once * k;
-    a.part = (float2 *)(a.part_top + at_once * plan.segs * k);
+    a.part_top = (unsigned long long *)((char *)p[10] + 4 * BEAM_COUNTERS);
+    a.part = (float2 *)(a.part_top + at_once * plan.lists * k);
     const cudaStream_t st = (cudaStream_t)stream;
     for (int64_t first = 0; first < rows; first += at_once) {
         const int64_t n = std::min(rows - first, at_once);
         a.row_first = first;
+        a.rows = (int)n;
         NC_TRY(type == KV_F32 ? launch_beams<KV_F32>(st, a, n) : type == KV_F16 ? launch_beams<KV_F16>(st, a, n) : launch_beams<KV_BF16>(st, a, n));
     }
     return NC_OK;
