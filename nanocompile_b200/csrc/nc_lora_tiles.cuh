@@ -52,7 +52,10 @@ inline LoraTilesPlan lora_tiles_plan(int targets, int rank, int parts, int cols)
     p.b_blocks = (rank + 31) / 32;
     p.sum_at = parts * p.h_blocks * LT_HALF;
     p.slot_at = p.sum_at + 2 * p.b_blocks * cols * 64;
-    p.slots = (LT_BYTES - p.slot_at) / LT_SLOT < LT_SLOTS ? (LT_BYTES - p.slot_at) / LT_SLOT : LT_SLOTS;
+    // Two or four, that a slot is always the same warps': they wait for every second tile only, and would take the round of a slot's
+    // barrier before the one that they wait for, of the same parity, for that.
+    p.slots = (LT_BYTES - p.slot_at) / LT_SLOT / 2 * 2;
+    if (p.slots > LT_SLOTS) p.slots = LT_SLOTS;
     p.bytes = p.slot_at + p.slots * LT_SLOT;
     const int sums = p.sum_at + (LT_ROWS + 12) * (p.wide + 4) * 4, stage = LT_BLOCK + p.a_bytes;  // the last CTA's share may be shorter
     if (sums > p.bytes) p.bytes = sums;
@@ -110,23 +113,34 @@ __device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t v) { asm vol
 __device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// Two values rounded to 16 bits, and what that leaves.
+// Two values rounded to 16 bits, and what that leaves: nothing of what is no number.  What would round to an infinity is cut off.
 template <int TW>
 __device__ __forceinline__ uint32_t lt_part(float2 &v) {
-    uint32_t w;
+    auto round = [](float2 f, float2 *r) {
+        uint32_t w;
+        if constexpr (TW == KV_BF16) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+            w = *reinterpret_cast<const uint32_t *>(&b);
+            *r = __bfloat1622float2(b);
+        } else {
+            const __half2 b = __floats2half2_rn(f.x, f.y);
+            w = *reinterpret_cast<const uint32_t *>(&b);
+            *r = __half22float2(b);
+        }
+        return w;
+    };
     float2 r;
-    if constexpr (TW == KV_BF16) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
-        w = *reinterpret_cast<const uint32_t *>(&b);
-        r = __bfloat1622float2(b);
-    } else {
-        const __half2 b = __floats2half2_rn(v.x, v.y);
-        w = *reinterpret_cast<const uint32_t *>(&b);
-        r = __half22float2(b);
+    uint32_t w = round(v, &r);
+    if (!(fabsf(r.x) < INFINITY && fabsf(r.y) < INFINITY)) {
+        constexpr float most = TW == KV_BF16 ? 3.3895314e38f : 65504.0f;
+        auto cut = [](float f) { return fabsf(f) < INFINITY ? fminf(fmaxf(f, -most), most) : f; };
+        w = round(make_float2(cut(v.x), cut(v.y)), &r);
+        v.x = fabsf(r.x) < INFINITY ? fsub(v.x, r.x) : 0.0f;
+        v.y = fabsf(r.y) < INFINITY ? fsub(v.y, r.y) : 0.0f;
+        return w;
     }
-    // Nothing is left of what is no number, or rounds to none.
-    v.x = fabsf(r.x) < INFINITY ? fsub(v.x, r.x) : 0.0f;
-    v.y = fabsf(r.y) < INFINITY ? fsub(v.y, r.y) : 0.0f;
+    v.x = fsub(v.x, r.x);
+    v.y = fsub(v.y, r.y);
     return w;
 }
 // Eight outputs from 16 bytes of base and float32 sums.

@@ -5,7 +5,7 @@
 // (nanocompile/models/qwen2.py:348-368); these operators have no counterpart there.
 #include "nc_api.cuh"
 #include "nc_beams.cuh"
-#include "nc_lora_tiles.cuh"
+#include "nc_lora_stream.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -49,7 +49,7 @@ int64_t lora_groups(int64_t seqs, int64_t slots) { return std::min(seqs, slots +
 // Rows of an item: by the mean of the largest number of groups, as only the device knows how many there are.
 int64_t lora_tile(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t mean = rows / std::max<int64_t>(1, lora_groups(seqs, slots));
-    return mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+    return mean <= 32 ? 8 : 128;               // the few items of an adapter read it from L2: 128 rows of 8 adapters of 1 MB 16 us by eights, 25 by 16 rows
 }
 int64_t lora_places(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t tile = lora_tile(rows, seqs, slots);
@@ -81,8 +81,58 @@ int32_t launch_lora(cudaStream_t st, const LoraArgs &a, int passes) {
     CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
     return check_launch("lora_rows_kernel");
 }
+// For items of eight rows.  False where a CTA's share of the inputs is too long, or its part of an adapter so small that the ring
+// takes longer than it saves (one row of 896 inputs to 1152 outputs at rank 16: 8.9 us without, 10.1 with).
+template <int TX, int TW>
+bool lora_stream_shape(const LoraArgs &a, int passes, int *ctas, LoraStreamPlan *plan) {
+    using S = LoraStream<TX, TW>;
+    const int units = (a.inputs + 31) / 32;
+    const double bytes = 2.0 * a.rank * ((double)a.targets * a.inputs + a.outputs) / passes;
+    // CTAs of a cluster, by rounds of CTAs: 10 us to start and to add up, then bytes at 22 a ns for each of two on an SM, 30 alone.  Measured:
+    // 64 adapters of 1 MB 24 us by 4 CTAs, 44 by 8; 128 of them 46 by 4 with two on an SM, 58 by 2 alone.
+    double best = 0.0;
+    *ctas = 0;
+    for (int n = 8; n >= 1; n /= 2) {
+        const LoraStreamPlan p = lora_stream_plan(a.pass_targets, a.rank, (units + n - 1) / n * 32, S::PX, S::PH);
+        if (!p.fits) break;
+        const bool two = p.bytes <= LS_BYTES;
+        const int64_t clusters = (int64_t)a.items * passes * n, places = two ? 2 * 148 : 148;
+        const double cost = (double)((clusters + places - 1) / places) * (10.0 + 1e-3 * bytes / n / (two ? 22.0 : 30.0));
+        if (*ctas != 0 && cost >= best) continue;
+        best = cost;
+        *ctas = n;
+        *plan = p;
+    }
+    return *ctas != 0 && bytes / *ctas > 24 * 1024;
+}
+template <int TX, int TW>
+int32_t launch_lora_stream(cudaStream_t st, const LoraArgs &a, int passes, int ctas, const LoraStreamPlan &plan) {
+    auto kernel = lora_stream_kernel<TX, TW>;
+    static std::atomic<uint64_t> allowed{0};
+    NC_TRY(allow_smem_once(kernel, LS_BYTES_ALONE, &allowed));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * ctas), (unsigned)passes);
+    cfg.blockDim = LS_THREADS;
+    cfg.dynamicSmemBytes = plan.bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, plan));
+    return check_launch("lora_stream_kernel");
+}
 template <int TX, int TW>
 int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes) {
+    if (a.tile == 8) {
+        int ctas;
+        LoraStreamPlan plan;
+        if (lora_stream_shape<TX, TW>(a, passes, &ctas, &plan)) return launch_lora_stream<TX, TW>(st, a, passes, ctas, plan);
+    }
     return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : a.tile == 16 ? launch_lora<TX, TW, 2>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
 }
 // For items of 128 rows.
