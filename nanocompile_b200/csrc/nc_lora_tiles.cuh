@@ -8,9 +8,9 @@
 // memory, a row to a thread, and store it, whole rows to half a warp; four others have the next tile.  The targets' h lie side by side,
 // whole 16s to each.
 //
-// Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (16 bits and the next 16: bfloat16 2^-17 of it is
-// lost, float16 2^-22; float16's h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its
-// range).  Sums are float32 in tensor memory.
+// Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-18 of it is lost, float16 2^-24; float16's
+// h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its range).  float32 rows and their h go
+// in three bfloat16 parts (2^-27 is lost), float16 weights beside them in two, which are exact.  Sums are float32 in tensor memory.
 #pragma once
 
 #include "nc_kv4_prompt.cuh"
@@ -29,35 +29,38 @@ constexpr int LT_SLOTS = 4;                    // tiles of base on their way or 
 
 __device__ unsigned int g_lora_fault;          // set when a matrix instruction did not come to its end within the wait limit
 
-template <int TX>
+template <int TX, int TW>
 struct LoraTiles {
-    static constexpr int PH = 2;                                       // parts of h
-    static constexpr int COLS = TX == KV_F32 ? 64 : 128;               // outputs of a tile
-    static constexpr int SIZE = TX == KV_F32 ? 4 : 2;
+    static constexpr bool F32 = TX == KV_F32;
+    static constexpr int T = F32 ? (int)KV_BF16 : TX;                  // of the operands
+    static constexpr int PX = F32 ? 3 : 1, PW = F32 && TW == KV_F16 ? 2 : 1, PH = F32 ? 3 : 2;   // parts of x, of weights, of h
+    static constexpr int COLS = F32 ? 64 : 128;                        // outputs of a tile
+    static constexpr int SIZE = F32 ? 4 : 2;
 };
 
 // How shared memory is laid out, by the most rows of h in a pass: h's operand, then the sums of h; over these two tiles of B and the
 // slots of base; over all of it the stages of the first products.
 struct LoraTilesPlan {
     int wide;                                  // rows of h in whole 16s
-    int stages, a_bytes;                       // of a stage: LT_BLOCK for rows, a_bytes for A
+    int stages, a_bytes;                       // of a stage: LT_BLOCK for a part of the rows, a_bytes for one of A
     int h_blocks, b_blocks;                    // blocks of 32 for a part of h, for B
     int sum_at, slot_at, slots, bytes;
 };
-inline LoraTilesPlan lora_tiles_plan(int targets, int rank, int parts, int cols) {
+template <typename S>
+inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
     LoraTilesPlan p{};
     p.wide = targets * ((rank + 15) / 16 * 16);
     p.a_bytes = p.wide * 128;
     p.h_blocks = (p.wide + 31) / 32;
     p.b_blocks = (rank + 31) / 32;
-    p.sum_at = parts * p.h_blocks * LT_HALF;
-    p.slot_at = p.sum_at + 2 * p.b_blocks * cols * 64;
+    p.sum_at = S::PH * p.h_blocks * LT_HALF;
+    p.slot_at = p.sum_at + 2 * S::PW * p.b_blocks * S::COLS * 64;
     // Two or four, that a slot is always the same warps': they wait for every second tile only, and would take the round of a slot's
     // barrier before the one that they wait for, of the same parity, for that.
     p.slots = (LT_BYTES - p.slot_at) / LT_SLOT / 2 * 2;
     if (p.slots > LT_SLOTS) p.slots = LT_SLOTS;
     p.bytes = p.slot_at + p.slots * LT_SLOT;
-    const int sums = p.sum_at + (LT_ROWS + 12) * (p.wide + 4) * 4, stage = LT_BLOCK + p.a_bytes;  // the last CTA's share may be shorter
+    const int sums = p.sum_at + (LT_ROWS + 12) * (p.wide + 4) * 4, stage = S::PX * LT_BLOCK + S::PW * p.a_bytes;  // the last CTA's share may be shorter
     if (sums > p.bytes) p.bytes = sums;
     p.stages = LT_BYTES / stage < LT_STAGES ? LT_BYTES / stage : LT_STAGES;
     if (p.stages * stage > p.bytes) p.bytes = p.stages * stage;
@@ -143,9 +146,13 @@ __device__ __forceinline__ uint32_t lt_part(float2 &v) {
     v.y = fsub(v.y, r.y);
     return w;
 }
-// Eight outputs from 16 bytes of base and float32 sums.
+// 16 bytes of outputs from those of base and float32 sums.
 template <int TX>
-__device__ __forceinline__ uint4 lt_add(const uint4 &was, const float (&v)[8], float scale) {
+__device__ __forceinline__ uint4 lt_add(const uint4 &was, const uint32_t *sums, float scale) {
+    const float *const v = reinterpret_cast<const float *>(sums);
+    if constexpr (TX == KV_F32)
+        return make_uint4(__float_as_uint(__fmaf_rn(scale, v[0], __uint_as_float(was.x))), __float_as_uint(__fmaf_rn(scale, v[1], __uint_as_float(was.y))),
+                          __float_as_uint(__fmaf_rn(scale, v[2], __uint_as_float(was.z))), __float_as_uint(__fmaf_rn(scale, v[3], __uint_as_float(was.w))));
     const uint32_t u[4] = {was.x, was.y, was.z, was.w};
     uint32_t w[4];
 #pragma unroll
@@ -163,9 +170,37 @@ __device__ __forceinline__ uint4 lt_add(const uint4 &was, const float (&v)[8], f
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int TX>
+// What a worker has of a block of float32 rows, and of float16 weights beside them.
+struct LtBlock {
+    float4 x[8];
+    uint4 w[LORA_PASS / 32];
+};
+// The products of parts that count: of p + q up to the third.
+template <int P, int Q, typename F>
+__device__ __forceinline__ void lt_parts(F use) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (p + q < 3) use(p, q);
+}
+// Eight float16 weights in two bfloat16 parts, which hold them exactly.
+__device__ __forceinline__ void lt_two_parts(const uint4 &w, uint4 *high, uint4 *low) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        h[i] = lt_part<KV_BF16>(f);
+        l[i] = lt_part<KV_BF16>(f);
+    }
+    *high = make_uint4(h[0], h[1], h[2], h[3]);
+    *low = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <int TX, int TW>
 __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraTilesPlan plan) {
-    using S = LoraTiles<TX>;
+    using S = LoraTiles<TX, TW>;
     extern __shared__ __align__(1024) char lt_raw[];
     char *const tiles = lt_raw + ((1024 - (kvt_smem(lt_raw) & 1023)) & 1023);
     __shared__ LoraTilesShared sh;
@@ -228,16 +263,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         g_lora_fault = 1;
         return false;
     };
-    const int stage_bytes = LT_BLOCK + plan.a_bytes, c = tid & 7, line = tid >> 3;               // a worker's 16 bytes of every 32nd row
+    const int stage_bytes = S::PX * LT_BLOCK + S::PW * plan.a_bytes, c = tid & 7, line = tid >> 3;             // a worker's 16 bytes of every 32nd row
 
     // h, in parts: D1 = x A^T over this CTA's inputs.
     if (worker) {
-        const char *x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = sh.row[line + 32 * i];
-            x[i] = row < 0 ? nullptr : (const char *)a.x + (int64_t)row * a.x_stride * 2;
-        }
         int from[LORA_PASS / 32];                                      // of A's rows; -1: none there
 #pragma unroll
         for (int i = 0; i < LORA_PASS / 32; ++i) {
@@ -245,37 +274,116 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             from[i] = j < wide && j - t * rp < r ? (t * a.rank + j - t * rp) * a.inputs : -1;
         }
         const uint32_t swizzled = (uint32_t)line * 128 + (uint32_t)((c ^ (line & 7)) << 4);
-        auto issue = [&](int k) {
-            const uint32_t to = base_at + (uint32_t)(k % plan.stages) * stage_bytes + swizzled;
+        auto ask_a = [&](int k) {
+            const uint32_t to = base_at + (uint32_t)(k % plan.stages) * stage_bytes + S::PX * LT_BLOCK + swizzled;
             const int e = (k_low + k) * 64 + 8 * c;
-            const bool in = e < a.inputs;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lt_copy16(to + i * 4096, in && x[i] ? x[i] + e * 2 : a.x, in && x[i] ? 16 : 0);
-#pragma unroll
-            for (int i = 0; i < LORA_PASS / 32; ++i)
-                if (line + 32 * i < wide) lt_copy16(to + LT_BLOCK + i * 4096, in && from[i] >= 0 ? wa + (int64_t)(from[i] + e) * 2 : wa, in && from[i] >= 0 ? 16 : 0);
+            for (int i = 0; i < LORA_PASS / 32; ++i) {
+                const bool there = e < a.inputs && from[i] >= 0;
+                if (line + 32 * i < wide) lt_copy16(to + i * 4096, there ? wa + (int64_t)(from[i] + e) * 2 : wa, there ? 16 : 0);
+            }
         };
-        // A stage is asked for again when the products two blocks back are done with it, not those just begun.
-        const int ahead = max(1, plan.stages - 2);
-        for (int k = 0; k < ahead; ++k) {
-            if (k < k_blocks) issue(k);
-            lt_commit();
-        }
-        for (int k = 0; k < k_blocks; ++k) {
-            const int next = k + ahead;
-            if (next < k_blocks) {
-                if (next >= plan.stages) wait(&sh.empty[next % plan.stages], (next / plan.stages - 1) & 1);
-                issue(next);
+        if constexpr (!S::F32) {
+            const char *x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = sh.row[line + 32 * i];
+                x[i] = row < 0 ? nullptr : (const char *)a.x + (int64_t)row * a.x_stride * 2;
             }
-            lt_commit();
-            switch (ahead) {                                           // the oldest of `ahead` + 1 groups is there
-                case 1: lt_wait_copies<1>(); break;
-                case 2: lt_wait_copies<2>(); break;
-                case 3: lt_wait_copies<3>(); break;
-                default: lt_wait_copies<4>(); break;
+            auto issue = [&](int k) {
+                const uint32_t to = base_at + (uint32_t)(k % plan.stages) * stage_bytes + swizzled;
+                const int e = (k_low + k) * 64 + 8 * c;
+                const bool in = e < a.inputs;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lt_copy16(to + i * 4096, in && x[i] ? x[i] + e * 2 : a.x, in && x[i] ? 16 : 0);
+                ask_a(k);
+            };
+            // A stage is asked for again when the products two blocks back are done with it, not those just begun.
+            const int ahead = max(1, plan.stages - 2);
+            for (int k = 0; k < ahead; ++k) {
+                if (k < k_blocks) issue(k);
+                lt_commit();
             }
-            lt_async_fence();
-            lt_arrive(&sh.full[k % plan.stages]);
+            for (int k = 0; k < k_blocks; ++k) {
+                const int next = k + ahead;
+                if (next < k_blocks) {
+                    if (next >= plan.stages) wait(&sh.empty[next % plan.stages], (next / plan.stages - 1) & 1);
+                    issue(next);
+                }
+                lt_commit();
+                switch (ahead) {                                       // the oldest of `ahead` + 1 groups is there
+                    case 1: lt_wait_copies<1>(); break;
+                    case 2: lt_wait_copies<2>(); break;
+                    case 3: lt_wait_copies<3>(); break;
+                    default: lt_wait_copies<4>(); break;
+                }
+                lt_async_fence();
+                lt_arrive(&sh.full[k % plan.stages]);
+            }
+        } else {
+            // float32 rows go through registers, a block ahead: four values of every 16th row to a thread, split into parts on the way.
+            const int c4 = tid & 15, line4 = tid >> 4;
+            auto load = [&](int k, LtBlock &block) {
+                const int e = (k_low + k) * 64 + 4 * c4;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = sh.row[line4 + 16 * i];
+                    block.x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (row >= 0 && e < a.inputs) block.x[i] = __ldg((const float4 *)((const float *)a.x + (int64_t)row * a.x_stride + e));
+                }
+                if constexpr (S::PW == 1) {
+                    ask_a(k);
+                } else {
+                    const int ea = (k_low + k) * 64 + 8 * c;
+#pragma unroll
+                    for (int i = 0; i < LORA_PASS / 32; ++i) {
+                        block.w[i] = make_uint4(0, 0, 0, 0);
+                        if (from[i] >= 0 && ea < a.inputs) block.w[i] = __ldg((const uint4 *)(wa + (int64_t)(from[i] + ea) * 2));
+                    }
+                }
+                lt_commit();
+            };
+            auto store = [&](int k, const LtBlock &block) {
+                const uint32_t at = base_at + (uint32_t)(k % plan.stages) * stage_bytes;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = line4 + 16 * i;
+                    const uint32_t to = at + (uint32_t)row * 128 + (uint32_t)(((c4 >> 1) ^ (row & 7)) << 4) + (uint32_t)(c4 & 1) * 8;
+                    float2 x = make_float2(block.x[i].x, block.x[i].y), y = make_float2(block.x[i].z, block.x[i].w);
+#pragma unroll
+                    for (int p = 0; p < S::PX; ++p)
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + p * LT_BLOCK), "r"(lt_part<KV_BF16>(x)), "r"(lt_part<KV_BF16>(y)) : "memory");
+                }
+                if constexpr (S::PW == 2) {
+#pragma unroll
+                    for (int i = 0; i < LORA_PASS / 32; ++i) {
+                        if (line + 32 * i >= wide) continue;
+                        uint4 high, low;
+                        lt_two_parts(block.w[i], &high, &low);
+                        const uint32_t to = at + S::PX * LT_BLOCK + swizzled + i * 4096;
+                        store16_shared(to, high.x, high.y, high.z, high.w);
+                        store16_shared(to + plan.a_bytes, low.x, low.y, low.z, low.w);
+                    }
+                }
+            };
+            auto step = [&](int k, const LtBlock &now, LtBlock &next) {
+                if (k + 1 < k_blocks) {
+                    if (k + 1 >= plan.stages) wait(&sh.empty[(k + 1) % plan.stages], ((k + 1) / plan.stages - 1) & 1);
+                    load(k + 1, next);
+                } else {
+                    lt_commit();
+                }
+                store(k, now);
+                lt_wait_copies<1>();
+                lt_async_fence();
+                lt_arrive(&sh.full[k % plan.stages]);
+            };
+            LtBlock even, odd;
+            if (k_blocks > 0) load(0, even);
+            for (int k = 0; k < k_blocks; k += 2) {
+                step(k, even, odd);
+                if (k + 1 < k_blocks) step(k + 1, odd, even);
+            }
         }
         lt_wait_copies<0>();
     } else if (warp == LT_MMA && lane == 0) {
@@ -285,7 +393,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             kvt_after();
             const uint32_t at = base_at + (uint32_t)stage * stage_bytes;
             const int steps = min(4, (a.inputs - (k_low + k) * 64 + 15) / 16);
-            for (int s = 0; s < steps; ++s) lt_mma<TX>(tmem, kvt_desc(at + 32 * s), kvt_desc(at + LT_BLOCK + 32 * s), wide, k > 0 || s > 0);
+            for (int s = 0; s < steps; ++s)
+                lt_parts<S::PX, S::PW>([&](int p, int q) {
+                    lt_mma<S::T>(tmem, kvt_desc(at + p * LT_BLOCK + 32 * s), kvt_desc(at + S::PX * LT_BLOCK + q * plan.a_bytes + 32 * s), wide, k > 0 || s > 0 || p > 0 || q > 0);
+                });
             kvt_commit(&sh.empty[stage]);
         }
         kvt_commit(&sh.d1_done);
@@ -361,7 +472,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 if (!(keep >> (4 * m) & 4)) continue;
 #pragma unroll
                 for (int p = 0; p < S::PH; ++p)
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<TX>(v[m])) : "memory");
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<S::T>(v[m])) : "memory");
             }
         }
         lt_async_fence();
@@ -396,7 +507,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         }
         return (tile_low + i - tile0) * S::COLS;                       // the tile's first output of its target
     };
-    const int b_bytes = plan.b_blocks * S::COLS * 64;
+    const int b_part = plan.b_blocks * S::COLS * 64, b_bytes = S::PW * b_part;
     const bool staged = a.wide != 0;
     if (warp > LT_MMA) {
         // B's rows in blocks of 32, 64 bytes each, 16 of every 32nd row to a thread; base's rows, 16 bytes of every eighth to a thread.
@@ -408,14 +519,21 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                     const uint32_t dst = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
                     const char *const from = wb + (((int64_t)n_target + n0 + n) * a.rank + j) * 2;
                     const bool there = n0 + n < a.width[target];
-                    if (j + 8 <= r || j >= r || !there) {
+                    if (S::PW == 1 && (j + 8 <= r || j >= r || !there)) {
                         lt_copy16(dst, there && j < r ? from : wb, there && j < r ? 16 : 0);
                     } else {                                           // what lies past the adapter's own rank may be anything
-                        const uint4 w = __ldg((const uint4 *)from);
+                        const uint4 w = there && j < r ? __ldg((const uint4 *)from) : make_uint4(0, 0, 0, 0);
                         uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) u[e] = j + 2 * e >= r ? 0u : j + 2 * e + 1 >= r ? u[e] & 0xffffu : u[e];
-                        store16_shared(dst, u[0], u[1], u[2], u[3]);
+                        if constexpr (S::PW == 1) {
+                            store16_shared(dst, u[0], u[1], u[2], u[3]);
+                        } else {
+                            uint4 high, low;
+                            lt_two_parts(make_uint4(u[0], u[1], u[2], u[3]), &high, &low);
+                            store16_shared(dst, high.x, high.y, high.z, high.w);
+                            store16_shared(dst + b_part, low.x, low.y, low.z, low.w);
+                        }
                     }
                 }
             lt_commit();
@@ -460,12 +578,13 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 kvt_after();
                 const uint32_t b = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
                 bool add = false;
-                for (int p = 0; p < S::PH; ++p)
+                lt_parts<S::PH, S::PW>([&](int p, int q) {
                     for (int j = 0; j < rp; j += 16, add = true) {
                         const int at = (target - t0) * rp + j;
-                        lt_mma<TX>(tmem + (uint32_t)(i & 1) * 128, lt_desc64(base_at + (uint32_t)(p * plan.h_blocks + (at >> 5)) * LT_HALF + (uint32_t)(at & 31) * 2),
-                                   lt_desc64(b + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)(j & 31) * 2), S::COLS, add);
+                        lt_mma<S::T>(tmem + (uint32_t)(i & 1) * 128, lt_desc64(base_at + (uint32_t)(p * plan.h_blocks + (at >> 5)) * LT_HALF + (uint32_t)(at & 31) * 2),
+                                     lt_desc64(b + q * b_part + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)(j & 31) * 2), S::COLS, add);
                     }
+                });
                 kvt_commit(&sh.d2_done[i & 1]);
             }
             kvt_commit(&sh.drained);
@@ -476,6 +595,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         if constexpr (TX == KV_F16) wait(&sh.h_full, 0);               // the rows' scales
         const int at = 32 * (warp & 3) + lane, row = sh.row[at], half = warp >> 2, cc = lane & 15, cl = lane >> 4;
         const float by = TX == KV_F16 ? scale * sh.row_scale[at] : scale;
+        constexpr int STEP = 16 / S::SIZE;                             // outputs of 16 bytes
         const uint32_t d2 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)half * 128;
         for (int i = half; i < my_tiles; i += 2) {
             const int n0 = look_up(i), left = min(S::COLS, a.width[target] - n0), n = n_target + n0, slot_i = i % plan.slots;
@@ -495,16 +615,15 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 }
                 if (row < 0 || m >= left) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    const float f[8] = {__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]),
-                                        __uint_as_float(v[e + 4]), __uint_as_float(v[e + 5]), __uint_as_float(v[e + 6]), __uint_as_float(v[e + 7])};
-                    if (staged && m + e + 8 <= left) {
+                for (int e = 0; e < 32; e += STEP) {
+                    if (staged && m + e + STEP <= left) {
                         uint4 *const was = (uint4 *)(slot_line + (m + e) * S::SIZE);
-                        *was = lt_add<TX>(a.base ? *was : make_uint4(0, 0, 0, 0), f, by);
+                        *was = lt_add<TX>(a.base ? *was : make_uint4(0, 0, 0, 0), v + e, by);
                     } else {
                         const int64_t to = (int64_t)row * a.out_stride + n + m + e, was = (int64_t)row * a.base_stride + n + m + e;
-                        for (int k = 0; k < min(8, left - m - e); ++k)
-                            kv_store(a.out, to + k, TX, __fmaf_rn(by, f[k], a.base ? kv_load(a.base, was + k, TX) : 0.0f));
+#pragma unroll
+                        for (int k = 0; k < STEP; ++k)
+                            if (m + e + k < left) kv_store(a.out, to + k, TX, __fmaf_rn(by, __uint_as_float(v[e + k]), a.base ? kv_load(a.base, was + k, TX) : 0.0f));
                     }
                 }
             }

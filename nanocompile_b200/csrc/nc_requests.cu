@@ -126,25 +126,20 @@ int32_t launch_lora_stream(cudaStream_t st, const LoraArgs &a, int passes, int c
     CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, plan));
     return check_launch("lora_stream_kernel");
 }
+// For items of 128 rows.  False where shared memory is too small for the rank (float16 adapters above 96 beside float32 rows).
 template <int TX, int TW>
-int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes) {
-    if (a.tile == 8) {
-        int ctas;
-        LoraStreamPlan plan;
-        if (lora_stream_shape<TX, TW>(a, passes, &ctas, &plan)) return launch_lora_stream<TX, TW>(st, a, passes, ctas, plan);
-    }
-    return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : a.tile == 16 ? launch_lora<TX, TW, 2>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
+bool lora_tiles_shape(LoraArgs *a, LoraTilesPlan *plan) {
+    using S = LoraTiles<TX, TW>;
+    a->pass_targets = std::min(a->targets, std::max(1, LORA_PASS / ((a->rank + 15) / 16 * 16)));
+    *plan = lora_tiles_plan<S>(a->pass_targets, a->rank);
+    while ((plan->slots < 2 || plan->stages < 2) && a->pass_targets > 1) *plan = lora_tiles_plan<S>(--a->pass_targets, a->rank);
+    return plan->slots >= 2 && plan->stages >= 2;
 }
-// For items of 128 rows.
-template <int TX>
-int32_t launch_lora_tiles(cudaStream_t st, LoraArgs a) {
-    using S = LoraTiles<TX>;
-    auto kernel = lora_tiles_kernel<TX>;
+template <int TX, int TW>
+int32_t launch_lora_tiles(cudaStream_t st, const LoraArgs &a, const LoraTilesPlan &plan) {
+    auto kernel = lora_tiles_kernel<TX, TW>;
     static std::atomic<uint64_t> allowed{0};
     NC_TRY(allow_smem_once(kernel, LT_BYTES + 1024, &allowed));
-    a.pass_targets = std::min(a.targets, std::max(1, LORA_PASS / ((a.rank + 15) / 16 * 16)));
-    LoraTilesPlan plan = lora_tiles_plan(a.pass_targets, a.rank, S::PH, S::COLS);
-    while (plan.slots < 2 && a.pass_targets > 1) plan = lora_tiles_plan(--a.pass_targets, a.rank, S::PH, S::COLS);
     const int passes = (a.targets + a.pass_targets - 1) / a.pass_targets;
     const size_t bytes = (size_t)plan.bytes + 1024;
     const int ctas = (int)std::clamp<int64_t>(148 / ((int64_t)a.items * passes), 1, 8);          // one on an SM
@@ -164,9 +159,24 @@ int32_t launch_lora_tiles(cudaStream_t st, LoraArgs a) {
     CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, plan));
     return check_launch("lora_tiles_kernel");
 }
+template <int TX, int TW>
+int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes, bool tiles) {
+    if constexpr (TX == TW || TX == KV_F32)
+        if (tiles) {
+            LoraArgs t = a;
+            LoraTilesPlan plan;
+            if (lora_tiles_shape<TX, TW>(&t, &plan)) return launch_lora_tiles<TX, TW>(st, t, plan);
+        }
+    if (a.tile == 8) {
+        int ctas;
+        LoraStreamPlan plan;
+        if (lora_stream_shape<TX, TW>(a, passes, &ctas, &plan)) return launch_lora_stream<TX, TW>(st, a, passes, ctas, plan);
+    }
+    return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
+}
 template <int TX>
-int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes) {
-    return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes) : launch_lora_n<TX, KV_BF16>(st, a, passes);
+int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes, bool tiles) {
+    return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes, tiles) : launch_lora_n<TX, KV_BF16>(st, a, passes, tiles);
 }
 
 }  // namespace
@@ -278,9 +288,8 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     const int passes = (int)((targets + a.pass_targets - 1) / a.pass_targets);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool tiles = a.tile == LT_ROWS && a.x_vectors && targets * rank * inputs <= I32;
-    if (tiles && type == KV_BF16 && wtype == KV_BF16) return launch_lora_tiles<KV_BF16>(st, a);
-    if (tiles && type == KV_F16 && wtype == KV_F16) return launch_lora_tiles<KV_F16>(st, a);
-    return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes) : launch_lora_w<KV_BF16>(st, a, passes);
+    return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes, tiles) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes, tiles)
+                                                                                         : launch_lora_w<KV_BF16>(st, a, passes, tiles);
 }
 
 // ---- beams --------------------------------------------------------------------------------------
