@@ -38,13 +38,14 @@ struct LoraTiles {
     static constexpr int SIZE = F32 ? 4 : 2;
 };
 
-// How shared memory is laid out, by the most rows of h in a pass: h's operand, then the sums of h; over these two tiles of B and the
-// slots of base; over all of it the stages of the first products.
+// How shared memory is laid out, by the most rows of h in a pass: h's operand, two tiles of B, the slots of base; over these the stages of
+// the first products.  Where there is room the sums of h lie past the stages and the first two slots (`early`): then they may come while
+// a CTA is still at its stages, and the first tiles of B and base while they are added up.  Else they lie over B and the slots.
 struct LoraTilesPlan {
     int wide;                                  // rows of h in whole 16s
     int stages, a_bytes;                       // of a stage: LT_BLOCK for a part of the rows, a_bytes for one of A
     int h_blocks, b_blocks;                    // blocks of 32 for a part of h, for B
-    int sum_at, slot_at, slots, bytes;
+    int b_at, slot_at, slots, sum_at, early, bytes;
 };
 template <typename S>
 inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
@@ -53,16 +54,20 @@ inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
     p.a_bytes = p.wide * 128;
     p.h_blocks = (p.wide + 31) / 32;
     p.b_blocks = (rank + 31) / 32;
-    p.sum_at = S::PH * p.h_blocks * LT_HALF;
-    p.slot_at = p.sum_at + 2 * S::PW * p.b_blocks * S::COLS * 64;
+    p.b_at = S::PH * p.h_blocks * LT_HALF;
+    p.slot_at = p.b_at + 2 * S::PW * p.b_blocks * S::COLS * 64;
     // Two or four, that a slot is always the same warps': they wait for every second tile only, and would take the round of a slot's
     // barrier before the one that they wait for, of the same parity, for that.
     p.slots = (LT_BYTES - p.slot_at) / LT_SLOT / 2 * 2;
     if (p.slots > LT_SLOTS) p.slots = LT_SLOTS;
     p.bytes = p.slot_at + p.slots * LT_SLOT;
-    const int sums = p.sum_at + (LT_ROWS + 12) * (p.wide + 4) * 4, stage = S::PX * LT_BLOCK + S::PW * p.a_bytes;  // the last CTA's share may be shorter
-    if (sums > p.bytes) p.bytes = sums;
-    p.stages = LT_BYTES / stage < LT_STAGES ? LT_BYTES / stage : LT_STAGES;
+    const int sums = (LT_ROWS + 12) * (p.wide + 4) * 4, stage = S::PX * LT_BLOCK + S::PW * p.a_bytes;            // the last CTA's share may be shorter
+    p.sum_at = p.slot_at + 2 * LT_SLOT;
+    p.early = p.sum_at + sums <= LT_BYTES && 2 * stage <= p.sum_at;
+    if (!p.early) p.sum_at = p.b_at;
+    if (p.sum_at + sums > p.bytes) p.bytes = p.sum_at + sums;
+    const int room = p.early ? p.sum_at : LT_BYTES;
+    p.stages = room / stage < LT_STAGES ? room / stage : LT_STAGES;
     if (p.stages * stage > p.bytes) p.bytes = p.stages * stage;
     return p;
 }
@@ -218,14 +223,16 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         if (t < t0) n_first += a.width[t];
         else n_pass += a.width[t], n_tiles += (a.width[t] + S::COLS - 1) / S::COLS;
     }
-    const int r = slot < 0 ? 0 : a.ranks ? min(max(a.ranks[slot], 0), a.rank) : a.rank;
+    // What depends on the item is asked for together.
+    const int my_row = tid < count ? (int)lora_row(a, order, first + tid) : -1, rank = a.ranks ? a.ranks[max(slot, 0)] : a.rank;
+    const float scale = a.scales ? a.scales[max(slot, 0)] : 1.0f;
+    const int r = slot < 0 ? 0 : min(max(rank, 0), a.rank);
     if (r == 0) {
         const int64_t n = n_pass;
         lora_copy<TX>(a, order, first, count, n_first + (int)(n * cta / ctas), n_first + (int)(n * (cta + 1) / ctas));
         return;
     }
     const int rp = (r + 15) / 16 * 16, wide = (t1 - t0) * rp;
-    const float scale = a.scales ? a.scales[slot] : 1.0f;
     const char *const wa = (const char *)a.a + ((int64_t)slot * a.targets + t0) * a.rank * a.inputs * 2;
     const char *const wb = (const char *)a.b + (int64_t)slot * a.outputs * a.rank * 2;
     const int tile_low = (int)((int64_t)n_tiles * cta / ctas), tile_high = (int)((int64_t)n_tiles * (cta + 1) / ctas), my_tiles = tile_high - tile_low;
@@ -249,11 +256,12 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < LT_ROWS) sh.row[tid] = tid < count ? (int)lora_row(a, order, first + tid) : -1;
+    if (tid < LT_ROWS) sh.row[tid] = my_row;
     kvt_before();
     __syncthreads();
     kvt_after();
     release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
+    if (plan.early) lora_cluster_arrive();     // this CTA is there: peers may write to its shared memory
     const uint32_t tmem = sh.tmem, base_at = kvt_smem(tiles);
     const long long limit = g_wait_cycles;
     // A wait that runs out is the last one: the CTA goes on without waiting and its outputs are not to be used.
@@ -404,7 +412,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     __syncwarp();
     wait(&sh.d1_done, 0);
     kvt_after();
-    lora_cluster_arrive();                     // every CTA is done with its stages: sums may lie over them
+    __syncwarp();
+    if (!plan.early) lora_cluster_arrive();    // this CTA is done with its stages: sums may lie over them
     lora_cluster_wait();
     const int mine = (LT_ROWS / 4 + ctas - 1) / ctas * 4, pitch = plan.wide + 4;     // rows that a CTA adds up; the last one's may be fewer
     if (worker) {
@@ -426,8 +435,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         }
     }
     kvt_before();
+    __syncwarp();
     lora_cluster_arrive();
-    lora_cluster_wait();
+    if (warp <= LT_MMA) lora_cluster_wait();   // those that load go on
     kvt_after();
     if (worker) {
         // A row to a warp, two columns of every 64 to a lane.
@@ -438,46 +448,65 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             const int col = 64 * m + 2 * lane, j = col % rp;
             if (col < wide) keep |= (uint32_t)((j < r) | (j + 1 < r) << 1 | 4) << (4 * m);
         }
-        for (int i = warp; i < min(mine, LT_ROWS - cta * mine); i += LT_WARPS) {
-            const int row = cta * mine + i;
-            float2 v[LORA_PASS / 64];
-            float most = 0.0f;
+        // Four rows at a time, that their loads do not wait for one another.
+        constexpr int M = LORA_PASS / 64, R = 4;
+        const int rows = min(mine, LT_ROWS - cta * mine);
+        for (int i0 = warp; i0 < rows; i0 += R * LT_WARPS) {
+            float2 v[R][M];
 #pragma unroll
-            for (int m = 0; m < LORA_PASS / 64; ++m) {
-                v[m] = make_float2(0.0f, 0.0f);
-                if (!(keep >> (4 * m) & 4)) continue;
-                for (int k = 0; k < ctas; ++k) {
-                    const float2 p = *(const float2 *)(sums + (k * mine + i) * pitch + 64 * m);
-                    v[m].x = fadd(v[m].x, p.x);
-                    v[m].y = fadd(v[m].y, p.y);
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int m = 0; m < M; ++m) v[u][m] = make_float2(0.0f, 0.0f);
+            for (int k = 0; k < ctas; ++k)
+#pragma unroll
+                for (int u = 0; u < R; ++u) {
+                    const int i = min(i0 + u * LT_WARPS, rows - 1);
+#pragma unroll
+                    for (int m = 0; m < M; ++m) {
+                        if (!(keep >> (4 * m) & 4)) continue;
+                        const float2 p = *(const float2 *)(sums + (k * mine + i) * pitch + 64 * m);
+                        v[u][m].x = fadd(v[u][m].x, p.x);
+                        v[u][m].y = fadd(v[u][m].y, p.y);
+                    }
                 }
-                if (!(keep >> (4 * m) & 1)) v[m].x = 0.0f;
-                if (!(keep >> (4 * m) & 2)) v[m].y = 0.0f;
-                most = fmaxf(most, fmaxf(fabsf(v[m].x), fabsf(v[m].y)));
-            }
-            if constexpr (TX == KV_F16) {
-                const uint32_t exponent = __reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23;
-                float back = 1.0f;
-                if (exponent > 20 && exponent < 255) {                 // 2^14 <= most * 2^(141 - exponent) < 2^15
-                    const float to = __uint_as_float((268 - exponent) << 23);
-                    back = __uint_as_float((exponent - 14) << 23);
 #pragma unroll
-                    for (int m = 0; m < LORA_PASS / 64; ++m) v[m].x = fmul(v[m].x, to), v[m].y = fmul(v[m].y, to);
+            for (int u = 0; u < R; ++u) {
+                if (i0 + u * LT_WARPS >= rows) break;
+                const int row = cta * mine + i0 + u * LT_WARPS;
+                float most = 0.0f;
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    if (!(keep >> (4 * m) & 1)) v[u][m].x = 0.0f;
+                    if (!(keep >> (4 * m) & 2)) v[u][m].y = 0.0f;
+                    most = fmaxf(most, fmaxf(fabsf(v[u][m].x), fabsf(v[u][m].y)));
                 }
-                if (lane == 0) sh.row_scale[row] = back;
-            }
-            const uint32_t at = base_at + (uint32_t)(lane >> 4) * LT_HALF + (uint32_t)row * 64 + (uint32_t)(((lane >> 2 & 3) ^ ((row >> 1) & 3)) << 4) + (uint32_t)(lane & 3) * 4;
+                if constexpr (TX == KV_F16) {
+                    const uint32_t exponent = __reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23;
+                    float back = 1.0f;
+                    if (exponent > 20 && exponent < 255) {             // 2^14 <= most * 2^(141 - exponent) < 2^15
+                        const float to = __uint_as_float((268 - exponent) << 23);
+                        back = __uint_as_float((exponent - 14) << 23);
 #pragma unroll
-            for (int m = 0; m < LORA_PASS / 64; ++m) {
-                if (!(keep >> (4 * m) & 4)) continue;
+                        for (int m = 0; m < M; ++m) v[u][m].x = fmul(v[u][m].x, to), v[u][m].y = fmul(v[u][m].y, to);
+                    }
+                    if (lane == 0) sh.row_scale[row] = back;
+                }
+                const uint32_t at = base_at + (uint32_t)(lane >> 4) * LT_HALF + (uint32_t)row * 64 + (uint32_t)(((lane >> 2 & 3) ^ ((row >> 1) & 3)) << 4) + (uint32_t)(lane & 3) * 4;
 #pragma unroll
-                for (int p = 0; p < S::PH; ++p)
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<S::T>(v[m])) : "memory");
+                for (int m = 0; m < M; ++m) {
+                    if (!(keep >> (4 * m) & 4)) continue;
+#pragma unroll
+                    for (int p = 0; p < S::PH; ++p)
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<S::T>(v[u][m])) : "memory");
+                }
             }
         }
         lt_async_fence();
     }
-    if (warp != LT_MMA) asm volatile("bar.sync 1, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");       // h's rows of this CTA are there, the sums read
+    if (worker) {
+        asm volatile("bar.sync 1, %0;" ::"n"(LT_WORKERS) : "memory");  // h's rows of this CTA are there, and the sums read:
+        asm volatile("bar.arrive 2, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");             // what lies over them may come
+    }
     if (warp == 0) {
         // To each peer this CTA's rows of every block, 64 bytes each, and their scales: one bulk copy a lane.
         const int from_row = cta * mine, rows = min(mine, LT_ROWS - from_row), used = (wide + 31) / 32, per = S::PH * used + (TX == KV_F16);
@@ -513,7 +542,17 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         // B's rows in blocks of 32, 64 bytes each, 16 of every 32nd row to a thread; base's rows, 16 bytes of every eighth to a thread.
         const int at = tid - LT_WORKERS - 32, bc = at & 3, bl = at >> 2, cc = at & 15, cl = at >> 4;
         auto issue_b = [&](int i, int n0) {
-            const uint32_t to = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
+            const uint32_t to = base_at + plan.b_at + (uint32_t)(i & 1) * b_bytes;
+            if (S::PW == 1 && r == rp && n0 + S::COLS <= a.width[target]) {
+                const char *const from = wb + (((int64_t)n_target + n0 + bl) * a.rank + 8 * bc) * 2;
+                const uint32_t dst = to + (uint32_t)bl * 64 + (uint32_t)((bc ^ ((bl >> 1) & 3)) << 4);     // the same for every 32nd row
+                for (int j = 0; 8 * bc + j < rp; j += 32)
+#pragma unroll
+                    for (int n = 0; n < S::COLS; n += LT_LOADERS / 4)
+                        lt_copy16(dst + (uint32_t)(j >> 5) * (S::COLS * 64) + n * 64, from + ((int64_t)n * a.rank + j) * 2, 16);
+                lt_commit();
+                return;
+            }
             for (int n = bl; n < S::COLS; n += LT_LOADERS / 4)
                 for (int j = 8 * bc; j < rp; j += 32) {
                     const uint32_t dst = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
@@ -540,8 +579,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         };
         // Tile i's B is waited for once the next one's is asked for; base is asked for as slots become free, and its copies
         // report to the slot's barrier themselves.
+        const bool all_rows = count == LT_ROWS;
+        const int late = plan.early ? min(2, my_tiles) : 0;            // the first tile that lies over the sums
         for (int i = 0; i <= my_tiles; ++i) {
             int n0 = 0;
+            if (i == late) asm volatile("bar.sync 2, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");
             if (i < my_tiles) {
                 if (i >= 2) wait(&sh.d2_done[i & 1], ((i >> 1) - 1) & 1);
                 n0 = look_up(i);
@@ -558,7 +600,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             if (i >= plan.slots) wait(&sh.slot_free[slot_i], (i / plan.slots - 1) & 1);
             const uint32_t to = base_at + plan.slot_at + (uint32_t)(slot_i * LT_SLOT + cc * 16);
             const char *const from = (const char *)a.base + ((int64_t)n_target + n0) * S::SIZE + cc * 16;
-            if ((cc + 1) * (16 / S::SIZE) <= left)
+            if (all_rows && left >= S::COLS) {
+#pragma unroll
+                for (int k = 0; k < LT_ROWS; k += LT_LOADERS / 16)
+                    lt_copy16(to + (k + cl) * LT_LINE, from + (int64_t)sh.row[k + cl] * a.base_stride * S::SIZE, 16);
+            } else if ((cc + 1) * (16 / S::SIZE) <= left)
 #pragma unroll 4
                 for (int k = cl; k < LT_ROWS; k += LT_LOADERS / 16) {
                     const int row = sh.row[k];
@@ -567,6 +613,8 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(kvt_smem(&sh.slot_full[slot_i])) : "memory");
         }
         lt_wait_copies<0>();
+        __syncwarp();
+        lora_cluster_wait();                   // for the sums
     } else if (warp == LT_MMA) {
         if (lane == 0) {
             const bool ready = wait(&sh.h_full, 0);
@@ -576,7 +624,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 if (!wait(&sh.b_full[i & 1], (i >> 1) & 1)) break;
                 if (i >= 2 && !wait(&sh.d2_free[i & 1], ((i >> 1) - 1) & 1)) break;
                 kvt_after();
-                const uint32_t b = base_at + plan.sum_at + (uint32_t)(i & 1) * b_bytes;
+                const uint32_t b = base_at + plan.b_at + (uint32_t)(i & 1) * b_bytes;
                 bool add = false;
                 lt_parts<S::PH, S::PW>([&](int p, int q) {
                     for (int j = 0; j < rp; j += 16, add = true) {
@@ -596,6 +644,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         const int at = 32 * (warp & 3) + lane, row = sh.row[at], half = warp >> 2, cc = lane & 15, cl = lane >> 4;
         const float by = TX == KV_F16 ? scale * sh.row_scale[at] : scale;
         constexpr int STEP = 16 / S::SIZE;                             // outputs of 16 bytes
+        const bool full_rows = __all_sync(0xffffffffu, row >= 0);
         const uint32_t d2 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)half * 128;
         for (int i = half; i < my_tiles; i += 2) {
             const int n0 = look_up(i), left = min(S::COLS, a.width[target] - n0), n = n_target + n0, slot_i = i % plan.slots;
@@ -603,6 +652,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             wait(&sh.d2_done[half], (i >> 1) & 1);
             kvt_after();
             if (staged && a.base) wait(&sh.slot_full[slot_i], (i / plan.slots) & 1);
+            const bool whole = staged && left == S::COLS;
 #pragma unroll 1
             for (int m = 0; m < S::COLS; m += 32) {
                 uint32_t v[32];
@@ -612,6 +662,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 if (m + 32 == S::COLS) {
                     kvt_before();
                     lt_arrive(&sh.d2_free[half]);
+                }
+                if (whole) {                                           // the same way for all rows, also those that are none
+                    uint4 was[32 / STEP];
+#pragma unroll
+                    for (int e = 0; e < 32 / STEP; ++e) was[e] = a.base ? *(const uint4 *)(slot_line + (m + e * STEP) * S::SIZE) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 32 / STEP; ++e) *(uint4 *)(slot_line + (m + e * STEP) * S::SIZE) = lt_add<TX>(was[e], v + e * STEP, by);
+                    continue;
                 }
                 if (row < 0 || m >= left) continue;
 #pragma unroll
@@ -631,7 +689,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             __syncwarp();
             const char *const from = tiles + plan.slot_at + slot_i * LT_SLOT + (32 * (warp & 3)) * LT_LINE + cc * 16;
             char *const to = (char *)a.out + (int64_t)n * S::SIZE + cc * 16;
-            if ((cc + 1) * (16 / S::SIZE) <= left)
+            if (whole && full_rows) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 2)
+                    __stcs((uint4 *)(to + (int64_t)sh.row[32 * (warp & 3) + k + cl] * a.out_stride * S::SIZE), *(const uint4 *)(from + (k + cl) * LT_LINE));
+            } else if ((cc + 1) * STEP <= left)
 #pragma unroll 4
                 for (int k = cl; k < 32; k += 2) {
                     const int to_row = sh.row[32 * (warp & 3) + k];

@@ -484,3 +484,8 @@ def test_states_past_32_bits(cuda):
     got = np.zeros(4096, np.uint8)
     runtime.check(lib.nc_copy_to_host(got.ctypes.data, ctypes.c_void_p(new.data_ptr() + 2 * size - 4096), 4096))
     assert (got == line).all()
+
+
+def test_no_wait_has_run_out(cuda):
+    """After all of the above: the kernels' waits end because what they wait for comes."""
+    runtime.check(runtime.library().nc_device_faults())
