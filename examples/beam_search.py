@@ -1,10 +1,13 @@
-"""Beam search on the GPU over a paged 4-bit key/value cache: ``python examples/beam_search.py [beams] [tokens]``.
+"""Beam search on the GPU over a paged 4-bit key/value cache: ``python examples/beam_search.py [beams] [tokens] [requests]``.
 
 A small int8 Qwen2-shaped decoder with random weights, run from the library's fused groups; its history is held by the
 serving operators (``nanocompile_b200.serving``). One prompt is prefilled into the first sequence and forked into
 ``beams``; each step appends and attends over the 4-bit cache, takes every beam's best tokens with their log
 probabilities, and hands the pages of the beams that go on to their successors. Only token ids, scores and parents
 cross to the host.
+
+With several requests (:func:`beam_search_requests`) the beams are chosen on the device too, and each request may have a
+low-rank adapter of its own beside the shared projections; the token histories come to the host at the end.
 """
 
 from __future__ import annotations
@@ -29,11 +32,33 @@ class Beam:
     score: float                       # the sum of its tokens' log probabilities
 
 
+class Adapters:
+    """Low-rank adapters of a model's q, k, v, o and down projections: ``slots`` of them, with ranks of their own."""
+
+    NAMES = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.down_proj")
+
+    def __init__(self, shape: model.ModelShape, slots: int, rank: int, seed: int = 0):
+        rng = np.random.default_rng(seed)
+        self.slots = slots
+        self.ranks = DeviceArray.of(np.array([max(1, rank >> s % 3) for s in range(slots)], np.int32))
+        self.scales = DeviceArray.of(np.full(slots, 2.0, np.float32))
+        inputs = {"self_attn.o_proj": shape.q_rows, "mlp.down_proj": shape.inter}
+        outputs = {"self_attn.q_proj": shape.q_rows, "self_attn.k_proj": shape.kv_rows, "self_attn.v_proj": shape.kv_rows}
+        self.layouts, self.weights = {}, {}
+        for name in self.NAMES:
+            k, n = inputs.get(name, shape.hidden), outputs.get(name, shape.hidden)
+            self.layouts[name] = layout = serving.LoraLayout(k, (n,), rank)
+            for layer in range(shape.layers):
+                self.weights[layer, name] = [DeviceArray.of((rng.standard_normal(size) * scale).astype(np.float16))
+                                             for size, scale in ((layout.a_shape(slots), k ** -0.5), (layout.b_shape(slots), 0.05))]
+
+
 class Decoder:
-    """An int8 decoder over a 4-bit paged cache of ``seqs`` sequences of up to ``length`` positions."""
+    """An int8 decoder over a 4-bit paged cache of ``seqs`` sequences of up to ``length`` positions; ``adapters`` beside its
+    projections, one for each sequence (:meth:`use`)."""
 
     def __init__(self, shape: model.ModelShape, weights: dict[str, np.ndarray], seqs: int, length: int, page_size: int = 16,
-                 top: int = 8):
+                 top: int = 8, adapters: Adapters | None = None):
         self.shape, self.seqs, self.length, self.top = shape, seqs, length, top
         self.lib = runtime.library()
         self.layout = serving.KV4Layout(shape.heads, shape.kv_heads, shape.head_dim, page_size, shape.layers)
@@ -49,6 +74,11 @@ class Decoder:
         angles = np.arange(length, dtype=np.float32)[:, None] * shape.rope_rates()
         self.rope = DeviceArray.of(np.cos(angles)), DeviceArray.of(np.sin(angles))
         self.rows = 0
+        self.adapters, self.adapter_ids = adapters, DeviceArray.of(np.full(seqs, -1, np.int32))
+
+    def use(self, adapters) -> None:
+        """The adapter of each sequence from now on (-1: none)."""
+        self.adapter_ids.upload(np.asarray(adapters, np.int32))
 
     def _packed(self, values: np.ndarray) -> DeviceArray:
         out, values = DeviceArray(values.shape, np.uint8), np.ascontiguousarray(values)
@@ -79,6 +109,15 @@ class Decoder:
         self.score_scratch = DeviceArray.zeros((serving.token_logprobs_scratch_bytes(rows, s.vocab, self.top),), np.uint8)
         self.attention_scratch = DeviceArray.zeros(
             (serving.kv4_attention_scratch_bytes(self.layout, rows, self.seqs, self.length, rows),), np.uint8)
+        if self.adapters:
+            self.batch = serving.LoraBatch(rows, self.seqs, self.adapters.slots)
+            self.plan = DeviceArray((self.batch.plan_bytes,), np.uint8)
+
+    def _adapt(self, layer: int, name: str, out, x) -> None:
+        if self.adapters:
+            a, b = self.adapters.weights[layer, name]
+            serving.lora_project(self.adapters.layouts[name], self.batch, out, x, a, b, self.plan, base=out, ranks=self.adapters.ranks,
+                                 scales=self.adapters.scales)
 
     def _project(self, out, name: str, n: int, k: int, epilogue: int, operand=None, second=None) -> None:
         w = self.weights
@@ -87,9 +126,9 @@ class Decoder:
 
     def update(self, parent, grow) -> None:
         """Sequences continue ``parent`` (-1: none) with ``grow`` more positions; raises if the pool has too few pages."""
+        parent, grow = (v if isinstance(v, DeviceArray) else DeviceArray.of(np.asarray(v, np.int32)) for v in (parent, grow))
         serving.kv_pages_update(self.tables[1], self.lengths[1], self.tables[0], self.lengths[0], self.pool, self.status,
-                                self.pages_scratch, page_size=self.layout.page_size,
-                                parent=DeviceArray.of(np.asarray(parent, np.int32)), grow=DeviceArray.of(np.asarray(grow, np.int32)))
+                                self.pages_scratch, page_size=self.layout.page_size, parent=parent, grow=grow)
         missing = int(self.status.numpy()[0])
         if missing:
             raise runtime.InterpreterError(f"the cache lacks {missing} pages")
@@ -97,31 +136,39 @@ class Decoder:
         self.lengths.reverse()
 
     def step(self, ids, counts, targets=None) -> None:
-        """Token rows ``ids``, the last ``counts[i]`` positions of each sequence i (already grown by :meth:`update`); leaves
-        the rows' top tokens, and the log probabilities of ``targets``, on the device."""
+        """Token rows ``ids`` (on the host or the device), the last ``counts[i]`` positions of each sequence i (already grown by
+        :meth:`update`); leaves the rows' logits and top tokens, and the log probabilities of ``targets``, on the device."""
         s, w, at = self.shape, self.weights, (self.tables[0], self.lengths[0])
-        self._room(len(ids))
+        self._room(sum(counts))
         rows, eps = self.rows, int(np.array([s.eps], np.float32).view(np.uint32)[0])
-        self.ids.upload(np.asarray(ids, np.int64))
+        if not isinstance(ids, DeviceArray):
+            self.ids.upload(np.asarray(ids, np.int64))
+            ids = self.ids
         self.row_start.upload(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
-        self._group("nc_gather_rows", [self.x, self.ids, w["model.embed_tokens.weight"], self.error], [rows, s.vocab, s.hidden])
+        if self.adapters:                                            # the rows of each adapter, for all layers and projections
+            serving.lora_plan(self.batch, self.plan, self.adapter_ids, row_start=self.row_start)
+        normed = self.normed if self.adapters else None              # the adapters' products take what is not quantised
+        self._group("nc_gather_rows", [self.x, ids, w["model.embed_tokens.weight"], self.error], [rows, s.vocab, s.hidden])
         for layer in range(s.layers):
             p = f"model.layers.{layer}"
-            self._group("nc_rms_norm_quantize", [None, self.x, w[f"{p}.input_layernorm.weight"], self.xq, self.xs, self.offset, None],
+            self._group("nc_rms_norm_quantize", [normed, self.x, w[f"{p}.input_layernorm.weight"], self.xq, self.xs, self.offset, None],
                         [rows, s.hidden, eps])
             for out, name, n in ((self.q, "q_proj", s.q_rows), (self.k, "k_proj", s.kv_rows), (self.v, "v_proj", s.kv_rows)):
                 self._project(out, f"{p}.self_attn.{name}.weight", n, s.hidden, 1, w[f"{p}.self_attn.{name}.bias"])
+                self._adapt(layer, f"self_attn.{name}", out, normed)
             serving.kv4_append(self.layout, self.pool, self.k, self.v, *at, row_start=self.row_start, rope=self.rope, layer=layer)
             serving.kv4_attention(self.layout, self.ctx, self.q, self.pool, *at, self.attention_scratch, max_length=self.length,
                                   row_start=self.row_start, max_rows=rows, rope=self.rope, layer=layer)
             self._group("nc_quantize_blocks", [self.xq, self.ctx, self.xs, self.offset, None], [rows, s.q_rows])
             self._project(self.x2, f"{p}.self_attn.o_proj.weight", s.hidden, s.q_rows, 2, self.x)
+            self._adapt(layer, "self_attn.o_proj", self.x2, self.ctx)
             self._group("nc_rms_norm_quantize", [None, self.x2, w[f"{p}.post_attention_layernorm.weight"], self.xq, self.xs, self.offset, None],
                         [rows, s.hidden, eps])
             self._project(self.mlp, f"{p}.mlp.gate_proj.weight", s.inter, s.hidden, 3, w[f"{p}.mlp.up_proj.weight@int8"],
                           w[f"{p}.mlp.up_proj.weight@scales"])
             self._group("nc_quantize_blocks", [self.xq, self.mlp, self.xs, self.offset, None], [rows, s.inter])
             self._project(self.x, f"{p}.mlp.down_proj.weight", s.hidden, s.inter, 2, self.x2)
+            self._adapt(layer, "mlp.down_proj", self.x, self.mlp)
         self._group("nc_rms_norm_quantize", [self.normed, self.x, w["model.norm.weight"], None, None, None, None], [rows, s.hidden, eps])
         self._group("nc_lm_head_argmax", [self.logits, self.normed, w["model.embed_tokens.weight"], None, self.head_scratch],
                     [rows, s.vocab, s.hidden])
@@ -157,9 +204,52 @@ def beam_search(decoder: Decoder, prompt, tokens: int) -> list[Beam]:
     return beams
 
 
-def main(beams: int = 4, tokens: int = 24) -> None:
+def beam_search_requests(decoder: Decoder, prompts, beams: int, tokens: int, adapters=None, end: int = -1) -> list[list[Beam]]:
+    """The best continuations of each of several prompts, of up to ``tokens`` tokens or to the token ``end``, best first: request g has
+    the cache's sequences ``g * beams ..``, and of a decoder's adapters ``adapters[g]``. The choice, the histories and the
+    pages stay on the device."""
+    n, groups = decoder.seqs, len(prompts)
+    first = [0 if i % beams else len(prompts[i // beams]) - 1 for i in range(n)]
+    if adapters is not None:
+        decoder.use([adapters[i // beams] for i in range(n)])
+    decoder.update([-1] * n, [0] * n)
+    decoder.update(range(n), first)
+    if any(first):
+        decoder.step([t for p in prompts for t in p[:-1]], first)
+    # The prompts' last tokens, and from there on the chosen ones: the first beam of each request is the only one to begin with.
+    decoder.update(range(n), [int(i % beams == 0) for i in range(n)])
+    ids = DeviceArray.of(np.array([prompts[i // beams][-1] for i in range(n)], np.int64))
+    scores = [DeviceArray.of(np.where(np.arange(n) % beams == 0, 0, -np.inf).astype(np.float32)), DeviceArray((n,), np.float32)]
+    finished = [DeviceArray.zeros((n,), np.int32) for _ in range(2)]
+    histories = [DeviceArray.zeros((n, tokens), np.int64) for _ in range(2)]
+    lengths = [DeviceArray.zeros((n,), np.int32) for _ in range(2)]
+    parent, grow, pages, more = DeviceArray((n,), np.int32), DeviceArray((n,), np.int32), DeviceArray((n,), np.int32), DeviceArray.of(np.ones(n, np.int32))
+    scratch = DeviceArray.zeros((serving.beam_select_scratch_bytes(n, decoder.shape.vocab, beams),), np.uint8)
+    for step in range(tokens):
+        decoder.step(ids, [1] * n)
+        serving.beam_select(parent, ids, scores[1], decoder.logits, scores[0], scratch, beams=beams, end=end,
+                            finished=finished[0] if end >= 0 else None, new_finished=finished[1], grow=grow, history=pages)
+        serving.beam_reorder(histories[1], histories[0], parent, lengths=lengths[0], new_lengths=lengths[1], append=ids, grow=grow)
+        for pair in (scores, finished, histories, lengths):
+            pair.reverse()
+        if step + 1 < tokens:
+            decoder.update(pages, more)
+    found = zip(histories[0].numpy(), lengths[0].numpy(), scores[0].numpy())
+    every = [Beam([int(t) for t in history[:length]], float(score)) for history, length, score in found]
+    return [every[g * beams: (g + 1) * beams] for g in range(groups)]
+
+
+def main(beams: int = 4, tokens: int = 24, requests: int = 1) -> None:
     shape = model.SMALL
     prompt = model.synthetic_prompt(shape.vocab, 37)
+    if requests > 1:
+        adapters = Adapters(shape, slots=3, rank=16)
+        decoder = Decoder(shape, model.synthetic_weights(shape, seed=3, std=0.08), beams * requests, len(prompt) + tokens, adapters=adapters)
+        prompts = [prompt[: len(prompt) - g] for g in range(requests)]
+        for g, found in enumerate(beam_search_requests(decoder, prompts, beams, tokens, adapters=[g % 4 - 1 for g in range(requests)], end=5)):
+            for beam in found:
+                print(f"{g}: {beam.score:9.4f}  {' '.join(map(str, beam.tokens))}")
+        return
     decoder = Decoder(shape, model.synthetic_weights(shape, seed=3, std=0.08), beams, len(prompt) + tokens)
     for beam in beam_search(decoder, prompt, tokens):
         print(f"{beam.score:9.4f}  {' '.join(map(str, beam.tokens))}")
