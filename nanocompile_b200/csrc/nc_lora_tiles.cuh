@@ -703,8 +703,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             lt_arrive(&sh.slot_free[slot_i]);
         }
     }
+    // What this CTA has been sent is there, also where a wait for it has run out; so what it has sent is, once every CTA has come here.
+    kvt_mbar_wait(&sh.h_full, 0, NC_DRAIN_CYCLES);
     __syncwarp();
-    // What this CTA has sent is there once every CTA has come here.
     lora_cluster_arrive();
     // Nothing reads or writes tensor memory any more once the last matrix instruction has come to its end.
     kvt_mbar_wait(&sh.drained, 0, NC_DRAIN_CYCLES);

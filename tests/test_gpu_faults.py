@@ -128,3 +128,22 @@ def test_a_4_bit_prompt_stops_on_a_short_wait_and_its_scratch_stays_good(short_w
         got = case.check(layout, query, "bfloat16", counts, **bounds)
         assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(got, want))
     cuda.device_faults()
+
+
+@pytest.mark.parametrize("dtype,wtype", [("float32", "bfloat16"), ("float32", "float16"), ("bfloat16", "bfloat16"), ("float16", "float16")])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [300, 70, 128, 2]])
+def test_adapters_stop_on_a_short_wait(short_waits, dtype, wtype, counts):
+    """Waits cut short end the adapters' kernels, for single tokens and for prompts; the next call is right."""
+    from tests.test_gpu_requests import Adapted
+
+    cuda = short_waits
+    case = Adapted(1, dtype, wtype, 2048, (1000, 264), 32, 3, [0, 2, 1, -1], counts)
+    want = case.run().check()
+    cuda.set_wait_limit(1)
+    for _ in range(2):
+        case.run()
+    with pytest.raises(cuda.KernelError, match="adapters.*wait limit"):
+        cuda.device_faults()
+    cuda.set_wait_limit(0)
+    assert np.array_equal(bits(case.run().check()), bits(want))
+    cuda.device_faults()
