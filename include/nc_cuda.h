@@ -171,7 +171,7 @@ int32_t nc_attention_cache(void **p, const int64_t *s, void *stream);
 
 /* NC_ERR_KERNEL if a kernel recorded a device-side fault since the last call (a TMA stage of
  * the grouped attention kernel that did not arrive within its bounded wait, or a copy or a matrix
- * instruction of nc_kv4_attention's prompts, whose output is then missing in part); clears it. */
+ * instruction of nc_kv4_attention's prompts or of nc_lora_project, whose output is then missing in part); clears it. */
 int32_t nc_device_faults(void);
 
 /* Bounds the library's abandonable device-side waits (pipeline stages of the tensor-core
@@ -291,7 +291,8 @@ int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
  * [outputs][rank] (16-bit, contiguous); the targets share x (q, k and v, say) and their outputs follow one another.  Row r of
  * a sequence with adapter a, output n of target t:
  *   out[r, n] = base[r, n] + scales[a] * sum_{j < ranks[a]} B_a[n, j] * sum_k A_a[t * rank + j, k] * x[r, k]
- * What a slot holds past ranks[a] is not read.  Rows of sequences without an adapter are base's (nought without base).
+ * What a slot holds past ranks[a] does not count.  Rows of sequences without an adapter, or with one of rank 0, are base's (nought
+ * without base).
  *
  * The plan: the rows of a call grouped by adapter, made once for all projections and layers of a batch.  Adapters outside
  * 0 .. slots - 1 are none; the smallest sequence with one from `slots` on is put into the error word.  Rows outside
@@ -303,11 +304,12 @@ int32_t nc_lora_plan(void **p, const int64_t *s, void *stream);
 int64_t nc_lora_plan_bytes(int64_t rows, int64_t seqs, int64_t slots);
 
 /* Adds the adapters' shares to projections' outputs; the plan was made for the same rows, seqs and slots.
- * p: [0] out [rows, outputs] (may be base)  [1] x [rows, inputs]  [2] base (nullable)  [3] A  [4] B  [5] plan
+ * p: [0] out [rows, outputs] (may be base, at its stride; overlaps nothing else)  [1] x [rows, inputs]  [2] base (nullable)  [3] A  [4] B  [5] plan
  *    [6] ranks i32[slots] (null: rank)  [7] scales f32[slots] (null: 1)
  * s: rows, seqs, slots, inputs, rank (both multiples of 8; rank 128 at most), targets (8 at most), element type of x, base
  *    and out, element type of A and B (1 or 2), plan bytes, x row stride (elements), base row stride, out row stride,
- *    outputs of each target */
+ *    outputs of each target (2^23 inputs or outputs in all at most).
+ * A wait in it that runs out (see nc_set_wait_limit) leaves outputs that are not to be used; nc_device_faults tells. */
 int32_t nc_lora_project(void **p, const int64_t *s, void *stream);
 
 /* Beam search's choice.  Rows g * beams .. (g + 1) * beams - 1 are request g's.  scores[r]: the sum of the log

@@ -3,6 +3,7 @@
 
 #include "../../include/nc_cuda.h"
 
+#include <atomic>
 #include <cstdint>
 #include <cstdlib>
 
@@ -46,6 +47,11 @@ inline bool pdl_enabled() {
     return on;
 }
 
+constexpr int64_t I32 = (int64_t(1) << 31) - 1;
+// Whether an address or a number of bytes is no multiple of n, a power of two.
+inline bool misaligned(const void *p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) != 0; }
+inline bool misaligned(int64_t v, int64_t n) { return (v & (n - 1)) != 0; }
+
 inline int sm_count() {
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -72,6 +78,17 @@ template <typename K>
 cudaError_t allow_smem(K kernel, size_t bytes) {
     if (bytes <= 48 * 1024) return cudaSuccess;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+// Raises a kernel's limit of shared memory, once on each device (`allowed`: a bit for each).
+template <typename K>
+int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) {
+    int device = 0;
+    CUDA_TRY(cudaGetDevice(&device));
+    if (device < 64 && (allowed->load(std::memory_order_relaxed) >> device & 1)) return NC_OK;
+    CUDA_TRY(allow_smem(kernel, bytes));
+    if (device < 64) allowed->fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    return NC_OK;
 }
 
 inline int32_t check_launch(const char *what) {

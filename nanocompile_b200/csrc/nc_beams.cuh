@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(LP_THREADS, BEAM_RESIDENT) beam_select_kernel(
         __syncthreads();
     }
     if (tid == 0) shared.ndone = 0;
-    const int all = live * a.batches, ctas = (int)gridDim.x;       // below 2^20: a request has few segments
+    const int all = live * a.batches, ctas = (int)gridDim.x;       // below 2^24: a row has at most 16 batches to each of 512 segments
     const BeamShare share{max(a.least, (all + ctas - 1) / ctas), a.batches};
     int at = (int)blockIdx.x * share.size;
     const int end = min(all, at + share.size);

@@ -22,6 +22,7 @@
 namespace nc {
 
 constexpr int LORA_TARGETS = 8, LORA_RANK = 128, LORA_SEQS = 8192;
+constexpr int LORA_LINE = 1 << 23;             // inputs or outputs of a row at most: those of 128 rows are counted in 32 bits
 constexpr int LORA_THREADS = 256, LORA_WARPS = LORA_THREADS / 32;
 constexpr int LORA_PASS = 192;                 // rows of h at most in a pass: targets x rank in whole 32s
 constexpr int LORA_HEAD = 4;                   // words before the plan's items
@@ -250,10 +251,10 @@ __device__ __forceinline__ int64_t lora_row(const LoraArgs &a, const int32_t *or
     const int row = order[at];
     return row >= 0 && row < a.rows ? row : -1;
 }
-// Rows without an adapter: columns [from, to) of base, or nought.
+// Rows without an adapter, or with one of rank 0: columns [from, to) of base, or nought.
 template <int TX>
 __device__ __forceinline__ void lora_copy(const LoraArgs &a, const int32_t *order, int start, int count, int from, int to) {
-    if (a.out == a.base && a.out_stride == a.base_stride) return;
+    if (a.out == a.base) return;
     for (int i = threadIdx.x; i < (to - from) * count; i += blockDim.x) {
         const int64_t row = lora_row(a, order, start + i / (to - from));
         const int n = from + i % (to - from);
@@ -290,12 +291,12 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
         if (t < t0) n_first += a.width[t];
         else n_pass += a.width[t], n_tiles += (a.width[t] + 15) / 16;
     }
-    if (slot < 0) {
+    const int r = slot < 0 ? 0 : a.ranks ? min(max(a.ranks[slot], 0), a.rank) : a.rank;
+    if (r == 0) {
         const int64_t n = n_pass;
         lora_copy<TX>(a, order, first, count, n_first + (int)(n * cta / ctas), n_first + (int)(n * (cta + 1) / ctas));
         return;
     }
-    const int r = a.ranks ? min(max(a.ranks[slot], 0), a.rank) : a.rank;
     const float scale = a.scales ? a.scales[slot] : 1.0f;
     const char *const wa = (const char *)a.a + (int64_t)slot * a.targets * a.rank * a.inputs * 2;
     const char *const wb = (const char *)a.b + (int64_t)slot * a.outputs * a.rank * 2;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
             for (int i = 0; i < S::TB; ++i)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int t = (tb + i) / max(per, 1), j = (tb + i - t * per) * 16 + 8 * k + g;
+                    const int t = (tb + i) / per, j = (tb + i - t * per) * 16 + 8 * k + g;
                     from[i][k] = tb + i < tiles && j < r ? (const uint16_t *)wa + ((int64_t)(t0 + t) * a.rank + j) * a.inputs + 8 * c : nullptr;
                 }
 #pragma unroll 2

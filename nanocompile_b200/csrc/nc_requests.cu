@@ -8,27 +8,10 @@
 #include "nc_lora_stream.cuh"
 
 #include <algorithm>
-#include <atomic>
 
 using namespace nc;
 
 namespace {
-
-constexpr int64_t I32 = (int64_t(1) << 31) - 1;
-
-bool misaligned(const void *p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) != 0; }
-bool misaligned(int64_t v, int64_t n) { return (v & (n - 1)) != 0; }
-
-// Raises a kernel's limit of shared memory, once on each device (`allowed`: a bit for each).
-template <typename K>
-int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) {
-    int device = 0;
-    CUDA_TRY(cudaGetDevice(&device));
-    if (device < 64 && (allowed->load(std::memory_order_relaxed) >> device & 1)) return NC_OK;
-    CUDA_TRY(allow_smem(kernel, bytes));
-    if (device < 64) allowed->fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
-    return NC_OK;
-}
 
 int32_t check_type(int64_t type) {
     if (type < KV_F32 || type > KV_BF16) return fail(NC_ERR_ARGUMENT, "element type %lld: 0 float32, 1 float16, 2 bfloat16", (long long)type);
@@ -237,14 +220,16 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     NC_TRY(lora_batch(rows, seqs, slots));
     NC_TRY(check_type(type));
     if (wtype != KV_F16 && wtype != KV_BF16) return fail(NC_ERR_ARGUMENT, "adapters of element type %lld: 1 float16 or 2 bfloat16", (long long)wtype);
-    if (inputs <= 0 || inputs % 8 || inputs > I32 || rank <= 0 || rank % 8 || rank > LORA_RANK)
-        return fail(NC_ERR_ARGUMENT, "%lld inputs, rank %lld: multiples of 8, the rank %d at most", (long long)inputs, (long long)rank, LORA_RANK);
+    if (inputs <= 0 || inputs % 8 || inputs > LORA_LINE || rank <= 0 || rank % 8 || rank > LORA_RANK)
+        return fail(NC_ERR_ARGUMENT, "%lld inputs (%d at most), rank %lld: multiples of 8, the rank %d at most", (long long)inputs, LORA_LINE, (long long)rank,
+                    LORA_RANK);
     if (targets <= 0 || targets > LORA_TARGETS) return fail(NC_ERR_ARGUMENT, "%lld targets: 1 to %d", (long long)targets, LORA_TARGETS);
     int64_t outputs = 0;
     bool even = true;
     for (int t = 0; t < targets; ++t) {
         const int64_t width = s[12 + t];
-        if (width <= 0 || width > I32 / LORA_TARGETS) return fail(NC_ERR_ARGUMENT, "a target of %lld outputs", (long long)width);
+        if (width <= 0 || width > LORA_LINE - outputs)
+            return fail(NC_ERR_ARGUMENT, "a target of %lld outputs after %lld: %d at most", (long long)width, (long long)outputs, LORA_LINE);
         even = even && outputs % 2 == 0;
         a.width[t] = (int)width;
         outputs += width;
@@ -269,6 +254,9 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     if (misaligned(a.x, bytes) || misaligned(a.out, bytes) || misaligned(a.base, bytes)) return fail(NC_ERR_ARGUMENT, "misaligned rows");
     if (a.x_stride < inputs || a.out_stride < outputs || (a.base && a.base_stride < outputs))
         return fail(NC_ERR_ARGUMENT, "rows of %lld inputs or %lld outputs overlap", (long long)inputs, (long long)outputs);
+    if (a.out == a.x) return fail(NC_ERR_ARGUMENT, "the outputs are the inputs");
+    if (a.out == a.base && a.out_stride != a.base_stride)
+        return fail(NC_ERR_ARGUMENT, "outputs in place of base at a stride of %lld, base's is %lld", (long long)a.out_stride, (long long)a.base_stride);
     a.rows = (int)rows;
     a.items = (int)lora_places(rows, seqs, slots);
     a.tile = (int)lora_tile(rows, seqs, slots);
@@ -309,11 +297,12 @@ struct BeamPlan {
 };
 BeamPlan beam_plan(int64_t batches, int64_t beams) {
     auto lists = [&](int64_t least) { return std::min(batches, (std::max<int64_t>(batches - 2, 0)) / least + 2 + batches / BEAM_BATCHES); };
+    if (lists(batches) * beams > BEAM_LISTS) return BeamPlan{0, 0};
     int64_t least = std::max<int64_t>(1, batches * beams / BEAM_LISTS);
     // Two batches where that leaves half of the candidates that are taken at once: 4 beams of 151936 float32 logits 13.2 us, 14.7 with one.
     if (least == 1 && batches > 1 && lists(1) * beams * beams > 512 && lists(2) * beams * beams <= 512) least = 2;
-    while (least < batches && lists(least) * beams > BEAM_LISTS) ++least;
-    return lists(least) * beams > BEAM_LISTS ? BeamPlan{0, 0} : BeamPlan{least, lists(least)};
+    while (lists(least) * beams > BEAM_LISTS) ++least;
+    return BeamPlan{least, lists(least)};
 }
 int64_t beam_launch_rows(int64_t rows, int64_t beams) { return std::min<int64_t>(rows, BEAM_ROWS / beams * beams); }
 
@@ -393,8 +382,8 @@ template <typename V>
 int32_t launch_reorder(cudaStream_t st, ReorderArgs a) {
     const int64_t chunk = (int64_t)sizeof(V) * BEAM_COPY_THREADS * BEAM_COPY_VECS;
     a.chunks = std::max<int64_t>(1, (a.capacity * a.line + chunk - 1) / chunk);
-    const int64_t ctas = (int64_t)a.rows * a.planes * a.chunks;
-    if (ctas > I32) return fail(NC_ERR_ARGUMENT, "%d rows of %d planes of %lld bytes in one call", a.rows, a.planes, (long long)(a.capacity * a.line));
+    const int64_t ctas = (int64_t)a.rows * a.planes <= I32 / a.chunks ? a.rows * a.planes * a.chunks : 0;
+    if (ctas == 0) return fail(NC_ERR_ARGUMENT, "%d rows of %d planes of %lld bytes in one call", a.rows, a.planes, (long long)(a.capacity * a.line));
     CUDA_TRY(launch_k(beam_reorder_kernel<V>, (unsigned)ctas, BEAM_COPY_THREADS, 0, st, a));
     return check_launch("beam_reorder_kernel");
 }

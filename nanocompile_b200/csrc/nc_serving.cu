@@ -10,30 +10,14 @@
 #include "nc_logprobs.cuh"
 
 #include <algorithm>
-#include <atomic>
 #include <cstring>
 
 using namespace nc;
 
 namespace {
 
-constexpr int64_t I32 = (int64_t(1) << 31) - 1;
-
-bool misaligned(const void *p, int64_t n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) != 0; }
-
 int32_t check_type(int64_t type) {
     if (type < KV_F32 || type > KV_BF16) return fail(NC_ERR_ARGUMENT, "element type %lld: 0 float32, 1 float16, 2 bfloat16", (long long)type);
-    return NC_OK;
-}
-
-// Raises a kernel's limit of shared memory, once on each device (`allowed`: a bit for each).
-template <typename K>
-int32_t allow_smem_once(K kernel, size_t bytes, std::atomic<uint64_t> *allowed) {
-    int device = 0;
-    CUDA_TRY(cudaGetDevice(&device));
-    if (device < 64 && (allowed->load(std::memory_order_relaxed) >> device & 1)) return NC_OK;
-    CUDA_TRY(allow_smem(kernel, bytes));
-    if (device < 64) allowed->fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
     return NC_OK;
 }
 

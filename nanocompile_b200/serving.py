@@ -461,7 +461,7 @@ def lora_project(layout: LoraLayout, batch: LoraBatch, out, x, a, b, plan, *, ba
                  stream: int = 0) -> None:
     """Add the adapters' shares to the outputs of projections of ``x`` (``nc_lora_project``).
 
-    ``out`` = ``base`` (default: nought; may be ``out`` itself) + ``scales`` * B (A x), each row with its sequence's adapter.
+    ``out`` = ``base`` (default: nought; may be ``out`` itself, at its stride) + ``scales`` * B (A x), each row with its sequence's adapter.
     ``a`` and ``b``: float16 or bfloat16, as :meth:`LoraLayout.a_shape` and ``b_shape`` say. ``ranks`` (int32 ``[slots]``): the adapters' own
     ranks, where lower; ``scales``: float32 ``[slots]``. float32 rows keep float32 accuracy.
     """

@@ -272,6 +272,26 @@ def test_a_plan_serves_many_projections_and_streams(cuda):
         case.check(out.cpu().numpy())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inputs,widths,rank,counts", [(64, (32, 7), 8, [1] * 4), (4864, (896,), 64, [1] * 4), (256, (160, 33), 32, [90, 3, 200, 1])])
+def test_adapters_of_rank_nought_are_none(cuda, dtype, inputs, widths, rank, counts):
+    """Whatever they hold and whatever their scale: base as it is, also in place."""
+    wtype = "float16" if dtype == "float16" else BF16
+    case = Adapted(14, dtype, wtype, inputs, widths, rank, 4, [0, 1, 2, 1], counts, ranks=[rank, 0, -3, rank])
+    case.a[1:3] = case.b[1:3] = np.nan
+    case.scales[1:3] = np.inf, np.nan
+    got = decode(case.run().d_out.numpy(), dtype)
+    base = device(case.base, dtype)
+    in_place = decode(case.run(base=base, out=base).d_out.numpy(), dtype)
+    for i in (1, 2, 3):
+        at = slice(case.row_start[i], case.row_start[i + 1])
+        assert (got[at] == case.base[at]).all() and (in_place[at] == case.base[at]).all()
+    case.a[1:3] = case.b[1:3] = 0
+    case.scales[1:3] = 1
+    case.check(got)
+    case.check(in_place)
+
+
 # -- beams -----------------------------------------------------------------------------------------------------
 
 
@@ -412,6 +432,46 @@ def test_a_beam_scratch_serves_smaller_calls_and_is_left_as_the_next_needs_it(cu
     scratch = DeviceArray.zeros((serving.beam_select_scratch_bytes(96, 60000, 16),), np.uint8)
     for rows, vocab, beams in ((96, 60000, 16), (4, 60000, 4), (90, 59999, 9), (1, 17, 1), (96, 60000, 16)):
         Beams(language(rng, rows, vocab), rng.standard_normal(rows), beams).run(scratch=scratch).check()
+
+
+def test_a_captured_choice_and_its_reordering_follow_their_inputs(cuda):
+    """A step captured into a graph, replayed with other logits, scores and states: what the calls outside a graph give."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(15)
+    groups, beams, vocab = 3, 4, 20011
+    rows = groups * beams
+    put = lambda v: torch.from_numpy(np.ascontiguousarray(v)).cuda()                                  # noqa: E731
+    logits, scores, states = put(language(rng, rows, vocab)), put(np.zeros(rows, np.float32)), put(rng.standard_normal((rows, 9)).astype(np.float32))
+    scratch = torch.zeros(serving.beam_select_scratch_bytes(rows, vocab, beams), dtype=torch.uint8, device="cuda")
+    parent, tokens = (torch.empty(rows, dtype=t, device="cuda") for t in (torch.int32, torch.int64))
+    totals, moved = torch.empty(rows, device="cuda"), torch.empty_like(states)
+
+    def step():
+        at = torch.cuda.current_stream().cuda_stream
+        serving.beam_select(parent, tokens, totals, logits, scores, scratch, beams=beams, stream=at)
+        serving.beam_reorder(moved, states, parent, stream=at)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for live in (rows, 5, 1):
+        case = Beams(language(rng, rows, vocab), np.where(np.arange(rows) < live, rng.standard_normal(rows) - 4, -np.inf), beams).run().check()
+        logits.copy_(put(case.host))
+        scores.copy_(put(case.scores))
+        states.copy_(put(rng.standard_normal((rows, 9)).astype(np.float32)))
+        before = moved.cpu().numpy()
+        graph.replay()
+        torch.cuda.synchronize()
+        for have, want in zip((parent, tokens, totals), case.got):
+            assert (have.cpu().numpy() == want).all()
+        was, now = states.cpu().numpy(), moved.cpu().numpy()
+        for i, p in enumerate(case.got[0]):
+            assert (now[i] == (was[p] if p >= 0 else before[i])).all()
 
 
 # -- states ----------------------------------------------------------------------------------------------------

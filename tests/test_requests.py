@@ -30,6 +30,11 @@ def project(**change):
     (dict(plan=Fake((4096,), np.uint8, address=4100)), "16-byte boundary"), (dict(plan=Fake((64, 64), np.uint8)), "scratch"),
     (dict(ranks=Fake((3,), np.int32)), "ranks"), (dict(scales=Fake((4,), np.float16)), "scales"),
     (dict(out=Fake((5, 48), np.float32, address=0)), "null output"), (dict(x=Fake((5, 64), np.float32, address=4098)), "misaligned"),
+    (dict(x=Fake((5, 64), np.float32, address=8192)), "the outputs are the inputs"),
+    (dict(base=Fake((5, 48), np.float32, address=8192, strides=(50, 1))), "in place of base"),
+    (dict(layout=serving.LoraLayout(2 ** 23 + 8, (32, 16), 8), x=Fake((5, 2 ** 23 + 8), np.float32), a=Fake((4, 16, 2 ** 23 + 8), np.float16)), "8388608 at most"),
+    (dict(layout=serving.LoraLayout(64, (32, 2 ** 23), 8), out=Fake((5, 2 ** 23 + 32), np.float32, address=8192), b=Fake((4, 2 ** 23 + 32, 8), np.float16)),
+     "8388608 outputs after 32"),
 ])
 def test_projections_refuse(change, what):
     with pytest.raises(runtime.InterpreterError, match=what):
@@ -74,7 +79,7 @@ def test_plan_bytes_hold_every_item_and_row():
     (dict(scores=Fake((6,), np.float64)), "scores"), (dict(scores=Fake((6,), np.float32, address=12288)), "are the old ones"),
     (dict(finished=Fake((6,), np.int32), new_finished=Fake((6,), np.int32), end=1), "are the old ones"), (dict(norms=Fake((5,), np.float32)), "norms"),
     (dict(logits=Fake((6, 50), np.float32, address=4098)), "misaligned"), (dict(scratch=Fake((1 << 20,), np.uint8, address=4104)), "scratch"),
-    (dict(logits=Fake((6, 0), np.float32)), "0 logits")])
+    (dict(logits=Fake((6, 0), np.float32)), "0 logits"), (dict(logits=Fake((6, 2 ** 31), np.float32)), "too large for 3 beams")])
 def test_selections_refuse(change, what):
     given = {"parent": Fake((6,), np.int32), "tokens": Fake((6,), np.int64), "new_scores": Fake((6,), np.float32, address=12288),
              "logits": Fake((6, 50), np.float32), "scores": Fake((6,), np.float32), "scratch": Fake((1 << 20,), np.uint8), "beams": 3, **change}
@@ -95,7 +100,9 @@ def test_a_beam_scratch_covers_every_smaller_call():
     (dict(new=Fake((3, 2, 8, 4), np.float64)), "expected"), (dict(new_lengths=Fake((3,), np.int32)), "without lengths"),
     (dict(append=Fake((3, 2, 4), np.float32)), "without lengths"), (dict(lengths=Fake((3,), np.int32), append=Fake((3, 4), np.float32)), "append"),
     (dict(lengths=Fake((3,), np.int32), grow=Fake((3,), np.int32)), "grow without"),
-    (dict(lengths=Fake((3,), np.int32), new_lengths=Fake((3,), np.int32)), "are the old ones")])
+    (dict(lengths=Fake((3,), np.int32), new_lengths=Fake((3,), np.int32)), "are the old ones"),
+    (dict(new=Fake((2 ** 30, 2 ** 30, 64, 2 ** 16), np.uint8, address=8192, strides=(2 ** 52, 2 ** 22, 2 ** 16, 1)), parent=Fake((2 ** 30,), np.int32),
+          old=Fake((2 ** 30, 2 ** 30, 64, 2 ** 16), np.uint8, strides=(2 ** 52, 2 ** 22, 2 ** 16, 1))), "in one call")])
 def test_reorders_refuse(change, what):
     given = {"new": Fake((3, 2, 8, 4), np.float32, address=8192), "old": Fake((3, 2, 8, 4), np.float32), "parent": Fake((3,), np.int32), **change}
     with pytest.raises(runtime.InterpreterError, match=what):
