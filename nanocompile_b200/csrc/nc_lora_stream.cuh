@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) lora_stream_kernel(const __grid
         const int64_t row = warp < count ? lora_row(a, order, first + warp) : -1;
         // 1024 inputs at a time; where they are scaled, a first time for the largest.
         constexpr int M = 4;
-        float v[M][8], by = 1.0f;
+        float v[M][8], by = 1.0f, largest = 0.0f;                  // largest: of the row, once scaled, where that is a number
         auto load = [&](int from) {
 #pragma unroll
             for (int m = 0; m < M; ++m) {
@@ -275,20 +275,35 @@ __global__ void __launch_bounds__(LS_THREADS, 2) lora_stream_kernel(const __grid
             by = ls_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), &back);
             if (lane == 0) x_back[warp] = back;
             if (slice > 256 * M) load(0);
+            if (__any_sync(0xffffffffu, !(most < INFINITY))) largest = INFINITY;
         }
         for (int from = 0; from * 2 < plan.x_line - 16; from += 256 * M) {
             if (from > 0) load(from);
+            if constexpr (S::PX > 1 && !S::SCALED_X) {
+                largest = 0.0f;
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const int e = from + 256 * m + 8 * lane;
-                if (e * 2 >= plan.x_line - 16) continue;
-                float2 pair[4];
+                for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pair[i] = S::SCALED_X ? make_float2(fmul(v[m][2 * i], by), fmul(v[m][2 * i + 1], by)) : make_float2(v[m][2 * i], v[m][2 * i + 1]);
-#pragma unroll
-                for (int p = 0; p < S::PX; ++p)
-                    *(uint4 *)(x_room + (p * 8 + warp) * plan.x_line + e * 2) = make_uint4(lt_part<TW>(pair[0]), lt_part<TW>(pair[1]), lt_part<TW>(pair[2]), lt_part<TW>(pair[3]));
+                    for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(v[m][i]));
             }
+            lt_sure<TW>(largest, [&](auto sure) {                      // rows of the weights' type are their only part, whatever they are
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    const int e = from + 256 * m + 8 * lane;
+                    if (e * 2 >= plan.x_line - 16) continue;
+                    float2 pair[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        pair[i] = S::SCALED_X ? make_float2(fmul(v[m][2 * i], by), fmul(v[m][2 * i + 1], by)) : make_float2(v[m][2 * i], v[m][2 * i + 1]);
+#pragma unroll
+                    for (int p = 0; p < S::PX; ++p) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = lt_part<TW, decltype(sure)::value>(pair[i]);
+                        *(uint4 *)(x_room + (p * 8 + warp) * plan.x_line + e * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            });
         }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(LORA_THREADS) : "memory");
@@ -361,14 +376,17 @@ __global__ void __launch_bounds__(LS_THREADS, 2) lora_stream_kernel(const __grid
             if (lane == 0) h_back[warp] = back;
 #pragma unroll
             for (int m = 0; m < M; ++m) v[m].x = fmul(v[m].x, by), v[m].y = fmul(v[m].y, by);
+            if (most < INFINITY) most = fmul(most, by);                // where the row has an infinity it is as it was, and may be too large
         }
+        lt_sure<TW>(most, [&](auto sure) {
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            const int at = 64 * m + 2 * lane;
-            if (at >= rp * (t1 - t0)) continue;
+            for (int m = 0; m < M; ++m) {
+                const int at = 64 * m + 2 * lane;
+                if (at >= rp * (t1 - t0)) continue;
 #pragma unroll
-            for (int p = 0; p < S::PH; ++p) *(uint32_t *)(h_room + (p * 8 + warp) * plan.h_line + at * 2) = lt_part<TW>(v[m]);
-        }
+                for (int p = 0; p < S::PH; ++p) *(uint32_t *)(h_room + (p * 8 + warp) * plan.h_line + at * 2) = lt_part<TW, decltype(sure)::value>(v[m]);
+            }
+        });
     }
     lora_cluster_arrive();                                             // the peers' sums are read; they may go once all CTAs are here
     asm volatile("cp.async.wait_all;" ::: "memory");

@@ -16,6 +16,8 @@
 #include "nc_kv4_prompt.cuh"
 #include "nc_lora.cuh"
 
+#include <type_traits>
+
 namespace nc {
 
 constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_LOADERS = 128, LT_TMEM = 256;
@@ -25,6 +27,12 @@ constexpr int LT_HALF = LT_ROWS * 64;          // 128 rows of 64 bytes
 constexpr int LT_STAGES = 6;                   // of the first products at most
 constexpr int LT_BYTES = 216 * 1024;           // of tiles at most
 constexpr int LT_LINE = 272, LT_SLOT = LT_ROWS * LT_LINE;              // bytes from a row to the next of a tile of base: no bank twice in a quarter
+// Rows that a CTA adds up, whole fours, and of all CTAs' shares at most: the last one's may be shorter (six CTAs have 24 rows each).
+__host__ __device__ constexpr int lt_share(int ctas) { return (LT_ROWS / 4 + ctas - 1) / ctas * 4; }
+constexpr int LT_SUM_ROWS = 144;
+static_assert(2 * lt_share(2) <= LT_SUM_ROWS && 3 * lt_share(3) <= LT_SUM_ROWS && 4 * lt_share(4) <= LT_SUM_ROWS && 5 * lt_share(5) <= LT_SUM_ROWS &&
+                  6 * lt_share(6) <= LT_SUM_ROWS && 7 * lt_share(7) <= LT_SUM_ROWS && 8 * lt_share(8) <= LT_SUM_ROWS,
+              "room for the sums of every share");
 constexpr int LT_SLOTS = 4;                    // tiles of base on their way or in work, at most
 
 __device__ unsigned int g_lora_fault;          // set when a matrix instruction did not come to its end within the wait limit
@@ -61,7 +69,7 @@ inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
     p.slots = (LT_BYTES - p.slot_at) / LT_SLOT / 2 * 2;
     if (p.slots > LT_SLOTS) p.slots = LT_SLOTS;
     p.bytes = p.slot_at + p.slots * LT_SLOT;
-    const int sums = (LT_ROWS + 12) * (p.wide + 4) * 4, stage = S::PX * LT_BLOCK + S::PW * p.a_bytes;            // the last CTA's share may be shorter
+    const int sums = LT_SUM_ROWS * (p.wide + 4) * 4, stage = S::PX * LT_BLOCK + S::PW * p.a_bytes;
     p.sum_at = p.slot_at + 2 * LT_SLOT;
     p.early = p.sum_at + sums <= LT_BYTES && 2 * stage <= p.sum_at;
     if (!p.early) p.sum_at = p.b_at;
@@ -121,8 +129,11 @@ __device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t v) { asm vol
 __device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// Two values rounded to 16 bits, and what that leaves: nothing of what is no number.  What would round to an infinity is cut off.
 template <int TW>
+__device__ constexpr float lt_most() { return TW == KV_BF16 ? 3.3895314e38f : 65504.0f; }        // the largest number
+// Two values rounded to 16 bits, and what that leaves: nothing of an infinity.  What would round to an infinity is cut off.  SURE: neither is
+// larger than lt_most, nor an infinity.
+template <int TW, bool SURE = false>
 __device__ __forceinline__ uint32_t lt_part(float2 &v) {
     auto round = [](float2 f, float2 *r) {
         uint32_t w;
@@ -139,8 +150,8 @@ __device__ __forceinline__ uint32_t lt_part(float2 &v) {
     };
     float2 r;
     uint32_t w = round(v, &r);
-    if (!(fabsf(r.x) < INFINITY && fabsf(r.y) < INFINITY)) {
-        constexpr float most = TW == KV_BF16 ? 3.3895314e38f : 65504.0f;
+    if (!SURE && !(fabsf(r.x) < INFINITY && fabsf(r.y) < INFINITY)) {
+        constexpr float most = lt_most<TW>();
         auto cut = [](float f) { return fabsf(f) < INFINITY ? fminf(fmaxf(f, -most), most) : f; };
         w = round(make_float2(cut(v.x), cut(v.y)), &r);
         v.x = fabsf(r.x) < INFINITY ? fsub(v.x, r.x) : 0.0f;
@@ -189,16 +200,30 @@ __device__ __forceinline__ void lt_parts(F use) {
         for (int q = 0; q < Q; ++q)
             if (p + q < 3) use(p, q);
 }
+// use(std::true_type) where numbers up to `most` are sure, else use(std::false_type).
+template <int TW, typename F>
+__device__ __forceinline__ void lt_sure(float most, F use) {
+    if (most <= lt_most<TW>()) use(std::true_type());
+    else use(std::false_type());
+}
 // Eight float16 weights in two bfloat16 parts, which hold them exactly.
 __device__ __forceinline__ void lt_two_parts(const uint4 &w, uint4 *high, uint4 *low) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     uint32_t h[4], l[4];
+    float2 f[4];
+    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        h[i] = lt_part<KV_BF16>(f);
-        l[i] = lt_part<KV_BF16>(f);
+        f[i] = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        most = fmaxf(most, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
     }
+    lt_sure<KV_BF16>(most, [&](auto sure) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[i] = lt_part<KV_BF16, decltype(sure)::value>(f[i]);
+            l[i] = lt_part<KV_BF16, decltype(sure)::value>(f[i]);
+        }
+    });
     *high = make_uint4(h[0], h[1], h[2], h[3]);
     *low = make_uint4(l[0], l[1], l[2], l[3]);
 }
@@ -353,15 +378,23 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             };
             auto store = [&](int k, const LtBlock &block) {
                 const uint32_t at = base_at + (uint32_t)(k % plan.stages) * stage_bytes;
+                float most = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = line4 + 16 * i;
-                    const uint32_t to = at + (uint32_t)row * 128 + (uint32_t)(((c4 >> 1) ^ (row & 7)) << 4) + (uint32_t)(c4 & 1) * 8;
-                    float2 x = make_float2(block.x[i].x, block.x[i].y), y = make_float2(block.x[i].z, block.x[i].w);
+                for (int i = 0; i < 8; ++i)
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(block.x[i].x), fabsf(block.x[i].y))), fmaxf(fabsf(block.x[i].z), fabsf(block.x[i].w)));
+                lt_sure<KV_BF16>(most, [&](auto sure) {
 #pragma unroll
-                    for (int p = 0; p < S::PX; ++p)
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + p * LT_BLOCK), "r"(lt_part<KV_BF16>(x)), "r"(lt_part<KV_BF16>(y)) : "memory");
-                }
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = line4 + 16 * i;
+                        const uint32_t to = at + (uint32_t)row * 128 + (uint32_t)(((c4 >> 1) ^ (row & 7)) << 4) + (uint32_t)(c4 & 1) * 8;
+                        float2 x = make_float2(block.x[i].x, block.x[i].y), y = make_float2(block.x[i].z, block.x[i].w);
+#pragma unroll
+                        for (int p = 0; p < S::PX; ++p) {
+                            const uint32_t u = lt_part<KV_BF16, decltype(sure)::value>(x), v = lt_part<KV_BF16, decltype(sure)::value>(y);
+                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + p * LT_BLOCK), "r"(u), "r"(v) : "memory");
+                        }
+                    }
+                });
                 if constexpr (S::PW == 2) {
 #pragma unroll
                     for (int i = 0; i < LORA_PASS / 32; ++i) {
@@ -415,7 +448,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     __syncwarp();
     if (!plan.early) lora_cluster_arrive();    // this CTA is done with its stages: sums may lie over them
     lora_cluster_wait();
-    const int mine = (LT_ROWS / 4 + ctas - 1) / ctas * 4, pitch = plan.wide + 4;     // rows that a CTA adds up; the last one's may be fewer
+    const int mine = lt_share(ctas), pitch = plan.wide + 4;
     if (worker) {
         // The CTA's sums go to the CTAs that add them up: a row to a thread, 16 columns at a time, a half of them to a warp.
         const int row = 32 * (warp & 3) + lane;
@@ -488,17 +521,22 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                         back = __uint_as_float((exponent - 14) << 23);
 #pragma unroll
                         for (int m = 0; m < M; ++m) v[u][m].x = fmul(v[u][m].x, to), v[u][m].y = fmul(v[u][m].y, to);
+                        most = 1.0f;                               // some number
                     }
                     if (lane == 0) sh.row_scale[row] = back;
                 }
                 const uint32_t at = base_at + (uint32_t)(lane >> 4) * LT_HALF + (uint32_t)row * 64 + (uint32_t)(((lane >> 2 & 3) ^ ((row >> 1) & 3)) << 4) + (uint32_t)(lane & 3) * 4;
+                lt_sure<S::T>(most, [&](auto sure) {
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    if (!(keep >> (4 * m) & 4)) continue;
+                    for (int m = 0; m < M; ++m) {
+                        if (!(keep >> (4 * m) & 4)) continue;
 #pragma unroll
-                    for (int p = 0; p < S::PH; ++p)
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(lt_part<S::T>(v[u][m])) : "memory");
-                }
+                        for (int p = 0; p < S::PH; ++p) {
+                            const uint32_t w = lt_part<S::T, decltype(sure)::value>(v[u][m]);
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(p * plan.h_blocks + 2 * m) * LT_HALF), "r"(w) : "memory");
+                        }
+                    }
+                });
             }
         }
         lt_async_fence();

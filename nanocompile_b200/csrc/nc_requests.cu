@@ -38,6 +38,20 @@ int64_t lora_places(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t tile = lora_tile(rows, seqs, slots);
     return (rows + tile - 1) / tile + lora_groups(seqs, slots);
 }
+// Items of them at most: a group has a row at least.
+int lora_items_most(int64_t rows, int64_t seqs, int64_t slots) {
+    const int64_t groups = std::min(rows, lora_groups(seqs, slots));
+    return (int)(groups + (rows - groups) / lora_tile(rows, seqs, slots));
+}
+// Clusters of 1 to 8 CTAs that a B200 holds at once, with one CTA on an SM and with two: fewer than its SMs would hold, as a cluster lies
+// within one of its processing clusters, and for two twice as many, as they come to lie (32 clusters of 8: 26 us, 24 of them 16).  A
+// device with other processing clusters only has a rule that fits it less well.
+constexpr int CLUSTERS_ALONE[8] = {148, 74, 45, 33, 26, 22, 15, 15}, CLUSTERS_TWO[8] = {296, 148, 90, 66, 52, 44, 30, 30};
+// Rounds in which `clusters` of `n` CTAs run.
+int lora_rounds(int64_t clusters, int n, bool two) {
+    const int at_once = (two ? CLUSTERS_TWO : CLUSTERS_ALONE)[n - 1];
+    return (int)((clusters + at_once - 1) / at_once);
+}
 
 template <int TX, int TW, int NT>
 int32_t launch_lora(cudaStream_t st, const LoraArgs &a, int passes) {
@@ -67,20 +81,19 @@ int32_t launch_lora(cudaStream_t st, const LoraArgs &a, int passes) {
 // For items of eight rows.  False where a CTA's share of the inputs is too long, or its part of an adapter so small that the ring
 // takes longer than it saves (one row of 896 inputs to 1152 outputs at rank 16: 8.9 us without, 10.1 with).
 template <int TX, int TW>
-bool lora_stream_shape(const LoraArgs &a, int passes, int *ctas, LoraStreamPlan *plan) {
+bool lora_stream_shape(const LoraArgs &a, int passes, int items, int *ctas, LoraStreamPlan *plan) {
     using S = LoraStream<TX, TW>;
     const int units = (a.inputs + 31) / 32;
     const double bytes = 2.0 * a.rank * ((double)a.targets * a.inputs + a.outputs) / passes;
-    // CTAs of a cluster, by rounds of CTAs: 10 us to start and to add up, then bytes at 22 a ns for each of two on an SM, 30 alone.  Measured:
+    // CTAs of a cluster, by rounds: 10 us to start and to add up, then bytes at 22 a ns for each of two on an SM, 30 alone.  Measured:
     // 64 adapters of 1 MB 24 us by 4 CTAs, 44 by 8; 128 of them 46 by 4 with two on an SM, 58 by 2 alone.
     double best = 0.0;
     *ctas = 0;
-    for (int n = 8; n >= 1; n /= 2) {
+    for (int n = 8; n >= 1; --n) {
         const LoraStreamPlan p = lora_stream_plan(a.pass_targets, a.rank, (units + n - 1) / n * 32, S::PX, S::PH);
         if (!p.fits) break;
         const bool two = p.bytes <= LS_BYTES;
-        const int64_t clusters = (int64_t)a.items * passes * n, places = two ? 2 * 148 : 148;
-        const double cost = (double)((clusters + places - 1) / places) * (10.0 + 1e-3 * bytes / n / (two ? 22.0 : 30.0));
+        const double cost = lora_rounds((int64_t)items * passes, n, two) * (10.0 + 1e-3 * bytes / n / (two ? 22.0 : 30.0));
         if (*ctas != 0 && cost >= best) continue;
         best = cost;
         *ctas = n;
@@ -119,13 +132,23 @@ bool lora_tiles_shape(LoraArgs *a, LoraTilesPlan *plan) {
     return plan->slots >= 2 && plan->stages >= 2;
 }
 template <int TX, int TW>
-int32_t launch_lora_tiles(cudaStream_t st, const LoraArgs &a, const LoraTilesPlan &plan) {
+int32_t launch_lora_tiles(cudaStream_t st, const LoraArgs &a, int items, const LoraTilesPlan &plan) {
     auto kernel = lora_tiles_kernel<TX, TW>;
     static std::atomic<uint64_t> allowed{0};
     NC_TRY(allow_smem_once(kernel, LT_BYTES + 1024, &allowed));
     const int passes = (a.targets + a.pass_targets - 1) / a.pass_targets;
     const size_t bytes = (size_t)plan.bytes + 1024;
-    const int ctas = (int)std::clamp<int64_t>(148 / ((int64_t)a.items * passes), 1, 8);          // one on an SM
+    // CTAs of a cluster, one on an SM, by rounds: 14 us for what does not depend on an item's size, then its bytes.
+    const double size = TX == KV_F32 ? 4 : 2, rate = TX == KV_F32 ? 20.0 : 33.0;
+    const double moved = LT_ROWS * size * ((double)a.inputs + (a.base ? 2.0 : 1.0) * a.outputs / passes);
+    double best = 0.0;
+    int ctas = 0;
+    for (int n = 8; n >= 1; --n) {
+        const double cost = lora_rounds((int64_t)items * passes, n, false) * (14.0 + 1e-3 * moved / n / rate);
+        if (ctas != 0 && cost >= best) continue;
+        best = cost;
+        ctas = n;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.items * ctas), (unsigned)passes);
     cfg.blockDim = LT_THREADS;
@@ -143,23 +166,23 @@ int32_t launch_lora_tiles(cudaStream_t st, const LoraArgs &a, const LoraTilesPla
     return check_launch("lora_tiles_kernel");
 }
 template <int TX, int TW>
-int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes, bool tiles) {
+int32_t launch_lora_n(cudaStream_t st, const LoraArgs &a, int passes, int items, bool tiles) {
     if constexpr (TX == TW || TX == KV_F32)
         if (tiles) {
             LoraArgs t = a;
             LoraTilesPlan plan;
-            if (lora_tiles_shape<TX, TW>(&t, &plan)) return launch_lora_tiles<TX, TW>(st, t, plan);
+            if (lora_tiles_shape<TX, TW>(&t, &plan)) return launch_lora_tiles<TX, TW>(st, t, items, plan);
         }
     if (a.tile == 8) {
         int ctas;
         LoraStreamPlan plan;
-        if (lora_stream_shape<TX, TW>(a, passes, &ctas, &plan)) return launch_lora_stream<TX, TW>(st, a, passes, ctas, plan);
+        if (lora_stream_shape<TX, TW>(a, passes, items, &ctas, &plan)) return launch_lora_stream<TX, TW>(st, a, passes, ctas, plan);
     }
     return a.tile == 8 ? launch_lora<TX, TW, 1>(st, a, passes) : launch_lora<TX, TW, 4>(st, a, passes);
 }
 template <int TX>
-int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes, bool tiles) {
-    return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes, tiles) : launch_lora_n<TX, KV_BF16>(st, a, passes, tiles);
+int32_t launch_lora_w(cudaStream_t st, const LoraArgs &a, int passes, int items, bool tiles) {
+    return a.wtype == KV_F16 ? launch_lora_n<TX, KV_F16>(st, a, passes, items, tiles) : launch_lora_n<TX, KV_BF16>(st, a, passes, items, tiles);
 }
 
 }  // namespace
@@ -276,8 +299,9 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     const int passes = (int)((targets + a.pass_targets - 1) / a.pass_targets);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool tiles = a.tile == LT_ROWS && a.x_vectors && targets * rank * inputs <= I32;
-    return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes, tiles) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes, tiles)
-                                                                                         : launch_lora_w<KV_BF16>(st, a, passes, tiles);
+    const int items = lora_items_most(rows, seqs, slots);
+    return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes, items, tiles) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes, items, tiles)
+                                                                                                : launch_lora_w<KV_BF16>(st, a, passes, items, tiles);
 }
 
 // ---- beams --------------------------------------------------------------------------------------

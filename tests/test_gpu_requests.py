@@ -272,6 +272,19 @@ def test_a_plan_serves_many_projections_and_streams(cuda):
         case.check(out.cpu().numpy())
 
 
+@pytest.mark.parametrize("dtype,wtype", [("float32", BF16), ("float16", "float16"), (BF16, BF16)])
+@pytest.mark.parametrize("items", [1, 15, 16, 22, 26, 33, 45, 74, 148, 149])
+def test_prompts_of_every_cluster_size(cuda, dtype, wtype, items):
+    """Rows of one adapter in so many whole items of 128, and one row more."""
+    Adapted(17, dtype, wtype, 136, (64, 72), 80, 1, [0], [128 * (items - 1) + 1]).run().check()
+
+
+@pytest.mark.parametrize("dtype,wtype", [("float32", BF16), (BF16, BF16)])
+@pytest.mark.parametrize("seqs", [1, 15, 33, 37, 45, 56, 71, 93, 148, 296, 300])
+def test_single_tokens_of_every_cluster_size(cuda, dtype, wtype, seqs):
+    Adapted(18, dtype, wtype, 1024, (256, 40), 32, seqs, list(range(seqs)), [1] * seqs).run().check()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("inputs,widths,rank,counts", [(64, (32, 7), 8, [1] * 4), (4864, (896,), 64, [1] * 4), (256, (160, 33), 32, [90, 3, 200, 1])])
 def test_adapters_of_rank_nought_are_none(cuda, dtype, inputs, widths, rank, counts):
