@@ -294,6 +294,8 @@ int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
  * What a slot holds past ranks[a] does not count.  Rows of sequences without an adapter, or with one of rank 0, are base's (nought
  * without base).
  *
+ * An infinity or a NaN in x makes its row's outputs such (a NaN also of an infinity, beside float16 adapters).
+ *
  * The plan: the rows of a call grouped by adapter, made once for all projections and layers of a batch.  Adapters outside
  * 0 .. slots - 1 are none; the smallest sequence with one from `slots` on is put into the error word.  Rows outside
  * row_start[0] .. row_start[seqs] - 1 are left as they are by the projections.

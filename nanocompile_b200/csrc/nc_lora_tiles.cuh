@@ -210,20 +210,14 @@ __device__ __forceinline__ void lt_sure(float most, F use) {
 __device__ __forceinline__ void lt_two_parts(const uint4 &w, uint4 *high, uint4 *low) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     uint32_t h[4], l[4];
-    float2 f[4];
-    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[i] = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-        most = fmaxf(most, fmaxf(fabsf(f[i].x), fabsf(f[i].y)));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+        float2 rest = f;
+        h[i] = lt_part<KV_BF16, true>(rest);
+        rest = make_float2(fabsf(f.x) < INFINITY ? rest.x : 0.0f, fabsf(f.y) < INFINITY ? rest.y : 0.0f);
+        l[i] = lt_part<KV_BF16, true>(rest);
     }
-    lt_sure<KV_BF16>(most, [&](auto sure) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[i] = lt_part<KV_BF16, decltype(sure)::value>(f[i]);
-            l[i] = lt_part<KV_BF16, decltype(sure)::value>(f[i]);
-        }
-    });
     *high = make_uint4(h[0], h[1], h[2], h[3]);
     *low = make_uint4(l[0], l[1], l[2], l[3]);
 }
@@ -354,16 +348,19 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 lt_arrive(&sh.full[k % plan.stages]);
             }
         } else {
-            // float32 rows go through registers, a block ahead: four values of every 16th row to a thread, split into parts on the way.
+            // float32 rows go through registers, a block ahead: four values of every 16th row to a thread, split into parts on the way.  Few
+            // instructions count here, more than loads further ahead: 8192 rows 4096 -> 6144 take 165 us, 178 with two blocks ahead, 172 with
+            // the loop unrolled and the parts of seldom numbers in it.
             const int c4 = tid & 15, line4 = tid >> 4;
+            auto fetch = [&](int k, int i) {
+                const int e = (k_low + k) * 64 + 4 * c4, row = sh.row[line4 + 16 * i];
+                return row >= 0 && e < a.inputs ? __ldg((const float4 *)((const float *)a.x + (int64_t)row * a.x_stride + e)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            };
             auto load = [&](int k, LtBlock &block) {
-                const int e = (k_low + k) * 64 + 4 * c4;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = sh.row[line4 + 16 * i];
-                    block.x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (row >= 0 && e < a.inputs) block.x[i] = __ldg((const float4 *)((const float *)a.x + (int64_t)row * a.x_stride + e));
-                }
+                for (int i = 0; i < 8; ++i) block.x[i] = fetch(k, i);
+            };
+            auto load_a = [&](int k, LtBlock &block) {
                 if constexpr (S::PW == 1) {
                     ask_a(k);
                 } else {
@@ -382,19 +379,21 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     most = fmaxf(fmaxf(most, fmaxf(fabsf(block.x[i].x), fabsf(block.x[i].y))), fmaxf(fabsf(block.x[i].z), fabsf(block.x[i].w)));
-                lt_sure<KV_BF16>(most, [&](auto sure) {
+                auto put = [&](int i, const float4 &from, auto sure) {
+                    const int row = line4 + 16 * i;
+                    const uint32_t to = at + (uint32_t)row * 128 + (uint32_t)(((c4 >> 1) ^ (row & 7)) << 4) + (uint32_t)(c4 & 1) * 8;
+                    float2 x = make_float2(from.x, from.y), y = make_float2(from.z, from.w);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = line4 + 16 * i;
-                        const uint32_t to = at + (uint32_t)row * 128 + (uint32_t)(((c4 >> 1) ^ (row & 7)) << 4) + (uint32_t)(c4 & 1) * 8;
-                        float2 x = make_float2(block.x[i].x, block.x[i].y), y = make_float2(block.x[i].z, block.x[i].w);
-#pragma unroll
-                        for (int p = 0; p < S::PX; ++p) {
-                            const uint32_t u = lt_part<KV_BF16, decltype(sure)::value>(x), v = lt_part<KV_BF16, decltype(sure)::value>(y);
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + p * LT_BLOCK), "r"(u), "r"(v) : "memory");
-                        }
+                    for (int p = 0; p < S::PX; ++p) {
+                        const uint32_t u = lt_part<KV_BF16, decltype(sure)::value>(x), v = lt_part<KV_BF16, decltype(sure)::value>(y);
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + p * LT_BLOCK), "r"(u), "r"(v) : "memory");
                     }
-                });
+                };
+#pragma unroll
+                for (int i = 0; i < 8; ++i) put(i, block.x[i], std::true_type());
+                if (!(most <= lt_most<KV_BF16>()))                     // seldom: once more, in few instructions
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) put(i, fetch(k, i), std::false_type());
                 if constexpr (S::PW == 2) {
 #pragma unroll
                     for (int i = 0; i < LORA_PASS / 32; ++i) {
@@ -407,10 +406,14 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                     }
                 }
             };
-            auto step = [&](int k, const LtBlock &now, LtBlock &next) {
+            LtBlock now, next;
+            if (k_blocks > 0) load(0, now), load_a(0, now);
+#pragma unroll 1
+            for (int k = 0; k < k_blocks; ++k) {
                 if (k + 1 < k_blocks) {
+                    load(k + 1, next);                                 // before the wait: 8192 rows 194 us behind it
                     if (k + 1 >= plan.stages) wait(&sh.empty[(k + 1) % plan.stages], ((k + 1) / plan.stages - 1) & 1);
-                    load(k + 1, next);
+                    load_a(k + 1, next);
                 } else {
                     lt_commit();
                 }
@@ -418,12 +421,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 lt_wait_copies<1>();
                 lt_async_fence();
                 lt_arrive(&sh.full[k % plan.stages]);
-            };
-            LtBlock even, odd;
-            if (k_blocks > 0) load(0, even);
-            for (int k = 0; k < k_blocks; k += 2) {
-                step(k, even, odd);
-                if (k + 1 < k_blocks) step(k + 1, odd, even);
+                now = next;
             }
         }
         lt_wait_copies<0>();

@@ -38,10 +38,10 @@ int64_t lora_places(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t tile = lora_tile(rows, seqs, slots);
     return (rows + tile - 1) / tile + lora_groups(seqs, slots);
 }
-// Items of them at most: a group has a row at least.
-int lora_items_most(int64_t rows, int64_t seqs, int64_t slots) {
-    const int64_t groups = std::min(rows, lora_groups(seqs, slots));
-    return (int)(groups + (rows - groups) / lora_tile(rows, seqs, slots));
+// Items that are to be expected of them: one to a group, or half an item for the end of each.
+int lora_items(int64_t rows, int64_t seqs, int64_t slots) {
+    const int64_t groups = std::min(rows, lora_groups(seqs, slots)), tile = lora_tile(rows, seqs, slots);
+    return (int)std::max(groups, (2 * rows + tile * groups + 2 * tile - 1) / (2 * tile));
 }
 // Clusters of 1 to 8 CTAs that a B200 holds at once, with one CTA on an SM and with two: fewer than its SMs would hold, as a cluster lies
 // within one of its processing clusters, and for two twice as many, as they come to lie (32 clusters of 8: 26 us, 24 of them 16).  A
@@ -93,7 +93,9 @@ bool lora_stream_shape(const LoraArgs &a, int passes, int items, int *ctas, Lora
         const LoraStreamPlan p = lora_stream_plan(a.pass_targets, a.rank, (units + n - 1) / n * 32, S::PX, S::PH);
         if (!p.fits) break;
         const bool two = p.bytes <= LS_BYTES;
-        const double cost = lora_rounds((int64_t)items * passes, n, two) * (10.0 + 1e-3 * bytes / n / (two ? 22.0 : 30.0));
+        const int rounds = lora_rounds((int64_t)items * passes, n, two);
+        if (rounds > 1 && (n & (n - 1))) continue; // clusters of odd sizes do not take each other's places: 200 adapters of 1 MB 97 us by 3, 79 by 4
+        const double cost = rounds * (10.0 + 1e-3 * bytes / n / (two ? 22.0 : 30.0));
         if (*ctas != 0 && cost >= best) continue;
         best = cost;
         *ctas = n;
@@ -299,7 +301,7 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     const int passes = (int)((targets + a.pass_targets - 1) / a.pass_targets);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool tiles = a.tile == LT_ROWS && a.x_vectors && targets * rank * inputs <= I32;
-    const int items = lora_items_most(rows, seqs, slots);
+    const int items = lora_items(rows, seqs, slots);
     return type == KV_F32 ? launch_lora_w<KV_F32>(st, a, passes, items, tiles) : type == KV_F16 ? launch_lora_w<KV_F16>(st, a, passes, items, tiles)
                                                                                                 : launch_lora_w<KV_BF16>(st, a, passes, items, tiles);
 }

@@ -206,6 +206,22 @@ def test_an_infinity_is_one_in_float32(cuda):
     assert np.allclose(case.run().d_out.numpy(), case.x[0, 7], rtol=2.0 ** -22)
 
 
+@pytest.mark.parametrize("wtype", [BF16, "float16"])
+@pytest.mark.parametrize("count", [8, 300])
+def test_the_largest_numbers_of_float32_rows(cuda, wtype, count):
+    """What rounds to an infinity in 16 bits, and an infinity."""
+    case = Adapted(16, "float32", wtype, 64, (32,), 8, 1, [0], [count], base=False, scales=False)
+    case.a[...], case.b[...] = 1, 0
+    case.b[..., 0] = 1
+    case.x[1], case.x[2], case.x[5, 9] = 0, 0, np.inf
+    case.x[1, 7], case.x[2, 40] = 3.4e38, -3.39e38
+    got = case.run().d_out.numpy()
+    assert np.allclose(got[1], 3.4e38, rtol=2.0 ** -22) and np.allclose(got[2], -3.39e38, rtol=2.0 ** -22)
+    assert np.isnan(got[5]).all()                                        # every h is infinite, and seven of them are multiplied by 0
+    case.x[5] = got[5] = 0
+    case.check(got)
+
+
 def test_adapters_outside_the_slots_are_none_and_recorded(cuda):
     error = error_word()
     case = Adapted(8, "float32", BF16, 64, (32,), 8, 3, [1, 7, -5, 3, 2], [1, 2, 1, 1, 4]).run(error=error)
