@@ -7,6 +7,10 @@
 // units of 32 inputs, or two tiles of 16 outputs, at once: with one, its chain of loads, products and sums took as long.  The rows' shares
 // of x are in shared memory from the start, as operands, and those of base where they fit.
 //
+// Bound by the adapters' bytes where each request has its own, beside a start of 10 us (the plan's words, x as operands, the sums'
+// way through the cluster).  Adapters of 4096 inputs and outputs at rank 64 (1 MB each), bfloat16, with the plan: one 11.7 us, 16
+// of them 14.5, 64 23.5 (2.9 TB/s), 128 45 (3.0 TB/s of 6.5: two rounds of clusters; 67 with one tile of outputs to a warp at a time).
+//
 // Accuracy.  Products are mma m16n8k16 of the weights' type.  Rows of that type are taken as they are, others and h go in parts: three of
 // bfloat16 for float32 rows (2^-27 is lost), else two (bfloat16: 2^-18, beside outputs of 8 bits; float16: 2^-24).  For
 // float16 a row of x or h is first brought to [2^14, 2^15) by a power of two, so that no size leaves its range.  A chain of

@@ -8,6 +8,11 @@
 // memory, a row to a thread, and store it, whole rows to half a warp; four others have the next tile.  The targets' h lie side by side,
 // whole 16s to each.
 //
+// Bound by the bytes of x, base and outputs, behind 14 us that no size takes away (tensor memory, two ways through the cluster).  8192
+// bfloat16 rows of 4096 inputs to 6144 outputs at rank 32: 82 us (3.3 TB/s of 6.5; its products are 21 GFLOP, 13 us); 512 of them 30; float32
+// rows 164 (3.3 TB/s), beside float16 weights 226.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
+// by the warps that add it 122, in bulk copies of a row each 201.
+//
 // Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-18 of it is lost, float16 2^-24; float16's
 // h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its range).  float32 rows and their h go
 // in three bfloat16 parts (2^-27 is lost), float16 weights beside them in two, which are exact.  Sums are float32 in tensor memory.
@@ -577,9 +582,44 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     if (warp > LT_MMA) {
         // B's rows in blocks of 32, 64 bytes each, 16 of every 32nd row to a thread; base's rows, 16 bytes of every eighth to a thread.
         const int at = tid - LT_WORKERS - 32, bc = at & 3, bl = at >> 2, cc = at & 15, cl = at >> 4;
+        // float16 weights beside float32 rows go through registers, a tile ahead.
+        constexpr int BN = S::PW == 2 ? S::COLS / 32 : 1, BJ = S::PW == 2 ? LORA_RANK / 32 : 1;
+        uint4 held[BN][BJ];
+        auto fetch_b = [&](int n0) {
+#pragma unroll
+            for (int n = 0; n < BN; ++n)
+#pragma unroll
+                for (int j = 0; j < BJ; ++j) {
+                    held[n][j] = make_uint4(0, 0, 0, 0);
+                    if (32 * j + 8 * bc < r && n0 + bl + 32 * n < a.width[target])
+                        held[n][j] = __ldg((const uint4 *)(wb + (((int64_t)n_target + n0 + bl + 32 * n) * a.rank + 32 * j + 8 * bc) * 2));
+                }
+        };
+        // What lies past the adapter's own rank may be anything.
+        auto within = [&](const uint4 &w, int j) {
+            uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = j + 2 * e >= r ? 0u : j + 2 * e + 1 >= r ? u[e] & 0xffffu : u[e];
+            return make_uint4(u[0], u[1], u[2], u[3]);
+        };
         auto issue_b = [&](int i, int n0) {
             const uint32_t to = base_at + plan.b_at + (uint32_t)(i & 1) * b_bytes;
-            if (S::PW == 1 && r == rp && n0 + S::COLS <= a.width[target]) {
+            if constexpr (S::PW == 2) {
+#pragma unroll
+                for (int n = 0; n < BN; ++n)
+#pragma unroll
+                    for (int j = 0; j < BJ; ++j) {
+                        if (32 * j + 8 * bc >= rp) continue;
+                        const uint32_t dst = to + (uint32_t)(j * S::COLS + bl + 32 * n) * 64 + (uint32_t)((bc ^ ((bl >> 1) & 3)) << 4);
+                        uint4 high, low;
+                        lt_two_parts(within(held[n][j], 32 * j + 8 * bc), &high, &low);
+                        store16_shared(dst, high.x, high.y, high.z, high.w);
+                        store16_shared(dst + b_part, low.x, low.y, low.z, low.w);
+                    }
+                lt_commit();
+                return;
+            }
+            if (r == rp && n0 + S::COLS <= a.width[target]) {
                 const char *const from = wb + (((int64_t)n_target + n0 + bl) * a.rank + 8 * bc) * 2;
                 const uint32_t dst = to + (uint32_t)bl * 64 + (uint32_t)((bc ^ ((bl >> 1) & 3)) << 4);     // the same for every 32nd row
                 for (int j = 0; 8 * bc + j < rp; j += 32)
@@ -594,44 +634,17 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                     const uint32_t dst = to + (uint32_t)(j >> 5) * (S::COLS * 64) + (uint32_t)n * 64 + (uint32_t)((bc ^ ((n >> 1) & 3)) << 4);
                     const char *const from = wb + (((int64_t)n_target + n0 + n) * a.rank + j) * 2;
                     const bool there = n0 + n < a.width[target];
-                    if (S::PW == 1 && (j + 8 <= r || j >= r || !there)) {
+                    if (j + 8 <= r || j >= r || !there) {
                         lt_copy16(dst, there && j < r ? from : wb, there && j < r ? 16 : 0);
-                    } else {                                           // what lies past the adapter's own rank may be anything
-                        const uint4 w = there && j < r ? __ldg((const uint4 *)from) : make_uint4(0, 0, 0, 0);
-                        uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] = j + 2 * e >= r ? 0u : j + 2 * e + 1 >= r ? u[e] & 0xffffu : u[e];
-                        if constexpr (S::PW == 1) {
-                            store16_shared(dst, u[0], u[1], u[2], u[3]);
-                        } else {
-                            uint4 high, low;
-                            lt_two_parts(make_uint4(u[0], u[1], u[2], u[3]), &high, &low);
-                            store16_shared(dst, high.x, high.y, high.z, high.w);
-                            store16_shared(dst + b_part, low.x, low.y, low.z, low.w);
-                        }
+                    } else {
+                        const uint4 w = within(__ldg((const uint4 *)from), j);
+                        store16_shared(dst, w.x, w.y, w.z, w.w);
                     }
                 }
             lt_commit();
         };
-        // Tile i's B is waited for once the next one's is asked for; base is asked for as slots become free, and its copies
-        // report to the slot's barrier themselves.
         const bool all_rows = count == LT_ROWS;
-        const int late = plan.early ? min(2, my_tiles) : 0;            // the first tile that lies over the sums
-        for (int i = 0; i <= my_tiles; ++i) {
-            int n0 = 0;
-            if (i == late) asm volatile("bar.sync 2, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");
-            if (i < my_tiles) {
-                if (i >= 2) wait(&sh.d2_done[i & 1], ((i >> 1) - 1) & 1);
-                n0 = look_up(i);
-                issue_b(i, n0);
-            }
-            if (i > 0) {
-                if (i < my_tiles) lt_wait_copies<1>();
-                else lt_wait_copies<0>();
-                lt_async_fence();
-                lt_arrive(&sh.b_full[(i - 1) & 1]);
-            }
-            if (i == my_tiles || !staged || !a.base) continue;
+        auto ask_base = [&](int i, int n0) {
             const int slot_i = i % plan.slots, left = a.width[target] - n0;
             if (i >= plan.slots) wait(&sh.slot_free[slot_i], (i / plan.slots - 1) & 1);
             const uint32_t to = base_at + plan.slot_at + (uint32_t)(slot_i * LT_SLOT + cc * 16);
@@ -647,6 +660,30 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                     if (row >= 0) lt_copy16(to + k * LT_LINE, from + (int64_t)row * a.base_stride * S::SIZE, 16);
                 }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(kvt_smem(&sh.slot_full[slot_i])) : "memory");
+        };
+        // Tile i's B is waited for once the next one's is asked for; base is asked for as slots become free, and its copies
+        // report to the slot's barrier themselves.
+        const int late = plan.early ? min(2, my_tiles) : 0;            // the first tile that lies over the sums
+        if constexpr (S::PW == 2)
+            if (my_tiles > 0) fetch_b(look_up(0));
+        for (int i = 0; i <= my_tiles; ++i) {
+            int n0 = 0;
+            if (i == late) asm volatile("bar.sync 2, %0;" ::"n"(LT_WORKERS + LT_LOADERS) : "memory");
+            if (i < my_tiles) {
+                if (i >= 2) wait(&sh.d2_done[i & 1], ((i >> 1) - 1) & 1);
+                n0 = look_up(i);
+                issue_b(i, n0);
+            }
+            if (i > 0) {
+                if (i < my_tiles) lt_wait_copies<1>();
+                else lt_wait_copies<0>();
+                lt_async_fence();
+                lt_arrive(&sh.b_full[(i - 1) & 1]);
+            }
+            if (i == my_tiles) break;
+            if (staged && a.base) ask_base(i, n0);
+            if constexpr (S::PW == 2)
+                if (i + 1 < my_tiles) fetch_b(look_up(i + 1));
         }
         lt_wait_copies<0>();
         __syncwarp();
