@@ -4,8 +4,8 @@
 //   out[r, n] = base[r, n] + scale[s] sum_j B[s, n, j] h[j],   h[j] = sum_k A[s, t rank + j, k] x[r, k],   j < ranks[s].
 //
 // The plan groups a call's rows by adapter: sequences sorted by adapter (a bitonic sort in shared memory, in their order among
-// equals), rows counted along them, and the groups cut into items of up to `tile` rows.  Group g's j-th item, from its
-// start s_g in the order, has the place (s_g + j tile) / tile + g: distinct, below rows / tile + groups, found without a sum over items.
+// equals), rows counted along them, and the groups cut into items of up to `tile` rows, one after another: places for items that there might
+// have been come last, so that their clusters take no other's room (64 adapters of 1 MB for two rows each: 38 us with them in between).
 // One CTA, bound by its barriers: 4.8 us for 64 sequences, 87 for 8192, once for all layers and projections of a batch.
 //
 // An item to a cluster of CTAs, in one launch: each multiplies its share of the inputs k, the CTAs add their sums of h through
@@ -66,11 +66,11 @@ __device__ __forceinline__ int lora_scan(int v, int *sums) {
     return v;
 }
 
-// One CTA.  Shared memory: size keys, then size + 1 row offsets, group starts and group adapters.
+// One CTA.  Shared memory: size keys, then size + 1 row offsets, group starts, group adapters and the groups' first items.
 __global__ void __launch_bounds__(1024, 1) lora_plan_kernel(const __grid_constant__ LoraPlanArgs a) {
     extern __shared__ __align__(16) char lora_smem[];
     unsigned long long *const key = (unsigned long long *)lora_smem;
-    int *const offset = (int *)(key + a.size), *const start = offset + a.size + 1, *const group = start + a.size + 1;
+    int *const offset = (int *)(key + a.size), *const start = offset + a.size + 1, *const group = start + a.size + 1, *const place = group + a.size + 1;
     __shared__ int sums[33];
     const int tid = threadIdx.x, threads = blockDim.x;
     release_dependents();
@@ -126,18 +126,28 @@ __global__ void __launch_bounds__(1024, 1) lora_plan_kernel(const __grid_constan
         a.plan[1] = groups;
     }
     __syncthreads();
+    int count = 0;                                                 // of items
+    for (int base = 0; base < groups; base += threads) {
+        const int i = base + tid, n = i < groups ? max(0, start[i + 1] - start[i] + a.tile - 1) / a.tile : 0;
+        const int upto = lora_scan(n, sums) + count;
+        if (i < groups) place[i] = upto - n;
+        if (tid == threads - 1) sums[32] = upto;
+        __syncthreads();
+        count = sums[32];
+        __syncthreads();
+    }
     int4 *const items = lora_items(a.plan);
     for (int i = tid; i < a.items; i += threads) {
-        int low = 0, high = groups;                                // the last group whose first place is i or before
+        int low = 0, high = groups;                                // the last group whose first item is i or before: those without rows have none
         while (high - low > 1) {
             const int mid = (low + high) >> 1;
-            if (start[mid] / a.tile + mid <= i) low = mid;
+            if (place[mid] <= i) low = mid;
             else high = mid;
         }
         int4 item = make_int4(-1, 0, 0, 0);
-        if (groups > 0) {
-            const int at = start[low] + (i - (start[low] / a.tile + low)) * a.tile;
-            if (at < start[low + 1]) item = make_int4(group[low] < a.slots ? group[low] : -1, at, min(a.tile, start[low + 1] - at), 0);
+        if (i < count) {
+            const int at = start[low] + (i - place[low]) * a.tile;
+            item = make_int4(group[low] < a.slots ? group[low] : -1, at, min(a.tile, start[low + 1] - at), 0);
         }
         items[i] = item;
     }

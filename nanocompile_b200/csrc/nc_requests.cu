@@ -32,16 +32,19 @@ int64_t lora_groups(int64_t seqs, int64_t slots) { return std::min(seqs, slots +
 // Rows of an item: by the mean of the largest number of groups, as only the device knows how many there are.
 int64_t lora_tile(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t mean = rows / std::max<int64_t>(1, lora_groups(seqs, slots));
-    return mean <= 32 ? 8 : 128;               // the few items of an adapter read it from L2: 128 rows of 8 adapters of 1 MB 16 us by eights, 25 by 16 rows
+    // The few items of an adapter by eights read it from L2.  Adapters of 45 KB, 64 of them for 16 rows each: 17 us by eights, 37 by 128; of 1 MB,
+    // 8 of them for 16 rows each 30 and 25, 24 rows each 31 and 25.
+    return mean <= 16 ? 8 : 128;
 }
+// Items at most: a group that has any has a row.
 int64_t lora_places(int64_t rows, int64_t seqs, int64_t slots) {
-    const int64_t tile = lora_tile(rows, seqs, slots);
-    return (rows + tile - 1) / tile + lora_groups(seqs, slots);
+    const int64_t groups = std::min(rows, lora_groups(seqs, slots));
+    return groups + (rows - groups) / lora_tile(rows, seqs, slots);
 }
 // Items that are to be expected of them: one to a group, or half an item for the end of each.
 int lora_items(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t groups = std::min(rows, lora_groups(seqs, slots)), tile = lora_tile(rows, seqs, slots);
-    return (int)std::max(groups, (2 * rows + tile * groups + 2 * tile - 1) / (2 * tile));
+    return (int)std::min(lora_places(rows, seqs, slots), std::max(groups, (2 * rows + tile * groups + 2 * tile - 1) / (2 * tile)));
 }
 // Clusters of 1 to 8 CTAs that a B200 holds at once, with one CTA on an SM and with two: fewer than its SMs would hold, as a cluster lies
 // within one of its processing clusters, and for two twice as many, as they come to lie (32 clusters of 8: 26 us, 24 of them 16).  A
@@ -232,9 +235,9 @@ extern "C" int32_t nc_lora_plan(void **p, const int64_t *s, void *stream) {
     // Threads for the longer of the sort's pairs, the items and the rows, as barriers of fewer warps are cheaper.
     const int64_t work = std::max<int64_t>({a.size / 2, a.items, rows / 4});
     const unsigned threads = work <= 128 ? 128 : work <= 256 ? 256 : work <= 512 ? 512 : 1024;
-    const size_t bytes = (size_t)a.size * 8 + (size_t)3 * 4 * (a.size + 1);
+    const size_t bytes = (size_t)a.size * 8 + (size_t)4 * 4 * (a.size + 1);
     static std::atomic<uint64_t> allowed{0};
-    NC_TRY(allow_smem_once(lora_plan_kernel, (size_t)LORA_SEQS * 8 + (size_t)3 * 4 * (LORA_SEQS + 1), &allowed));
+    NC_TRY(allow_smem_once(lora_plan_kernel, (size_t)LORA_SEQS * 8 + (size_t)4 * 4 * (LORA_SEQS + 1), &allowed));
     CUDA_TRY(launch_k(lora_plan_kernel, 1, threads, bytes, (cudaStream_t)stream, a));
     return check_launch("lora_plan_kernel");
 }

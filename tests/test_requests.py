@@ -68,7 +68,8 @@ def test_plans_refuse(change, what):
 
 def test_plan_bytes_hold_every_item_and_row():
     for rows, seqs, slots in ((1, 1, 1), (64, 64, 8), (8192, 8, 5), (8192, 8192, 10000), (0, 0, 1)):
-        assert serving.LoraBatch(rows, seqs, slots).plan_bytes >= 4 * rows + 16 * (rows // 128 + min(seqs, slots + 1))
+        groups = min(rows, seqs, slots + 1)                              # with a row each; the others fill whole items at best
+        assert serving.LoraBatch(rows, seqs, slots).plan_bytes >= 4 * rows + 16 * (groups + (rows - groups) // 128)
 
 
 @pytest.mark.parametrize("change,what", [
