@@ -12,8 +12,8 @@
 // distributed shared memory, in the order of the CTAs, and each expands its share of the outputs.  Three kernels do so: for items of up
 // to eight rows with much to read nc_lora_stream.cuh, for 128 rows nc_lora_tiles.cuh, and for the others the one here.
 //
-// lora_rows_kernel: weights are the matrix instruction's 16 rows, eight rows of x its columns (NT = 1), or 32 rows (NT = 4) where 128 are of
-// 16-bit types other than the weights', or their vectors are not aligned.  Weights go straight into operands, B's share is asked of L2
+// lora_rows_kernel: weights are the matrix instruction's 16 rows, eight rows of x its columns (NT = 1), or 32 rows (NT = 4) where the 128 of an item
+// are of a 16-bit type other than the weights', not aligned, or of a rank that leaves no room.  Weights go straight into operands, B's share is asked of L2
 // at the start.  Bound by its chain of dependent loads: one row of 896 inputs to 1152 outputs at rank 16 takes 8.8 us with the plan.
 //
 // Accuracy.  Products are mma m16n8k8 tf32: 16-bit weights and rows are tf32 numbers as they are, float32 rows and h go in two parts
