@@ -173,7 +173,7 @@ struct LoraArgs {
     const int32_t *plan, *ranks;               // ranks: [slots] or null
     const float *scales;                       // [slots] or null
     int64_t x_stride, base_stride, out_stride;
-    int rows, items, tile, inputs, outputs, rank, slots, targets, pass_targets, type, wtype;
+    int rows, items, tile, inputs, outputs, rank, slots, targets, pass_targets, wtype;
     int x_vectors, pairs, wide;                // 16-byte loads of x; two outputs to an access; 16 bytes of them
     int width[LORA_TARGETS];
 };

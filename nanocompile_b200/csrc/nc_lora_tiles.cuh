@@ -115,7 +115,6 @@ __device__ __forceinline__ uint64_t lt_desc64(uint32_t address) {
     return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
 }
 __device__ __forceinline__ void lt_async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void lt_async_fence_cluster() { asm volatile("fence.proxy.async.shared::cluster;" ::: "memory"); }
 // 16 bytes from `from`, of which `bytes` are there: the others become nought.
 __device__ __forceinline__ void lt_copy16(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -130,7 +129,6 @@ __device__ __forceinline__ uint32_t lt_peer(uint32_t at, uint32_t rank) {       
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void lt_store_peer(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }

@@ -293,7 +293,6 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     a.rank = (int)rank;
     a.slots = (int)slots;
     a.targets = (int)targets;
-    a.type = (int)type;
     a.wtype = (int)wtype;
     a.x_vectors = !misaligned(a.x, 16) && !misaligned(a.x_stride * bytes, 16);
     a.pairs = even && !misaligned(a.out, 2 * bytes) && !misaligned(a.base, 2 * bytes) && a.out_stride % 2 == 0 && (!a.base || a.base_stride % 2 == 0);

@@ -321,6 +321,27 @@ def test_adapters_of_rank_nought_are_none(cuda, dtype, inputs, widths, rank, cou
     case.check(in_place)
 
 
+def test_calls_on_two_streams_at_once(cuda):
+    """Plans and projections of different kernels, each stream with a plan of its own."""
+    torch = pytest.importorskip("torch")
+    cases = [Adapted(19, "float32", BF16, 512, (256, 64), 32, 3, [0, 2, 1], [300, 5, 200]), Adapted(20, BF16, BF16, 1024, (512,), 64, 40, list(range(40)), [1] * 40),
+             Adapted(21, "float16", "float16", 256, (640,), 16, 2, [1, 0], [700, 129]), Adapted(22, "float32", "float16", 64, (48,), 8, 4, [3, -1, 0], [1, 1, 1])]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for case in cases:
+        case.run()                                                       # its arrays
+    torch.cuda.synchronize()
+    for case in cases:
+        case.d_out.upload(np.zeros_like(case.d_out.numpy()))
+    for _ in range(20):
+        for case, stream in zip(cases, streams):
+            serving.lora_plan(case.batch, case.plan, case.d_adapters, row_start=case.d_start, stream=stream.cuda_stream)
+            serving.lora_project(case.layout, case.batch, case.d_out, case.d_x, case.d_a, case.d_b, case.plan, base=case.d_base, scales=case.d_scales,
+                                 stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for case in cases:
+        case.check()
+
+
 # -- beams -----------------------------------------------------------------------------------------------------
 
 
