@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     }
     if (tid < LT_ROWS) sh.row[tid] = my_row;
     kvt_before();
-    __syncthreads();
+    const bool all_rows = __syncthreads_and(tid >= LT_ROWS || my_row >= 0);    // 128 of them, and each is one of the call
     kvt_after();
     release_dependents();                      // not before this CTA has its tensor memory: a dependent may hold all the rest
     if (plan.early) lora_cluster_arrive();     // this CTA is there: peers may write to its shared memory
@@ -641,7 +641,6 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 }
             lt_commit();
         };
-        const bool all_rows = count == LT_ROWS;
         auto ask_base = [&](int i, int n0) {
             const int slot_i = i % plan.slots, left = a.width[target] - n0;
             if (i >= plan.slots) wait(&sh.slot_free[slot_i], (i / plan.slots - 1) & 1);

@@ -251,6 +251,28 @@ def test_a_row_start_that_does_not_ascend_stays_in_bounds(cuda):
     case.run().d_out.numpy()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts,inputs,rank", [([1] * 9, 256, 16), ([1] * 9, 4096, 32), ([300], 256, 16), ([128, 1, 256], 256, 16)])
+def test_rows_of_a_plan_that_are_none_of_the_call(cuda, dtype, counts, inputs, rank):
+    """They are neither read nor written, wherever they lie in an item: a plan's last words are its rows."""
+    case = Adapted(23, dtype, "float16" if dtype == "float16" else BF16, inputs, (256, 64), rank, 3, [i % 3 for i in range(len(counts))], counts)
+    case.run()
+    rows = case.batch.rows
+    plan = case.plan.numpy().copy()
+    order = plan[plan.size - 4 * rows:].view(np.int32)
+    at = [0, rows // 2, rows - 1]
+    none = order[at].copy()
+    order[at] = -1, rows, -2 ** 31
+    assert len(set(none.tolist())) == 3 and ((none >= 0) & (none < rows)).all()
+    case.plan.upload(plan)
+    case.d_out.upload(encode(np.full((rows, 320), 55, np.float32), dtype))
+    serving.lora_project(case.layout, case.batch, case.d_out, case.d_x, case.d_a, case.d_b, case.plan, base=case.d_base, scales=case.d_scales)
+    got = decode(case.d_out.numpy(), dtype)
+    assert (got[none] == 55).all()
+    got[none] = ref.lora(case.x, case.a, case.b, case.widths, rank, case.adapters, case.row_start, case.base, None, case.scales)[0][none]
+    case.check(got)
+
+
 def test_no_rows(cuda):
     case = Adapted(12, "float32", BF16, 64, (32,), 8, 2, [], [])
     assert case.run().d_out.numpy().shape == (0, 32)
