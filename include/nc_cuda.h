@@ -171,7 +171,8 @@ int32_t nc_attention_cache(void **p, const int64_t *s, void *stream);
 
 /* NC_ERR_KERNEL if a kernel recorded a device-side fault since the last call (a TMA stage of
  * the grouped attention kernel that did not arrive within its bounded wait, or a copy or a matrix
- * instruction of nc_kv4_attention's prompts or of nc_lora_project, whose output is then missing in part); clears it. */
+ * instruction of nc_kv4_attention's prompts or of nc_lora_project, whose output is then missing in part, or a plan of other
+ * sizes than nc_lora_project's); clears it. */
 int32_t nc_device_faults(void);
 
 /* Bounds the library's abandonable device-side waits (pipeline stages of the tensor-core
@@ -305,7 +306,8 @@ int64_t nc_token_logprobs_scratch_bytes(int64_t rows, int64_t vocab, int64_t k);
 int32_t nc_lora_plan(void **p, const int64_t *s, void *stream);
 int64_t nc_lora_plan_bytes(int64_t rows, int64_t seqs, int64_t slots);
 
-/* Adds the adapters' shares to projections' outputs; the plan was made for the same rows, seqs and slots.
+/* Adds the adapters' shares to projections' outputs; the plan was made for the same rows, seqs and slots (with one that was not,
+ * or with none, the outputs stay as they were, and nc_device_faults tells).
  * p: [0] out [rows, outputs] (may be base, at its stride; overlaps nothing else)  [1] x [rows, inputs]  [2] base (nullable)  [3] A  [4] B  [5] plan
  *    [6] ranks i32[slots] (null: rank)  [7] scales f32[slots] (null: 1)
  * s: rows, seqs, slots, inputs, rank (both multiples of 8; rank 128 at most), targets (8 at most), element type of x, base

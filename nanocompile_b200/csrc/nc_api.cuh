@@ -19,7 +19,7 @@ __attribute__((visibility("hidden"))) int32_t prompt_fault(bool *fault);
 // Their g_wait_cycles: each source file has its own.
 __attribute__((visibility("hidden"))) int32_t set_prompt_wait_limit(long long cycles);
 // The same of the adapters' kernels (nc_requests.cu).
-__attribute__((visibility("hidden"))) int32_t requests_fault(bool *fault);
+__attribute__((visibility("hidden"))) int32_t requests_fault(const char **what);
 __attribute__((visibility("hidden"))) int32_t set_requests_wait_limit(long long cycles);
 
 #define CUDA_TRY(expr)                                                                           \

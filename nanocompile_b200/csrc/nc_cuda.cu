@@ -840,9 +840,9 @@ extern "C" int32_t nc_device_faults(void) {
     bool prompt = false;
     NC_TRY(prompt_fault(&prompt));
     if (prompt) return fail(NC_ERR_KERNEL, "4-bit attention: a copy or a matrix instruction did not complete within its wait limit");
-    bool adapters = false;
+    const char *adapters = nullptr;
     NC_TRY(requests_fault(&adapters));
-    if (adapters) return fail(NC_ERR_KERNEL, "adapters: a matrix instruction did not complete within its wait limit");
+    if (adapters) return fail(NC_ERR_KERNEL, "adapters: %s", adapters);
     return NC_OK;
 }
 

@@ -29,7 +29,11 @@ constexpr int LORA_TARGETS = 8, LORA_RANK = 128, LORA_SEQS = 8192;
 constexpr int LORA_LINE = 1 << 23;             // inputs or outputs of a row at most: those of 128 rows are counted in 32 bits
 constexpr int LORA_THREADS = 256, LORA_WARPS = LORA_THREADS / 32;
 constexpr int LORA_PASS = 192;                 // rows of h at most in a pass: targets x rank in whole 32s
-constexpr int LORA_HEAD = 4;                   // words before the plan's items
+constexpr int LORA_HEAD = 4;                   // words before the plan's items: the rows, sequences and slots it was made for
+
+// What went wrong in a kernel since it was last asked for: LORA_LATE a wait that ran out, LORA_OTHER a plan of other sizes than the call's.
+__device__ unsigned int g_lora_fault;
+constexpr unsigned int LORA_LATE = 1, LORA_OTHER = 2;
 
 struct LoraPlanArgs {
     const int32_t *adapters;                   // [seqs]; outside 0 .. slots - 1: none
@@ -122,8 +126,7 @@ __global__ void __launch_bounds__(1024, 1) lora_plan_kernel(const __grid_constan
     rows = min(max(rows, 0), a.rows);                              // otherwise only where row_start does not ascend
     if (tid == 0) {
         start[groups] = rows;
-        a.plan[0] = rows;
-        a.plan[1] = groups;
+        *(int4 *)a.plan = make_int4(a.rows, a.seqs, a.slots, 0);
     }
     __syncthreads();
     int count = 0;                                                 // of items
@@ -173,7 +176,7 @@ struct LoraArgs {
     const int32_t *plan, *ranks;               // ranks: [slots] or null
     const float *scales;                       // [slots] or null
     int64_t x_stride, base_stride, out_stride;
-    int rows, items, tile, inputs, outputs, rank, slots, targets, pass_targets, wtype;
+    int rows, seqs, items, tile, inputs, outputs, rank, slots, targets, pass_targets, wtype;
     int x_vectors, pairs, wide;                // 16-byte loads of x; two outputs to an access; 16 bytes of them
     int width[LORA_TARGETS];
 };
@@ -260,6 +263,17 @@ __device__ __forceinline__ void lora_store2(void *p, int64_t at, float2 v, bool 
     }
 }
 
+// An item of the plan: slot (-1: none), first place of its rows in the plan's order, how many; no rows where the plan is of other sizes.
+__device__ __forceinline__ int4 lora_item(const LoraArgs &a, int i) {
+    const int4 head = *(const int4 *)a.plan;
+    int4 item = lora_items(a.plan)[i];
+    if (head.x != a.rows || head.y != a.seqs || head.z != a.slots) {
+        if (threadIdx.x == 0) atomicOr(&g_lora_fault, LORA_OTHER);
+        item.z = 0;
+    }
+    if (item.z < 0 || item.z > a.rows || item.y < 0 || item.y > a.rows - item.z || item.x >= a.slots) item.z = 0;
+    return item;
+}
 // The row at a place of the plan's order; -1 for what is no row of the call.
 __device__ __forceinline__ int64_t lora_row(const LoraArgs &a, const int32_t *order, int at) {
     const int row = order[at];
@@ -295,10 +309,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
     release_dependents();
     wait_for_producer();
     // An item's rows from blockIdx.z COLS on.
-    const int4 item = lora_items(a.plan)[blockIdx.x / ctas];
+    const int4 item = lora_item(a, blockIdx.x / ctas);
     const int32_t *const order = (const int32_t *)(lora_items(a.plan) + a.items);
     const int slot = item.x, first = item.y + (int)blockIdx.z * COLS, count = min(COLS, item.z - (int)blockIdx.z * COLS);
-    if (count <= 0 || first < 0 || first > a.rows - count || slot >= a.slots) return;        // nothing there, or no plan of this call's sizes
+    if (count <= 0) return;
     const int t0 = (int)blockIdx.y * a.pass_targets, t1 = min(a.targets, t0 + a.pass_targets);
     int n_first = 0, n_pass = 0, n_tiles = 0;                      // outputs before the pass, of it, tiles of 16 of them
     for (int t = 0; t < t1; ++t) {

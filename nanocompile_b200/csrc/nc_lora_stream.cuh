@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(LS_THREADS, 2) lora_stream_kernel(const __grid
     const int ctas = (int)lora_cluster_size(), cta = (int)lora_rank_of_cluster();
     release_dependents();
     wait_for_producer();
-    const int4 item = lora_items(a.plan)[blockIdx.x / ctas];
+    const int4 item = lora_item(a, blockIdx.x / ctas);
     const int32_t *const order = (const int32_t *)(lora_items(a.plan) + a.items);
     const int slot = item.x, first = item.y, count = min(8, item.z);
-    if (count <= 0 || first < 0 || first > a.rows - count || slot >= a.slots) return;        // nothing there, or no plan of this call's sizes
+    if (count <= 0) return;
     const int t0 = (int)blockIdx.y * a.pass_targets, t1 = min(a.targets, t0 + a.pass_targets);
     int n_first = 0, n_pass = 0, n_tiles = 0;                          // outputs before the pass, of it, tiles of 16 of them
     for (int t = 0; t < t1; ++t) {
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) lora_stream_kernel(const __grid
     auto wait = [&](uint64_t *bar, unsigned parity) {                  // one that runs out is the last one
         if (kvt_mbar_wait(bar, parity, *(volatile int *)&failed ? 0 : limit)) return true;
         *(volatile int *)&failed = 1;
-        g_lora_fault = 1;
+        atomicOr(&g_lora_fault, LORA_LATE);
         return false;
     };
     // B's stages: tiles [tile, tile + n) of one target, from output n0 on.

@@ -40,8 +40,6 @@ static_assert(2 * lt_share(2) <= LT_SUM_ROWS && 3 * lt_share(3) <= LT_SUM_ROWS &
               "room for the sums of every share");
 constexpr int LT_SLOTS = 4;                    // tiles of base on their way or in work, at most
 
-__device__ unsigned int g_lora_fault;          // set when a matrix instruction did not come to its end within the wait limit
-
 template <int TX, int TW>
 struct LoraTiles {
     static constexpr bool F32 = TX == KV_F32;
@@ -235,10 +233,10 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     const bool worker = warp < LT_WARPS;
     const int ctas = (int)lora_cluster_size(), cta = (int)lora_rank_of_cluster();
     wait_for_producer();
-    const int4 item = lora_items(a.plan)[blockIdx.x / ctas];
+    const int4 item = lora_item(a, blockIdx.x / ctas);
     const int32_t *const order = (const int32_t *)(lora_items(a.plan) + a.items);
     const int slot = item.x, first = item.y, count = min(LT_ROWS, item.z);
-    if (count <= 0 || first < 0 || first > a.rows - count || slot >= a.slots) return;        // nothing there, or no plan of this call's sizes
+    if (count <= 0) return;
     const int t0 = (int)blockIdx.y * a.pass_targets, t1 = min(a.targets, t0 + a.pass_targets);
     int n_first = 0, n_pass = 0, n_tiles = 0;                          // outputs before the pass, of it, tiles of them
     for (int t = 0; t < t1; ++t) {
@@ -290,7 +288,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     auto wait = [&](uint64_t *bar, unsigned parity) {
         if (kvt_mbar_wait(bar, parity, *(volatile int *)&sh.failed ? 0 : limit)) return true;
         *(volatile int *)&sh.failed = 1;
-        g_lora_fault = 1;
+        atomicOr(&g_lora_fault, LORA_LATE);
         return false;
     };
     const int stage_bytes = S::PX * LT_BLOCK + S::PW * plan.a_bytes, c = tid & 7, line = tid >> 3;             // a worker's 16 bytes of every 32nd row

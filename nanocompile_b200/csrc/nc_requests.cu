@@ -197,13 +197,15 @@ int32_t nc::set_requests_wait_limit(long long cycles) {
     return NC_OK;
 }
 
-// Whether a wait has run out since the last call; clears it.
-int32_t nc::requests_fault(bool *fault) {
+// What went wrong in the adapters' kernels since the last call, or null; clears it.
+int32_t nc::requests_fault(const char **what) {
     unsigned int word = 0;
     CUDA_TRY(cudaMemcpyFromSymbol(&word, g_lora_fault, sizeof(word)));
-    *fault = word != 0;
+    *what = word & LORA_LATE    ? "a copy or a matrix instruction did not complete within its wait limit"
+            : word & LORA_OTHER ? "a plan was made for other rows, sequences or slots than the projection's"
+                                : nullptr;
     word = 0;
-    if (*fault) CUDA_TRY(cudaMemcpyToSymbol(g_lora_fault, &word, sizeof(word)));
+    if (*what) CUDA_TRY(cudaMemcpyToSymbol(g_lora_fault, &word, sizeof(word)));
     return NC_OK;
 }
 
@@ -286,6 +288,7 @@ extern "C" int32_t nc_lora_project(void **p, const int64_t *s, void *stream) {
     if (a.out == a.base && a.out_stride != a.base_stride)
         return fail(NC_ERR_ARGUMENT, "outputs in place of base at a stride of %lld, base's is %lld", (long long)a.out_stride, (long long)a.base_stride);
     a.rows = (int)rows;
+    a.seqs = (int)seqs;
     a.items = (int)lora_places(rows, seqs, slots);
     a.tile = (int)lora_tile(rows, seqs, slots);
     a.inputs = (int)inputs;

@@ -162,7 +162,8 @@ def set_wait_limit(cycles: int) -> None:
 
 
 def device_faults() -> None:
-    """Raise :class:`KernelError` if a device-side wait gave up since the last check (and clear it)."""
+    """Raise :class:`KernelError` if a device-side wait gave up, or an adapters' plan was of other sizes than its call, since the last
+    check (and clear it)."""
     check(library().nc_device_faults())
 
 

@@ -273,6 +273,31 @@ def test_rows_of_a_plan_that_are_none_of_the_call(cuda, dtype, counts, inputs, r
     case.check(got)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,other", [(([1] * 9, 256), ([1] * 10, 256)), (([1] * 9, 4096), ([2] + [1] * 8, 4096)), (([300, 2], 256), ([300, 3], 256)),
+                                         (([300, 212], 256), ([512], 256)), (([128, 128, 256], 256), ([1] * 600, 256)), (([600], 256), None)])
+def test_a_plan_of_other_sizes_changes_nothing_and_is_reported(cuda, dtype, batch, other):
+    """A plan that lies in a buffer for both, of another batch or of none."""
+    wtype = "float16" if dtype == "float16" else BF16
+    case = Adapted(24, dtype, wtype, batch[1], (256, 64), 32, 3, [i % 3 for i in range(len(batch[0]))], batch[0]).run()
+    case.check()
+    room = DeviceArray.zeros((1 << 16,), np.uint8)
+    if other:
+        stale = Adapted(25, dtype, wtype, other[1], (256, 64), 32, 3, [i % 3 for i in range(len(other[0]))], other[0])
+        serving.lora_plan(stale.batch, room, DeviceArray.of(stale.adapters), row_start=DeviceArray.of(stale.row_start))
+    runtime.device_faults()
+    case.d_out.upload(encode(np.full((case.batch.rows, 320), 55, np.float32), dtype))
+    project = lambda plan: serving.lora_project(case.layout, case.batch, case.d_out, case.d_x, case.d_a, case.d_b, plan, base=case.d_base,      # noqa: E731
+                                                scales=case.d_scales)
+    project(room)
+    assert (decode(case.d_out.numpy(), dtype) == 55).all()
+    with pytest.raises(runtime.KernelError, match="other rows, sequences or slots"):
+        runtime.device_faults()
+    project(case.plan)
+    case.check()
+    runtime.device_faults()
+
+
 def test_no_rows(cuda):
     case = Adapted(12, "float32", BF16, 64, (32,), 8, 2, [], [])
     assert case.run().d_out.numpy().shape == (0, 32)
