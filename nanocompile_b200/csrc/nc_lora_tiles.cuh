@@ -1,7 +1,8 @@
 // nc_lora_tiles.cuh -- low-rank adapters for prompts: what nc_lora.cuh computes, for items of up to 128 rows, on the tensor cores.
 //
 // An item to a cluster.  First each CTA multiplies its share of the inputs, 64 at a time: D1 [128 rows][h] += x A^T, tcgen05.mma with the
-// rows and the adapter's A copied asynchronously into 128-byte swizzled tiles, D1 in tensor memory.  The CTAs' sums of h are added
+// rows and the adapter's A copied asynchronously into 128-byte swizzled tiles, D1 in tensor memory (float32 rows: each 64 inputs a D1 of
+// their own, two in turn where there is room, added up by the four warps that load later).  The CTAs' sums of h are added
 // through distributed shared memory: each CTA is sent its share of the rows, and copies them, added up and split into the
 // operand's parts, to all.  Then each CTA expands its share of the outputs, 256 bytes of a row at a time: D2 [128][outputs] = h B^T in two
 // halves of tensor memory.  Four warps ask for B and, up to four tiles ahead, for base; four warps add a tile's D2 to its base in shared
@@ -10,12 +11,16 @@
 //
 // Bound by the bytes of x, base and outputs, behind 14 us that no size takes away (tensor memory, two ways through the cluster).  8192
 // bfloat16 rows of 4096 inputs to 6144 outputs at rank 32: 82 us (3.3 TB/s of 6.5; its products are 21 GFLOP, 13 us); 512 of them 30; float32
-// rows 164 (3.3 TB/s), beside float16 weights 226.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
+// rows 165 (3.3 TB/s), beside float16 weights 230.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
 // by the warps that add it 122, in bulk copies of a row each 201.
 //
 // Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-18 of it is lost, float16 2^-24; float16's
 // h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its range).  float32 rows and their h go
-// in three bfloat16 parts (2^-27 is lost), float16 weights beside them in two, which are exact.  Sums are float32 in tensor memory.
+// in three bfloat16 parts (2^-27 is lost), float16 weights beside them in two, which are exact.  Sums are float32 in tensor memory; the
+// matrix unit cuts them off at each step, always towards nought, which adds up along a chain.  So float32 rows have chains of 64 inputs,
+// the largest parts' four steps last, added in float32: 8192 rows of 4096 inputs are 1.6e-7 of the result (rms) from 64 bits; in a chain
+// of 2048 inputs they were 7.0e-6 beside bfloat16 weights, 1.2e-5 beside float16.  16-bit rows have one chain (float16: 1.7e-6 towards
+// nought there, in outputs that are rounded by 2e-4).
 #pragma once
 
 #include "nc_kv4_prompt.cuh"
@@ -25,7 +30,7 @@
 
 namespace nc {
 
-constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_LOADERS = 128, LT_TMEM = 256;
+constexpr int LT_ROWS = 128, LT_WARPS = 8, LT_WORKERS = 32 * LT_WARPS, LT_LOADERS = 128;
 constexpr int LT_MMA = LT_WARPS, LT_THREADS = LT_WORKERS + 32 + LT_LOADERS;            // the warp after the workers', then those that load
 constexpr int LT_BLOCK = LT_ROWS * 128;        // 128 rows of 128 bytes
 constexpr int LT_HALF = LT_ROWS * 64;          // 128 rows of 64 bytes
@@ -47,6 +52,7 @@ struct LoraTiles {
     static constexpr int PX = F32 ? 3 : 1, PW = F32 && TW == KV_F16 ? 2 : 1, PH = F32 ? 3 : 2;   // parts of x, of weights, of h
     static constexpr int COLS = F32 ? 64 : 128;                        // outputs of a tile
     static constexpr int SIZE = F32 ? 4 : 2;
+    static constexpr int TMEM = F32 ? 512 : 256;                       // columns: two halves of D2, before them D1, of float32 rows the chains and their sums
 };
 
 // How shared memory is laid out, by the most rows of h in a pass: h's operand, two tiles of B, the slots of base; over these the stages of
@@ -57,6 +63,7 @@ struct LoraTilesPlan {
     int stages, a_bytes;                       // of a stage: LT_BLOCK for a part of the rows, a_bytes for one of A
     int h_blocks, b_blocks;                    // blocks of 32 for a part of h, for B
     int b_at, slot_at, slots, sum_at, early, bytes;
+    int chains, chain_step;                    // float32 rows: chains of products in tensor memory, 32s of columns apart, and their sums behind
 };
 template <typename S>
 inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
@@ -80,11 +87,13 @@ inline LoraTilesPlan lora_tiles_plan(int targets, int rank) {
     const int room = p.early ? p.sum_at : LT_BYTES;
     p.stages = room / stage < LT_STAGES ? room / stage : LT_STAGES;
     if (p.stages * stage > p.bytes) p.bytes = p.stages * stage;
+    p.chain_step = p.h_blocks * 32;
+    p.chains = 3 * p.chain_step <= S::TMEM ? 2 : 1;
     return p;
 }
 
 struct LoraTilesShared {                       // before the tiles
-    uint64_t full[LT_STAGES], empty[LT_STAGES], d1_done, b_full[2], d2_done[2], d2_free[2], slot_full[LT_SLOTS], slot_free[LT_SLOTS], h_full, drained;
+    uint64_t full[LT_STAGES], empty[LT_STAGES], chain_full[2], chain_free[2], d1_done, b_full[2], d2_done[2], d2_free[2], slot_full[LT_SLOTS], slot_free[LT_SLOTS], h_full, drained;
     __align__(16) float row_scale[LT_ROWS];
     int row[LT_ROWS];
     uint32_t tmem;
@@ -163,6 +172,15 @@ __device__ __forceinline__ uint32_t lt_part(float2 &v) {
     v.y = fsub(v.y, r.y);
     return w;
 }
+// v += sum.
+__device__ __forceinline__ void lt_sums(uint32_t (&v)[16], const uint32_t (&sum)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        const float2 f = unpack2(add2(pack2(__uint_as_float(sum[e]), __uint_as_float(sum[e + 1])), pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]))));
+        v[e] = __float_as_uint(f.x);
+        v[e + 1] = __float_as_uint(f.y);
+    }
+}
 // 16 bytes of outputs from those of base and float32 sums.
 template <int TX>
 __device__ __forceinline__ uint4 lt_add(const uint4 &was, const uint32_t *sums, float scale) {
@@ -192,14 +210,14 @@ struct LtBlock {
     float4 x[8];
     uint4 w[LORA_PASS / 32];
 };
-// The products of parts that count: of p + q up to the third.
+// The products of parts that count: of p + q up to the third, the largest last, as each step cuts off what the whole sum has no bits for.
 template <int P, int Q, typename F>
 __device__ __forceinline__ void lt_parts(F use) {
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int s = 2; s >= 0; --s)
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-            if (p + q < 3) use(p, q);
+            if (s - q >= 0 && s - q < P) use(s - q, q);
 }
 // use(std::true_type) where numbers up to `most` are sure, else use(std::false_type).
 template <int TW, typename F>
@@ -263,12 +281,13 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(wb + at), "r"((uint32_t)min((int64_t)4096, high - at)) : "memory");
     }
     if (warp == LT_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kvt_smem(&sh.tmem)), "n"(LT_TMEM) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kvt_smem(&sh.tmem)), "n"(S::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
         for (int i = 0; i < plan.stages; ++i) lt_init(&sh.full[i], LT_WORKERS), lt_init(&sh.empty[i], 1);
-        lt_init(&sh.d1_done, 1);
+        lt_init(&sh.d1_done, S::F32 ? LT_LOADERS : 1);
+        for (int i = 0; i < 2; ++i) lt_init(&sh.chain_full[i], 1), lt_init(&sh.chain_free[i], LT_LOADERS);
         lt_init(&sh.drained, 1);
         for (int i = 0; i < 2; ++i) lt_init(&sh.b_full[i], LT_LOADERS), lt_init(&sh.d2_done[i], 1), lt_init(&sh.d2_free[i], LT_ROWS);
         for (int i = 0; i < LT_SLOTS; ++i) lt_init(&sh.slot_full[i], LT_LOADERS), lt_init(&sh.slot_free[i], LT_ROWS);
@@ -293,7 +312,9 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     };
     const int stage_bytes = S::PX * LT_BLOCK + S::PW * plan.a_bytes, c = tid & 7, line = tid >> 3;             // a worker's 16 bytes of every 32nd row
 
-    // h, in parts: D1 = x A^T over this CTA's inputs.
+    // h, in parts: D1 = x A^T over this CTA's inputs.  Of float32 rows each block of 64 inputs is a chain of its own; the warps that load
+    // later add up all but the last in tensor memory.
+    const uint32_t d1 = S::F32 ? tmem + plan.chains * plan.chain_step : tmem;
     if (worker) {
         int from[LORA_PASS / 32];                                      // of A's rows; -1: none there
 #pragma unroll
@@ -428,21 +449,49 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         lt_wait_copies<0>();
     } else if (warp == LT_MMA && lane == 0) {
         for (int k = 0; k < k_blocks; ++k) {
-            const int stage = k % plan.stages;
+            const int stage = k % plan.stages, chain = S::F32 ? k % plan.chains : 0, turn = S::F32 ? k / plan.chains : 0;
+            const int steps = min(4, (a.inputs - (k_low + k) * 64 + 15) / 16);
+            const uint32_t at = base_at + (uint32_t)stage * stage_bytes, to = tmem + chain * plan.chain_step;
+            const uint64_t x = kvt_desc(at), w = kvt_desc(at + S::PX * LT_BLOCK);                 // addresses in them are in 16s of bytes
+            if (turn > 0 && !wait(&sh.chain_free[chain], (turn - 1) & 1)) break;
             if (!wait(&sh.full[stage], (k / plan.stages) & 1)) break;
             kvt_after();
-            const uint32_t at = base_at + (uint32_t)stage * stage_bytes;
-            const int steps = min(4, (a.inputs - (k_low + k) * 64 + 15) / 16);
-            for (int s = 0; s < steps; ++s)
-                lt_parts<S::PX, S::PW>([&](int p, int q) {
-                    lt_mma<S::T>(tmem, kvt_desc(at + p * LT_BLOCK + 32 * s), kvt_desc(at + S::PX * LT_BLOCK + q * plan.a_bytes + 32 * s), wide, k > 0 || s > 0 || p > 0 || q > 0);
-                });
+            bool add = !S::F32 && k > 0;
+            lt_parts<S::PX, S::PW>([&](int p, int q) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s, add = true)
+                    if (s < steps) lt_mma<S::T>(to, x + (p * LT_BLOCK + 32 * s) / 16, w + (q * plan.a_bytes + 32 * s) / 16, wide, add);
+            });
             kvt_commit(&sh.empty[stage]);
+            if (S::F32) kvt_commit(&sh.chain_full[chain]);
         }
-        kvt_commit(&sh.d1_done);
+        if (!S::F32) kvt_commit(&sh.d1_done);
+    } else if (S::F32 && warp > LT_MMA) {
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        for (int k = 0; k + 1 < k_blocks; ++k) {                       // the last one's stays where it is
+            const int chain = k % plan.chains;
+            wait(&sh.chain_full[chain], (k / plan.chains) & 1);
+            kvt_after();
+            __syncwarp();
+            for (int j = 0; j < wide; j += 16) {
+                uint32_t v[16], sum[16];
+                kvt_load16(tmem + lanes + chain * plan.chain_step + j, v);
+                if (k > 0) kvt_load16(d1 + lanes + j, sum);
+                kvt_wait_ld();
+                if (k > 0) lt_sums(v, sum);
+                kvt_store16(d1 + lanes + j, v);
+            }
+            kvt_before();
+            lt_arrive(&sh.chain_free[chain]);
+            kvt_wait_st();
+        }
+        kvt_before();
+        lt_arrive(&sh.d1_done);
     }
     __syncwarp();
     wait(&sh.d1_done, 0);
+    const uint32_t last = S::F32 && k_blocks > 0 ? (k_blocks - 1) % plan.chains : 0;
+    if (S::F32 && k_blocks > 0) wait(&sh.chain_full[last], ((k_blocks - 1) / plan.chains) & 1);
     kvt_after();
     __syncwarp();
     if (!plan.early) lora_cluster_arrive();    // this CTA is done with its stages: sums may lie over them
@@ -454,9 +503,11 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
         const bool here = row / mine == cta;
         const uint32_t at = base_at + plan.sum_at + (uint32_t)((cta * mine + row % mine) * pitch) * 4, to = lt_peer(at, row / mine);
         for (int j = 16 * (warp >> 2); j < wide; j += 32) {
-            uint32_t v[16];
-            kvt_load16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + j, v);
+            uint32_t v[16], sum[16];
+            kvt_load16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + last * plan.chain_step + j, v);
+            if (S::F32 && k_blocks > 1) kvt_load16(d1 + ((uint32_t)(32 * (warp & 3)) << 16) + j, sum);
             kvt_wait_ld();
+            if (S::F32 && k_blocks > 1) lt_sums(v, sum);
             if (k_blocks == 0)                                         // more CTAs than blocks of inputs
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = 0;
@@ -780,7 +831,7 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
     kvt_before();
     __syncthreads();
     kvt_after();
-    if (warp == LT_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(LT_TMEM) : "memory");
+    if (warp == LT_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::TMEM) : "memory");
     lora_cluster_wait();
 }
 

@@ -207,6 +207,24 @@ def test_an_infinity_is_one_in_float32(cuda):
 
 
 @pytest.mark.parametrize("wtype", [BF16, "float16"])
+@pytest.mark.parametrize("rows,inputs,outputs,rank", [(1024, 16384, 64, 8), (8192, 2048, 40, 16), (640, 4096, 96, 64), (1500, 512, 128, 96), (700, 1000, 64, 128),
+                                                      (600, 1032, 200, 80)])
+@pytest.mark.parametrize("positive", [False, True])
+def test_long_float32_prompts_keep_float32_accuracy(cuda, wtype, rows, inputs, outputs, rank, positive):
+    """Against the result, where other tests' bounds are of the terms: the matrix unit cuts its sums off at each step, always
+    towards nought, which adds up along a chain. A chain of 64 inputs, or of 64 of h, has four steps of full size, each off by
+    2^-23 of the sum at most: 2^-21 of h, and as much of the outputs. Up to 32 chains and 8 CTAs' sums are added in float32: 40
+    roundings of 2^-25 in the mean, as independent ones 2^-22; the parts that the operands go in, the scale and the output less than 2^-23."""
+    case = Adapted(26, "float32", wtype, inputs, (outputs,), rank, 1, [0], [rows], scales=False, base=False)
+    if positive:
+        case.x, case.a, case.b = np.abs(case.x), np.abs(case.a), np.abs(case.b)
+    got = case.run().check()
+    want, _ = ref.lora(case.x, case.a, case.b, case.widths, rank, case.adapters, case.row_start)
+    off = float(np.sqrt(np.mean((got - want) ** 2) / np.mean(want ** 2)))
+    assert off <= 2.0 ** -20 + 2.0 ** -22 + 2.0 ** -23
+
+
+@pytest.mark.parametrize("wtype", [BF16, "float16"])
 @pytest.mark.parametrize("count", [8, 300])
 def test_the_largest_numbers_of_float32_rows(cuda, wtype, count):
     """What rounds to an infinity in 16 bits, and an infinity."""
