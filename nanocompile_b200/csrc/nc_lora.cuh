@@ -17,7 +17,7 @@
 // at the start.  Bound by its chain of dependent loads: one row of 896 inputs to 1152 outputs at rank 16 takes 8.8 us with the plan.
 //
 // Accuracy.  Products are mma m16n8k8 tf32: 16-bit weights and rows are tf32 numbers as they are, float32 rows and h go in two parts
-// (11 bits and the next 11, rounded: 2^-24 of the value is lost, as by one float32 rounding).  The matrix unit cuts sums off rather
+// (11 bits and the next 11, rounded: 2^-23 of the value is lost at most, the last bit of some).  The matrix unit cuts sums off rather
 // than rounding them, so a chain is 32 inputs long, and the chains are added in float32.
 #pragma once
 

@@ -12,8 +12,9 @@
 // of them 14.5, 64 23.5 (2.9 TB/s), 128 45 (3.0 TB/s of 6.5: two rounds of clusters; 67 with one tile of outputs to a warp at a time).
 //
 // Accuracy.  Products are mma m16n8k16 of the weights' type.  Rows of that type are taken as they are, others and h go in parts: three of
-// bfloat16 for float32 rows (2^-27 is lost), else two (bfloat16: 2^-18, beside outputs of 8 bits; float16: 2^-24).  For
-// float16 a row of x or h is first brought to [2^14, 2^15) by a power of two, so that no size leaves its range.  A chain of
+// bfloat16 for float32 rows, which hold them, else two.  Two of bfloat16 hold float16 rows; of h they lose 2^-17 at most, where a bfloat16
+// output is rounded by 2^-8, a float16 one by 2^-11.  Two of float16 lose 2^-23 at most, or 2^-39 of the row's largest: a row of x or h is
+// first brought to [2^14, 2^15) by a power of two, so that no size leaves its range.  A chain of
 // the matrix unit, which cuts sums off, is 32 inputs long; chains are added in float32.
 #pragma once
 

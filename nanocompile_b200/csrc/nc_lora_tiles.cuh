@@ -14,9 +14,9 @@
 // rows 165 (3.3 TB/s), beside float16 weights 230.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
 // by the warps that add it 122, in bulk copies of a row each 201.
 //
-// Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-18 of it is lost, float16 2^-24; float16's
-// h is first brought to [2^14, 2^15) by a power of two for each row, so that no size leaves its range).  float32 rows and their h go
-// in three bfloat16 parts (2^-27 is lost), float16 weights beside them in two, which are exact.  Sums are float32 in tensor memory; the
+// Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-17 of it is lost at most, float16
+// 2^-23, or 2^-39 of the row's largest: that is first brought to [2^14, 2^15) by a power of two, so that no size leaves its range).  float32
+// rows and their h go in three bfloat16 parts, float16 weights beside them in two, which hold them; of the products' parts 2^-25 is left out.  Sums are float32 in tensor memory; the
 // matrix unit cuts them off at each step, always towards nought, which adds up along a chain.  So float32 rows have chains of 64 inputs,
 // the largest parts' four steps last, added in float32: 8192 rows of 4096 inputs are 1.6e-7 of the result (rms) from 64 bits; in a chain
 // of 2048 inputs they were 7.0e-6 beside bfloat16 weights, 1.2e-5 beside float16.  16-bit rows have one chain (float16: 1.7e-6 towards

@@ -131,6 +131,30 @@ def test_adapters(cuda, dtype, wtype, inputs, widths, rank, slots, adapters, cou
     Adapted(1, dtype, wtype, inputs, widths, rank, slots, adapters, counts).run().check()
 
 
+@pytest.mark.parametrize("inputs,widths,rank,slots,adapters,counts", CASES + [(4096, (1024, 40), 32, 3, [0, 2, 1, 0], [1] * 4)])
+def test_float16_rows_beside_bfloat16_adapters(cuda, inputs, widths, rank, slots, adapters, counts):
+    Adapted(27, "float16", BF16, inputs, widths, rank, slots, adapters, counts).run().check()
+
+
+@pytest.mark.parametrize("dtype,wtype", [("float16", BF16), (BF16, "float16")])
+@pytest.mark.parametrize("inputs,counts", [(256, [1] * 6), (4096, [1] * 6), (256, [90, 3, 200, 1, 0, 17])])
+def test_rows_and_adapters_of_different_16_bit_types(cuda, dtype, wtype, inputs, counts):
+    """Adapters of ranks of their own with NaN behind them, and rows with an infinity and a NaN."""
+    case = Adapted(28, dtype, wtype, inputs, (1000, 28), 64, 6, [0, 1, 2, 3, 4, 5], counts, ranks=[64, 1, 0, 13, 33, 16])
+    kept = case.a.copy(), case.b.copy(), case.x.copy()
+    for s, r in enumerate(case.ranks):
+        for t in range(2):
+            case.a[s, t * 64 + r: (t + 1) * 64] = np.nan
+        case.b[s, :, r:] = np.nan
+    bad = [case.row_start[0], case.row_start[3]]
+    case.x[bad[0], 3], case.x[bad[1], inputs - 1] = np.inf, np.nan
+    got = decode(case.run().d_out.numpy(), dtype)
+    assert not np.isfinite(got[bad]).any() and np.isnan(got[bad[1]]).all()
+    case.a, case.b, case.x = kept
+    case.x[bad] = case.base[bad] = got[bad] = 0
+    case.check(got)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("counts", [[1] * 6, [90, 3, 200, 1, 0, 17]])
 def test_adapters_of_ranks_of_their_own(cuda, dtype, counts):
