@@ -331,7 +331,7 @@ int32_t nc_lora_project(void **p, const int64_t *s, void *stream);
  *    [11] error word (nullable)
  * s: rows, vocab, logit row stride (elements), element type, beams (32 at most), end (-1: none), scratch bytes */
 int32_t nc_beam_select(void **p, const int64_t *s, void *stream);
-/* Enough for every call of this vocabulary, of any type, with up to so many rows and beams. */
+/* Enough for every call, of any type, with up to so many rows, logits of a row and beams. */
 int64_t nc_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int64_t beams);
 
 /* States reordered by parents: lines 0 .. lengths[parent[i]] - 1 (every line without lengths) of each plane of row parent[i] to

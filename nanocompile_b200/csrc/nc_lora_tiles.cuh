@@ -16,11 +16,11 @@
 //
 // Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-17 of it is lost at most, float16
 // 2^-23, or 2^-39 of the row's largest: that is first brought to [2^14, 2^15) by a power of two, so that no size leaves its range).  float32
-// rows and their h go in three bfloat16 parts, float16 weights beside them in two, which hold them; of the products' parts 2^-25 is left out.  Sums are float32 in tensor memory; the
-// matrix unit cuts them off at each step, always towards nought, which adds up along a chain.  So float32 rows have chains of 64 inputs,
-// the largest parts' four steps last, added in float32: 8192 rows of 4096 inputs are 1.6e-7 of the result (rms) from 64 bits; in a chain
-// of 2048 inputs they were 7.0e-6 beside bfloat16 weights, 1.2e-5 beside float16.  16-bit rows have one chain (float16: 1.7e-6 towards
-// nought there, in outputs that are rounded by 2e-4).
+// rows and their h go in three bfloat16 parts, float16 weights beside them in two, which hold them; of the products' parts 2^-25 is
+// left out.  Sums are float32 in tensor memory; the matrix unit cuts them off at each step, always towards nought, which adds up along a
+// chain.  So float32 rows have chains of 64 inputs, the largest parts' four steps last, added in float32: 8192 rows of 4096 inputs are
+// 1.6e-7 of the result (rms) from 64 bits; in a chain of 2048 inputs they were 7.0e-6 beside bfloat16 weights, 1.2e-5 beside float16.
+// 16-bit rows have one chain (float16: 1.7e-6 towards nought there, in outputs that are rounded by 2e-4).
 #pragma once
 
 #include "nc_kv4_prompt.cuh"

@@ -347,9 +347,10 @@ int32_t launch_beams(cudaStream_t st, const BeamArgs &a, int64_t rows) {
 
 extern "C" int64_t nc_beam_select_scratch_bytes(int64_t rows, int64_t vocab, int64_t beams) {
     if (rows <= 0 || vocab <= 0 || beams <= 0 || beams > LP_MAX_TOP) return 4 * BEAM_COUNTERS;
-    int64_t row = 0;                           // fewer beams may have more segments
-    for (int type : {KV_F32, KV_F16})
-        for (int64_t n = 1; n <= beams; ++n) row = std::max(row, beam_plan(beam_batches(vocab, type), n).lists * 8 * (1 + n));
+    // Of the most segments that any smaller vocabulary and number of beams may have (smaller ones can have more: 64 batches of 8 beams are
+    // cut into 64 segments, 65 into 37): a batch each, and BEAM_LISTS of a request.
+    int64_t row = 0;
+    for (int64_t n = 1; n <= beams; ++n) row = std::max(row, std::min<int64_t>(beam_batches(vocab, KV_F32), BEAM_LISTS / n) * 8 * (1 + n));
     return 4 * BEAM_COUNTERS + std::min<int64_t>(rows, BEAM_ROWS) * row;
 }
 

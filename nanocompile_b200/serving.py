@@ -486,7 +486,7 @@ def lora_project(layout: LoraLayout, batch: LoraBatch, out, x, a, b, plan, *, ba
 
 
 def beam_select_scratch_bytes(rows: int, vocab: int, beams: int) -> int:
-    """Scratch for :func:`beam_select` calls of up to ``rows`` rows and ``beams`` beams."""
+    """Scratch for :func:`beam_select` calls of up to ``rows`` rows of ``vocab`` logits and ``beams`` beams."""
     return int(library().nc_beam_select_scratch_bytes(rows, vocab, beams))
 
 

@@ -573,6 +573,15 @@ def test_a_beam_scratch_serves_smaller_calls_and_is_left_as_the_next_needs_it(cu
         Beams(language(rng, rows, vocab), rng.standard_normal(rows), beams).run(scratch=scratch).check()
 
 
+@pytest.mark.parametrize("rows,beams,vocab,smaller", [(4, 4, 132000, 108000), (8, 8, 264000, 234000), (32, 32, 66000, 62000)])
+def test_a_beam_scratch_serves_smaller_vocabularies(cuda, rows, beams, vocab, smaller):
+    """Also where those are cut into more segments."""
+    rng = np.random.default_rng(7)
+    scratch = DeviceArray.zeros((serving.beam_select_scratch_bytes(rows, vocab, beams),), np.uint8)
+    for n in (vocab, smaller, vocab):
+        Beams(language(rng, rows, n), rng.standard_normal(rows), beams).run(scratch=scratch).check()
+
+
 def test_a_captured_choice_and_its_reordering_follow_their_inputs(cuda):
     """A step captured into a graph, replayed with other logits, scores and states: what the calls outside a graph give."""
     torch = pytest.importorskip("torch")

@@ -89,6 +89,17 @@ def test_selections_refuse(change, what):
                             given.pop("scratch"), **given)
 
 
+@pytest.mark.parametrize("beams", [1, 2, 3, 4, 5, 8, 16, 31, 32])
+def test_a_beam_scratch_grows_with_every_size(beams):
+    """So that one for some rows, vocabulary and beams serves the calls of fewer of any of them."""
+    vocabularies = sorted({*range(1, 300000, 997), 54000, 62000, 66000, 108000, 132000, 234000, 264000})
+    for rows in (1, beams, 40 * beams):
+        sizes = [serving.beam_select_scratch_bytes(rows, v, beams) for v in vocabularies]
+        assert sizes == sorted(sizes)
+        assert all(serving.beam_select_scratch_bytes(rows + 1, v, beams) >= s and serving.beam_select_scratch_bytes(rows, v, max(1, beams - 1)) <= s
+                   for v, s in zip(vocabularies, sizes))
+
+
 def test_a_beam_scratch_covers_every_smaller_call():
     sizes = [serving.beam_select_scratch_bytes(r, v, k) for r, v, k in ((1, 100, 1), (1, 151936, 1), (64, 151936, 4), (256, 151936, 8), (4096, 151936, 32))]
     assert sizes == sorted(sizes)
