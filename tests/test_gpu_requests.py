@@ -294,6 +294,22 @@ def test_a_row_start_that_does_not_ascend_stays_in_bounds(cuda):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inputs,rows,row_start", [(64, 12, [5, 2, 400, -7, 12]), (4096, 12, [12, -3, 12, 0, 12]), (64, 700, [650, 0, 700, -7, 9000]),
+                                                   (64, 700, [0, 700, 0, 700, 0]), (64, 700, [700] * 5)])
+def test_a_row_start_that_does_not_ascend_writes_its_rows_alone(cuda, dtype, inputs, rows, row_start):
+    """Items of eight rows and of 128: what lies before, between and behind the outputs' rows stays as it was."""
+    case = Adapted(29, dtype, "float16" if dtype == "float16" else BF16, inputs, (320, 16), 32, 2, [0, 1, 0, 1], [rows // 4] * 4)
+    case.row_start = np.array(row_start, np.int32)
+    stride, skip = 336 + 24, 256
+    out, room = strided(np.full((rows, 336), 77), dtype, stride, skip)
+    _, behind = strided(np.full((rows, 336), 77), dtype, stride, skip)
+    case.run(out=out)
+    flat = decode(room.numpy(), dtype)
+    flat[skip + np.arange(rows)[:, None] * stride + np.arange(336)] = 77
+    assert (flat == 77).all() and (decode(behind.numpy(), dtype) == 77).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("counts,inputs,rank", [([1] * 9, 256, 16), ([1] * 9, 4096, 32), ([300], 256, 16), ([128, 1, 256], 256, 16)])
 def test_rows_of_a_plan_that_are_none_of_the_call(cuda, dtype, counts, inputs, rank):
     """They are neither read nor written, wherever they lie in an item: a plan's last words are its rows."""
