@@ -400,6 +400,16 @@ def test_prompts_of_every_cluster_size(cuda, dtype, wtype, items):
     Adapted(17, dtype, wtype, 136, (64, 72), 80, 1, [0], [128 * (items - 1) + 1]).run().check()
 
 
+@pytest.mark.parametrize("dtype,wtype", [("float32", BF16), ("float32", "float16"), ("float16", "float16"), ("float16", BF16), (BF16, BF16), (BF16, "float16")])
+@pytest.mark.parametrize("rank", [88, 96, 104, 128])
+@pytest.mark.parametrize("inputs,widths,counts", [(136, (64, 72), [300, 1, 128]), (520, (200, 16, 33), [129, 700])])
+def test_prompts_of_large_ranks(cuda, dtype, wtype, rank, inputs, widths, counts):
+    """Three or four blocks of B, one target to a pass or two; float32 rows beside float16 adapters above rank 96 in the general kernel."""
+    slots = len(counts)
+    Adapted(30, dtype, wtype, inputs, widths, rank, slots, list(range(slots)), counts).run().check()
+    Adapted(31, dtype, wtype, inputs, widths, rank, slots, list(range(slots)), counts, ranks=[rank - 7] + [rank - 40] * (slots - 1)).run().check()
+
+
 @pytest.mark.parametrize("dtype,wtype", [("float32", BF16), (BF16, BF16)])
 @pytest.mark.parametrize("seqs", [1, 15, 33, 37, 45, 56, 71, 93, 148, 296, 300])
 def test_single_tokens_of_every_cluster_size(cuda, dtype, wtype, seqs):
