@@ -18,7 +18,7 @@
 //
 // Accuracy.  Products are mma m16n8k8 tf32: 16-bit weights and rows are tf32 numbers as they are, float32 rows and h go in two parts
 // (11 bits and the next 11, rounded: 2^-23 of the value is lost at most, the last bit of some).  The matrix unit cuts sums off rather
-// than rounding them, so a chain is 32 inputs long, and the chains are added in float32.
+// than rounding them, so a chain is 32 inputs long, the small parts first or apart, and the chains are added in float32.
 #pragma once
 
 #include "nc_kv4.cuh"
@@ -386,10 +386,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
                     for (int n = 0; n < NT; ++n) {
                         float d[4] = {};
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            lora_mma(d, p[e], q[e], p[e + 1], q[e + 1], high[n][e], high[n][e + 1]);
+                        for (int e = 0; e < 8; e += 2)             // the small parts first, as each step cuts the whole sum off
                             if constexpr (TX == KV_F32) lora_mma(d, p[e], q[e], p[e + 1], q[e + 1], low[n][e], low[n][e + 1]);
-                        }
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) lora_mma(d, p[e], q[e], p[e + 1], q[e + 1], high[n][e], high[n][e + 1]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[i][n][e] = fadd(acc[i][n][e], d[e]);
                     }
@@ -472,17 +472,17 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_rows_kernel(const __grid
                 const float *const at = h + (8 * i + g) * S::HS + (target - t0) * rp + j + 8 * c;
                 const float4 h0 = *(const float4 *)at, h1 = *(const float4 *)(at + 4);
                 const float v[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
-                float d[4] = {};
+                float d[4] = {}, small[4] = {};                    // the small parts' sums apart, as each step cuts the whole sum off
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
                     uint32_t high[2], low[2];
                     lora_split(v[e], &high[0], &low[0]);
                     lora_split(v[e + 1], &high[1], &low[1]);
                     lora_mma(d, p[e], q[e], p[e + 1], q[e + 1], high[0], high[1]);
-                    lora_mma(d, p[e], q[e], p[e + 1], q[e + 1], low[0], low[1]);
+                    lora_mma(small, p[e], q[e], p[e + 1], q[e + 1], low[0], low[1]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][e] = fadd(acc[i][e], d[e]);
+                for (int e = 0; e < 4; ++e) acc[i][e] = fadd(acc[i][e], fadd(small[e], d[e]));
             }
         }
 #pragma unroll

@@ -15,7 +15,7 @@
 // bfloat16 for float32 rows, which hold them, else two.  Two of bfloat16 hold float16 rows; of h they lose 2^-17 at most, where a bfloat16
 // output is rounded by 2^-8, a float16 one by 2^-11.  Two of float16 lose 2^-23 at most, or 2^-39 of the row's largest: a row of x or h is
 // first brought to [2^14, 2^15) by a power of two, so that no size leaves its range.  A chain of
-// the matrix unit, which cuts sums off, is 32 inputs long; chains are added in float32.
+// the matrix unit, which cuts sums off, is 32 inputs long, the largest parts last; chains are added in float32.
 #pragma once
 
 #include "nc_lora_tiles.cuh"
@@ -83,7 +83,7 @@ template <int TW, int PARTS>
 __device__ __forceinline__ void ls_unit(float (&acc)[4], const uint4 &p, const uint4 &q, const char *column, int step) {
     float d[4] = {};
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
+    for (int i = PARTS - 1; i >= 0; --i) {                             // the largest last, as each step cuts the whole sum off
         const uint4 x = *(const uint4 *)(column + i * step);
         ls_mma<TW>(d, p.x, q.x, p.y, q.y, x.x, x.y);
         ls_mma<TW>(d, p.z, q.z, p.w, q.w, x.z, x.w);
