@@ -86,7 +86,8 @@ int32_t launch_lora(cudaStream_t st, const LoraArgs &a, int passes) {
 // rows of 8 adapters 12.4 and 10.6; 28 KB (896 -> 896 at 64) 9.5 and 8.8, 13.0 and 10.1; 30 KB (896 -> 1152 at 32) 11.4 and 11.8, 15.5 and
 // 13.2; 32 KB (4096 -> 4096 at 16) 10.3 and 11.2, 12.5 and 12.9; 64 KB (4096 -> 4096 at 32) 9.6 and 11.6, 12.9 and 13.5.  Most is saved where
 // outputs are many (896 -> 9728 at 16: 12.4 and 17.7); with few of them the ring may take up to a fifth longer (4864 -> 896 at 64: one row 11.7 and
-// 11.5, 64 rows of 8 bfloat16 adapters 15.3 and 12.5, 32 of 32 adapters 15.1 and 16.7).
+// 11.5, 64 rows of 8 bfloat16 adapters 15.3 and 12.5, 32 of 32 adapters 15.1 and 16.7).  With one CTA or two to many items it pays earlier:
+// 28 KB (128 adapters of 896 -> 896 at 16) 11.8 and 12.5.
 template <int TX, int TW>
 bool lora_stream_shape(const LoraArgs &a, int passes, int items, int *ctas, LoraStreamPlan *plan) {
     using S = LoraStream<TX, TW>;
@@ -108,7 +109,7 @@ bool lora_stream_shape(const LoraArgs &a, int passes, int items, int *ctas, Lora
         *ctas = n;
         *plan = p;
     }
-    return *ctas != 0 && bytes / *ctas > 28 * 1024;
+    return *ctas != 0 && bytes / *ctas > (*ctas > 2 ? 28 : 24) * 1024;
 }
 template <int TX, int TW>
 int32_t launch_lora_stream(cudaStream_t st, const LoraArgs &a, int passes, int ctas, const LoraStreamPlan &plan) {
