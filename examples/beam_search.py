@@ -33,7 +33,8 @@ class Beam:
 
 
 class Adapters:
-    """Low-rank adapters of a model's q, k, v, o and down projections: ``slots`` of them, with ranks of their own."""
+    """Low-rank adapters of a model's q, k, v, o and down projections: ``slots`` of them, with ranks of their own. Gate and up have none,
+    as their fused product leaves neither's output to add to."""
 
     NAMES = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.down_proj")
 

@@ -8,8 +8,8 @@
 // of x are in shared memory from the start, as operands, and those of base where they fit.
 //
 // Bound by the adapters' bytes where each request has its own, beside a start of 10 us (the plan's words, x as operands, the sums'
-// way through the cluster).  Adapters of 4096 inputs and outputs at rank 64 (1 MB each), bfloat16, with the plan: one 11.7 us, 16
-// of them 14.5, 64 23.5 (2.9 TB/s), 128 45 (3.0 TB/s of 6.5: two rounds of clusters; 67 with one tile of outputs to a warp at a time).
+// way through the cluster).  Adapters of 4096 inputs and outputs at rank 64 (1 MB each), bfloat16, with the plan: one 11.4 us, 16
+// of them 13.2, 64 23.0 (3.0 TB/s), 128 44.7 (3.1 TB/s of 6.5: two rounds of clusters; 67 with one tile of outputs to a warp at a time).
 //
 // Accuracy.  Products are mma m16n8k16 of the weights' type.  Rows of that type are taken as they are, others and h go in parts: three of
 // bfloat16 for float32 rows, which hold them, else two.  Two of bfloat16 hold float16 rows; of h they lose 2^-17 at most, where a bfloat16

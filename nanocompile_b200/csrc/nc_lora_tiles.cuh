@@ -10,7 +10,7 @@
 // whole 16s to each.
 //
 // Bound by the bytes of x, base and outputs, behind 14 us that no size takes away (tensor memory, two ways through the cluster).  8192
-// bfloat16 rows of 4096 inputs to 6144 outputs at rank 32: 82 us (3.3 TB/s of 6.5; its products are 13 GFLOP, 8 us at the measured rate); 512 of them 30; float32
+// bfloat16 rows of 4096 inputs to 6144 outputs at rank 32: 82 us (3.3 TB/s of 6.5; its products are 13 GFLOP, 8 us at the measured rate); 512 of them 29; float32
 // rows 165 (3.3 TB/s), beside float16 weights 230.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
 // by the warps that add it 122, in bulk copies of a row each 201.
 //

@@ -32,8 +32,8 @@ int64_t lora_groups(int64_t seqs, int64_t slots) { return std::min(seqs, slots +
 // Rows of an item: by the mean of the largest number of groups, as only the device knows how many there are.
 int64_t lora_tile(int64_t rows, int64_t seqs, int64_t slots) {
     const int64_t mean = rows / std::max<int64_t>(1, lora_groups(seqs, slots));
-    // The few items of an adapter by eights read it from L2.  Adapters of 45 KB, 64 of them for 16 rows each: 17 us by eights, 37 by 128; of 1 MB,
-    // 8 of them for 16 rows each 30 and 25, 24 rows each 31 and 25.
+    // The few items of an adapter by eights read it from L2.  Us by eights and by 128: adapters of 45 KB beside float32 rows, 64 of them for 16 rows
+    // each 18 and 37, for 48 55 and 39; of 1 MB beside bfloat16 rows, 64 of them for 16 rows each 64 and 68, for 24 93 and 69, 8 of them 17 and 25.
     return mean <= 16 ? 8 : 128;
 }
 // Items at most: a group that has any has a row.

@@ -463,7 +463,8 @@ def lora_project(layout: LoraLayout, batch: LoraBatch, out, x, a, b, plan, *, ba
 
     ``out`` = ``base`` (default: nought; may be ``out`` itself, at its stride) + ``scales`` * B (A x), each row with its sequence's adapter.
     ``a`` and ``b``: float16 or bfloat16, as :meth:`LoraLayout.a_shape` and ``b_shape`` say. ``ranks`` (int32 ``[slots]``): the adapters' own
-    ranks, where lower; ``scales``: float32 ``[slots]``. float32 rows keep float32 accuracy. With a plan of another batch's sizes
+    ranks, where lower; ``scales``: float32 ``[slots]``. float32 rows keep float32 accuracy (few rows beside float16 adapters: to 2^-39 of
+    the row's largest value, where that is coarser). With a plan of another batch's sizes
     ``out`` stays as it was, and ``runtime.device_faults`` raises.
     """
     rows, slots = batch.rows, batch.slots
