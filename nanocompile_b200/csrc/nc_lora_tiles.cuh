@@ -11,7 +11,7 @@
 //
 // Bound by the bytes of x, base and outputs, behind 14 us that no size takes away (tensor memory, two ways through the cluster).  8192
 // bfloat16 rows of 4096 inputs to 6144 outputs at rank 32: 82 us (3.3 TB/s of 6.5; its products are 13 GFLOP, 8 us at the measured rate); 512 of them 29; float32
-// rows 165 (3.3 TB/s), beside float16 weights 230.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
+// rows 165 (3.3 TB/s), beside float16 weights 212.  While the sums of h were read from the peers the bfloat16 rows took 171 us, with base loaded
 // by the warps that add it 122, in bulk copies of a row each 201.
 //
 // Accuracy.  16-bit rows and weights are multiplied as they are, h goes in two parts (bfloat16: 2^-17 of it is lost at most, float16
@@ -429,16 +429,20 @@ __global__ void __launch_bounds__(LT_THREADS, 1) lora_tiles_kernel(const __grid_
                 }
             };
             LtBlock now, next;
+            auto wait_for = [&](int k) {                               // the stage of block k
+                if (k >= plan.stages) wait(&sh.empty[k % plan.stages], (k / plan.stages - 1) & 1);
+            };
             if (k_blocks > 0) load(0, now), load_a(0, now);
 #pragma unroll 1
             for (int k = 0; k < k_blocks; ++k) {
                 if (k + 1 < k_blocks) {
                     load(k + 1, next);                                 // before the wait: 8192 rows 194 us behind it
-                    if (k + 1 >= plan.stages) wait(&sh.empty[(k + 1) % plan.stages], ((k + 1) / plan.stages - 1) & 1);
+                    if constexpr (S::PW == 1) wait_for(k + 1);
                     load_a(k + 1, next);
                 } else {
                     lt_commit();
                 }
+                if constexpr (S::PW == 2) wait_for(k);                 // its weights come through registers, and nothing before the store needs the stage
                 store(k, now);
                 lt_wait_copies<1>();
                 lt_async_fence();
